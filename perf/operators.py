@@ -105,7 +105,8 @@ def _blocks(x, dim):
 def _scales(amax):
     """(what the values are multiplied by, what stands in the scale) from the largest magnitude of a group."""
     amax = amax.clamp(min=TINY)
-    return E4M3_MAX / amax, amax / E4M3_MAX
+    most = torch.full_like(amax, E4M3_MAX)             # a quotient of tensors is rounded once, one with a number may not be
+    return most / amax, amax / most
 
 
 def _rounded(v, like):
@@ -428,12 +429,19 @@ def exact(case, seed):
     kind, D = case["kind"], torch.float64
     st = prepare(case, seed)
 
+    def quotients(m):
+        """A group's scale and multiplier: 32-bit numbers by definition."""
+        m = m.float()
+        top = torch.full_like(m, 448.0)
+        return (m / top).double(), (top / m).double()
+
     def groups_of(v, size):
         """[(first, last, scale, multiplier)] along the last dimension of v."""
         out = []
         for a in range(0, v.shape[-1], size):
             m = v[..., a:a + size].abs().amax(-1).clamp(min=TINY)
-            out.append((a, min(a + size, v.shape[-1]), (m.float() / 448).double(), (448 / m.float()).double()))
+            s, inv = quotients(m)
+            out.append((a, min(a + size, v.shape[-1]), s, inv))
         return out
 
     def held(v):
@@ -456,9 +464,8 @@ def exact(case, seed):
         for i in range(s.shape[0]):
             for j in range(s.shape[1]):
                 r, c = slice(128 * i, 128 * i + 128), slice(128 * j, 128 * j + 128)
-                m = w[r, c].abs().amax().float().clamp(min=TINY)
-                q[r, c] = held(w[r, c].double() * (448 / m).double())
-                s[i, j] = (m / 448).double()
+                s[i, j], inv = quotients(w[r, c].abs().amax().float().clamp(min=TINY))
+                q[r, c] = held(w[r, c].double() * inv)
                 deq[r, c] = q[r, c] * s[i, j]
         return deq, q, s
 
