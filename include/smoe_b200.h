@@ -470,6 +470,60 @@ int smoe_switch_loss(const void* logits, int bf16, const int32_t* freq, int64_t 
 int smoe_switch_loss_bwd(const void* logits, int bf16, const float* grad, const float* dloss, int64_t T, int64_t E,
                          void* dlogits, void* stream);
 
+/* ---- group-limited routing --------------------------------------------------
+ * No counterpart in the reference, whose router is the softmax over the K selected logits above.
+ * logits [T,E] (f32, or bf16 != 0), bias [E] f32 or null.  s = sigmoid(logit), or softmax over the E logits; c = s + bias (without
+ * a bias experts are ordered by their logits).  A group (E / groups neighbouring experts) scores the sum of its group_score (1 or 2)
+ * best c; the top_groups best groups stay, and of their experts the K best are taken: idx [T,K] in descending order, the first of
+ * equals before the others, scores [T,K] = scale * s / (sum of the K taken s + 1e-20), or scale * s without `normalize`.
+ * A logit of -inf closes its expert; slots beyond the open experts have index -1 and score 0.  NaN ranks lowest.  The selection is
+ * that of 64-bit arithmetic.  E <= 1024, K <= 32, groups <= 32, E % groups == 0, K <= top_groups * E / groups. */
+int smoe_group_routing(const void* logits, int bf16, const float* bias, int64_t T, int64_t E, int64_t K, int64_t groups,
+                       int64_t top_groups, int group_score, int softmax, int normalize, float scale, float* scores, int32_t* idx,
+                       void* stream);
+/* Gradient of the logits (of their type) from that of the scores; the selection and the bias are constants. */
+int smoe_group_routing_bwd(const void* logits, int bf16, const int32_t* idx, const float* dscores, int64_t T, int64_t E, int64_t K,
+                           int softmax, int normalize, float scale, void* dlogits, void* stream);
+
+/* ---- products with one f32 scale per block of 128 -------------------------------
+ * No counterpart in the reference, whose scales are ue8m0 per 1x32.  Activations carry a scale for each row and 128 columns
+ * (1x128), weights one for each 128 x 128, the operands of a weight gradient one for each column and 128 rows.  A block's scale is
+ * a / 448 and its payload e4m3(x * (448 / a)), a = max(max |x|, 2^-100), f32 throughout.
+ * Payload rows lie ceil(cols / 16) * 16 bytes apart; scales are dense.  Sizes are multiples of 8; payloads start on 16 bytes.
+ * Segments: efo [E+1] ascending multiples of 128 as smoe_topk_metadata leaves them, counts [E] live rows at a segment's start (null:
+ * all); efo null: one segment (E = 1) of all rows. */
+
+/* x bf16 [rows,K] -> q [rows,K], scales [rows, K/128].  swiglu: x is [rows,2K], gate / up interleaved, and what is quantised is
+ * silu(gate) * up (f32).  list != null: only the rows list[i], i < min(n_list, *n_live), are read and written. */
+int smoe_quant128_rows(const void* x_bf16, int64_t rows, int64_t K, int swiglu, const int32_t* list, const int32_t* n_live,
+                       int64_t n_list, void* q, float* scales, void* stream);
+/* x bf16 [T,K]: row t, quantised once, to the rows s_rev[naept[t]] .. s_rev[naept[t+1] - 1] of q [rows,K], scales [rows, K/128]. */
+int smoe_quant128_rows_scatter(const void* x_bf16, int64_t T, int64_t K, const int32_t* naept, const int32_t* s_rev, int64_t rows,
+                               void* q, float* scales, void* stream);
+/* Both forms of x bf16 [rows,K] from one read: q, scales as above (null: not written) and q_col [rows,K], col_scales
+ * [ceil(rows/128), K], where the rows of a segment behind its live ones count and leave zero.  128-row blocks without live rows
+ * have no column form. */
+int smoe_quant128_dual(const void* x_bf16, int64_t rows, int64_t K, const int32_t* efo, const int32_t* counts, int64_t E, void* q,
+                       float* scales, void* q_col, float* col_scales, void* stream);
+/* W bf16 [E,N,K] -> q [E,N,K], scales [E, N/128, K/128] (both rounded up). */
+int smoe_quant128_weight(const void* w_bf16, int64_t E, int64_t N, int64_t K, void* q, float* scales, void* stream);
+
+/* c[r,:] = a[r,:] . b[e(r)]^T, bf16 [rows,N]: a [rows,K] by rows, b [E,N,K] by blocks.  b_mn: b is stored [E,K,N] (a weight read
+ * the other way: the gradient of its input needs no transposed copy), its scales [E, K/128, N/128].  Rows that are not live are
+ * written as zero (zero_rest), or left as they are.  E <= 256.  pinned_host_word (may be null) receives a failure code at once. */
+int smoe_gemm128_rows(const void* a_fp8, const float* a_scales, const void* b_fp8, const float* b_scales, const int32_t* efo,
+                      const int32_t* counts, void* c_bf16, int64_t rows, int64_t N, int64_t K, int64_t E, int b_mn, int zero_rest,
+                      int32_t* status, int32_t* pinned_host_word, void* stream);
+/* The same made for few rows per expert (any counts are computed right), b [E,N,K]; rows that are not live are left as they are.
+ * live_rows: at most so many rows are live (0: not known); it only decides how the work is divided. */
+int smoe_gemm128_few(const void* a_fp8, const float* a_scales, const void* b_fp8, const float* b_scales, const int32_t* efo,
+                     const int32_t* counts, void* c_bf16, int64_t rows, int64_t N, int64_t K, int64_t E, int64_t live_rows,
+                     int32_t* status, int32_t* pinned_host_word, void* stream);
+/* c[e] (M x N) = a[seg_e]^T . b[seg_e], a [rows,M] and b [rows,N] by columns: f32, added to c or stored, or rounded to bf16. */
+int smoe_gemm128_wgrad(const void* a_fp8, const float* a_scales, const void* b_fp8, const float* b_scales, const int32_t* efo,
+                       const int32_t* counts, void* c, int64_t M, int64_t N, int64_t rows, int64_t E, int out_bf16, int accumulate,
+                       int32_t* status, int32_t* pinned_host_word, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -3,31 +3,15 @@
 #include <cuda_runtime.h>
 #include <cudaTypedefs.h>
 
-#include <mutex>
-
 #include "gemm.cuh"
 #include "gemm2.cuh"
 #include "gemm3.cuh"
 #include "gemm_few.cuh"
+#include "host.h"
 #include "smoe_b200.h"
 #include "smoe_internal.h"
 
 namespace smoe {
-
-static PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
-static std::once_flag g_encode_once;
-
-static bool load_encode() {
-  std::call_once(g_encode_once, [] {
-    void* fn = nullptr;
-    cudaDriverEntryPointQueryResult qres;
-    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &qres) ==
-            cudaSuccess &&
-        qres == cudaDriverEntryPointSuccess)
-      g_encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
-  });
-  return g_encode != nullptr;
-}
 
 // 2D row-major uint8 tensor [rows, cols], box {box_cols, box_rows}, 128-byte swizzle.
 static int make_tmap_u8(CUtensorMap* m, const void* base, uint64_t rows, uint64_t cols, uint32_t box_cols,
@@ -70,33 +54,6 @@ static int make_tmap_dw(CUtensorMap* m, const GemmParams& p, void* c, uint64_t r
 static int g_force_bn = 0;
 static int g_force_v1 = 0;
 static int g_force_gather4 = 0;     // A rows by index: TMA gather4 instead of the cp.async load warps
-
-// Per-device state: the SM count and the "large dynamic shared memory" function attribute belong to a device,
-// not to the process, so both are kept per device ordinal.
-constexpr int kMaxDevices = 64;
-static int g_sm_count[kMaxDevices] = {};
-
-static int current_device() {
-  int dev = 0;
-  cudaGetDevice(&dev);
-  return (dev >= 0 && dev < kMaxDevices) ? dev : 0;
-}
-
-static int sm_count() {
-  const int dev = current_device();
-  if (g_sm_count[dev] == 0) cudaDeviceGetAttribute(&g_sm_count[dev], cudaDevAttrMultiProcessorCount, dev);
-  return g_sm_count[dev];
-}
-
-// cudaFuncSetAttribute(MaxDynamicSharedMemorySize) once per (kernel instantiation, device)
-template <typename Kern>
-static bool ensure_smem_attr(Kern kern, int bytes, bool (&done)[kMaxDevices]) {
-  const int dev = current_device();
-  if (done[dev]) return true;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
-  done[dev] = true;
-  return true;
-}
 
 template <int BN, int MODE>
 static int launch(const CUtensorMap& ta, const CUtensorMap& tb, const GemmParams& p, int max_tiles,

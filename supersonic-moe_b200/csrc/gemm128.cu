@@ -1,0 +1,139 @@
+// Host side of the products with a scale per block of 128.
+#include "gemm128.cuh"
+#include "gemm128_few.cuh"
+#include "host.h"
+#include "smoe_b200.h"
+
+namespace smoe {
+
+// [depth, rows, cols] bytes, rows a multiple of 16 bytes apart, box {128, box_rows, 1} in the 128-byte swizzle; what lies beyond an
+// extent reads as zero
+static int make_tmap128(CUtensorMap* m, const void* base, uint64_t depth, uint64_t rows, uint64_t cols, uint32_t box_rows, int dims) {
+  if (!load_encode()) return SMOE_ERR_DRIVER;
+  if (reinterpret_cast<uintptr_t>(base) & 15) return SMOE_ERR_ALIGN;
+  const cuuint64_t pitch = (cols + 15) & ~(uint64_t)15;
+  cuuint64_t extent[3] = {cols, rows, depth};
+  cuuint64_t strides[2] = {pitch, pitch * rows};
+  cuuint32_t box[3] = {128, box_rows, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = g_encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, dims, const_cast<void*>(base), extent, strides, box, estr,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? SMOE_OK : SMOE_ERR_TMAP;
+}
+
+template <int MODE>
+static int launch128(const CUtensorMap& ta, const CUtensorMap& tb, const Gemm128Params& p, int64_t tiles, cudaStream_t stream) {
+  static bool attr_set[kMaxDevices] = {};
+  auto kern = gemm128_kernel<MODE>;
+  if (!ensure_smem_attr(kern, Gemm128Smem::TOTAL, attr_set)) return SMOE_ERR_LAUNCH;
+  int64_t pairs = sm_count() / 2;
+  if (tiles < pairs) pairs = tiles;
+  if (pairs <= 0) return SMOE_OK;
+  kern<<<(unsigned)(2 * pairs), Gemm128Smem::THREADS, Gemm128Smem::TOTAL, stream>>>(ta, tb, p);
+  return cudaGetLastError() == cudaSuccess ? SMOE_OK : SMOE_ERR_LAUNCH;
+}
+
+static bool size128(int64_t n) { return n > 0 && n % 8 == 0 && n < (int64_t)1 << 24; }
+
+static int check128(const void* a, const float* a_s, const void* b, const float* b_s, const int* efo, const int* counts, const void* c,
+                    int64_t rows, int64_t N, int64_t K, int64_t E, const int* status) {
+  if (rows < 0 || rows >= (int64_t)1 << 31 || !size128(N) || !size128(K) || E <= 0 || E > kMaxExperts2) return SMOE_ERR_SHAPE;
+  if (!efo && (E != 1 || counts)) return SMOE_ERR_ARG;
+  if (!status || (rows > 0 && (!a || !a_s || !b || !b_s || !c))) return SMOE_ERR_ARG;
+  if (((uintptr_t)a | (uintptr_t)b | (uintptr_t)c | (uintptr_t)a_s | (uintptr_t)b_s) & 15) return SMOE_ERR_ALIGN;
+  return SMOE_OK;
+}
+
+static int64_t up(int64_t n, int64_t m) { return (n + m - 1) / m; }
+
+}  // namespace smoe
+
+using namespace smoe;
+
+extern "C" {
+
+int smoe_gemm128_rows(const void* a_fp8, const float* a_scales, const void* b_fp8, const float* b_scales, const int32_t* efo,
+                      const int32_t* counts, void* c_bf16, int64_t rows, int64_t N, int64_t K, int64_t E, int b_mn,
+                      int zero_rest, int32_t* status, int32_t* pinned_host_word, void* stream) {
+  int rc = check128(a_fp8, a_scales, b_fp8, b_scales, efo, counts, c_bf16, rows, N, K, E, status);
+  if (rc || rows == 0) return rc;
+  CUtensorMap ta, tb;
+  rc = make_tmap128(&ta, a_fp8, 1, rows, K, 128, 2);
+  if (!rc) rc = b_mn ? make_tmap128(&tb, b_fp8, E, K, N, 128, 3) : make_tmap128(&tb, b_fp8, E, N, K, 128, 3);
+  if (rc) return rc;
+  Gemm128Params p{};
+  p.rows = (int)rows; p.N = (int)N; p.K = (int)K; p.E = (int)E;
+  p.efo = efo; p.counts = counts; p.a_s = a_scales; p.b_s = b_scales;
+  const int64_t nb = up(N, 128), kb = up(K, 128);
+  p.a_kb = (int)kb;
+  p.bs_e = nb * kb;
+  p.bs_n = b_mn ? 1 : kb;
+  p.bs_k = b_mn ? (int)nb : 1;
+  p.b_mn = b_mn != 0; p.c = c_bf16; p.zero_rest = zero_rest != 0; p.status = status; p.host_word = pinned_host_word;
+  // every segment may end in a tile that is not full, and so may the rows behind the last
+  const int64_t tiles = efo ? (rows / 256 + E + 1) * up(N, 256) : up(rows, 256) * up(N, 256);
+  return launch128<ROWS128>(ta, tb, p, tiles, (cudaStream_t)stream);
+}
+
+int smoe_gemm128_wgrad(const void* a_fp8, const float* a_scales, const void* b_fp8, const float* b_scales, const int32_t* efo,
+                       const int32_t* counts, void* c, int64_t M, int64_t N, int64_t rows, int64_t E, int out_bf16, int accumulate,
+                       int32_t* status, int32_t* pinned_host_word, void* stream) {
+  int rc = check128(a_fp8, a_scales, b_fp8, b_scales, efo, counts, c, rows, N, M, E, status);
+  if (rc) return rc;
+  if (out_bf16 && accumulate) return SMOE_ERR_ARG;
+  if (rows == 0) {                                  // an empty sum
+    if (accumulate) return SMOE_OK;
+    if (!c) return SMOE_ERR_ARG;
+    return cudaMemsetAsync(c, 0, (size_t)(E * M * N) * (out_bf16 ? 2 : 4), (cudaStream_t)stream) == cudaSuccess ? SMOE_OK
+                                                                                                             : SMOE_ERR_LAUNCH;
+  }
+  CUtensorMap ta, tb;
+  rc = make_tmap128(&ta, a_fp8, 1, rows, M, 128, 2);
+  if (!rc) rc = make_tmap128(&tb, b_fp8, 1, rows, N, 128, 3);
+  if (rc) return rc;
+  Gemm128Params p{};
+  p.rows = (int)rows; p.M = (int)M; p.N = (int)N; p.E = (int)E;
+  p.efo = efo; p.counts = counts; p.a_s = a_scales; p.b_s = b_scales;
+  p.c = c; p.out_bf16 = out_bf16 != 0; p.accumulate = accumulate != 0; p.status = status;
+  p.host_word = pinned_host_word;
+  return launch128<WGRAD128>(ta, tb, p, E * up(M, 256) * up(N, 256), (cudaStream_t)stream);
+}
+
+int smoe_gemm128_few(const void* a_fp8, const float* a_scales, const void* b_fp8, const float* b_scales, const int32_t* efo,
+                     const int32_t* counts, void* c_bf16, int64_t rows, int64_t N, int64_t K, int64_t E, int64_t live_rows,
+                     int32_t* status, int32_t* pinned_host_word, void* stream) {
+  int rc = check128(a_fp8, a_scales, b_fp8, b_scales, efo, counts, c_bf16, rows, N, K, E, status);
+  if (rc || rows == 0) return rc;
+  if (live_rows <= 0 || live_rows > rows) live_rows = rows;
+  CUtensorMap tw, tx;
+  rc = make_tmap128(&tw, b_fp8, E, N, K, 128, 3);
+  if (!rc) rc = make_tmap128(&tx, a_fp8, 1, rows, K, 16, 2);
+  if (rc) return rc;
+  static bool attr_set[kMaxDevices] = {};
+  if (!ensure_smem_attr(gemm128_few_kernel, Few128Smem::TOTAL, attr_set)) return SMOE_ERR_LAUNCH;
+  const int sms = sm_count();
+  const int64_t nw = up(N, 128), busy = live_rows < E ? live_rows : E;
+  const int64_t tiles = (live_rows / Few128Smem::NT + busy) * nw;       // as many as there can be
+  int split = 1;
+  while (split < 8 && tiles * split * 2 <= sms && split * 4 <= up(K, 128)) split *= 2;
+  Few128Params p{(int)rows, (int)N, (int)K, (int)E, efo, counts, b_scales, a_scales, (__nv_bfloat16*)c_bf16, split, status,
+                 pinned_host_word};
+  int64_t groups = sms / split;
+  if (tiles < groups) groups = tiles;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = (unsigned)split;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(groups * split));
+  cfg.blockDim = dim3(Few128Smem::THREADS);
+  cfg.dynamicSmemBytes = Few128Smem::TOTAL;
+  cfg.stream = (cudaStream_t)stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, gemm128_few_kernel, tw, tx, p) != cudaSuccess) return SMOE_ERR_LAUNCH;
+  return cudaGetLastError() == cudaSuccess ? SMOE_OK : SMOE_ERR_LAUNCH;
+}
+
+}  // extern "C"

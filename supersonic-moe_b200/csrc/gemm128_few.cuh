@@ -1,0 +1,281 @@
+// The product of gemm128.cuh for few rows per expert (single tokens, decoding): the weights are the M operand.
+//
+// Such a call is bound by the read of the weights.  A CTA computes 128 weight rows x up to 64 routed rows, so that each SM streams
+// weight tiles of its own; of the routed rows only as many 16-row pieces are fetched and multiplied as hold live ones.  The sum
+// of a block of 128 lies transposed in TMEM (lane = weight row, column = routed row) in one of eight buffers of 64 columns; the
+// epilogue warps scale it - one number a column, which every lane reads from shared memory - and keep 64 f32 sums a thread.
+//
+// Where the weight tiles are too few to occupy the SMs a cluster of 2, 4 or 8 CTAs shares one: each takes a stretch of the
+// reduction, leaves its sums in its shared memory, and adds up a share of the columns from all of them, in rank order.
+#pragma once
+#include "gemm128.cuh"
+
+namespace smoe {
+
+struct Few128Params {
+  int rows, N, K, E;
+  const int *efo, *counts;
+  const float *w_s, *x_s;    // [E, N/128, K/128], [rows, K/128]
+  __nv_bfloat16* c;          // [rows, N], live rows only are written
+  int split;                 // CTAs of a cluster
+  int* status;
+  volatile int* host_word;
+};
+
+struct Few128Smem {
+  static constexpr int NT = 64;                               // routed rows of a tile
+  static constexpr int A_BYTES = BM * BK, B_BYTES = NT * BK;
+  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES, STAGES = 7;
+  static constexpr int ACC = 8;                               // TMEM buffers
+  static constexpr int EPI_WARPS = 4;
+  static constexpr int PART_BYTES = NT * BM * 4;              // sums of this CTA: [column][weight row]
+  static constexpr int SX_BYTES = EPI_WARPS * 2 * NT * 4;     // scales of a block's columns, per warp, two buffers
+  static constexpr int AUX_BYTES = 512 + 3 * (kG128Segs + 1) * 4;
+  static constexpr int TOTAL = 1024 + STAGES * STAGE_BYTES + PART_BYTES + SX_BYTES + AUX_BYTES;
+  static constexpr int THREADS = 32 * (2 + EPI_WARPS);
+  static_assert(TOTAL <= 227 * 1024, "shared memory budget");
+  static_assert((2 * STAGES + 2 * ACC + 2) * 8 <= 496, "barrier storage");
+};
+
+// as mbar_wait, for data that other CTAs of the cluster left before they arrived
+__device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity) {
+  const uint64_t t0 = globaltimer_ns();
+  uint32_t spins = 0;
+  while (true) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity), "r"(kTryWaitHintNs)
+        : "memory");
+    if (ok) return true;
+    if ((++spins & 0x3ff) == 0 && globaltimer_ns() - t0 > kWaitLimitNs) return false;
+  }
+}
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+struct FewTile128 {
+  int e, w0, row0, live;     // live: 1 .. NT
+};
+// the row tiles of one weight tile are neighbours: L2 serves the weights
+__device__ __forceinline__ FewTile128 few_tile128(int tile, int nw, int E, const Segs128& s) {
+  FewTile128 t;
+  t.e = seg_of_tile(s.tiles, E, tile / nw);
+  const int n = s.tiles[t.e + 1] - s.tiles[t.e], r = tile - s.tiles[t.e] * nw;
+  t.w0 = r / n * BM;
+  t.row0 = s.start[t.e] + r % n * Few128Smem::NT;
+  t.live = min(s.live[t.e] - t.row0, Few128Smem::NT);
+  return t;
+}
+
+__global__ void __launch_bounds__(Few128Smem::THREADS, 1)
+gemm128_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, const Few128Params p) {
+  using S = Few128Smem;
+  constexpr int NT = S::NT;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float* part = reinterpret_cast<float*>(smem + S::STAGES * S::STAGE_BYTES);
+  uint8_t* sx_all = reinterpret_cast<uint8_t*>(part) + S::PART_BYTES;
+  uint8_t* aux = sx_all + S::SX_BYTES;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(aux);            // full[S], empty[S], tfull[ACC], tempty[ACC], pfull, pempty
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(aux + 496);
+  volatile int* s_abort = reinterpret_cast<volatile int*>(aux + 500);
+  Segs128 segs;
+  segs.start = reinterpret_cast<int*>(aux + 512);
+  segs.live = segs.start + kG128Segs + 1;
+  segs.tiles = segs.live + kG128Segs + 1;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int split = p.split, rank = split > 1 ? (int)cluster_ctarank() : 0;
+  const int group = blockIdx.x / split, n_groups = gridDim.x / split;
+  const uint32_t bar_full = smem_u32(bars), bar_empty = bar_full + 8 * S::STAGES;
+  const uint32_t bar_tfull = bar_empty + 8 * S::STAGES, bar_tempty = bar_tfull + 8 * S::ACC;
+  const uint32_t bar_pfull = bar_tempty + 8 * S::ACC, bar_pempty = bar_pfull + 8;
+
+  if (warp == 2) load_segs128(segs, p.efo, p.counts, p.E, p.rows, NT, true, lane);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S::STAGES; ++s) {
+      mbar_init(bar_full + 8 * s, 1);
+      mbar_init(bar_empty + 8 * s, 1);
+    }
+    for (int s = 0; s < S::ACC; ++s) {
+      mbar_init(bar_tfull + 8 * s, 1);
+      mbar_init(bar_tempty + 8 * s, S::EPI_WARPS);
+    }
+    mbar_init(bar_pfull, S::EPI_WARPS * split);
+    mbar_init(bar_pempty, S::EPI_WARPS * split);
+    *s_abort = 0;
+    fence_barrier_init();
+    fence_proxy_async_smem();
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_slot), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (split > 1) cluster_sync_all();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  const uint32_t smem_base = smem_u32(smem);
+  const int nw = (p.N + BM - 1) / BM, nkt = (p.K + 127) / 128;
+  const int n_total = segs.tiles[p.E] * nw;
+  const int k0 = rank * nkt / split, k1 = (rank + 1) * nkt / split;        // split <= nkt: nobody is without
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer
+    if (lane == 0) {
+      prefetch_tmap(&tmap_w);
+      prefetch_tmap(&tmap_x);
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int tile = group; tile < n_total && ok; tile += n_groups) {
+        const FewTile128 t = few_tile128(tile, nw, p.E, segs);
+        const int pieces = (t.live + 15) / 16;
+        for (int k = k0; k < k1; ++k) {
+          ok = mbar_wait(bar_empty + 8 * stage, phase ^ 1);
+          if (!ok) break;
+          const uint32_t full = bar_full + 8 * stage, a_dst = smem_base + stage * S::STAGE_BYTES, b_dst = a_dst + S::A_BYTES;
+          mbar_expect_tx(full, S::A_BYTES + pieces * 16 * BK);
+          tma_load_3d(a_dst, &tmap_w, full, k * 128, t.w0, t.e);
+          for (int i = 0; i < pieces; ++i) tma_load_2d(b_dst + i * 16 * BK, &tmap_x, full, k * 128, t.row0 + i * 16);
+          if (++stage == S::STAGES) { stage = 0; phase ^= 1; }
+        }
+      }
+      if (!ok) { *s_abort = 1; fail128(p.status, p.host_word, 501); }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
+    if (elect_one()) {
+      int stage = 0, as = 0;
+      uint32_t phase = 0, aphase = 0;
+      bool ok = true;
+      for (int tile = group; tile < n_total && ok; tile += n_groups) {
+        const FewTile128 t = few_tile128(tile, nw, p.E, segs);
+        const uint32_t idesc = make_idesc_f8(BM, (t.live + 15) / 16 * 16, false, false);
+        for (int k = k0; k < k1; ++k) {
+          ok = mbar_wait(bar_tempty + 8 * as, aphase ^ 1) && mbar_wait(bar_full + 8 * stage, phase);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t a_src = smem_base + stage * S::STAGE_BYTES;
+          const uint64_t a_desc = make_desc_kmajor_sw128(a_src), b_desc = make_desc_kmajor_sw128(a_src + S::A_BYTES);
+#pragma unroll
+          for (int kb = 0; kb < BK / 32; ++kb) mma_f8(tmem_base + as * NT, a_desc + 2 * kb, b_desc + 2 * kb, idesc, kb != 0);
+          tc_commit(bar_empty + 8 * stage);
+          tc_commit(bar_tfull + 8 * as);
+          if (++stage == S::STAGES) { stage = 0; phase ^= 1; }
+          if (++as == S::ACC) { as = 0; aphase ^= 1; }
+        }
+      }
+      if (!ok) { *s_abort = 1; fail128(p.status, p.host_word, 502); }
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------ epilogue: a warp owns 32 weight rows, its TMEM lanes
+    const int q = warp & 3;
+    float* sx = reinterpret_cast<float*>(sx_all) + (warp - 2) * 2 * NT;
+    int as = 0;
+    uint32_t aphase = 0, pphase = 0;
+    bool ok = true;
+    for (int tile = group; tile < n_total && ok; tile += n_groups) {
+      const FewTile128 t = few_tile128(tile, nw, p.E, segs);
+      const int w_row = t.w0 + q * 32 + lane;
+      float acc[NT];
+#pragma unroll
+      for (int i = 0; i < NT; ++i) acc[i] = 0.f;
+      const float* ws = p.w_s + ((int64_t)t.e * nw + t.w0 / 128) * nkt;
+      const bool in0 = lane < t.live, in1 = lane + 32 < t.live;
+      const float* xs0 = p.x_s + (int64_t)(t.row0 + (in0 ? lane : 0)) * nkt;
+      const float* xs1 = p.x_s + (int64_t)(t.row0 + (in1 ? lane + 32 : 0)) * nkt;
+      float n0 = xs0[k0] * ws[k0], n1 = xs1[k0] * ws[k0];
+      for (int k = k0; k < k1; ++k) {
+        float* sk = sx + (k & 1) * NT;
+        sk[lane] = n0;
+        sk[lane + 32] = n1;
+        __syncwarp();
+        if (k + 1 < k1) {
+          const float w = ws[k + 1];
+          n0 = xs0[k + 1] * w;
+          n1 = xs1[k + 1] * w;
+        }
+        ok = __all_sync(0xffffffffu, mbar_wait(bar_tfull + 8 * as, aphase));
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t src = tmem_base + ((uint32_t)(q * 32) << 16) + as * NT;
+#pragma unroll
+        for (int c = 0; c < NT / 16; ++c) {
+          if (c * 16 < t.live) {
+            uint32_t r[16];
+            tmem_ld16(src + c * 16, r);
+            tmem_ld_wait();
+            tmem_arrived(r);
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+              const float4 s4 = *reinterpret_cast<const float4*>(sk + c * 16 + i);
+              acc[c * 16 + i] = fmaf(__uint_as_float(r[i]), s4.x, acc[c * 16 + i]);
+              acc[c * 16 + i + 1] = fmaf(__uint_as_float(r[i + 1]), s4.y, acc[c * 16 + i + 1]);
+              acc[c * 16 + i + 2] = fmaf(__uint_as_float(r[i + 2]), s4.z, acc[c * 16 + i + 2]);
+              acc[c * 16 + i + 3] = fmaf(__uint_as_float(r[i + 3]), s4.w, acc[c * 16 + i + 3]);
+            }
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_tempty + 8 * as);
+        if (++as == S::ACC) { as = 0; aphase ^= 1; }
+      }
+      if (!ok) break;
+      if (split == 1) {
+        if (w_row < p.N) {
+          __nv_bfloat16* dst = p.c + (int64_t)t.row0 * p.N + w_row;
+#pragma unroll
+          for (int i = 0; i < NT; ++i)
+            if (i < t.live) dst[(int64_t)i * p.N] = __float2bfloat16_rn(acc[i]);
+        }
+      } else {
+        // everyone has read what this CTA left for the tile before
+        ok = __all_sync(0xffffffffu, mbar_wait_cluster(bar_pempty, pphase ^ 1));
+        if (!ok) break;
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+          if (i < t.live) part[i * BM + q * 32 + lane] = acc[i];
+        __syncwarp();
+        if (lane < split) mbar_arrive_cluster(map_to_cta(bar_pfull, lane));
+        ok = __all_sync(0xffffffffu, mbar_wait_cluster(bar_pfull, pphase));
+        if (!ok) break;
+        const uint32_t mine = smem_u32(part + q * 32 + lane);
+        for (int i = rank; i < t.live; i += split) {
+          float v = 0.f;
+          for (int r = 0; r < split; ++r) v += ld_cluster_f32(map_to_cta(mine + i * BM * 4, r));
+          if (w_row < p.N) p.c[(int64_t)(t.row0 + i) * p.N + w_row] = __float2bfloat16_rn(v);
+        }
+        __syncwarp();
+        if (lane < split) mbar_arrive_cluster(map_to_cta(bar_pempty, lane));
+        pphase ^= 1;
+      }
+    }
+    if (!ok && lane == 0) { *s_abort = 1; fail128(p.status, p.host_word, 503); }
+  }
+
+  // common exit: everyone arrives here, also after a failed wait
+  __syncthreads();
+  if (*s_abort) {                             // copies and MMAs in flight may still write this CTA's memory
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 2000000ull) __nanosleep(1000);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (split > 1) cluster_sync_all();          // the others may still read this CTA's sums
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem_base, 512);
+}
+
+}  // namespace smoe

@@ -6,6 +6,12 @@ __version__ = "0.1.0"
 
 from . import _lib  # noqa: F401
 from . import ops  # noqa: F401
+from .block128 import (  # noqa: F401
+    block128_experts,
+    block128_linear,
+    quantize_rows_block128,
+    quantize_weight_block128,
+)
 from .config import SonicMoEConfig, get_active_config, set_active_config  # noqa: F401
 from .count_cumsum import count_cumsum  # noqa: F401
 from .enums import ActivationType, KernelBackendMoE  # noqa: F401
@@ -25,4 +31,4 @@ from .functional import (  # noqa: F401
 from .interface import run_sonic_moe  # noqa: F401
 from .moe import MoE  # noqa: F401
 from .quack_utils import pack_blockscaled_1x32_scales  # noqa: F401
-from .routing import token_rounding_routing  # noqa: F401
+from .routing import group_limited_routing, token_rounding_routing  # noqa: F401

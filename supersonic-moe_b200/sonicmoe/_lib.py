@@ -7,12 +7,12 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_int, c_int64, c_void_p
+from ctypes import c_float, c_int, c_int64, c_void_p
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libsmoe_b200.so")
 
-_P, _I, _L = c_void_p, c_int, c_int64
+_P, _I, _L, _F = c_void_p, c_int, c_int64, c_float
 
 
 class LayerArgs(ctypes.Structure):
@@ -87,6 +87,15 @@ SIGNATURES = {
     "smoe_switch_loss_workspace": (_L, [_L]),
     "smoe_switch_loss": (_I, [_P, _I, _P, _L, _L, _P, _P, _P, _P]),
     "smoe_switch_loss_bwd": (_I, [_P, _I, _P, _P, _L, _L, _P, _P]),
+    "smoe_group_routing": (_I, [_P, _I, _P, _L, _L, _L, _L, _L, _I, _I, _I, _F, _P, _P, _P]),
+    "smoe_group_routing_bwd": (_I, [_P, _I, _P, _P, _L, _L, _L, _I, _I, _F, _P, _P]),
+    "smoe_quant128_rows": (_I, [_P, _L, _L, _I, _P, _P, _L, _P, _P, _P]),
+    "smoe_quant128_rows_scatter": (_I, [_P, _L, _L, _P, _P, _L, _P, _P, _P]),
+    "smoe_quant128_dual": (_I, [_P, _L, _L, _P, _P, _L, _P, _P, _P, _P, _P]),
+    "smoe_quant128_weight": (_I, [_P, _L, _L, _L, _P, _P, _P]),
+    "smoe_gemm128_rows": (_I, [_P] * 7 + [_L] * 4 + [_I, _I, _P, _P, _P]),
+    "smoe_gemm128_few": (_I, [_P] * 7 + [_L] * 5 + [_P, _P, _P]),
+    "smoe_gemm128_wgrad": (_I, [_P] * 7 + [_L] * 4 + [_I, _I, _P, _P, _P]),
 }
 
 # exported for the library's own tests only (csrc/smoe_internal.h); not product ABI

@@ -777,3 +777,236 @@ def switch_loss_bwd(logits, grad, dloss):
     check(lib.smoe_switch_loss_bwd(_p(logits), int(logits.dtype == torch.bfloat16), _p(grad), _p(dloss), T, E, _p(out),
                                    _stream()), "switch_loss_bwd")
     return out
+
+
+# ---------------------------------------------------------------- group-limited routing, products with a scale per block of 128
+def _on_their_device(fn):
+    """Launch where the tensors are: they have to be on one GPU, which need not be the current one."""
+    import functools
+
+    @functools.wraps(fn)
+    def wrapper(*a, **k):
+        dev = None
+        for t in (*a, *k.values()):
+            if isinstance(t, torch.Tensor):
+                if not t.is_cuda:
+                    raise RuntimeError("sonicmoe kernels need CUDA tensors (no CPU fallback)")
+                if dev is None:
+                    dev = t.device.index
+                elif t.device.index != dev:
+                    raise RuntimeError(f"{fn.__name__}: tensors on cuda:{dev} and cuda:{t.device.index}")
+        if dev is None or dev == torch.cuda.current_device():
+            return fn(*a, **k)
+        with torch.cuda.device(dev):
+            return fn(*a, **k)
+    return wrapper
+
+
+def _need(ok, what):
+    if not ok:
+        raise ValueError(what)
+
+
+@_timed
+@_on_their_device
+def group_routing(logits, K, bias=None, groups=1, top_groups=1, group_score=2, softmax=False, normalize=True, scale=1.0):
+    """Router logits [T,E] (f32, bf16) -> (scores f32 [T,K], expert indices i32 [T,K]); see `group_limited_routing`."""
+    _cuda(logits, bias)
+    _need(logits.ndim == 2 and logits.dtype in (torch.float32, torch.bfloat16), "group_routing: logits are f32 or bf16 [T,E]")
+    T, E = logits.shape
+    _need(bias is None or (bias.dtype == torch.float32 and tuple(bias.shape) == (E,)), f"group_routing: bias is f32 [{E}]")
+    scores = torch.empty(T, K, dtype=torch.float32, device=logits.device)
+    idx = torch.empty(T, K, dtype=_I32, device=logits.device)
+    check(lib.smoe_group_routing(_p(logits), int(logits.dtype == torch.bfloat16), _p(bias), T, E, K, groups, top_groups,
+                                 group_score, int(softmax), int(normalize), scale, _p(scores), _p(idx), _stream()),
+          "group_routing")
+    return scores, idx
+
+
+@_timed
+@_on_their_device
+def group_routing_bwd(logits, idx, dscores, softmax=False, normalize=True, scale=1.0):
+    """Gradient of the logits, in their type."""
+    _cuda(logits, idx, dscores)
+    T, E = logits.shape
+    _need(idx.dtype == _I32 and dscores.dtype == torch.float32 and idx.ndim == 2 and idx.shape[0] == T and idx.shape == dscores.shape,
+          "group_routing_bwd: idx i32 and dscores f32 [T,K]")
+    out = torch.empty_like(logits)
+    check(lib.smoe_group_routing_bwd(_p(logits), int(logits.dtype == torch.bfloat16), _p(idx), _p(dscores), T, E, idx.shape[1],
+                                     int(softmax), int(normalize), scale, _p(out), _stream()), "group_routing_bwd")
+    return out
+
+
+def _payload(shape, device):
+    """Uninitialised e4m3 bytes whose rows start on 16-byte boundaries."""
+    pitch = (shape[-1] + 15) // 16 * 16
+    q = torch.empty(*shape[:-1], pitch, dtype=_U8, device=device)
+    return q if pitch == shape[-1] else q[..., :shape[-1]]
+
+
+def _check_payload(q, what):
+    _need(q.element_size() == 1, f"{what}: the payload is e4m3")
+    pitch, expect = (q.shape[-1] + 15) // 16 * 16, 1
+    for n, s in zip(reversed(q.shape), reversed(q.stride())):
+        _need(n <= 1 or s == expect, f"{what}: payload rows are dense and {pitch} bytes apart")
+        expect = pitch if expect == 1 else expect * n
+
+
+def _blocks128(n):
+    return (n + 127) // 128
+
+
+def _need_bf16(x, dims, what):
+    _cuda(x)
+    _need(x.dtype == torch.bfloat16 and x.ndim == dims, f"{what}: a bf16 tensor of {dims} dimensions")
+
+
+def _need_segments(efo, counts, E, what):
+    _cuda(efo, counts)
+    _need(efo is None or (efo.dtype == _I32 and tuple(efo.shape) == (E + 1,)), f"{what}: efo is i32 [{E + 1}]")
+    _need(counts is None or (counts.dtype == _I32 and tuple(counts.shape) == (E,)), f"{what}: counts is i32 [{E}]")
+    _need(efo is not None or (E == 1 and counts is None), f"{what}: more than one expert, or counts, need efo")
+
+
+@_timed
+@_on_their_device
+def quant128_rows(x, swiglu=False, rows_list=None, n_live=None):
+    """bf16 [rows,K] -> (e4m3 bytes [rows,K], scales f32 [rows,K/128]).  `swiglu`: x is [rows,2K], gate and up interleaved, and
+    silu(gate) * up is quantised.  `rows_list` i32, `n_live` i32 (device): only the first n_live rows listed."""
+    _need_bf16(x, 2, "quant128_rows")
+    _cuda(rows_list, n_live)
+    rows, K = x.shape
+    if swiglu:
+        _need(K % 16 == 0, f"quant128_rows: {K} columns of gate and up are no multiple of 16")
+        K //= 2
+    _need(K > 0 and K % 8 == 0, f"quant128_rows: {K} columns are no multiple of 8")
+    _need((rows_list is None) == (n_live is None), "quant128_rows: rows_list and n_live go together")
+    _need(rows_list is None or (rows_list.dtype == _I32 and n_live.dtype == _I32), "quant128_rows: rows_list and n_live are i32")
+    q = _payload((rows, K), x.device)
+    s = torch.empty(rows, _blocks128(K), dtype=torch.float32, device=x.device)
+    check(lib.smoe_quant128_rows(_p(x), rows, K, int(swiglu), _p(rows_list), _p(n_live),
+                                 0 if rows_list is None else rows_list.numel(), _p(q), _p(s), _stream()), "quant128_rows")
+    return q, s
+
+
+@_timed
+@_on_their_device
+def quant128_rows_scatter(x, naept, s_rev, rows):
+    """bf16 [T,K], the routing metadata's token offsets and places -> (e4m3 bytes [rows,K], scales [rows,K/128]) in expert-sorted
+    order; rows without a token are left as they are."""
+    _need_bf16(x, 2, "quant128_rows_scatter")
+    _cuda(naept, s_rev)
+    T, K = x.shape
+    _need(K > 0 and K % 8 == 0, f"quant128_rows_scatter: {K} columns are no multiple of 8")
+    _need(naept.dtype == _I32 and naept.numel() == T + 1 and s_rev.dtype == _I32, "quant128_rows_scatter: naept i32 [T+1], s_rev i32")
+    q = _payload((rows, K), x.device)
+    s = torch.empty(rows, _blocks128(K), dtype=torch.float32, device=x.device)
+    check(lib.smoe_quant128_rows_scatter(_p(x), T, K, _p(naept), _p(s_rev), rows, _p(q), _p(s), _stream()),
+          "quant128_rows_scatter")
+    return q, s
+
+
+@_timed
+@_on_their_device
+def quant128_dual(x, efo=None, counts=None, with_rows=True):
+    """bf16 [rows,K] -> (row form e4m3 [rows,K], scales [rows,K/128]; both None without `with_rows`; column form e4m3 [rows,K], scales
+    [rows/128,K]) from one read."""
+    _need_bf16(x, 2, "quant128_dual")
+    rows, K = x.shape
+    _need(K > 0 and K % 8 == 0, f"quant128_dual: {K} columns are no multiple of 8")
+    E = 1 if efo is None else efo.numel() - 1
+    _need_segments(efo, counts, E, "quant128_dual")
+    f32 = lambda *shape: torch.empty(*shape, dtype=torch.float32, device=x.device)
+    q, s = (_payload((rows, K), x.device), f32(rows, _blocks128(K))) if with_rows else (None, None)
+    qc, sc = _payload((rows, K), x.device), f32(_blocks128(rows), K)
+    check(lib.smoe_quant128_dual(_p(x), rows, K, _p(efo), _p(counts), E, _p(q), _p(s), _p(qc), _p(sc), _stream()), "quant128_dual")
+    return q, s, qc, sc
+
+
+@_timed
+@_on_their_device
+def quant128_weight(w):
+    """bf16 [E,N,K] -> (e4m3 bytes [E,N,K], scales f32 [E,N/128,K/128])."""
+    _need_bf16(w, 3, "quant128_weight")
+    E, N, K = w.shape
+    _need(K > 0 and K % 8 == 0, f"quant128_weight: {K} columns are no multiple of 8")
+    q = _payload((E, N, K), w.device)
+    s = torch.empty(E, _blocks128(N), _blocks128(K), dtype=torch.float32, device=w.device)
+    check(lib.smoe_quant128_weight(_p(w), E, N, K, _p(q), _p(s), _stream()), "quant128_weight")
+    return q, s
+
+
+def _failure_words(device):
+    """Addresses of the status word and of its host mirror (which a capture must not be the first to allocate)."""
+    if _dev_index(device) not in _posted and torch.cuda.is_current_stream_capturing():
+        return status_word(device).data_ptr(), None
+    return status_pointers(device)
+
+
+def _product_args(a_q, a_s, b_q, b_s, efo, counts, E, N, K, b_blocks, what):
+    _cuda(a_s, b_s)
+    _check_payload(a_q, what)
+    _check_payload(b_q, what)
+    _need_segments(efo, counts, E, what)
+    _need(N % 8 == 0 and K % 8 == 0, f"{what}: sizes {N} x {K} are no multiples of 8")
+    _need(a_s.dtype == torch.float32 and tuple(a_s.shape) == (a_q.shape[0], _blocks128(K)),
+          f"{what}: the rows' scales are f32 [{a_q.shape[0]},{_blocks128(K)}]")
+    _need(b_s.dtype == torch.float32 and tuple(b_s.shape) == (E, *b_blocks), f"{what}: the weights' scales are f32 [{E},{b_blocks}]")
+
+
+@_timed
+@_on_their_device
+def gemm128_rows(a_q, a_s, b_q, b_s, efo=None, counts=None, b_mn=False, zero_rest=True):
+    """a e4m3 [rows,K] by rows, b e4m3 [E,N,K] by blocks (`b_mn`: [E,K,N], the reduction over its rows) -> bf16 [rows,N]; rows behind a
+    segment's live ones zero, or not written."""
+    _need(a_q.ndim == 2 and b_q.ndim == 3, "gemm128_rows: a [rows,K], b [E,N,K]")
+    rows, K = a_q.shape
+    E, N = b_q.shape[0], b_q.shape[2 if b_mn else 1]
+    _need(b_q.shape[1 if b_mn else 2] == K, f"gemm128_rows: reductions of {K} and {b_q.shape[1 if b_mn else 2]}")
+    nb, kb = _blocks128(N), _blocks128(K)
+    _product_args(a_q, a_s, b_q, b_s, efo, counts, E, N, K, (kb, nb) if b_mn else (nb, kb), "gemm128_rows")
+    c = torch.empty(rows, N, dtype=torch.bfloat16, device=a_q.device)
+    check(lib.smoe_gemm128_rows(_p(a_q), _p(a_s), _p(b_q), _p(b_s), _p(efo), _p(counts), _p(c), rows, N, K, E, int(b_mn),
+                                int(zero_rest), *_failure_words(a_q.device), _stream()), "gemm128_rows")
+    return c
+
+
+@_timed
+@_on_their_device
+def gemm128_few(a_q, a_s, b_q, b_s, efo=None, counts=None, live_rows=0):
+    """`gemm128_rows` made for few rows per expert; rows that are not live are not written.  `live_rows`: an upper bound of theirs, if
+    known."""
+    _need(a_q.ndim == 2 and b_q.ndim == 3, "gemm128_few: a [rows,K], b [E,N,K]")
+    rows, K = a_q.shape
+    E, N, Kb = b_q.shape
+    _need(Kb == K, f"gemm128_few: reductions of {K} and {Kb}")
+    _product_args(a_q, a_s, b_q, b_s, efo, counts, E, N, K, (_blocks128(N), _blocks128(K)), "gemm128_few")
+    c = torch.empty(rows, N, dtype=torch.bfloat16, device=a_q.device)
+    check(lib.smoe_gemm128_few(_p(a_q), _p(a_s), _p(b_q), _p(b_s), _p(efo), _p(counts), _p(c), rows, N, K, E, live_rows,
+                               *_failure_words(a_q.device), _stream()), "gemm128_few")
+    return c
+
+
+@_timed
+@_on_their_device
+def gemm128_wgrad(a_q, a_s, b_q, b_s, efo=None, counts=None, out=None, accumulate=False, E=1):
+    """a e4m3 [rows,M], b e4m3 [rows,N], both by columns -> bf16 [E,M,N], the products of each segment's live rows; or into `out` f32
+    [E,M,N], overwritten or added to."""
+    _cuda(a_s, b_s, out)
+    _need(a_q.ndim == 2 and b_q.ndim == 2 and a_q.shape[0] == b_q.shape[0], "gemm128_wgrad: a [rows,M], b [rows,N]")
+    _check_payload(a_q, "gemm128_wgrad")
+    _check_payload(b_q, "gemm128_wgrad")
+    (rows, M), N = a_q.shape, b_q.shape[1]
+    E = E if efo is None else efo.numel() - 1
+    _need_segments(efo, counts, E, "gemm128_wgrad")
+    rb = _blocks128(rows)
+    _need(M % 8 == 0 and N % 8 == 0, f"gemm128_wgrad: sizes {M} x {N} are no multiples of 8")
+    _need(a_s.dtype == b_s.dtype == torch.float32 and tuple(a_s.shape) == (rb, M) and tuple(b_s.shape) == (rb, N),
+          f"gemm128_wgrad: scales are f32 [{rb},{M}] and [{rb},{N}]")
+    _need(out is not None or not accumulate, "gemm128_wgrad: nothing to accumulate into")
+    if out is not None:
+        _need(out.dtype == torch.float32 and tuple(out.shape) == (E, M, N), f"gemm128_wgrad: out is f32 [{E},{M},{N}]")
+    c = out if out is not None else torch.empty(E, M, N, dtype=torch.bfloat16, device=a_q.device)
+    check(lib.smoe_gemm128_wgrad(_p(a_q), _p(a_s), _p(b_q), _p(b_s), _p(efo), _p(counts), _p(c), M, N, rows, E, int(out is None),
+                                 int(accumulate), *_failure_words(a_q.device), _stream()), "gemm128_wgrad")
+    return c

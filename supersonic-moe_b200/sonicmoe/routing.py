@@ -1,4 +1,5 @@
-"""Routers that produce (score, token, expert) pair lists for `moe_general_routing_inputs`.
+"""Routers beside the layer's own softmax top-k: `group_limited_routing` makes the [T,K] tables that `run_sonic_moe` and
+`block128_experts` take, `token_rounding_routing` (score, token, expert) pair lists for `moe_general_routing_inputs`.
 
 `token_rounding_routing` restates the token-rounding router of the reference's benchmark
 (benchmarks/moe-token-rounding.py:139-181): a token-choice top-K pass fixes each expert's load, the load is rounded
@@ -10,8 +11,60 @@ from __future__ import annotations
 
 import torch
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
+from . import ops
 from .count_cumsum import count_cumsum
+
+
+class _GroupLimitedRouting(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, K, bias, groups, top_groups, group_score, softmax, normalize, scale):
+        scores, idx = ops.group_routing(logits, K, bias, groups, top_groups, group_score, softmax, normalize, scale)
+        ctx.save_for_backward(logits, idx)
+        ctx.rule = (softmax, normalize, scale)
+        ctx.mark_non_differentiable(idx)
+        return scores, idx
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dscores, _didx):
+        logits, idx = ctx.saved_tensors
+        return (ops.group_routing_bwd(logits, idx, dscores.float().contiguous(), *ctx.rule),) + (None,) * 8
+
+
+def group_limited_routing(router_logits: torch.Tensor, K: int, *, score: str = "sigmoid", bias: torch.Tensor | None = None,
+                          groups: int = 1, top_groups: int | None = None, group_score: int = 2, normalize: bool = True,
+                          scale: float = 1.0):
+    """Router logits [T,E] (f32 or bf16) -> (scores f32 [T,K], expert indices i32 [T,K]), differentiable in the logits.
+
+    An expert's score is the sigmoid of its logit, or (`score="softmax"`) its softmax over all experts.  Experts are chosen by score +
+    `bias` (f32 [E], a constant that balances their load; it has no part in the scores returned).  With `groups` > 1 the experts
+    are that many runs of neighbours, a group ranks by the sum of its `group_score` (1 or 2) best experts, and only those of the
+    `top_groups` best groups are eligible.  The K best, in descending order, the first of equals first, get scale * score / sum of
+    the K scores (`normalize`) or scale * score.
+
+    A logit of -inf closes its expert; a row with fewer than K open experts ends in slots of index -1 and score 0 (the layer's
+    mark of a slot without an expert), so that a padded token is a row of -inf.  NaN ranks lowest.  The selection is that of 64-bit
+    arithmetic: it does not depend on how an exponential is rounded.  E <= 1024, K <= 32, groups <= 32."""
+    if score not in ("sigmoid", "softmax"):
+        raise ValueError(f"score={score!r}: 'sigmoid' or 'softmax'")
+    if router_logits.ndim != 2 or router_logits.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError(f"router logits are f32 or bf16 [T,E], got {router_logits.dtype} {tuple(router_logits.shape)}")
+    E = router_logits.shape[1]
+    top_groups = groups if top_groups is None else top_groups
+    if not (1 <= groups <= 32 and E % groups == 0 and 1 <= top_groups <= groups):
+        raise ValueError(f"groups={groups}, top_groups={top_groups}: at most 32 groups that divide {E} experts evenly")
+    if not (1 <= E <= 1024 and 1 <= K <= min(32, top_groups * (E // groups))):
+        raise ValueError(f"K={K}: 1 to 32, at most the {top_groups * (E // groups)} experts of the groups chosen (E={E}, at most 1024)")
+    if group_score not in (1, 2):
+        raise ValueError(f"group_score={group_score}: 1 or 2")
+    if bias is not None:
+        if bias.shape != (E,):
+            raise ValueError(f"bias {tuple(bias.shape)}: one value for each of {E} experts")
+        bias = bias.detach().float().contiguous()
+    return _GroupLimitedRouting.apply(router_logits.contiguous(), K, bias, groups, top_groups, group_score, score == "softmax",
+                                      normalize, float(scale))
 
 
 def token_rounding_routing(router_logits: torch.Tensor, K: int, Mtile: int = 128, routing: str = "nr"):
