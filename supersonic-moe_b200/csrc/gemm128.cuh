@@ -98,11 +98,6 @@ __device__ __forceinline__ void tmem_arrived(uint32_t (&r)[16]) {
   asm volatile("" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
                "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]));
 }
-__device__ __forceinline__ F2 f2_bits(uint32_t lo, uint32_t hi) {
-  F2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "r"(lo), "r"(hi));
-  return r;
-}
 
 // Segments from efo / counts, any values taken as they fit: 0 <= start <= end <= rows, start <= live end <= end
 struct Segs128 {
@@ -332,9 +327,9 @@ gemm128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
       const Tile128 t = tile128<MODE>(tile, rank, p, segs);
       const int row = t.m0 + q * 32 + lane;               // of c (WGRAD128: of the expert's)
       const int col0 = t.n0 + half * 128;
-      F2 acc[64];
+      float acc[128];
 #pragma unroll
-      for (int i = 0; i < 64; ++i) acc[i] = f2(0.f, 0.f);
+      for (int i = 0; i < 128; ++i) acc[i] = 0.f;
       // scales: one number a lane for its row, one for the 128 columns (ROWS128) or one a column (WGRAD128)
       const float* sa = p.a_s;
       const float* sb = p.b_s;
@@ -380,7 +375,6 @@ gemm128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
         tc_fence_after();
         const uint32_t src = tmem_base + ((uint32_t)(q * 32) << 16) + as * 256 + half * 128;
         const float f = MODE == WGRAD128 ? sa_now : sa_now * sb_now;
-        const F2 f_2 = f2(f, f);
         uint32_t r[2][16];
         tmem_ld16(src, r[0]);
 #pragma unroll
@@ -396,13 +390,17 @@ gemm128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
           }
           const uint32_t(&v)[16] = r[c & 1];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            F2 x = f2_bits(v[2 * i], v[2 * i + 1]);
+          for (int i = 0; i < 16; i += 4) {
             if (MODE == WGRAD128) {
-              const float2 s2 = *reinterpret_cast<const float2*>(sbk + c * 16 + 2 * i);
-              x = x * f2(s2.x, s2.y);
+              const float4 s4 = *reinterpret_cast<const float4*>(sbk + c * 16 + i);
+              const float x[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                acc[c * 16 + i + j] = fmaf(__uint_as_float(v[i + j]) * x[j], f, acc[c * 16 + i + j]);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) acc[c * 16 + i + j] = fmaf(__uint_as_float(v[i + j]), f, acc[c * 16 + i + j]);
             }
-            acc[c * 8 + i] = f2_fma(x, f_2, acc[c * 8 + i]);
           }
         }
         if (++as == 2) { as = 0; aphase ^= 1; }
@@ -417,8 +415,7 @@ gemm128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
           uint32_t w[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const float2 v = f2_get(acc[cc * 16 + i]);
-            w[i] = row_in ? pack_bf16x2(v.x, v.y) : 0u;
+            w[i] = row_in ? pack_bf16x2(acc[cc * 32 + 2 * i], acc[cc * 32 + 2 * i + 1]) : 0u;
           }
           store_slab128(stg, lane, w, [&](int r, int j, const uint4& v) {
             const int gr = t.m0 + q * 32 + r, gc = col0 + cc * 32 + j * 8;
@@ -431,11 +428,7 @@ gemm128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
         for (int cc = 0; cc < 8; ++cc) {
           uint32_t w[16];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float2 v = f2_get(acc[cc * 8 + i]);
-            w[2 * i] = __float_as_uint(v.x);
-            w[2 * i + 1] = __float_as_uint(v.y);
-          }
+          for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(acc[cc * 16 + i]);
           store_slab128(stg, lane, w, [&](int r, int j, const uint4& v) {
             const int gr = t.m0 + q * 32 + r, gc = col0 + cc * 16 + j * 4;
             if (gr < t.end && gc < p.N) {
