@@ -524,6 +524,28 @@ int smoe_gemm128_wgrad(const void* a_fp8, const float* a_scales, const void* b_f
                        const int32_t* counts, void* c, int64_t M, int64_t N, int64_t rows, int64_t E, int out_bf16, int accumulate,
                        int32_t* status, int32_t* pinned_host_word, void* stream);
 
+/* y = x W^T by segments from bf16 operands, in one call: x is quantised by rows into `scratch` (and by columns into `saved`, with
+ * SMOE_B128_DW), w [E,N,K] is e4m3 with scales, or bf16 with SMOE_B128_QUANT_W and then left quantised in `saved`.  The second call
+ * turns dy into dx [rows,K] (SMOE_B128_DX) and dw [E,N,K] (SMOE_B128_DW; bf16, or added to f32) with what the first one saved: its
+ * flags are the first call's plus those of the gradients wanted.  Arenas: smoe_block128_bytes(..., which) bytes, 256-byte aligned;
+ * which = 0 saved, 1 forward scratch, 2 backward scratch; -1 for sizes that are not taken. */
+enum { SMOE_B128_QUANT_W = 1, SMOE_B128_DW = 2, SMOE_B128_DX = 4 };
+int64_t smoe_block128_bytes(int64_t rows, int64_t N, int64_t K, int64_t E, int flags, int which);
+int smoe_block128_linear(const void* x_bf16, const void* w, const float* w_scales, const int32_t* efo, const int32_t* counts,
+                         void* y_bf16, void* saved, void* scratch, int64_t rows, int64_t N, int64_t K, int64_t E, int flags,
+                         int32_t* status, int32_t* pinned_host_word, void* stream);
+int smoe_block128_linear_bwd(const void* dy_bf16, const void* w_fp8, const float* w_scales, const int32_t* efo,
+                             const int32_t* counts, const void* saved, void* scratch, void* dx_bf16, void* dw, int64_t rows,
+                             int64_t N, int64_t K, int64_t E, int flags, int dw_f32_accumulate, int32_t* status,
+                             int32_t* pinned_host_word, void* stream);
+/* SwiGLU experts on routed tokens, inference, in one call: out[t,:] = sum_k scores[t,k] W2[e] (silu(gate) * up) with gate / up
+ * interleaved in W1[e] x[t], e = idx[t,k] (valid iff 0 <= e < E, a token's distinct).  w1 [E,2I,H], w2 [E,H,I] with their scales.
+ * scratch: smoe_block128_experts_bytes bytes, 256-byte aligned (-1 for sizes that are not taken; K <= 16). */
+int64_t smoe_block128_experts_bytes(int64_t T, int64_t H, int64_t I, int64_t E, int64_t K);
+int smoe_block128_experts(const void* x_bf16, const int32_t* idx, const float* scores, const void* w1_fp8, const float* w1_scales,
+                          const void* w2_fp8, const float* w2_scales, void* out_bf16, void* scratch, int64_t T, int64_t H,
+                          int64_t I, int64_t E, int64_t K, int32_t* status, int32_t* pinned_host_word, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

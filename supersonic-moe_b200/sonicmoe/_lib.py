@@ -96,6 +96,11 @@ SIGNATURES = {
     "smoe_gemm128_rows": (_I, [_P] * 7 + [_L] * 4 + [_I, _I, _P, _P, _P]),
     "smoe_gemm128_few": (_I, [_P] * 7 + [_L] * 5 + [_P, _P, _P]),
     "smoe_gemm128_wgrad": (_I, [_P] * 7 + [_L] * 4 + [_I, _I, _P, _P, _P]),
+    "smoe_block128_bytes": (_L, [_L] * 4 + [_I, _I]),
+    "smoe_block128_linear": (_I, [_P] * 8 + [_L] * 4 + [_I, _P, _P, _P]),
+    "smoe_block128_linear_bwd": (_I, [_P] * 9 + [_L] * 4 + [_I, _I, _P, _P, _P]),
+    "smoe_block128_experts_bytes": (_L, [_L] * 5),
+    "smoe_block128_experts": (_I, [_P] * 9 + [_L] * 5 + [_P, _P, _P]),
 }
 
 # exported for the library's own tests only (csrc/smoe_internal.h); not product ABI

@@ -780,233 +780,337 @@ def switch_loss_bwd(logits, grad, dloss):
 
 
 # ---------------------------------------------------------------- group-limited routing, products with a scale per block of 128
-def _on_their_device(fn):
-    """Launch where the tensors are: they have to be on one GPU, which need not be the current one."""
+_current = torch._C._cuda_getDevice
+
+
+def _on_its_device(fn):
+    """Launch on the GPU of the first argument, which need not be the current one."""
     import functools
 
     @functools.wraps(fn)
-    def wrapper(*a, **k):
-        dev = None
-        for t in (*a, *k.values()):
-            if isinstance(t, torch.Tensor):
-                if not t.is_cuda:
-                    raise RuntimeError("sonicmoe kernels need CUDA tensors (no CPU fallback)")
-                if dev is None:
-                    dev = t.device.index
-                elif t.device.index != dev:
-                    raise RuntimeError(f"{fn.__name__}: tensors on cuda:{dev} and cuda:{t.device.index}")
-        if dev is None or dev == torch.cuda.current_device():
-            return fn(*a, **k)
-        with torch.cuda.device(dev):
-            return fn(*a, **k)
+    def wrapper(x, *a, **k):
+        d = x.get_device()
+        if d < 0:
+            raise RuntimeError("sonicmoe kernels need CUDA tensors (no CPU fallback)")
+        if d == _current():
+            return fn(x, *a, **k)
+        with torch.cuda.device(d):
+            return fn(x, *a, **k)
     return wrapper
 
 
-def _need(ok, what):
-    if not ok:
-        raise ValueError(what)
+def _check_same_gpu(what, *ts):
+    d = ts[0].get_device()
+    for t in ts:
+        if t is not None and t.get_device() != d:
+            raise RuntimeError(f"{what}: tensors on different devices ({ts[0].device} and {t.device})")
+
+
+def _check_dense(what, *ts):
+    """On one GPU and contiguous."""
+    d = ts[0].get_device()
+    for t in ts:
+        if t is not None and (t.get_device() != d or not t.is_contiguous()):
+            _check_same_gpu(what, *ts)
+            raise RuntimeError("sonicmoe kernels need contiguous tensors")
 
 
 @_timed
-@_on_their_device
+@_on_its_device
 def group_routing(logits, K, bias=None, groups=1, top_groups=1, group_score=2, softmax=False, normalize=True, scale=1.0):
     """Router logits [T,E] (f32, bf16) -> (scores f32 [T,K], expert indices i32 [T,K]); see `group_limited_routing`."""
-    _cuda(logits, bias)
-    _need(logits.ndim == 2 and logits.dtype in (torch.float32, torch.bfloat16), "group_routing: logits are f32 or bf16 [T,E]")
+    _check_dense("group_routing", logits, bias)
+    bf16 = logits.dtype == torch.bfloat16
+    if logits.ndim != 2 or not (bf16 or logits.dtype == torch.float32):
+        raise ValueError(f"group_routing: logits are f32 or bf16 [T,E], got {logits.dtype} {tuple(logits.shape)}")
     T, E = logits.shape
-    _need(bias is None or (bias.dtype == torch.float32 and tuple(bias.shape) == (E,)), f"group_routing: bias is f32 [{E}]")
-    scores = torch.empty(T, K, dtype=torch.float32, device=logits.device)
-    idx = torch.empty(T, K, dtype=_I32, device=logits.device)
-    check(lib.smoe_group_routing(_p(logits), int(logits.dtype == torch.bfloat16), _p(bias), T, E, K, groups, top_groups,
-                                 group_score, int(softmax), int(normalize), scale, _p(scores), _p(idx), _stream()),
+    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (E,)):
+        raise ValueError(f"group_routing: bias is f32 [{E}], got {bias.dtype} {tuple(bias.shape)}")
+    scores, idx = logits.new_empty((T, K), dtype=torch.float32), logits.new_empty((T, K), dtype=_I32)
+    check(lib.smoe_group_routing(logits.data_ptr(), bf16, None if bias is None else bias.data_ptr(), T, E, K, groups, top_groups,
+                                 group_score, softmax, normalize, scale, scores.data_ptr(), idx.data_ptr(), _stream()),
           "group_routing")
     return scores, idx
 
 
 @_timed
-@_on_their_device
+@_on_its_device
 def group_routing_bwd(logits, idx, dscores, softmax=False, normalize=True, scale=1.0):
     """Gradient of the logits, in their type."""
-    _cuda(logits, idx, dscores)
+    _check_dense("group_routing_bwd", logits, idx, dscores)
     T, E = logits.shape
-    _need(idx.dtype == _I32 and dscores.dtype == torch.float32 and idx.ndim == 2 and idx.shape[0] == T and idx.shape == dscores.shape,
-          "group_routing_bwd: idx i32 and dscores f32 [T,K]")
+    bf16 = logits.dtype == torch.bfloat16
+    if not (bf16 or logits.dtype == torch.float32):
+        raise ValueError(f"group_routing_bwd: logits are f32 or bf16 [T,E], got {logits.dtype}")
+    if idx.dtype != _I32 or dscores.dtype != torch.float32 or idx.ndim != 2 or idx.shape[0] != T or idx.shape != dscores.shape:
+        raise ValueError("group_routing_bwd: idx i32 and dscores f32 [T,K]")
     out = torch.empty_like(logits)
-    check(lib.smoe_group_routing_bwd(_p(logits), int(logits.dtype == torch.bfloat16), _p(idx), _p(dscores), T, E, idx.shape[1],
-                                     int(softmax), int(normalize), scale, _p(out), _stream()), "group_routing_bwd")
+    check(lib.smoe_group_routing_bwd(logits.data_ptr(), bf16, idx.data_ptr(), dscores.data_ptr(), T, E, idx.shape[1], softmax,
+                                     normalize, scale, out.data_ptr(), _stream()), "group_routing_bwd")
     return out
-
-
-def _payload(shape, device):
-    """Uninitialised e4m3 bytes whose rows start on 16-byte boundaries."""
-    pitch = (shape[-1] + 15) // 16 * 16
-    q = torch.empty(*shape[:-1], pitch, dtype=_U8, device=device)
-    return q if pitch == shape[-1] else q[..., :shape[-1]]
-
-
-def _check_payload(q, what):
-    _need(q.element_size() == 1, f"{what}: the payload is e4m3")
-    pitch, expect = (q.shape[-1] + 15) // 16 * 16, 1
-    for n, s in zip(reversed(q.shape), reversed(q.stride())):
-        _need(n <= 1 or s == expect, f"{what}: payload rows are dense and {pitch} bytes apart")
-        expect = pitch if expect == 1 else expect * n
 
 
 def _blocks128(n):
     return (n + 127) // 128
 
 
-def _need_bf16(x, dims, what):
-    _cuda(x)
-    _need(x.dtype == torch.bfloat16 and x.ndim == dims, f"{what}: a bf16 tensor of {dims} dimensions")
+def _payload(like, *shape):
+    """Uninitialised e4m3 bytes whose rows start on 16-byte boundaries."""
+    K = shape[-1]
+    if K % 16 == 0:
+        return like.new_empty(shape, dtype=_U8)
+    return like.new_empty((*shape[:-1], (K + 15) // 16 * 16), dtype=_U8)[..., :K]
 
 
-def _need_segments(efo, counts, E, what):
-    _cuda(efo, counts)
-    _need(efo is None or (efo.dtype == _I32 and tuple(efo.shape) == (E + 1,)), f"{what}: efo is i32 [{E + 1}]")
-    _need(counts is None or (counts.dtype == _I32 and tuple(counts.shape) == (E,)), f"{what}: counts is i32 [{E}]")
-    _need(efo is not None or (E == 1 and counts is None), f"{what}: more than one expert, or counts, need efo")
+def check_payload(q, what):
+    """e4m3 rows as the quantisers leave them: dense, each on a 16-byte boundary."""
+    if q.element_size() != 1:
+        raise ValueError(f"{what}: the payload is e4m3, got {q.dtype}")
+    if q.shape[-1] % 16 == 0 and q.is_contiguous():
+        return
+    expect = 1
+    for n, stride in zip(reversed(q.shape), reversed(q.stride())):
+        if n > 1 and stride != expect:
+            raise ValueError(f"{what}: payload rows are dense and {(q.shape[-1] + 15) // 16 * 16} bytes apart, got strides {q.stride()}")
+        expect = (q.shape[-1] + 15) // 16 * 16 if expect == 1 else expect * n
+
+
+def _check_bf16(x, dims, K, what):
+    if x.dtype != torch.bfloat16 or x.ndim != dims:
+        raise ValueError(f"{what}: a bf16 tensor of {dims} dimensions, got {x.dtype} {tuple(x.shape)}")
+    if K <= 0 or K % 8:
+        raise ValueError(f"{what}: {K} columns are no multiple of 8")
+
+
+def check_segments(efo, counts, E, what):
+    """efo i32 [E+1] and counts i32 [E], where there are several experts."""
+    if efo is None:
+        if E != 1 or counts is not None:
+            raise ValueError(f"{what}: several experts, or counts, need efo")
+        return
+    if efo.dtype != _I32 or efo.shape != (E + 1,) or not efo.is_contiguous():
+        raise ValueError(f"{what}: efo is i32 [{E + 1}], got {efo.dtype} {tuple(efo.shape)}")
+    if counts is not None and (counts.dtype != _I32 or counts.shape != (E,) or not counts.is_contiguous()):
+        raise ValueError(f"{what}: counts is i32 [{E}], got {counts.dtype} {tuple(counts.shape)}")
 
 
 @_timed
-@_on_their_device
+@_on_its_device
 def quant128_rows(x, swiglu=False, rows_list=None, n_live=None):
     """bf16 [rows,K] -> (e4m3 bytes [rows,K], scales f32 [rows,K/128]).  `swiglu`: x is [rows,2K], gate and up interleaved, and
     silu(gate) * up is quantised.  `rows_list` i32, `n_live` i32 (device): only the first n_live rows listed."""
-    _need_bf16(x, 2, "quant128_rows")
-    _cuda(rows_list, n_live)
-    rows, K = x.shape
+    _check_dense("quant128_rows", x, rows_list, n_live)
+    K = x.shape[-1] if x.ndim else 0
     if swiglu:
-        _need(K % 16 == 0, f"quant128_rows: {K} columns of gate and up are no multiple of 16")
+        if K % 2:
+            raise ValueError(f"quant128_rows: {K} columns are no pairs of gate and up")
         K //= 2
-    _need(K > 0 and K % 8 == 0, f"quant128_rows: {K} columns are no multiple of 8")
-    _need((rows_list is None) == (n_live is None), "quant128_rows: rows_list and n_live go together")
-    _need(rows_list is None or (rows_list.dtype == _I32 and n_live.dtype == _I32), "quant128_rows: rows_list and n_live are i32")
-    q = _payload((rows, K), x.device)
-    s = torch.empty(rows, _blocks128(K), dtype=torch.float32, device=x.device)
-    check(lib.smoe_quant128_rows(_p(x), rows, K, int(swiglu), _p(rows_list), _p(n_live),
-                                 0 if rows_list is None else rows_list.numel(), _p(q), _p(s), _stream()), "quant128_rows")
+    _check_bf16(x, 2, K, "quant128_rows")
+    rows = x.shape[0]
+    if (rows_list is None) != (n_live is None) or (rows_list is not None and not rows_list.dtype == n_live.dtype == _I32):
+        raise ValueError("quant128_rows: rows_list and n_live go together, both i32")
+    q, s = _payload(x, rows, K), x.new_empty((rows, _blocks128(K)), dtype=torch.float32)
+    check(lib.smoe_quant128_rows(x.data_ptr(), rows, K, swiglu, _p(rows_list), _p(n_live),
+                                 0 if rows_list is None else rows_list.numel(), q.data_ptr(), s.data_ptr(), _stream()),
+          "quant128_rows")
     return q, s
 
 
 @_timed
-@_on_their_device
+@_on_its_device
 def quant128_rows_scatter(x, naept, s_rev, rows):
     """bf16 [T,K], the routing metadata's token offsets and places -> (e4m3 bytes [rows,K], scales [rows,K/128]) in expert-sorted
     order; rows without a token are left as they are."""
-    _need_bf16(x, 2, "quant128_rows_scatter")
-    _cuda(naept, s_rev)
+    _check_dense("quant128_rows_scatter", x, naept, s_rev)
+    _check_bf16(x, 2, x.shape[-1] if x.ndim else 0, "quant128_rows_scatter")
     T, K = x.shape
-    _need(K > 0 and K % 8 == 0, f"quant128_rows_scatter: {K} columns are no multiple of 8")
-    _need(naept.dtype == _I32 and naept.numel() == T + 1 and s_rev.dtype == _I32, "quant128_rows_scatter: naept i32 [T+1], s_rev i32")
-    q = _payload((rows, K), x.device)
-    s = torch.empty(rows, _blocks128(K), dtype=torch.float32, device=x.device)
-    check(lib.smoe_quant128_rows_scatter(_p(x), T, K, _p(naept), _p(s_rev), rows, _p(q), _p(s), _stream()),
-          "quant128_rows_scatter")
+    if naept.dtype != _I32 or naept.numel() != T + 1 or s_rev.dtype != _I32:
+        raise ValueError("quant128_rows_scatter: naept i32 [T+1], s_rev i32")
+    q, s = _payload(x, rows, K), x.new_empty((rows, _blocks128(K)), dtype=torch.float32)
+    check(lib.smoe_quant128_rows_scatter(x.data_ptr(), T, K, naept.data_ptr(), s_rev.data_ptr(), rows, q.data_ptr(), s.data_ptr(),
+                                         _stream()), "quant128_rows_scatter")
     return q, s
 
 
 @_timed
-@_on_their_device
+@_on_its_device
 def quant128_dual(x, efo=None, counts=None, with_rows=True):
     """bf16 [rows,K] -> (row form e4m3 [rows,K], scales [rows,K/128]; both None without `with_rows`; column form e4m3 [rows,K], scales
     [rows/128,K]) from one read."""
-    _need_bf16(x, 2, "quant128_dual")
+    _check_dense("quant128_dual", x, efo, counts)
+    _check_bf16(x, 2, x.shape[-1] if x.ndim else 0, "quant128_dual")
     rows, K = x.shape
-    _need(K > 0 and K % 8 == 0, f"quant128_dual: {K} columns are no multiple of 8")
     E = 1 if efo is None else efo.numel() - 1
-    _need_segments(efo, counts, E, "quant128_dual")
-    f32 = lambda *shape: torch.empty(*shape, dtype=torch.float32, device=x.device)
-    q, s = (_payload((rows, K), x.device), f32(rows, _blocks128(K))) if with_rows else (None, None)
-    qc, sc = _payload((rows, K), x.device), f32(_blocks128(rows), K)
-    check(lib.smoe_quant128_dual(_p(x), rows, K, _p(efo), _p(counts), E, _p(q), _p(s), _p(qc), _p(sc), _stream()), "quant128_dual")
+    check_segments(efo, counts, E, "quant128_dual")
+    q, s = (_payload(x, rows, K), x.new_empty((rows, _blocks128(K)), dtype=torch.float32)) if with_rows else (None, None)
+    qc, sc = _payload(x, rows, K), x.new_empty((_blocks128(rows), K), dtype=torch.float32)
+    check(lib.smoe_quant128_dual(x.data_ptr(), rows, K, _p(efo), _p(counts), E, _p(q), _p(s), qc.data_ptr(), sc.data_ptr(),
+                                 _stream()), "quant128_dual")
     return q, s, qc, sc
 
 
 @_timed
-@_on_their_device
+@_on_its_device
 def quant128_weight(w):
     """bf16 [E,N,K] -> (e4m3 bytes [E,N,K], scales f32 [E,N/128,K/128])."""
-    _need_bf16(w, 3, "quant128_weight")
+    _check_dense("quant128_weight", w)
+    _check_bf16(w, 3, w.shape[-1] if w.ndim else 0, "quant128_weight")
     E, N, K = w.shape
-    _need(K > 0 and K % 8 == 0, f"quant128_weight: {K} columns are no multiple of 8")
-    q = _payload((E, N, K), w.device)
-    s = torch.empty(E, _blocks128(N), _blocks128(K), dtype=torch.float32, device=w.device)
-    check(lib.smoe_quant128_weight(_p(w), E, N, K, _p(q), _p(s), _stream()), "quant128_weight")
+    q, s = _payload(w, E, N, K), w.new_empty((E, _blocks128(N), _blocks128(K)), dtype=torch.float32)
+    check(lib.smoe_quant128_weight(w.data_ptr(), E, N, K, q.data_ptr(), s.data_ptr(), _stream()), "quant128_weight")
     return q, s
 
 
-def _failure_words(device):
+def failure_words(device):
     """Addresses of the status word and of its host mirror (which a capture must not be the first to allocate)."""
     if _dev_index(device) not in _posted and torch.cuda.is_current_stream_capturing():
         return status_word(device).data_ptr(), None
     return status_pointers(device)
 
 
-def _product_args(a_q, a_s, b_q, b_s, efo, counts, E, N, K, b_blocks, what):
-    _cuda(a_s, b_s)
-    _check_payload(a_q, what)
-    _check_payload(b_q, what)
-    _need_segments(efo, counts, E, what)
-    _need(N % 8 == 0 and K % 8 == 0, f"{what}: sizes {N} x {K} are no multiples of 8")
-    _need(a_s.dtype == torch.float32 and tuple(a_s.shape) == (a_q.shape[0], _blocks128(K)),
-          f"{what}: the rows' scales are f32 [{a_q.shape[0]},{_blocks128(K)}]")
-    _need(b_s.dtype == torch.float32 and tuple(b_s.shape) == (E, *b_blocks), f"{what}: the weights' scales are f32 [{E},{b_blocks}]")
+def _check_product(a_q, a_s, b_q, b_s, efo, counts, E, N, K, b_blocks, what):
+    _check_same_gpu(what, a_q, a_s, b_q, b_s, efo, counts)
+    check_payload(a_q, what)
+    check_payload(b_q, what)
+    check_segments(efo, counts, E, what)
+    if N % 8 or K % 8:
+        raise ValueError(f"{what}: sizes {N} x {K} are no multiples of 8")
+    if a_s.dtype != torch.float32 or a_s.shape != (a_q.shape[0], _blocks128(K)) or not a_s.is_contiguous():
+        raise ValueError(f"{what}: the rows' scales are f32 [{a_q.shape[0]},{_blocks128(K)}], got {a_s.dtype} {tuple(a_s.shape)}")
+    if b_s.dtype != torch.float32 or b_s.shape != (E, *b_blocks) or not b_s.is_contiguous():
+        raise ValueError(f"{what}: the weights' scales are f32 {(E, *b_blocks)}, got {b_s.dtype} {tuple(b_s.shape)}")
 
 
 @_timed
-@_on_their_device
+@_on_its_device
 def gemm128_rows(a_q, a_s, b_q, b_s, efo=None, counts=None, b_mn=False, zero_rest=True):
     """a e4m3 [rows,K] by rows, b e4m3 [E,N,K] by blocks (`b_mn`: [E,K,N], the reduction over its rows) -> bf16 [rows,N]; rows behind a
     segment's live ones zero, or not written."""
-    _need(a_q.ndim == 2 and b_q.ndim == 3, "gemm128_rows: a [rows,K], b [E,N,K]")
+    if a_q.ndim != 2 or b_q.ndim != 3 or b_q.shape[1 if b_mn else 2] != a_q.shape[1]:
+        raise ValueError(f"gemm128_rows: a [rows,K] against b {'[E,K,N]' if b_mn else '[E,N,K]'}, got {tuple(a_q.shape)}, {tuple(b_q.shape)}")
     rows, K = a_q.shape
     E, N = b_q.shape[0], b_q.shape[2 if b_mn else 1]
-    _need(b_q.shape[1 if b_mn else 2] == K, f"gemm128_rows: reductions of {K} and {b_q.shape[1 if b_mn else 2]}")
     nb, kb = _blocks128(N), _blocks128(K)
-    _product_args(a_q, a_s, b_q, b_s, efo, counts, E, N, K, (kb, nb) if b_mn else (nb, kb), "gemm128_rows")
-    c = torch.empty(rows, N, dtype=torch.bfloat16, device=a_q.device)
-    check(lib.smoe_gemm128_rows(_p(a_q), _p(a_s), _p(b_q), _p(b_s), _p(efo), _p(counts), _p(c), rows, N, K, E, int(b_mn),
-                                int(zero_rest), *_failure_words(a_q.device), _stream()), "gemm128_rows")
+    _check_product(a_q, a_s, b_q, b_s, efo, counts, E, N, K, (kb, nb) if b_mn else (nb, kb), "gemm128_rows")
+    c = a_s.new_empty((rows, N), dtype=torch.bfloat16)
+    check(lib.smoe_gemm128_rows(a_q.data_ptr(), a_s.data_ptr(), b_q.data_ptr(), b_s.data_ptr(), _p(efo), _p(counts), c.data_ptr(),
+                                rows, N, K, E, b_mn, zero_rest, *failure_words(a_q.device), _stream()), "gemm128_rows")
     return c
 
 
 @_timed
-@_on_their_device
+@_on_its_device
 def gemm128_few(a_q, a_s, b_q, b_s, efo=None, counts=None, live_rows=0):
     """`gemm128_rows` made for few rows per expert; rows that are not live are not written.  `live_rows`: an upper bound of theirs, if
     known."""
-    _need(a_q.ndim == 2 and b_q.ndim == 3, "gemm128_few: a [rows,K], b [E,N,K]")
+    if a_q.ndim != 2 or b_q.ndim != 3 or b_q.shape[2] != a_q.shape[1]:
+        raise ValueError(f"gemm128_few: a [rows,K] against b [E,N,K], got {tuple(a_q.shape)}, {tuple(b_q.shape)}")
     rows, K = a_q.shape
-    E, N, Kb = b_q.shape
-    _need(Kb == K, f"gemm128_few: reductions of {K} and {Kb}")
-    _product_args(a_q, a_s, b_q, b_s, efo, counts, E, N, K, (_blocks128(N), _blocks128(K)), "gemm128_few")
-    c = torch.empty(rows, N, dtype=torch.bfloat16, device=a_q.device)
-    check(lib.smoe_gemm128_few(_p(a_q), _p(a_s), _p(b_q), _p(b_s), _p(efo), _p(counts), _p(c), rows, N, K, E, live_rows,
-                               *_failure_words(a_q.device), _stream()), "gemm128_few")
+    E, N = b_q.shape[:2]
+    _check_product(a_q, a_s, b_q, b_s, efo, counts, E, N, K, (_blocks128(N), _blocks128(K)), "gemm128_few")
+    c = a_s.new_empty((rows, N), dtype=torch.bfloat16)
+    check(lib.smoe_gemm128_few(a_q.data_ptr(), a_s.data_ptr(), b_q.data_ptr(), b_s.data_ptr(), _p(efo), _p(counts), c.data_ptr(),
+                               rows, N, K, E, live_rows, *failure_words(a_q.device), _stream()), "gemm128_few")
     return c
 
 
 @_timed
-@_on_their_device
-def gemm128_wgrad(a_q, a_s, b_q, b_s, efo=None, counts=None, out=None, accumulate=False, E=1):
+@_on_its_device
+def gemm128_wgrad(a_q, a_s, b_q, b_s, efo=None, counts=None, out=None, accumulate=False):
     """a e4m3 [rows,M], b e4m3 [rows,N], both by columns -> bf16 [E,M,N], the products of each segment's live rows; or into `out` f32
     [E,M,N], overwritten or added to."""
-    _cuda(a_s, b_s, out)
-    _need(a_q.ndim == 2 and b_q.ndim == 2 and a_q.shape[0] == b_q.shape[0], "gemm128_wgrad: a [rows,M], b [rows,N]")
-    _check_payload(a_q, "gemm128_wgrad")
-    _check_payload(b_q, "gemm128_wgrad")
+    if a_q.ndim != 2 or b_q.ndim != 2 or a_q.shape[0] != b_q.shape[0]:
+        raise ValueError(f"gemm128_wgrad: a [rows,M] against b [rows,N], got {tuple(a_q.shape)}, {tuple(b_q.shape)}")
+    _check_same_gpu("gemm128_wgrad", a_q, a_s, b_q, b_s, efo, counts, out)
+    check_payload(a_q, "gemm128_wgrad")
+    check_payload(b_q, "gemm128_wgrad")
     (rows, M), N = a_q.shape, b_q.shape[1]
-    E = E if efo is None else efo.numel() - 1
-    _need_segments(efo, counts, E, "gemm128_wgrad")
+    E = 1 if efo is None else efo.numel() - 1
+    check_segments(efo, counts, E, "gemm128_wgrad")
     rb = _blocks128(rows)
-    _need(M % 8 == 0 and N % 8 == 0, f"gemm128_wgrad: sizes {M} x {N} are no multiples of 8")
-    _need(a_s.dtype == b_s.dtype == torch.float32 and tuple(a_s.shape) == (rb, M) and tuple(b_s.shape) == (rb, N),
-          f"gemm128_wgrad: scales are f32 [{rb},{M}] and [{rb},{N}]")
-    _need(out is not None or not accumulate, "gemm128_wgrad: nothing to accumulate into")
-    if out is not None:
-        _need(out.dtype == torch.float32 and tuple(out.shape) == (E, M, N), f"gemm128_wgrad: out is f32 [{E},{M},{N}]")
-    c = out if out is not None else torch.empty(E, M, N, dtype=torch.bfloat16, device=a_q.device)
-    check(lib.smoe_gemm128_wgrad(_p(a_q), _p(a_s), _p(b_q), _p(b_s), _p(efo), _p(counts), _p(c), M, N, rows, E, int(out is None),
-                                 int(accumulate), *_failure_words(a_q.device), _stream()), "gemm128_wgrad")
+    if M % 8 or N % 8:
+        raise ValueError(f"gemm128_wgrad: sizes {M} x {N} are no multiples of 8")
+    for s, n in ((a_s, M), (b_s, N)):
+        if s.dtype != torch.float32 or s.shape != (rb, n) or not s.is_contiguous():
+            raise ValueError(f"gemm128_wgrad: scales are f32 [{rb},{n}], got {s.dtype} {tuple(s.shape)}")
+    if out is None:
+        if accumulate:
+            raise ValueError("gemm128_wgrad: nothing to accumulate into")
+        c = a_s.new_empty((E, M, N), dtype=torch.bfloat16)
+    else:
+        c = out
+        if out.dtype != torch.float32 or out.shape != (E, M, N) or not out.is_contiguous():
+            raise ValueError(f"gemm128_wgrad: out is f32 [{E},{M},{N}], got {out.dtype} {tuple(out.shape)}")
+    check(lib.smoe_gemm128_wgrad(a_q.data_ptr(), a_s.data_ptr(), b_q.data_ptr(), b_s.data_ptr(), _p(efo), _p(counts), c.data_ptr(),
+                                 M, N, rows, E, out is None, accumulate, *failure_words(a_q.device), _stream()), "gemm128_wgrad")
     return c
+
+
+# flags and arenas of the calls that launch a whole pass
+B128_QUANT_W, B128_DW, B128_DX = 1, 2, 4
+_bytes128 = {}
+
+
+def block128_bytes(rows, N, K, E, flags, which):
+    """Bytes of an arena of `block128_linear` / `block128_linear_bwd`: which = 0 saved, 1 forward scratch, 2 backward scratch."""
+    key = (rows, N, K, E, flags, which)
+    n = _bytes128.get(key)
+    if n is None:
+        if len(_bytes128) >= 4096:            # sizes follow from the key alone: forgetting costs a call
+            _bytes128.clear()
+        n = _bytes128[key] = lib.smoe_block128_bytes(*key)
+        if n < 0:
+            del _bytes128[key]
+            raise ValueError(f"block128: {rows} rows, {E} experts of {N} x {K}: sizes are multiples of 8, at most 256 experts")
+    return n
+
+
+@_timed
+@_on_its_device
+def block128_linear(x, w, w_s, efo, counts, E, N, K, flags):
+    """x bf16 [rows,K] and w (e4m3 with scales, or bf16 with B128_QUANT_W) -> (y bf16 [rows,N], arena for the backward pass or None)."""
+    _check_same_gpu("block128_linear", x, w, w_s, efo, counts)
+    rows = x.shape[0]
+    y = x.new_empty((rows, N))
+    n = block128_bytes(rows, N, K, E, flags, 0)
+    saved = x.new_empty(n, dtype=_U8) if n else None
+    scratch = x.new_empty(block128_bytes(rows, N, K, E, flags, 1), dtype=_U8)
+    check(lib.smoe_block128_linear(x.data_ptr(), w.data_ptr(), _p(w_s), _p(efo), _p(counts), y.data_ptr(), _p(saved),
+                                   scratch.data_ptr(), rows, N, K, E, flags, *failure_words(x.device), _stream()), "block128_linear")
+    return y, saved
+
+
+@_timed
+@_on_its_device
+def block128_linear_bwd(dy, w, w_s, efo, counts, saved, E, N, K, flags, main_grad=None):
+    """dy bf16 [rows,N] -> (dx bf16 [rows,K] or None, dw bf16 [E,N,K] or None, where it is added to `main_grad` f32)."""
+    rows = dy.shape[0]
+    dx = dy.new_empty((rows, K)) if flags & B128_DX else None
+    dw = None
+    if flags & B128_DW:
+        dw = dy.new_empty((E, N, K)) if main_grad is None else main_grad
+        _check_same_gpu("block128_linear", dy, dw)
+    scratch = dy.new_empty(block128_bytes(rows, N, K, E, flags, 2), dtype=_U8)
+    check(lib.smoe_block128_linear_bwd(dy.data_ptr(), _p(w), _p(w_s), _p(efo), _p(counts), _p(saved), scratch.data_ptr(), _p(dx),
+                                       _p(dw), rows, N, K, E, flags, main_grad is not None, *failure_words(dy.device), _stream()),
+          "block128_linear_bwd")
+    return dx, (dw if main_grad is None else None)
+
+
+@_timed
+@_on_its_device
+def block128_experts(x, idx, scores, w1, w1_s, w2, w2_s, E, I):
+    """x bf16 [T,H], idx i32 and scores f32 [T,K], quantised weights -> bf16 [T,H]; see `sonicmoe.block128_experts`."""
+    _check_same_gpu("block128_experts", x, idx, scores, w1, w1_s, w2, w2_s)
+    T, H = x.shape
+    K = idx.shape[1]
+    n = lib.smoe_block128_experts_bytes(T, H, I, E, K)
+    if n < 0:
+        raise ValueError(f"block128_experts: {T} tokens of {H}, {E} experts of {I}, {K} a token: sizes are multiples of 8, at most "
+                         "256 experts and 16 a token")
+    out = x.new_empty((T, H))
+    scratch = x.new_empty(n, dtype=_U8)
+    check(lib.smoe_block128_experts(x.data_ptr(), idx.data_ptr(), scores.data_ptr(), w1.data_ptr(), w1_s.data_ptr(), w2.data_ptr(),
+                                    w2_s.data_ptr(), out.data_ptr(), scratch.data_ptr(), T, H, I, E, K, *failure_words(x.device),
+                                    _stream()), "block128_experts")
+    return out

@@ -63,8 +63,10 @@ def group_limited_routing(router_logits: torch.Tensor, K: int, *, score: str = "
         if bias.shape != (E,):
             raise ValueError(f"bias {tuple(bias.shape)}: one value for each of {E} experts")
         bias = bias.detach().float().contiguous()
-    return _GroupLimitedRouting.apply(router_logits.contiguous(), K, bias, groups, top_groups, group_score, score == "softmax",
-                                      normalize, float(scale))
+    rule = (bias, groups, top_groups, group_score, score == "softmax", bool(normalize), float(scale))
+    if router_logits.requires_grad and torch.is_grad_enabled():
+        return _GroupLimitedRouting.apply(router_logits.contiguous(), K, *rule)
+    return ops.group_routing(router_logits.detach().contiguous(), K, *rule)
 
 
 def token_rounding_routing(router_logits: torch.Tensor, K: int, Mtile: int = 128, routing: str = "nr"):
