@@ -22,15 +22,30 @@ static int make_tmap128(CUtensorMap* m, const void* base, uint64_t depth, uint64
   return r == CUDA_SUCCESS ? SMOE_OK : SMOE_ERR_TMAP;
 }
 
+// The result [depth, rows, cols], box of 32 rows of 64 bytes
+static int make_tmap128_out(CUtensorMap* m, void* base, bool bf16, uint64_t depth, uint64_t rows, uint64_t cols) {
+  if (!load_encode()) return SMOE_ERR_DRIVER;
+  const cuuint64_t es = bf16 ? 2 : 4;
+  cuuint64_t extent[3] = {cols, rows, depth};
+  cuuint64_t strides[2] = {cols * es, cols * rows * es};
+  cuuint32_t box[3] = {(cuuint32_t)(64 / es), 32, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = g_encode(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, base, extent, strides,
+                              box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? SMOE_OK : SMOE_ERR_TMAP;
+}
+
 template <int MODE>
-static int launch128(const CUtensorMap& ta, const CUtensorMap& tb, const Gemm128Params& p, int64_t tiles, cudaStream_t stream) {
+static int launch128(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, const Gemm128Params& p, int64_t tiles,
+                     cudaStream_t stream) {
   static bool attr_set[kMaxDevices] = {};
   auto kern = gemm128_kernel<MODE>;
   if (!ensure_smem_attr(kern, Gemm128Smem::TOTAL, attr_set)) return SMOE_ERR_LAUNCH;
   int64_t pairs = sm_count() / 2;
   if (tiles < pairs) pairs = tiles;
   if (pairs <= 0) return SMOE_OK;
-  kern<<<(unsigned)(2 * pairs), Gemm128Smem::THREADS, Gemm128Smem::TOTAL, stream>>>(ta, tb, p);
+  kern<<<(unsigned)(2 * pairs), Gemm128Smem::THREADS, Gemm128Smem::TOTAL, stream>>>(ta, tb, tc, p);
   return cudaGetLastError() == cudaSuccess ? SMOE_OK : SMOE_ERR_LAUNCH;
 }
 
@@ -58,8 +73,9 @@ int smoe_gemm128_rows(const void* a_fp8, const float* a_scales, const void* b_fp
                       int zero_rest, int32_t* status, int32_t* pinned_host_word, void* stream) {
   int rc = check128(a_fp8, a_scales, b_fp8, b_scales, efo, counts, c_bf16, rows, N, K, E, status);
   if (rc || rows == 0) return rc;
-  CUtensorMap ta, tb;
+  CUtensorMap ta, tb, tc;
   rc = make_tmap128(&ta, a_fp8, 1, rows, K, 128, 2);
+  if (!rc) rc = make_tmap128_out(&tc, c_bf16, true, 1, rows, N);
   if (!rc) rc = b_mn ? make_tmap128(&tb, b_fp8, E, K, N, 128, 3) : make_tmap128(&tb, b_fp8, E, N, K, 128, 3);
   if (rc) return rc;
   Gemm128Params p{};
@@ -73,7 +89,7 @@ int smoe_gemm128_rows(const void* a_fp8, const float* a_scales, const void* b_fp
   p.b_mn = b_mn != 0; p.c = c_bf16; p.zero_rest = zero_rest != 0; p.status = status; p.host_word = pinned_host_word;
   // every segment may end in a tile that is not full, and so may the rows behind the last
   const int64_t tiles = efo ? (rows / 256 + E + 1) * up(N, 256) : up(rows, 256) * up(N, 256);
-  return launch128<ROWS128>(ta, tb, p, tiles, (cudaStream_t)stream);
+  return launch128<ROWS128>(ta, tb, tc, p, tiles, (cudaStream_t)stream);
 }
 
 int smoe_gemm128_wgrad(const void* a_fp8, const float* a_scales, const void* b_fp8, const float* b_scales, const int32_t* efo,
@@ -88,8 +104,9 @@ int smoe_gemm128_wgrad(const void* a_fp8, const float* a_scales, const void* b_f
     return cudaMemsetAsync(c, 0, (size_t)(E * M * N) * (out_bf16 ? 2 : 4), (cudaStream_t)stream) == cudaSuccess ? SMOE_OK
                                                                                                              : SMOE_ERR_LAUNCH;
   }
-  CUtensorMap ta, tb;
+  CUtensorMap ta, tb, tc;
   rc = make_tmap128(&ta, a_fp8, 1, rows, M, 128, 2);
+  if (!rc) rc = make_tmap128_out(&tc, c, out_bf16, E, M, N);
   if (!rc) rc = make_tmap128(&tb, b_fp8, 1, rows, N, 128, 3);
   if (rc) return rc;
   Gemm128Params p{};
@@ -97,7 +114,7 @@ int smoe_gemm128_wgrad(const void* a_fp8, const float* a_scales, const void* b_f
   p.efo = efo; p.counts = counts; p.a_s = a_scales; p.b_s = b_scales;
   p.c = c; p.out_bf16 = out_bf16 != 0; p.accumulate = accumulate != 0; p.status = status;
   p.host_word = pinned_host_word;
-  return launch128<WGRAD128>(ta, tb, p, E * up(M, 256) * up(N, 256), (cudaStream_t)stream);
+  return launch128<WGRAD128>(ta, tb, tc, p, E * up(M, 256) * up(N, 256), (cudaStream_t)stream);
 }
 
 int smoe_gemm128_few(const void* a_fp8, const float* a_scales, const void* b_fp8, const float* b_scales, const int32_t* efo,

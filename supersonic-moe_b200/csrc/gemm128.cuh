@@ -44,18 +44,21 @@ constexpr int kG128Segs = kMaxExperts2 + 1;        // the rows behind the last s
 
 struct Gemm128Smem {
   static constexpr int A_BYTES = BM * BK, B_BYTES = 128 * BK;
-  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES, STAGES = 6;
+  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES, STAGES = 5;
   static constexpr int EPI_WARPS = 8;
-  static constexpr int STG_BYTES = 2048;                    // output staging of a warp
-  static constexpr int SB_BYTES = 2 * 512;                  // WGRAD128: scales of a warp's 128 columns, two blocks
+  static constexpr int STG_TILE = 2048, STG_TILES = 3;      // output staging of a warp: 32 rows x 64 bytes
+  static constexpr int STG_BYTES = STG_TILES * STG_TILE;
+  // WGRAD128: scales of this CTA's 128 rows and of the 256 columns in a block, in a ring of their own, filled by a warp of its own:
+  // every block reads new lines of them, and a register's worth of look-ahead does not cover HBM (measured: 1650 clocks a block)
+  static constexpr int SC_BYTES = (128 + 256) * 4, SC_SLOTS = 6;
   static constexpr int AUX_BYTES = 512 + 4 * (kG128Segs + 1) * 4;
-  static constexpr int TOTAL = 1024 + STAGES * STAGE_BYTES + EPI_WARPS * (STG_BYTES + SB_BYTES) + AUX_BYTES;
+  static constexpr int TOTAL = 1024 + STAGES * STAGE_BYTES + EPI_WARPS * STG_BYTES + SC_SLOTS * SC_BYTES + AUX_BYTES;
   // Two warpgroups of epilogue warps and one with the producer and the MMA issuer.  A thread of the former needs more than the 168
   // registers that three warps on each quarter of the SM leave: 2 x 224 + 56 = 3 x 168.
   static constexpr int THREADS = 32 * (EPI_WARPS + 4), EPI_REGS = 224, OTHER_REGS = 56;
   static constexpr uint32_t TX_BYTES = 2u * STAGE_BYTES;
   static_assert(TOTAL <= 227 * 1024, "shared memory budget");
-  static_assert((2 * STAGES + 4) * 8 <= 496, "barrier storage");
+  static_assert((2 * STAGES + 4 + 2 * SC_SLOTS) * 8 <= 496, "barrier storage");
 };
 
 // tcgen05.mma kind::f8f6f4: e4m3 x e4m3 -> f32
@@ -91,6 +94,17 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* tmap, uint
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
       ::"r"(dst), "l"(tmap), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+// 16 lanes x 32 columns: thread t gets, of each 8 columns, columns 2 (t % 4) and the next of lanes t / 4 (r[4g], r[4g+1]) and
+// t / 4 + 8 (r[4g+2], r[4g+3])
+__device__ __forceinline__ void tmem_ld_16x32(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
       : "memory");
 }
 // the values of a TMEM load are there from here on: nothing that reads them moves ahead of the wait
@@ -173,33 +187,47 @@ __device__ __forceinline__ Tile128 tile128(int tile, int rank, const Gemm128Para
   return t;
 }
 
-// 32 columns (bf16) or 16 (f32) of a warp's 32 rows through its staging tile: lanes hold rows, the stores take 64 bytes of a row
-// each.  w: the lane's 16 words.  word0: column of the first word in 32-bit words from the row's start; words of a row.
-template <typename F>
-__device__ __forceinline__ void store_slab128(uint32_t stg, int lane, const uint32_t (&w)[16], F store) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-    st_shared_v4(stg + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4), w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+// A warp's staged 32 rows x 32 bf16 columns (16-byte pieces of a row at places xor (row / 2) % 4, the 64-byte TMA swizzle), where
+// not all rows are to be written: four lanes a row
+__device__ __forceinline__ void store_slab128(uint32_t stg, int lane, uint16_t* c, int N, int row0, int end, int col0) {
   __syncwarp();
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int r = i * 8 + (lane >> 2), j = lane & 3;
+    const int r = i * 8 + (lane >> 2), j = lane & 3, gr = row0 + r, gc = col0 + j * 8;
     uint4 v;
     ld_shared_v4(stg + r * 64 + ((j ^ ((r >> 1) & 3)) << 4), v.x, v.y, v.z, v.w);
-    store(r, j, v);
+    if (gr < end && gc < N) *reinterpret_cast<uint4*>(c + (int64_t)gr * N + gc) = v;
   }
   __syncwarp();
+}
+__device__ __forceinline__ void tma_store_3d(const void* tmap, uint32_t src, int c0, int c1, int c2) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];"
+               ::"l"(tmap), "r"(src), "r"(c0), "r"(c1), "r"(c2)
+               : "memory");
+}
+__device__ __forceinline__ void tma_reduce_add_3d(const void* tmap, uint32_t src, int c0, int c1, int c2) {
+  asm volatile("cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3, %4}], [%1];"
+               ::"l"(tmap), "r"(src), "r"(c0), "r"(c1), "r"(c2)
+               : "memory");
+}
+__device__ __forceinline__ void st_shared_v2(uint32_t addr, uint32_t a, uint32_t b) {
+  asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(addr), "r"(a), "r"(b) : "memory");
+}
+__device__ __forceinline__ void st_shared_b32(uint32_t addr, uint32_t v) {
+  asm volatile("st.shared.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
 
 template <int MODE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Gemm128Smem::THREADS, 1)
-gemm128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const Gemm128Params p) {
+gemm128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
+               const __grid_constant__ CUtensorMap tmap_c, const Gemm128Params p) {
   using S = Gemm128Smem;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* epi = smem + S::STAGES * S::STAGE_BYTES;
-  uint8_t* aux = epi + S::EPI_WARPS * (S::STG_BYTES + S::SB_BYTES);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(aux);            // full[S], empty[S], tfull[2], tempty[2]
+  uint8_t* scales = epi + S::EPI_WARPS * S::STG_BYTES;
+  uint8_t* aux = scales + S::SC_SLOTS * S::SC_BYTES;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(aux);            // full[S], empty[S], tfull[2], tempty[2], scfull[], scempty[]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(aux + 496);
   volatile int* s_abort = reinterpret_cast<volatile int*>(aux + 500);
   Segs128 segs;
@@ -212,8 +240,9 @@ gemm128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
   const int pair_id = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
   const uint32_t bar_full = smem_u32(bars), bar_empty = bar_full + 8 * S::STAGES;
   const uint32_t bar_tfull = bar_empty + 8 * S::STAGES, bar_tempty = bar_tfull + 16;
+  const uint32_t bar_scfull = bar_tempty + 16, bar_scempty = bar_scfull + 8 * S::SC_SLOTS;
 
-  constexpr int PRODUCER = S::EPI_WARPS, ISSUER = S::EPI_WARPS + 1;
+  constexpr int PRODUCER = S::EPI_WARPS, ISSUER = S::EPI_WARPS + 1, SCALER = S::EPI_WARPS + 2;
   if (warp == 2) load_segs128(segs, p.efo, p.counts, p.E, p.rows, 256, false, lane);
   if (threadIdx.x == 0) {
     for (int s = 0; s < S::STAGES; ++s) {
@@ -223,6 +252,10 @@ gemm128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
     for (int s = 0; s < 2; ++s) {
       mbar_init(bar_tfull + 8 * s, 1);                    // commit arrival, in each CTA
       mbar_init(bar_tempty + 8 * s, 2 * S::EPI_WARPS);    // leader's: the epilogue warps of both CTAs
+    }
+    for (int s = 0; s < S::SC_SLOTS; ++s) {
+      mbar_init(bar_scfull + 8 * s, 1);                   // of this CTA alone
+      mbar_init(bar_scempty + 8 * s, S::EPI_WARPS);
     }
     *s_abort = 0;
     fence_barrier_init();
@@ -245,7 +278,7 @@ gemm128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::OTHER_REGS));
   if (warp == PRODUCER) {
     // ------------------------------------------------------------ producer (both CTAs), one elected lane issues
-    if (lane == 0) { prefetch_tmap(&tmap_a); prefetch_tmap(&tmap_b); }
+    if (lane == 0) { prefetch_tmap(&tmap_a); prefetch_tmap(&tmap_b); prefetch_tmap(&tmap_c); }
     const uint32_t full0 = map_to_cta(bar_full, 0);
     int stage = 0;
     uint32_t phase = 0;
@@ -312,6 +345,29 @@ gemm128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
       if (!ok && lane == 0) { *s_abort = 1; fail128(p.status, p.host_word, 402); }
     }
     __syncwarp();
+  } else if (MODE == WGRAD128 && warp == SCALER) {
+    // ------------------------------------------------------------ scales (both CTAs, each its own)
+    if (lane == 0) {
+      int slot = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int tile = pair_id; tile < n_total && ok; tile += n_pairs) {
+        const Tile128 t = tile128<MODE>(tile, rank, p, segs);
+        const uint32_t a_bytes = max(min(128, p.M - t.m0), 0) * 4, b_bytes = min(256, p.N - t.n0) * 4;      // multiples of 32
+        for (int k = 0; k < t.nkt; ++k) {
+          ok = mbar_wait(bar_scempty + 8 * slot, phase ^ 1);
+          if (!ok) break;
+          const uint32_t full = bar_scfull + 8 * slot, dst = smem_u32(scales) + slot * S::SC_BYTES;
+          const int64_t block = t.t0 / 128 + k;
+          mbar_expect_tx(full, a_bytes + b_bytes);
+          if (a_bytes) bulk_load(dst, p.a_s + block * p.M + t.m0, a_bytes, full);
+          bulk_load(dst + 512, p.b_s + block * p.N + t.n0, b_bytes, full);
+          if (++slot == S::SC_SLOTS) { slot = 0; phase ^= 1; }
+        }
+      }
+      if (!ok) { *s_abort = 1; fail128(p.status, p.host_word, 404); }
+    }
+    __syncwarp();
   }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::EPI_REGS));
@@ -319,131 +375,182 @@ gemm128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
     const int q = warp & 3, half = warp >> 2;
     const uint32_t tempty0 = map_to_cta(bar_tempty, 0);
     const uint32_t stg = smem_u32(epi) + warp * S::STG_BYTES;
-    float* sb_buf = reinterpret_cast<float*>(epi + S::EPI_WARPS * S::STG_BYTES + warp * S::SB_BYTES);
-    int as = 0;
-    uint32_t aphase = 0;
+    int as = 0, slot = 0, buf = 0;
+    uint32_t aphase = 0, scphase = 0;
     bool ok = true;
-    for (int tile = pair_id; tile < n_total && ok; tile += n_pairs) {
-      const Tile128 t = tile128<MODE>(tile, rank, p, segs);
-      const int row = t.m0 + q * 32 + lane;               // of c (WGRAD128: of the expert's)
-      const int col0 = t.n0 + half * 128;
+    // A staging tile is free again once the store before the last one has been read out of shared memory
+    auto staging = [&] {
+      if (lane == 0) bulk_wait_group_read<S::STG_TILES - 1>();
+      __syncwarp();
+      const uint32_t at = stg + buf * S::STG_TILE;
+      if (++buf == S::STG_TILES) buf = 0;
+      return at;
+    };
+    auto staged = [&](uint32_t at, int col, int row, int e) {
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        if (MODE == WGRAD128 && p.accumulate) tma_reduce_add_3d(&tmap_c, at, col, row, e);
+        else tma_store_3d(&tmap_c, at, col, row, e);
+        bulk_commit_group();
+      }
+    };
+    auto release = [&] {                                  // the buffer's values are in registers
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster_relaxed(tempty0 + 8 * as);
+    };
+    Tile128 t{};
+    const float *sa = nullptr, *sb = nullptr;             // ROWS128: scales of a lane's row, of the columns
+    float sa_next = 0.f, sb_next = 0.f;
+    // The next tile and its first scales are asked for before the results of the one before it are written
+    auto begin = [&](int tile) {
+      t = tile128<MODE>(tile, rank, p, segs);
+      if (MODE == ROWS128 && t.nkt > 0) {
+        const int row = t.m0 + q * 32 + lane;
+        sa = p.a_s + (int64_t)(row < t.live ? row : 0) * p.a_kb;
+        sb = p.b_s + t.e * p.bs_e + (int64_t)min(t.n0 / 128 + half, (p.N - 1) / 128) * p.bs_n;
+        sa_next = *sa;
+        sb_next = *sb;
+      }
+    };
+    if (pair_id < n_total) begin(pair_id);
+    for (int tile = pair_id; tile < n_total; tile += n_pairs) {
       float acc[128];
 #pragma unroll
       for (int i = 0; i < 128; ++i) acc[i] = 0.f;
-      // scales: one number a lane for its row, one for the 128 columns (ROWS128) or one a column (WGRAD128)
-      const float* sa = p.a_s;
-      const float* sb = p.b_s;
-      int sa_k, sb_k;
-      bool sb_in = true, row_in;
-      if (MODE == WGRAD128) {
-        row_in = row < p.M;
-        sa += (int64_t)(t.t0 / 128) * p.M + (row_in ? row : 0);
-        sb_in = col0 + lane * 4 < p.N;
-        sb += (int64_t)(t.t0 / 128) * p.N + (sb_in ? col0 + lane * 4 : 0);
-        sa_k = p.M;
-        sb_k = p.N;
-      } else {
-        row_in = row < t.live;
-        sa += (int64_t)(row_in ? row : 0) * p.a_kb;
-        sb += t.e < p.E ? t.e * p.bs_e + (int64_t)min(col0 / 128, (p.N - 1) / 128) * p.bs_n : 0;
-        sa_k = 1;
-        sb_k = p.bs_k;
-      }
-      float sa_next = 0.f, sb_next = 0.f;
-      float4 sb4_next = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (t.nkt > 0) {
-        sa_next = *sa;
-        if (MODE == WGRAD128) { if (sb_in) sb4_next = *reinterpret_cast<const float4*>(sb); }
-        else sb_next = *sb;
-      }
+      const int r4 = lane >> 2, c2 = (lane & 3) * 2;
       for (int k = 0; k < t.nkt; ++k) {
-        const float sa_now = sa_next, sb_now = sb_next;
-        float* sbk = sb_buf + (k & 1) * 128;
-        if (MODE == WGRAD128) {
-          reinterpret_cast<float4*>(sbk)[lane] = sb4_next;
-          __syncwarp();
-        }
-        if (k + 1 < t.nkt) {
-          sa += sa_k;
-          sb += sb_k;
-          sa_next = *sa;
-          if (MODE == WGRAD128) { if (sb_in) sb4_next = *reinterpret_cast<const float4*>(sb); }
-          else sb_next = *sb;
-        }
-        ok = __all_sync(0xffffffffu, mbar_wait(bar_tfull + 8 * as, aphase));
-        if (!ok) break;
-        tc_fence_after();
         const uint32_t src = tmem_base + ((uint32_t)(q * 32) << 16) + as * 256 + half * 128;
-        const float f = MODE == WGRAD128 ? sa_now : sa_now * sb_now;
-        uint32_t r[2][16];
-        tmem_ld16(src, r[0]);
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          tmem_ld_wait();
-          tmem_arrived(r[c & 1]);
-          if (c < 7) {
-            tmem_ld16(src + (c + 1) * 16, r[(c + 1) & 1]);
-          } else {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster_relaxed(tempty0 + 8 * as);
+        if (MODE == ROWS128) {
+          // A lane is a row, a register a column: one factor a thread and block, the row's scale times the weight's.
+          const float f = sa_next * sb_next;
+          if (k + 1 < t.nkt) {
+            sa_next = *++sa;
+            sb += p.bs_k;
+            sb_next = *sb;
           }
-          const uint32_t(&v)[16] = r[c & 1];
+          ok = __all_sync(0xffffffffu, mbar_wait(bar_tfull + 8 * as, aphase));
+          if (!ok) break;
+          tc_fence_after();
+          uint32_t r[2][16];
+          tmem_ld16(src, r[0]);
 #pragma unroll
-          for (int i = 0; i < 16; i += 4) {
-            if (MODE == WGRAD128) {
-              const float4 s4 = *reinterpret_cast<const float4*>(sbk + c * 16 + i);
-              const float x[4] = {s4.x, s4.y, s4.z, s4.w};
+          for (int c = 0; c < 8; ++c) {
+            tmem_ld_wait();
+            tmem_arrived(r[c & 1]);
+            if (c < 7) tmem_ld16(src + (c + 1) * 16, r[(c + 1) & 1]);
+            else release();
 #pragma unroll
-              for (int j = 0; j < 4; ++j)
-                acc[c * 16 + i + j] = fmaf(__uint_as_float(v[i + j]) * x[j], f, acc[c * 16 + i + j]);
-            } else {
+            for (int i = 0; i < 16; ++i) acc[c * 16 + i] = fmaf(__uint_as_float(r[c & 1][i]), f, acc[c * 16 + i]);
+          }
+        } else {
+          // Both operands have a scale of their own in every block: two multiplications a value.  With a lane a row every lane
+          // would read the scales of all 128 columns, 128 KB a block and SM out of shared memory; in the matrix layout a thread
+          // has four rows and a quarter of the columns.
+          ok = __all_sync(0xffffffffu, mbar_wait(bar_scfull + 8 * slot, scphase));
+          if (!ok) break;
+          const float* sak = reinterpret_cast<const float*>(scales + slot * S::SC_BYTES) + q * 32 + r4;
+          const float* sbk = reinterpret_cast<const float*>(scales + slot * S::SC_BYTES + 512) + half * 128 + c2;
+          float f[4];
+          float2 s2[2][4];
 #pragma unroll
-              for (int j = 0; j < 4; ++j) acc[c * 16 + i + j] = fmaf(__uint_as_float(v[i + j]), f, acc[c * 16 + i + j]);
+          for (int j = 0; j < 4; ++j) {
+            f[j] = sak[8 * j];
+            s2[0][j] = *reinterpret_cast<const float2*>(sbk + j * 8);
+          }
+          ok = __all_sync(0xffffffffu, mbar_wait(bar_tfull + 8 * as, aphase));
+          if (!ok) break;
+          tc_fence_after();
+          uint32_t r[2][16];
+          tmem_ld_16x32(src, r[0]);
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {                   // 32 columns (c / 2) of 16 rows (c % 2)
+            tmem_ld_wait();
+            tmem_arrived(r[c & 1]);
+            if (c < 7) tmem_ld_16x32(src + ((uint32_t)(((c + 1) & 1) * 16) << 16) + ((c + 1) >> 1) * 32, r[(c + 1) & 1]);
+            else release();
+            if ((c & 1) == 0 && c < 6) {
+#pragma unroll
+              for (int g = 0; g < 4; ++g)
+                s2[((c >> 1) + 1) & 1][g] = *reinterpret_cast<const float2*>(sbk + ((c >> 1) + 1) * 32 + g * 8);
+            }
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const float2 s = s2[(c >> 1) & 1][g];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int at = c * 16 + g * 4 + i;
+                acc[at] = fmaf(__uint_as_float(r[c & 1][g * 4 + i]) * ((i & 1) ? s.y : s.x), f[(c & 1) * 2 + (i >> 1)], acc[at]);
+              }
             }
           }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar_scempty + 8 * slot);
+          if (++slot == S::SC_SLOTS) { slot = 0; scphase ^= 1; }
         }
         if (++as == 2) { as = 0; aphase ^= 1; }
       }
       if (!ok) break;
-      if (MODE == ROWS128 && t.m0 + q * 32 >= t.end) continue;      // nothing of this warp's rows is stored
       // ---- out
-      if (MODE == ROWS128 || p.out_bf16) {
-        uint16_t* c = reinterpret_cast<uint16_t*>(p.c) + (MODE == WGRAD128 ? (int64_t)t.e * p.M * p.N : 0);
+      const int row0 = t.m0 + q * 32, col0 = t.n0 + half * 128, end = t.end, e = t.e;
+      const bool row_in = row0 + lane < t.live;
+      if (tile + n_pairs < n_total) begin(tile + n_pairs);
+      if (row0 >= end) continue;                          // nothing of this warp's rows is stored
+      if (MODE == ROWS128) {
+        const bool whole = row0 + 32 <= end;
 #pragma unroll
         for (int cc = 0; cc < 4; ++cc) {
-          uint32_t w[16];
+          const int col = col0 + cc * 32;
+          if (col >= p.N) break;
+          const uint32_t at = staging();
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            w[i] = row_in ? pack_bf16x2(acc[cc * 32 + 2 * i], acc[cc * 32 + 2 * i + 1]) : 0u;
+          for (int j = 0; j < 4; ++j) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              w[i] = row_in ? pack_bf16x2(acc[cc * 32 + 8 * j + 2 * i], acc[cc * 32 + 8 * j + 2 * i + 1]) : 0u;
+            st_shared_v4(at + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4), w[0], w[1], w[2], w[3]);
           }
-          store_slab128(stg, lane, w, [&](int r, int j, const uint4& v) {
-            const int gr = t.m0 + q * 32 + r, gc = col0 + cc * 32 + j * 8;
-            if (gr < t.end && gc < p.N) *reinterpret_cast<uint4*>(c + (int64_t)gr * p.N + gc) = v;
-          });
+          if (whole) staged(at, col, row0, 0);
+          else store_slab128(at, lane, reinterpret_cast<uint16_t*>(p.c), p.N, row0, end, col);
+        }
+      } else if (p.out_bf16) {
+#pragma unroll
+        for (int cc = 0; cc < 4; ++cc) {
+          if (col0 + cc * 32 >= p.N) break;
+          const uint32_t at = staging();
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {                   // rows r4 + 8 j
+            const int r = r4 + 8 * j;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const int i = cc * 32 + (j >> 1) * 16 + g * 4 + (j & 1) * 2;
+              st_shared_b32(at + r * 64 + ((g ^ ((r >> 1) & 3)) << 4) + c2 * 2, pack_bf16x2(acc[i], acc[i + 1]));
+            }
+          }
+          staged(at, col0 + cc * 32, row0, e);
         }
       } else {
-        float* c = reinterpret_cast<float*>(p.c) + (int64_t)t.e * p.M * p.N;
 #pragma unroll
-        for (int cc = 0; cc < 8; ++cc) {
-          uint32_t w[16];
+        for (int cc = 0; cc < 8; ++cc) {                  // 16 columns
+          if (col0 + cc * 16 >= p.N) break;
+          const uint32_t at = staging();
 #pragma unroll
-          for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(acc[cc * 16 + i]);
-          store_slab128(stg, lane, w, [&](int r, int j, const uint4& v) {
-            const int gr = t.m0 + q * 32 + r, gc = col0 + cc * 16 + j * 4;
-            if (gr < t.end && gc < p.N) {
-              float4* dst = reinterpret_cast<float4*>(c + (int64_t)gr * p.N + gc);
-              float4 o = make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
-              if (p.accumulate) {
-                const float4 b = *dst;
-                o.x += b.x; o.y += b.y; o.z += b.z; o.w += b.w;
-              }
-              *dst = o;
+          for (int j = 0; j < 4; ++j) {
+            const int r = r4 + 8 * j;
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+              const int i = (cc >> 1) * 32 + (j >> 1) * 16 + ((cc & 1) * 2 + g) * 4 + (j & 1) * 2;
+              st_shared_v2(at + r * 64 + (((g * 2 + (c2 >> 2)) ^ ((r >> 1) & 3)) << 4) + (c2 & 2) * 4, __float_as_uint(acc[i]),
+                           __float_as_uint(acc[i + 1]));
             }
-          });
+          }
+          staged(at, col0 + cc * 16, row0, e);
         }
       }
     }
+    if (lane == 0) bulk_wait_group<0>();                  // all stores have left shared memory and are visible
     if (!ok && lane == 0) { *s_abort = 1; fail128(p.status, p.host_word, 403); }
   }
 
