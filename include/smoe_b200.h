@@ -500,11 +500,11 @@ int smoe_quant128_rows(const void* x_bf16, int64_t rows, int64_t K, int swiglu, 
 /* x bf16 [T,K]: row t, quantised once, to the rows s_rev[naept[t]] .. s_rev[naept[t+1] - 1] of q [rows,K], scales [rows, K/128]. */
 int smoe_quant128_rows_scatter(const void* x_bf16, int64_t T, int64_t K, const int32_t* naept, const int32_t* s_rev, int64_t rows,
                                void* q, float* scales, void* stream);
-/* Both forms of x bf16 [rows,K] from one read: q, scales as above (null: not written) and q_col [rows,K], col_scales
- * [ceil(rows/128), K], where the rows of a segment behind its live ones count and leave zero.  128-row blocks without live rows
- * have no column form. */
+/* Both forms of x bf16 [rows,K] from one read: q, scales as above (null: not written) and, transposed, q_t [K,rows] with a scale
+ * for each column of x and 128 rows, t_scales [ceil(rows/128), K]; the rows of a segment behind its live ones count and leave
+ * zero.  128-row blocks without live rows have no column form. */
 int smoe_quant128_dual(const void* x_bf16, int64_t rows, int64_t K, const int32_t* efo, const int32_t* counts, int64_t E, void* q,
-                       float* scales, void* q_col, float* col_scales, void* stream);
+                       float* scales, void* q_t, float* t_scales, void* stream);
 /* W bf16 [E,N,K] -> q [E,N,K], scales [E, N/128, K/128] (both rounded up). */
 int smoe_quant128_weight(const void* w_bf16, int64_t E, int64_t N, int64_t K, void* q, float* scales, void* stream);
 
@@ -519,7 +519,8 @@ int smoe_gemm128_rows(const void* a_fp8, const float* a_scales, const void* b_fp
 int smoe_gemm128_few(const void* a_fp8, const float* a_scales, const void* b_fp8, const float* b_scales, const int32_t* efo,
                      const int32_t* counts, void* c_bf16, int64_t rows, int64_t N, int64_t K, int64_t E, int64_t live_rows,
                      int32_t* status, int32_t* pinned_host_word, void* stream);
-/* c[e] (M x N) = a[seg_e]^T . b[seg_e], a [rows,M] and b [rows,N] by columns: f32, added to c or stored, or rounded to bf16. */
+/* c[e] (M x N) = a[:, seg_e] . b[:, seg_e]^T, a [M,rows] and b [N,rows] with scales [ceil(rows/128), M] and [.., N] as
+ * smoe_quant128_dual leaves them: f32, added to c or stored, or rounded to bf16. */
 int smoe_gemm128_wgrad(const void* a_fp8, const float* a_scales, const void* b_fp8, const float* b_scales, const int32_t* efo,
                        const int32_t* counts, void* c, int64_t M, int64_t N, int64_t rows, int64_t E, int out_bf16, int accumulate,
                        int32_t* status, int32_t* pinned_host_word, void* stream);

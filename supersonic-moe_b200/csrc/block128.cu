@@ -33,7 +33,7 @@ struct Saved128 {             // of a forward pass: the weight's payload, if the
       ws = m.floats(E * blocks128(N) * blocks128(K));
     }
     if (flags & SMOE_B128_DW) {
-      xc = m.take(rows * pitch128(K));
+      xc = m.take(K * pitch128(rows));
       xcs = m.floats(blocks128(rows) * K);
     }
     bytes = m.used;
@@ -61,7 +61,7 @@ struct Backward128 {          // dy in the forms that the gradients asked for re
       ds = m.floats(rows * blocks128(N));
     }
     if (flags & SMOE_B128_DW) {
-      dc = m.take(rows * pitch128(N));
+      dc = m.take(N * pitch128(rows));
       dcs = m.floats(blocks128(rows) * N);
     }
     bytes = m.used;

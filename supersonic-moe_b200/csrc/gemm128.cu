@@ -105,9 +105,9 @@ int smoe_gemm128_wgrad(const void* a_fp8, const float* a_scales, const void* b_f
                                                                                                              : SMOE_ERR_LAUNCH;
   }
   CUtensorMap ta, tb, tc;
-  rc = make_tmap128(&ta, a_fp8, 1, rows, M, 128, 2);
+  rc = make_tmap128(&ta, a_fp8, 1, M, rows, 128, 2);
   if (!rc) rc = make_tmap128_out(&tc, c, out_bf16, E, M, N);
-  if (!rc) rc = make_tmap128(&tb, b_fp8, 1, rows, N, 128, 3);
+  if (!rc) rc = make_tmap128(&tb, b_fp8, 1, N, rows, 128, 3);
   if (rc) return rc;
   Gemm128Params p{};
   p.rows = (int)rows; p.M = (int)M; p.N = (int)N; p.E = (int)E;

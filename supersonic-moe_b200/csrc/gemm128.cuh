@@ -1,14 +1,14 @@
 // Grouped products of e4m3 operands with one f32 scale per block of 128 (see quant128.cu), tcgen05 on CTA pairs.
 //
 //   ROWS128   c[r, n] = sum_kb as[r, kb] bs[e, n / 128, kb] (sum over the 128 k of kb of a[r, k] b[e][n, k])     rows by expert
-//   WGRAD128  c[e][m, n] (+)= sum_tb as[tb, m] bs[tb, n] (sum over the 128 rows t of tb of a[t, m] b[t, n])      rows summed over
+//   WGRAD128  c[e][m, n] (+)= sum_tb as[tb, m] bs[tb, n] (sum over the 128 rows t of tb of a[m, t] b[n, t])      rows summed over
 //
 // f32 scales are not what the block-scaled MMA takes (powers of two, 32 wide), so the plain e4m3 MMA sums one block of 128 at a
 // time into TMEM and the epilogue warps add it, scaled, to sums that stay in their registers: 128 f32 a thread, 256 x 256 outputs
 // a CTA pair.  Two TMEM buffers of 256 columns: the MMAs of one block (512 clocks) run while the block before is read out (256
 // clocks of TMEM reads, half as many of packed multiply-adds).
 //   B [E, N, K] is read K-major, or with b_mn as [E, K, N] as it lies: the gradient of the rows needs no transposed weights.
-//   Both operands of the weight gradient lie [rows, dim] and are read MN-major.
+//   Both operands of the weight gradient lie [dim, rows].
 #pragma once
 #include "gemm2.cuh"
 
@@ -96,21 +96,23 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* tmap, uint
       ::"r"(dst), "l"(tmap), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
       : "memory");
 }
-// 16 lanes x 32 columns: thread t gets, of each 8 columns, columns 2 (t % 4) and the next of lanes t / 4 (r[4g], r[4g+1]) and
-// t / 4 + 8 (r[4g+2], r[4g+3])
-__device__ __forceinline__ void tmem_ld_16x32(uint32_t taddr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr)
-      : "memory");
-}
 // the values of a TMEM load are there from here on: nothing that reads them moves ahead of the wait
 __device__ __forceinline__ void tmem_arrived(uint32_t (&r)[16]) {
   asm volatile("" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
                "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]));
+}
+// 16 lanes x 32 columns, complete when it returns: thread t gets, of each 8 columns g, columns 2 (t % 4) and the next of lanes t / 4
+// (the pair r[2g]) and t / 4 + 8 (r[2g+1]).
+__device__ __forceinline__ void tmem_matrix16x32(uint32_t taddr, F2 (&r)[8]) {
+  asm volatile(
+      "{\n\t.reg .b32 t<16>;\n\t"
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {t0,t1,t2,t3,t4,t5,t6,t7,t8,t9,t10,t11,t12,t13,t14,t15}, [%8];\n\t"
+      "tcgen05.wait::ld.sync.aligned;\n\t"
+      "mov.b64 %0, {t0,t1};\n\tmov.b64 %1, {t2,t3};\n\tmov.b64 %2, {t4,t5};\n\tmov.b64 %3, {t6,t7};\n\t"
+      "mov.b64 %4, {t8,t9};\n\tmov.b64 %5, {t10,t11};\n\tmov.b64 %6, {t12,t13};\n\tmov.b64 %7, {t14,t15};\n\t}"
+      : "=l"(r[0].v), "=l"(r[1].v), "=l"(r[2].v), "=l"(r[3].v), "=l"(r[4].v), "=l"(r[5].v), "=l"(r[6].v), "=l"(r[7].v)
+      : "r"(taddr)
+      : "memory");
 }
 
 // Segments from efo / counts, any values taken as they fit: 0 <= start <= end <= rows, start <= live end <= end
@@ -157,7 +159,7 @@ __device__ __forceinline__ int seg_of_tile(const int* tiles, int segs, int t) { 
 
 struct Tile128 {
   int e, m0, n0;             // m0: first row of this CTA's 128
-  int t0, nkt;               // WGRAD128: first row of the reduction; blocks of 128
+  int t0, nkt;               // WGRAD128: first row of the reduction (ROWS128: 0); blocks of 128
   int live, end;             // rows below live are computed, those up to end zero (WGRAD128: end = M)
 };
 template <int MODE>
@@ -170,8 +172,8 @@ __device__ __forceinline__ Tile128 tile128(int tile, int rank, const Gemm128Para
     const int r = tile - t.e * per;
     t.m0 = (r / nt) * 256 + rank * 128;
     t.n0 = (r % nt) * 256;
-    t.t0 = s.start[t.e];
-    t.nkt = (s.live[t.e] - t.t0 + 127) / 128;
+    t.t0 = s.start[t.e] & ~127;          // segments start there; a copy has to start on 16 bytes in any case
+    t.nkt = (s.live[t.e] - s.start[t.e] + 127) / 128;
     t.live = t.end = p.M;
   } else {
     const int pr = tile / nt;
@@ -210,8 +212,12 @@ __device__ __forceinline__ void tma_reduce_add_3d(const void* tmap, uint32_t src
                ::"l"(tmap), "r"(src), "r"(c0), "r"(c1), "r"(c2)
                : "memory");
 }
-__device__ __forceinline__ void st_shared_v2(uint32_t addr, uint32_t a, uint32_t b) {
-  asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(addr), "r"(a), "r"(b) : "memory");
+__device__ __forceinline__ uint32_t pack_bf16x2(F2 a) {
+  const float2 v = f2_get(a);
+  return pack_bf16x2(v.x, v.y);
+}
+__device__ __forceinline__ void st_shared_b64(uint32_t addr, F2 v) {
+  asm volatile("st.shared.b64 [%0], %1;" ::"r"(addr), "l"(v.v) : "memory");
 }
 __device__ __forceinline__ void st_shared_b32(uint32_t addr, uint32_t v) {
   asm volatile("st.shared.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
@@ -295,14 +301,9 @@ gemm128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
         const uint32_t a_dst = smem_base + stage * S::STAGE_BYTES, b_dst = a_dst + S::A_BYTES;
         if (elect_one()) {
           if (rank == 0) mbar_expect_tx(bar_full + 8 * stage, S::TX_BYTES);
-          if (MODE == WGRAD128) {
-            tma_load_2d_pair(a_dst, &tmap_a, full, m0, t0 + k * 128);
-            tma_load_3d_pair(b_dst, &tmap_b, full, n_row, t0 + k * 128, 0);
-          } else {
-            tma_load_2d_pair(a_dst, &tmap_a, full, k * 128, m0);
-            if (p.b_mn) tma_load_3d_pair(b_dst, &tmap_b, full, n_row, k * 128, e);
-            else tma_load_3d_pair(b_dst, &tmap_b, full, k * 128, n_row, e);
-          }
+          tma_load_2d_pair(a_dst, &tmap_a, full, t0 + k * 128, m0);
+          if (MODE == ROWS128 && p.b_mn) tma_load_3d_pair(b_dst, &tmap_b, full, n_row, k * 128, e);
+          else tma_load_3d_pair(b_dst, &tmap_b, full, t0 + k * 128, n_row, e);
         }
         if (++stage == S::STAGES) { stage = 0; phase ^= 1; }
       }
@@ -311,13 +312,13 @@ gemm128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
   } else if (warp == ISSUER) {
     // ------------------------------------------------------------ MMA issuer (leader CTA only)
     if (rank == 0) {
-      const bool a_mn = MODE == WGRAD128, b_mn = MODE == WGRAD128 || p.b_mn;
-      const uint32_t idesc = make_idesc_f8(256, 256, a_mn, b_mn);
+      const bool b_mn = MODE == ROWS128 && p.b_mn;
+      const uint32_t idesc = make_idesc_f8(256, 256, false, b_mn);
       // operand descriptors: see make_desc_kmajor_sw128 / make_desc_mnmajor_sw128; a step of 32 along the reduction is 32 bytes
       // (K-major) or 32 rows of 128 bytes
       const uint32_t desc_hi = (1024u >> 4) | (1u << 14) | (2u << 29);
-      const uint32_t a_step = a_mn ? 256u : 2u, b_step = b_mn ? 256u : 2u;
-      const uint32_t a_lo0 = ((smem_base & 0x3FFFF) >> 4) | ((a_mn ? (uint32_t)(S::A_BYTES >> 4) : 1u) << 16);
+      const uint32_t b_step = b_mn ? 256u : 2u;
+      const uint32_t a_lo0 = ((smem_base & 0x3FFFF) >> 4) | (1u << 16);
       const uint32_t b_lo0 = (((smem_base + S::A_BYTES) & 0x3FFFF) >> 4) | ((b_mn ? (uint32_t)(S::B_BYTES >> 4) : 1u) << 16);
       int stage = 0, as = 0;
       uint32_t phase = 0, aphase = 0;
@@ -325,16 +326,18 @@ gemm128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
       for (int tile = pair_id; tile < n_total && ok; tile += n_pairs) {
         const int nkt = __shfl_sync(0xffffffffu, tile128<MODE>(tile, 0, p, segs).nkt, 0);
         for (int k = 0; k < nkt; ++k) {
-          ok = __all_sync(0xffffffffu, mbar_wait(bar_tempty + 8 * as, aphase ^ 1));
-          if (!ok) break;
+          // (the operands first: they are there long before the buffer is, and a look at a barrier takes some 200 clocks while the
+          // MMAs read shared memory)
           ok = __all_sync(0xffffffffu, mbar_wait(bar_full + 8 * stage, phase));
+          if (!ok) break;
+          ok = __all_sync(0xffffffffu, mbar_wait(bar_tempty + 8 * as, aphase ^ 1));
           if (!ok) break;
           tc_fence_after();
           const uint32_t a_lo = a_lo0 + stage * (S::STAGE_BYTES >> 4), b_lo = b_lo0 + stage * (S::STAGE_BYTES >> 4);
           if (elect_one()) {
 #pragma unroll
             for (int kb = 0; kb < BK / 32; ++kb)
-              mma_f8_pair_lo(tmem_base + as * 256, a_lo + a_step * kb, b_lo + b_step * kb, desc_hi, idesc, kb != 0);
+              mma_f8_pair_lo(tmem_base + as * 256, a_lo + 2 * kb, b_lo + b_step * kb, desc_hi, idesc, kb != 0);
             tc_commit_pair(bar_empty + 8 * stage, 3);
             tc_commit_pair(bar_tfull + 8 * as, 3);
           }
@@ -416,9 +419,12 @@ gemm128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
     };
     if (pair_id < n_total) begin(pair_id);
     for (int tile = pair_id; tile < n_total; tile += n_pairs) {
-      float acc[128];
+      float acc[MODE == ROWS128 ? 128 : 1];               // [column]
+      F2 acc2[MODE == WGRAD128 ? 64 : 1];                 // [32 columns][16 rows][8 columns][row r4, row r4 + 8]: two columns
 #pragma unroll
-      for (int i = 0; i < 128; ++i) acc[i] = 0.f;
+      for (int i = 0; i < (MODE == ROWS128 ? 128 : 0); ++i) acc[i] = 0.f;
+#pragma unroll
+      for (int i = 0; i < (MODE == WGRAD128 ? 64 : 0); ++i) acc2[i] = f2(0.f, 0.f);
       const int r4 = lane >> 2, c2 = (lane & 3) * 2;
       for (int k = 0; k < t.nkt; ++k) {
         const uint32_t src = tmem_base + ((uint32_t)(q * 32) << 16) + as * 256 + half * 128;
@@ -447,47 +453,50 @@ gemm128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
         } else {
           // Both operands have a scale of their own in every block: two multiplications a value.  With a lane a row every lane
           // would read the scales of all 128 columns, 128 KB a block and SM out of shared memory; in the matrix layout a thread
-          // has four rows and a quarter of the columns.
-          ok = __all_sync(0xffffffffu, mbar_wait(bar_scfull + 8 * slot, scphase));
-          if (!ok) break;
-          const float* sak = reinterpret_cast<const float*>(scales + slot * S::SC_BYTES) + q * 32 + r4;
+          // has four rows and a quarter of the columns.  Two columns an instruction, which is half the issue (a load shape that
+          // reads TMEM in half the time, 16x128b, pairs rows instead and needs more of it: 213 -> 227 us).
+          // A look at a barrier or at shared memory takes some 200 clocks beside the MMAs: both are asked early.
           const float* sbk = reinterpret_cast<const float*>(scales + slot * S::SC_BYTES + 512) + half * 128 + c2;
-          float f[4];
-          float2 s2[2][4];
+          F2 f[4], s2[2][4];
+          if (k == 0) {
+            ok = __all_sync(0xffffffffu, mbar_wait(bar_scfull + 8 * slot, scphase));
+            if (!ok) break;
+          }
+          const float* sak = reinterpret_cast<const float*>(scales + slot * S::SC_BYTES) + q * 32 + r4;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            f[j] = sak[8 * j];
-            s2[0][j] = *reinterpret_cast<const float2*>(sbk + j * 8);
+            f[j] = f2(sak[8 * j], sak[8 * j]);
+            s2[0][j].v = *reinterpret_cast<const uint64_t*>(sbk + j * 8);
           }
           ok = __all_sync(0xffffffffu, mbar_wait(bar_tfull + 8 * as, aphase));
           if (!ok) break;
           tc_fence_after();
-          uint32_t r[2][16];
-          tmem_ld_16x32(src, r[0]);
+          const int next_slot = slot + 1 == S::SC_SLOTS ? 0 : slot + 1;
+          const uint32_t next_phase = scphase ^ (next_slot == 0 ? 1u : 0u);
+          bool seen = true;
 #pragma unroll
           for (int c = 0; c < 8; ++c) {                   // 32 columns (c / 2) of 16 rows (c % 2)
-            tmem_ld_wait();
-            tmem_arrived(r[c & 1]);
-            if (c < 7) tmem_ld_16x32(src + ((uint32_t)(((c + 1) & 1) * 16) << 16) + ((c + 1) >> 1) * 32, r[(c + 1) & 1]);
-            else release();
+            F2 r[8];
+            tmem_matrix16x32(src + ((uint32_t)((c & 1) * 16) << 16) + (c >> 1) * 32, r);
+            if (c == 7) release();
             if ((c & 1) == 0 && c < 6) {
 #pragma unroll
               for (int g = 0; g < 4; ++g)
-                s2[((c >> 1) + 1) & 1][g] = *reinterpret_cast<const float2*>(sbk + ((c >> 1) + 1) * 32 + g * 8);
+                s2[((c >> 1) + 1) & 1][g].v = *reinterpret_cast<const uint64_t*>(sbk + ((c >> 1) + 1) * 32 + g * 8);
             }
+            if (c == 6 && k + 1 < t.nkt) seen = mbar_try_wait(bar_scfull + 8 * next_slot, next_phase);
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              const float2 s = s2[(c >> 1) & 1][g];
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int at = c * 16 + g * 4 + i;
-                acc[at] = fmaf(__uint_as_float(r[c & 1][g * 4 + i]) * ((i & 1) ? s.y : s.x), f[(c & 1) * 2 + (i >> 1)], acc[at]);
-              }
-            }
+            for (int j = 0; j < 8; ++j)
+              acc2[c * 8 + j] = f2_fma(r[j] * s2[(c >> 1) & 1][j >> 1], f[(c & 1) * 2 + (j & 1)], acc2[c * 8 + j]);
           }
           __syncwarp();
           if (lane == 0) mbar_arrive(bar_scempty + 8 * slot);
-          if (++slot == S::SC_SLOTS) { slot = 0; scphase ^= 1; }
+          slot = next_slot;
+          scphase = next_phase;
+          if (k + 1 < t.nkt && !__all_sync(0xffffffffu, seen)) {
+            ok = __all_sync(0xffffffffu, mbar_wait(bar_scfull + 8 * slot, scphase));
+            if (!ok) break;
+          }
         }
         if (++as == 2) { as = 0; aphase ^= 1; }
       }
@@ -524,10 +533,9 @@ gemm128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
           for (int j = 0; j < 4; ++j) {                   // rows r4 + 8 j
             const int r = r4 + 8 * j;
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              const int i = cc * 32 + (j >> 1) * 16 + g * 4 + (j & 1) * 2;
-              st_shared_b32(at + r * 64 + ((g ^ ((r >> 1) & 3)) << 4) + c2 * 2, pack_bf16x2(acc[i], acc[i + 1]));
-            }
+            for (int g = 0; g < 4; ++g)
+              st_shared_b32(at + r * 64 + ((g ^ ((r >> 1) & 3)) << 4) + c2 * 2,
+                            pack_bf16x2(acc2[cc * 16 + (j >> 1) * 8 + g * 2 + (j & 1)]));
           }
           staged(at, col0 + cc * 32, row0, e);
         }
@@ -540,11 +548,9 @@ gemm128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
           for (int j = 0; j < 4; ++j) {
             const int r = r4 + 8 * j;
 #pragma unroll
-            for (int g = 0; g < 2; ++g) {
-              const int i = (cc >> 1) * 32 + (j >> 1) * 16 + ((cc & 1) * 2 + g) * 4 + (j & 1) * 2;
-              st_shared_v2(at + r * 64 + (((g * 2 + (c2 >> 2)) ^ ((r >> 1) & 3)) << 4) + (c2 & 2) * 4, __float_as_uint(acc[i]),
-                           __float_as_uint(acc[i + 1]));
-            }
+            for (int g = 0; g < 2; ++g)
+              st_shared_b64(at + r * 64 + (((g * 2 + (c2 >> 2)) ^ ((r >> 1) & 3)) << 4) + (c2 & 2) * 4,
+                            acc2[(cc >> 1) * 16 + (j >> 1) * 8 + ((cc & 1) * 2 + g) * 2 + (j & 1)]);
           }
           staged(at, col0 + cc * 16, row0, e);
         }

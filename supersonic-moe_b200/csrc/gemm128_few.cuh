@@ -22,6 +22,8 @@ struct Few128Params {
   volatile int* host_word;
 };
 
+constexpr int kFewBars = 640;        // bytes of barriers
+
 struct Few128Smem {
   static constexpr int NT = 64;                               // routed rows of a tile
   static constexpr int A_BYTES = BM * BK, B_BYTES = NT * BK;
@@ -29,12 +31,14 @@ struct Few128Smem {
   static constexpr int ACC = 8;                               // TMEM buffers
   static constexpr int EPI_WARPS = 4;
   static constexpr int PART_BYTES = NT * BM * 4;              // sums of this CTA: [column][weight row]
-  static constexpr int SX_BYTES = EPI_WARPS * 2 * NT * 4;     // scales of a block's columns, per warp, two buffers
-  static constexpr int AUX_BYTES = 512 + 3 * (kG128Segs + 1) * 4;
+  static constexpr int SX_GROUP = 8;                          // blocks whose factors travel together
+  static constexpr int SX_SLOTS = 4, SX_BYTES = SX_SLOTS * SX_GROUP * NT * 4;
+  static constexpr int AUX_BYTES = kFewBars + 16 + 3 * (kG128Segs + 1) * 4;
   static constexpr int TOTAL = 1024 + STAGES * STAGE_BYTES + PART_BYTES + SX_BYTES + AUX_BYTES;
-  static constexpr int THREADS = 32 * (2 + EPI_WARPS);
+  static constexpr int SCALER = 2 + EPI_WARPS;                // warp
+  static constexpr int THREADS = 32 * (SCALER + 1);
   static_assert(TOTAL <= 227 * 1024, "shared memory budget");
-  static_assert((2 * STAGES + 2 * ACC + 2) * 8 <= 496, "barrier storage");
+  static_assert((2 * STAGES + 2 * ACC + 2 + 2 * SX_SLOTS) * 8 <= kFewBars, "barrier storage");
 };
 
 // as mbar_wait, for data that other CTAs of the cluster left before they arrived
@@ -83,11 +87,11 @@ gemm128_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
   float* part = reinterpret_cast<float*>(smem + S::STAGES * S::STAGE_BYTES);
   uint8_t* sx_all = reinterpret_cast<uint8_t*>(part) + S::PART_BYTES;
   uint8_t* aux = sx_all + S::SX_BYTES;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(aux);            // full[S], empty[S], tfull[ACC], tempty[ACC], pfull, pempty
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(aux + 496);
-  volatile int* s_abort = reinterpret_cast<volatile int*>(aux + 500);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(aux);            // full[S], empty[S], tfull[ACC], tempty[ACC], pfull, pempty, sfull[], sempty[]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(aux + kFewBars);
+  volatile int* s_abort = reinterpret_cast<volatile int*>(aux + kFewBars + 4);
   Segs128 segs;
-  segs.start = reinterpret_cast<int*>(aux + 512);
+  segs.start = reinterpret_cast<int*>(aux + kFewBars + 16);
   segs.live = segs.start + kG128Segs + 1;
   segs.tiles = segs.live + kG128Segs + 1;
 
@@ -97,6 +101,7 @@ gemm128_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
   const uint32_t bar_full = smem_u32(bars), bar_empty = bar_full + 8 * S::STAGES;
   const uint32_t bar_tfull = bar_empty + 8 * S::STAGES, bar_tempty = bar_tfull + 8 * S::ACC;
   const uint32_t bar_pfull = bar_tempty + 8 * S::ACC, bar_pempty = bar_pfull + 8;
+  const uint32_t bar_sfull = bar_pempty + 8, bar_sempty = bar_sfull + 8 * S::SX_SLOTS;
 
   if (warp == 2) load_segs128(segs, p.efo, p.counts, p.E, p.rows, NT, true, lane);
   if (threadIdx.x == 0) {
@@ -107,6 +112,10 @@ gemm128_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
     for (int s = 0; s < S::ACC; ++s) {
       mbar_init(bar_tfull + 8 * s, 1);
       mbar_init(bar_tempty + 8 * s, S::EPI_WARPS);
+    }
+    for (int s = 0; s < S::SX_SLOTS; ++s) {
+      mbar_init(bar_sfull + 8 * s, 1);
+      mbar_init(bar_sempty + 8 * s, S::EPI_WARPS);
     }
     mbar_init(bar_pfull, S::EPI_WARPS * split);
     mbar_init(bar_pempty, S::EPI_WARPS * split);
@@ -178,12 +187,76 @@ gemm128_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
       if (!ok) { *s_abort = 1; fail128(p.status, p.host_word, 502); }
     }
     __syncwarp();
+  } else if (warp == S::SCALER) {
+    // ------------------------------------------------------------ factors of the columns, the row's scale times the weight's
+    // Rows of scales lie [rows, K/128]: a lane walks two of them, eight blocks at a time, and asks for the next eight, of whichever
+    // tile, before it hands over these, so that nobody waits for HBM (one block ahead in the epilogue's registers: 4.6 TB/s).
+    constexpr int G = S::SX_GROUP;
+    float* sx = reinterpret_cast<float*>(sx_all);
+    int slot = 0, tile = group, k = k0;
+    uint32_t phase = 0;
+    bool ok = true;
+    const float *ws = nullptr, *xs0 = nullptr, *xs1 = nullptr;
+    bool in0 = false, in1 = false;
+    auto at_tile = [&] {
+      if (tile >= n_total) return;
+      const FewTile128 t = few_tile128(tile, nw, p.E, segs);
+      ws = p.w_s + ((int64_t)t.e * nw + t.w0 / 128) * nkt;
+      in0 = lane < t.live;
+      in1 = lane + 32 < t.live;
+      xs0 = p.x_s + (int64_t)(t.row0 + (in0 ? lane : 0)) * nkt;
+      xs1 = p.x_s + (int64_t)(t.row0 + (in1 ? lane + 32 : 0)) * nkt;
+    };
+    auto ask = [&](float (&x0)[G], float (&x1)[G]) {          // and steps on
+#pragma unroll
+      for (int i = 0; i < G; ++i) {
+        const int kk = min(k + i, k1 - 1);
+        const float w = ws[kk];
+        x0[i] = in0 ? xs0[kk] * w : 0.f;
+        x1[i] = in1 ? xs1[kk] * w : 0.f;
+      }
+      k += G;
+      if (k >= k1) {
+        k = k0;
+        tile += n_groups;
+        at_tile();
+      }
+    };
+    auto give = [&](const float (&x0)[G], const float (&x1)[G]) {
+      ok = __all_sync(0xffffffffu, mbar_wait(bar_sempty + 8 * slot, phase ^ 1));
+      if (!ok) return;
+      float* to = sx + slot * G * NT;
+#pragma unroll
+      for (int i = 0; i < G; ++i) {
+        to[i * NT + lane] = x0[i];
+        to[i * NT + 32 + lane] = x1[i];
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_sfull + 8 * slot);
+      if (++slot == S::SX_SLOTS) { slot = 0; phase ^= 1; }
+    };
+    at_tile();
+    float a0[G], a1[G], b0[G], b1[G];
+    if (tile < n_total) {
+      ask(a0, a1);
+      while (ok) {
+        const bool more = tile < n_total;
+        if (more) ask(b0, b1);
+        give(a0, a1);
+        if (!more || !ok) break;
+        const bool again = tile < n_total;
+        if (again) ask(a0, a1);
+        give(b0, b1);
+        if (!again) break;
+      }
+    }
+    if (!ok && lane == 0) { *s_abort = 1; fail128(p.status, p.host_word, 504); }
   } else {
     // ------------------------------------------------------------ epilogue: a warp owns 32 weight rows, its TMEM lanes
     const int q = warp & 3;
-    float* sx = reinterpret_cast<float*>(sx_all) + (warp - 2) * 2 * NT;
-    int as = 0;
-    uint32_t aphase = 0, pphase = 0;
+    const float* sx = reinterpret_cast<const float*>(sx_all);
+    int as = 0, slot = 0;
+    uint32_t aphase = 0, pphase = 0, sphase = 0;
     bool ok = true;
     for (int tile = group; tile < n_total && ok; tile += n_groups) {
       const FewTile128 t = few_tile128(tile, nw, p.E, segs);
@@ -191,21 +264,13 @@ gemm128_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
       float acc[NT];
 #pragma unroll
       for (int i = 0; i < NT; ++i) acc[i] = 0.f;
-      const float* ws = p.w_s + ((int64_t)t.e * nw + t.w0 / 128) * nkt;
-      const bool in0 = lane < t.live, in1 = lane + 32 < t.live;
-      const float* xs0 = p.x_s + (int64_t)(t.row0 + (in0 ? lane : 0)) * nkt;
-      const float* xs1 = p.x_s + (int64_t)(t.row0 + (in1 ? lane + 32 : 0)) * nkt;
-      float n0 = xs0[k0] * ws[k0], n1 = xs1[k0] * ws[k0];
       for (int k = k0; k < k1; ++k) {
-        float* sk = sx + (k & 1) * NT;
-        sk[lane] = n0;
-        sk[lane + 32] = n1;
-        __syncwarp();
-        if (k + 1 < k1) {
-          const float w = ws[k + 1];
-          n0 = xs0[k + 1] * w;
-          n1 = xs1[k + 1] * w;
+        const int in_group = (k - k0) % S::SX_GROUP;
+        if (in_group == 0) {
+          ok = __all_sync(0xffffffffu, mbar_wait(bar_sfull + 8 * slot, sphase));
+          if (!ok) break;
         }
+        const float* sk = sx + (slot * S::SX_GROUP + in_group) * NT;
         ok = __all_sync(0xffffffffu, mbar_wait(bar_tfull + 8 * as, aphase));
         if (!ok) break;
         tc_fence_after();
@@ -229,24 +294,39 @@ gemm128_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar_tempty + 8 * as);
+        if (lane == 0) {
+          mbar_arrive(bar_tempty + 8 * as);
+          if (in_group == S::SX_GROUP - 1 || k == k1 - 1) mbar_arrive(bar_sempty + 8 * slot);
+        }
+        if (in_group == S::SX_GROUP - 1 || k == k1 - 1) {
+          if (++slot == S::SX_SLOTS) { slot = 0; sphase ^= 1; }
+        }
         if (++as == S::ACC) { as = 0; aphase ^= 1; }
       }
       if (!ok) break;
       if (split == 1) {
-        if (w_row < p.N) {
-          __nv_bfloat16* dst = p.c + (int64_t)t.row0 * p.N + w_row;
+        // (64 stores under a condition each took longer than three blocks: 3800 clocks for four rows)
+        __nv_bfloat16* dst = p.c + (int64_t)t.row0 * p.N + w_row;
 #pragma unroll
-          for (int i = 0; i < NT; ++i)
-            if (i < t.live) dst[(int64_t)i * p.N] = __float2bfloat16_rn(acc[i]);
+        for (int c = 0; c < NT; c += 16) {
+          if (c >= t.live) break;
+          const int n = w_row < p.N ? t.live - c : 0;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            if (i < n) *dst = __float2bfloat16_rn(acc[c + i]);
+            dst += p.N;
+          }
         }
       } else {
         // everyone has read what this CTA left for the tile before
         ok = __all_sync(0xffffffffu, mbar_wait_cluster(bar_pempty, pphase ^ 1));
         if (!ok) break;
 #pragma unroll
-        for (int i = 0; i < NT; ++i)
-          if (i < t.live) part[i * BM + q * 32 + lane] = acc[i];
+        for (int c = 0; c < NT; c += 16) {
+          if (c >= t.live) break;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) part[(c + i) * BM + q * 32 + lane] = acc[c + i];
+        }
         __syncwarp();
         if (lane < split) mbar_arrive_cluster(map_to_cta(bar_pfull, lane));
         ok = __all_sync(0xffffffffu, mbar_wait_cluster(bar_pfull, pphase));

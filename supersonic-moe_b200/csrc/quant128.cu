@@ -119,6 +119,8 @@ __global__ void __launch_bounds__(256) quant128_rows_kernel(const Rows128Args a)
 // A block holds a tile in registers (eight rows of eight values a thread) and takes from it what is asked for: a scale a row, a
 // scale a column, or one for all.  ROWS and COLS from one read is what a training step needs of an activation and of a
 // gradient: the row form feeds the products over columns, the column form the weight gradient, whose sum runs over rows.
+// The column form leaves transposed: the tensor core reads 8-bit operands whose reduction is not contiguous at half the rate out of
+// shared memory (the weight gradient's MMAs: 950 clocks a block against 650).
 //   efo, counts (column form): rows of a segment behind its live ones count as zero and leave zero; tiles without live rows stay
 //   unwritten
 struct Tile128Args {
@@ -126,18 +128,19 @@ struct Tile128Args {
   int64_t rows;              // of a matrix
   int K, E;                  // columns; segments (or, WEIGHT, matrices)
   const int *efo, *counts;
-  uint8_t *q, *qc;
-  float *s, *sc;
+  uint8_t *q, *qt;           // [rows, K]; [K, rows]
+  float *s, *st;             // [rows, K/128] ([E, rows/128, K/128]); [rows/128, K]
 };
 
 template <bool ROWS, bool COLS, bool WEIGHT>
 __global__ void __launch_bounds__(256) quant128_tile_kernel(const Tile128Args a) {
   __shared__ uint32_t s_max[8][64];                       // per warp: column maxima, two a word
   __shared__ __align__(16) float s_mul[128];
+  __shared__ __align__(16) uint8_t s_t[COLS ? 128 * 128 : 16];      // the transposed tile, 16-byte pieces at places xor (column / 8) % 8
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int kb = (a.K + 127) / 128;
   const int64_t mat = WEIGHT ? blockIdx.z : 0;
-  const int64_t row0 = (int64_t)blockIdx.y * 128;
+  const int64_t row0 = (int64_t)blockIdx.y * 128, my_row = row0 + warp * 16 + (lane >> 4) * 8;
   const int c0 = blockIdx.x * 128, col = c0 + (lane & 15) * 8;
   int64_t end = a.rows;                                   // live rows end here
   if (COLS && a.efo) {
@@ -159,32 +162,28 @@ __global__ void __launch_bounds__(256) quant128_tile_kernel(const Tile128Args a)
   uint4 v[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const int64_t r = row0 + warp * 16 + i * 2 + (lane >> 4);
     v[i] = make_uint4(0, 0, 0, 0);
-    if (in_col && r < a.rows) v[i] = __ldcs((const uint4*)(x + r * a.K + col));
+    if (in_col && my_row + i < a.rows) v[i] = __ldcs((const uint4*)(x + (my_row + i) * a.K + col));
   }
   if (ROWS) {
     const uint32_t half = 0xFFFFu << (lane & 16);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int64_t r = row0 + warp * 16 + i * 2 + (lane >> 4);
       uint32_t m2 = q128_max(q128_max(q128_abs(v[i].x), q128_abs(v[i].y)), q128_max(q128_abs(v[i].z), q128_abs(v[i].w)));
 #pragma unroll
       for (int d = 8; d > 0; d >>= 1) m2 = q128_max(m2, __shfl_xor_sync(half, m2, d));
       const float amax = q128_max_of(m2);
-      if (r < a.rows) {
-        if (in_col) *(uint2*)(a.q + r * q128_pitch(a.K) + col) = q128_pack8(v[i], kE4m3Max / amax);
-        if ((lane & 15) == 0) a.s[r * kb + blockIdx.x] = amax / kE4m3Max;
+      if (my_row + i < a.rows) {
+        if (in_col) *(uint2*)(a.q + (my_row + i) * q128_pitch(a.K) + col) = q128_pack8(v[i], kE4m3Max / amax);
+        if ((lane & 15) == 0) a.s[(my_row + i) * kb + blockIdx.x] = amax / kE4m3Max;
       }
     }
   }
   if (COLS) {
     if (end <= row0) return;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int64_t r = row0 + warp * 16 + i * 2 + (lane >> 4);
-      if (r >= end) v[i] = make_uint4(0, 0, 0, 0);
-    }
+    for (int i = 0; i < 8; ++i)
+      if (my_row + i >= end) v[i] = make_uint4(0, 0, 0, 0);
   }
   if (COLS || WEIGHT) {
     uint32_t m[4] = {0, 0, 0, 0};
@@ -208,17 +207,12 @@ __global__ void __launch_bounds__(256) quant128_tile_kernel(const Tile128Args a)
       if (tid == 0) a.s[(mat * gridDim.y + blockIdx.y) * kb + blockIdx.x] = amax / kE4m3Max;
       uint8_t* q = a.q + mat * a.rows * q128_pitch(a.K);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int64_t r = row0 + warp * 16 + i * 2 + (lane >> 4);
-        if (in_col && r < a.rows) *(uint2*)(q + r * q128_pitch(a.K) + col) = q128_pack8(v[i], mul);
-      }
+      for (int i = 0; i < 8; ++i)
+        if (in_col && my_row + i < a.rows) *(uint2*)(q + (my_row + i) * q128_pitch(a.K) + col) = q128_pack8(v[i], mul);
     } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j) m[j] = q128_max(m[j], __shfl_xor_sync(0xffffffffu, m[j], 16));
-      if (lane < 16) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s_max[warp][lane * 4 + j] = m[j];
-      }
+      if (lane < 16) *(uint4*)&s_max[warp][lane * 4] = make_uint4(m[0], m[1], m[2], m[3]);
       __syncthreads();
       if (tid < 64) {
         uint32_t t = s_max[0][tid];
@@ -228,17 +222,29 @@ __global__ void __launch_bounds__(256) quant128_tile_kernel(const Tile128Args a)
         s_mul[2 * tid] = kE4m3Max / lo;
         s_mul[2 * tid + 1] = kE4m3Max / hi;
         const int c = c0 + 2 * tid;
-        if (c < a.K) *(float2*)(a.sc + (int64_t)blockIdx.y * a.K + c) = make_float2(lo / kE4m3Max, hi / kE4m3Max);
+        if (c < a.K) *(float2*)(a.st + (int64_t)blockIdx.y * a.K + c) = make_float2(lo / kE4m3Max, hi / kE4m3Max);
       }
       __syncthreads();
-      const float4 f0 = *(const float4*)(s_mul + (lane & 15) * 8), f1 = *(const float4*)(s_mul + (lane & 15) * 8 + 4);
+      // eight rows of a column are eight consecutive bytes of the transposed tile
+      const uint32_t* w = (const uint32_t*)v;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int64_t r = row0 + warp * 16 + i * 2 + (lane >> 4);
-        if (!in_col || r >= a.rows) continue;
-        *(uint2*)(a.qc + r * q128_pitch(a.K) + col) =
-            make_uint2(q128_pack4(q128_lo(v[i].x) * f0.x, q128_hi(v[i].x) * f0.y, q128_lo(v[i].y) * f0.z, q128_hi(v[i].y) * f0.w),
-                       q128_pack4(q128_lo(v[i].z) * f1.x, q128_hi(v[i].z) * f1.y, q128_lo(v[i].w) * f1.z, q128_hi(v[i].w) * f1.w));
+      for (int j = 0; j < 8; ++j) {
+        const int c = (lane & 15) * 8 + j;
+        const float f = s_mul[c];
+        float y[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = ((j & 1) ? q128_hi(w[i * 4 + j / 2]) : q128_lo(w[i * 4 + j / 2])) * f;
+        *(uint2*)(s_t + c * 128 + ((warp ^ (lane & 7)) << 4) + (lane >> 4) * 8) =
+            make_uint2(q128_pack4(y[0], y[1], y[2], y[3]), q128_pack4(y[4], y[5], y[6], y[7]));
+      }
+      __syncthreads();
+      const int64_t pitch = q128_pitch(a.rows);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = warp * 16 + i * 4 + (lane >> 3), piece = lane & 7;
+        if (c0 + c < a.K && row0 + piece * 16 < a.rows)
+          *(uint4*)(a.qt + (int64_t)(c0 + c) * pitch + row0 + piece * 16) =
+              *(const uint4*)(s_t + c * 128 + ((piece ^ ((c >> 3) & 7)) << 4));
       }
     }
   }
@@ -287,14 +293,15 @@ int smoe_quant128_rows_scatter(const void* x_bf16, int64_t T, int64_t K, const i
 }
 
 int smoe_quant128_dual(const void* x_bf16, int64_t rows, int64_t K, const int32_t* efo, const int32_t* counts, int64_t E, void* q,
-                       float* scales, void* q_col, float* col_scales, void* stream) {
-  int rc = quant128_check(x_bf16, q_col, col_scales, rows, K);
+                       float* scales, void* q_t, float* t_scales, void* stream) {
+  int rc = quant128_check(x_bf16, q_t, t_scales, rows, K);
   if (!rc && q) rc = quant128_check(x_bf16, q, scales, rows, K);
   if (rc) return rc;
-  if (((uintptr_t)col_scales & 7) || E < 0 || (efo && E <= 0) || (counts && !efo)) return ((uintptr_t)col_scales & 7) ? SMOE_ERR_ALIGN : SMOE_ERR_ARG;
+  if ((uintptr_t)t_scales & 7) return SMOE_ERR_ALIGN;
+  if (E < 0 || (efo && E <= 0) || (counts && !efo)) return SMOE_ERR_ARG;
   if (rows == 0) return SMOE_OK;
   if (rows > (int64_t)65535 * 128) return SMOE_ERR_SHAPE;
-  Tile128Args a{x_bf16, rows, (int)K, (int)E, efo, counts, (uint8_t*)q, (uint8_t*)q_col, scales, col_scales};
+  Tile128Args a{x_bf16, rows, (int)K, (int)E, efo, counts, (uint8_t*)q, (uint8_t*)q_t, scales, t_scales};
   const dim3 grid((unsigned)((K + 127) / 128), (unsigned)((rows + 127) / 128));
   if (q) quant128_tile_kernel<true, true, false><<<grid, 256, 0, (cudaStream_t)stream>>>(a);
   else quant128_tile_kernel<false, true, false><<<grid, 256, 0, (cudaStream_t)stream>>>(a);

@@ -935,18 +935,18 @@ def quant128_rows_scatter(x, naept, s_rev, rows):
 @_timed
 @_on_its_device
 def quant128_dual(x, efo=None, counts=None, with_rows=True):
-    """bf16 [rows,K] -> (row form e4m3 [rows,K], scales [rows,K/128]; both None without `with_rows`; column form e4m3 [rows,K], scales
-    [rows/128,K]) from one read."""
+    """bf16 [rows,K] -> (row form e4m3 [rows,K], scales [rows,K/128]; both None without `with_rows`; column form transposed, e4m3
+    [K,rows], scales [rows/128,K]) from one read."""
     _check_dense("quant128_dual", x, efo, counts)
     _check_bf16(x, 2, x.shape[-1] if x.ndim else 0, "quant128_dual")
     rows, K = x.shape
     E = 1 if efo is None else efo.numel() - 1
     check_segments(efo, counts, E, "quant128_dual")
     q, s = (_payload(x, rows, K), x.new_empty((rows, _blocks128(K)), dtype=torch.float32)) if with_rows else (None, None)
-    qc, sc = _payload(x, rows, K), x.new_empty((_blocks128(rows), K), dtype=torch.float32)
-    check(lib.smoe_quant128_dual(x.data_ptr(), rows, K, _p(efo), _p(counts), E, _p(q), _p(s), qc.data_ptr(), sc.data_ptr(),
+    qt, st = _payload(x, K, rows), x.new_empty((_blocks128(rows), K), dtype=torch.float32)
+    check(lib.smoe_quant128_dual(x.data_ptr(), rows, K, _p(efo), _p(counts), E, _p(q), _p(s), qt.data_ptr(), st.data_ptr(),
                                  _stream()), "quant128_dual")
-    return q, s, qc, sc
+    return q, s, qt, st
 
 
 @_timed
@@ -1017,14 +1017,14 @@ def gemm128_few(a_q, a_s, b_q, b_s, efo=None, counts=None, live_rows=0):
 @_timed
 @_on_its_device
 def gemm128_wgrad(a_q, a_s, b_q, b_s, efo=None, counts=None, out=None, accumulate=False):
-    """a e4m3 [rows,M], b e4m3 [rows,N], both by columns -> bf16 [E,M,N], the products of each segment's live rows; or into `out` f32
+    """a e4m3 [M,rows], b e4m3 [N,rows], the column forms of `quant128_dual` -> bf16 [E,M,N], the products of each segment's live rows; or into `out` f32
     [E,M,N], overwritten or added to."""
-    if a_q.ndim != 2 or b_q.ndim != 2 or a_q.shape[0] != b_q.shape[0]:
-        raise ValueError(f"gemm128_wgrad: a [rows,M] against b [rows,N], got {tuple(a_q.shape)}, {tuple(b_q.shape)}")
+    if a_q.ndim != 2 or b_q.ndim != 2 or a_q.shape[1] != b_q.shape[1]:
+        raise ValueError(f"gemm128_wgrad: a [M,rows] against b [N,rows], got {tuple(a_q.shape)}, {tuple(b_q.shape)}")
     _check_same_gpu("gemm128_wgrad", a_q, a_s, b_q, b_s, efo, counts, out)
     check_payload(a_q, "gemm128_wgrad")
     check_payload(b_q, "gemm128_wgrad")
-    (rows, M), N = a_q.shape, b_q.shape[1]
+    (M, rows), N = a_q.shape, b_q.shape[0]
     E = 1 if efo is None else efo.numel() - 1
     check_segments(efo, counts, E, "gemm128_wgrad")
     rb = _blocks128(rows)

@@ -38,7 +38,7 @@ def spread(*shape, seed=0):
 
 
 def same(q, s, ref):
-    assert torch.equal(q.cpu().view(torch.uint8), ref[0].view(torch.uint8))
+    assert torch.equal(q.cpu().contiguous().view(torch.uint8), ref[0].view(torch.uint8))
     assert torch.equal(s.cpu(), ref[1])
 
 
@@ -59,7 +59,7 @@ def test_quantisers_bit_for_bit(sonicmoe, rows, K):
         same(q, s, O.quant_rows(x))
         q, s, qc, sc = sonicmoe.ops.quant128_dual(x.to(DEV))
         same(q, s, O.quant_rows(x))
-        same(qc, sc, O.quant_cols(x))
+        same(qc.T, sc, O.quant_cols(x))
         w = make(3, rows, K, seed=seed + K)
         q, s = sonicmoe.quantize_weight_block128(w.to(DEV))
         same(q, s, O.quant_weight(w))
@@ -93,7 +93,7 @@ def test_column_form_of_segments(sonicmoe):
     busy = live.view(-1, 128).any(1)
     assert torch.equal(sc.cpu()[busy], ref_s[busy])
     keep = busy.repeat_interleave(128)
-    assert torch.equal(qc.cpu().view(torch.uint8)[keep], ref_q.view(torch.uint8)[keep])
+    assert torch.equal(qc.cpu().T[keep], ref_q.view(torch.uint8)[keep])
     want = O.quant_rows(x[live])
     assert torch.equal(q.cpu()[live].view(torch.uint8), want[0].view(torch.uint8)) and torch.equal(s.cpu()[live], want[1])
 
