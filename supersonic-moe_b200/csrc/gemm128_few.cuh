@@ -29,13 +29,13 @@ struct Few128Smem {
   static constexpr int A_BYTES = BM * BK, B_BYTES = NT * BK;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES, STAGES = 7;
   static constexpr int ACC = 8;                               // TMEM buffers
-  static constexpr int EPI_WARPS = 4;
+  static constexpr int EPI_WARPS = 4, EPI_SETS = 2;           // sets take turns by tile: one writes while the other reads sums
   static constexpr int PART_BYTES = NT * BM * 4;              // sums of this CTA: [column][weight row]
   static constexpr int SX_GROUP = 8;                          // blocks whose factors travel together
   static constexpr int SX_SLOTS = 4, SX_BYTES = SX_SLOTS * SX_GROUP * NT * 4;
   static constexpr int AUX_BYTES = kFewBars + 16 + 3 * (kG128Segs + 1) * 4;
   static constexpr int TOTAL = 1024 + STAGES * STAGE_BYTES + PART_BYTES + SX_BYTES + AUX_BYTES;
-  static constexpr int SCALER = 2 + EPI_WARPS;                // warp
+  static constexpr int SCALER = 2 + EPI_WARPS * EPI_SETS;                // warp
   static constexpr int THREADS = 32 * (SCALER + 1);
   static_assert(TOTAL <= 227 * 1024, "shared memory budget");
   static_assert((2 * STAGES + 2 * ACC + 2 + 2 * SX_SLOTS) * 8 <= kFewBars, "barrier storage");
@@ -136,6 +136,10 @@ gemm128_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
   const int nw = (p.N + BM - 1) / BM, nkt = (p.K + 127) / 128;
   const int n_total = segs.tiles[p.E] * nw;
   const int k0 = rank * nkt / split, k1 = (rank + 1) * nkt / split;        // split <= nkt: nobody is without
+  // Each set of epilogue warps has buffers and slots of its own, and meets every use of them in order: a wait by parity cannot
+  // tell a phase from the one after next.  CTAs that share a tile have few of them and use one set.
+  const int sets = split > 1 ? 1 : S::EPI_SETS, bufs = S::ACC / sets, slots = S::SX_SLOTS / sets;
+  const int blocks = k1 - k0, groups = (blocks + S::SX_GROUP - 1) / S::SX_GROUP;
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
@@ -164,13 +168,15 @@ gemm128_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
     if (elect_one()) {
-      int stage = 0, as = 0;
-      uint32_t phase = 0, aphase = 0;
+      int stage = 0, turn = 0;
+      uint32_t phase = 0;
       bool ok = true;
-      for (int tile = group; tile < n_total && ok; tile += n_groups) {
+      for (int tile = group; tile < n_total && ok; tile += n_groups, ++turn) {
         const FewTile128 t = few_tile128(tile, nw, p.E, segs);
+        const uint32_t use0 = (uint32_t)(turn / sets) * blocks;
         const uint32_t idesc = make_idesc_f8(BM, (t.live + 15) / 16 * 16, false, false);
         for (int k = k0; k < k1; ++k) {
+          const uint32_t use = use0 + (k - k0), as = turn % sets * bufs + use % bufs, aphase = use / bufs & 1;
           ok = mbar_wait(bar_tempty + 8 * as, aphase ^ 1) && mbar_wait(bar_full + 8 * stage, phase);
           if (!ok) break;
           tc_fence_after();
@@ -181,7 +187,6 @@ gemm128_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
           tc_commit(bar_empty + 8 * stage);
           tc_commit(bar_tfull + 8 * as);
           if (++stage == S::STAGES) { stage = 0; phase ^= 1; }
-          if (++as == S::ACC) { as = 0; aphase ^= 1; }
         }
       }
       if (!ok) { *s_abort = 1; fail128(p.status, p.host_word, 502); }
@@ -193,8 +198,8 @@ gemm128_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
     // tile, before it hands over these, so that nobody waits for HBM (one block ahead in the epilogue's registers: 4.6 TB/s).
     constexpr int G = S::SX_GROUP;
     float* sx = reinterpret_cast<float*>(sx_all);
-    int slot = 0, tile = group, k = k0;
-    uint32_t phase = 0;
+    int tile = group, k = k0;
+    uint32_t given = 0;                                       // groups handed over
     bool ok = true;
     const float *ws = nullptr, *xs0 = nullptr, *xs1 = nullptr;
     bool in0 = false, in1 = false;
@@ -223,7 +228,9 @@ gemm128_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
       }
     };
     auto give = [&](const float (&x0)[G], const float (&x1)[G]) {
-      ok = __all_sync(0xffffffffu, mbar_wait(bar_sempty + 8 * slot, phase ^ 1));
+      const uint32_t turn = given / groups, use = turn / sets * groups + given % groups;
+      const uint32_t slot = turn % sets * slots + use % slots;
+      ok = __all_sync(0xffffffffu, mbar_wait(bar_sempty + 8 * slot, (use / slots & 1) ^ 1));
       if (!ok) return;
       float* to = sx + slot * G * NT;
 #pragma unroll
@@ -233,7 +240,7 @@ gemm128_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(bar_sfull + 8 * slot);
-      if (++slot == S::SX_SLOTS) { slot = 0; phase ^= 1; }
+      ++given;
     };
     at_tile();
     float a0[G], a1[G], b0[G], b1[G];
@@ -253,12 +260,12 @@ gemm128_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
     if (!ok && lane == 0) { *s_abort = 1; fail128(p.status, p.host_word, 504); }
   } else {
     // ------------------------------------------------------------ epilogue: a warp owns 32 weight rows, its TMEM lanes
-    const int q = warp & 3;
+    const int q = warp & 3, set = (warp - 2) / S::EPI_WARPS;
     const float* sx = reinterpret_cast<const float*>(sx_all);
-    int as = 0, slot = 0;
-    uint32_t aphase = 0, pphase = 0, sphase = 0;
     bool ok = true;
-    for (int tile = group; tile < n_total && ok; tile += n_groups) {
+    int as = 0, slot = 0;                                     // of this set's
+    uint32_t aphase = 0, sphase = 0, pphase = 0;
+    for (int tile = set < sets ? group + set * n_groups : n_total; tile < n_total && ok; tile += sets * n_groups) {
       const FewTile128 t = few_tile128(tile, nw, p.E, segs);
       const int w_row = t.w0 + q * 32 + lane;
       float acc[NT];
@@ -267,14 +274,14 @@ gemm128_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
       for (int k = k0; k < k1; ++k) {
         const int in_group = (k - k0) % S::SX_GROUP;
         if (in_group == 0) {
-          ok = __all_sync(0xffffffffu, mbar_wait(bar_sfull + 8 * slot, sphase));
+          ok = __all_sync(0xffffffffu, mbar_wait(bar_sfull + 8 * (set * slots + slot), sphase));
           if (!ok) break;
         }
-        const float* sk = sx + (slot * S::SX_GROUP + in_group) * NT;
-        ok = __all_sync(0xffffffffu, mbar_wait(bar_tfull + 8 * as, aphase));
+        const float* sk = sx + ((set * slots + slot) * S::SX_GROUP + in_group) * NT;
+        ok = __all_sync(0xffffffffu, mbar_wait(bar_tfull + 8 * (set * bufs + as), aphase));
         if (!ok) break;
         tc_fence_after();
-        const uint32_t src = tmem_base + ((uint32_t)(q * 32) << 16) + as * NT;
+        const uint32_t src = tmem_base + ((uint32_t)(q * 32) << 16) + (set * bufs + as) * NT;
 #pragma unroll
         for (int c = 0; c < NT / 16; ++c) {
           if (c * 16 < t.live) {
@@ -295,13 +302,13 @@ gemm128_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
         tc_fence_before();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(bar_tempty + 8 * as);
-          if (in_group == S::SX_GROUP - 1 || k == k1 - 1) mbar_arrive(bar_sempty + 8 * slot);
+          mbar_arrive(bar_tempty + 8 * (set * bufs + as));
+          if (in_group == S::SX_GROUP - 1 || k == k1 - 1) mbar_arrive(bar_sempty + 8 * (set * slots + slot));
         }
         if (in_group == S::SX_GROUP - 1 || k == k1 - 1) {
-          if (++slot == S::SX_SLOTS) { slot = 0; sphase ^= 1; }
+          if (++slot == slots) { slot = 0; sphase ^= 1; }
         }
-        if (++as == S::ACC) { as = 0; aphase ^= 1; }
+        if (++as == bufs) { as = 0; aphase ^= 1; }
       }
       if (!ok) break;
       if (split == 1) {
