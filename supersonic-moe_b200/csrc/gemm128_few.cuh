@@ -339,10 +339,18 @@ gemm128_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
         ok = __all_sync(0xffffffffu, mbar_wait_cluster(bar_pfull, pphase));
         if (!ok) break;
         const uint32_t mine = smem_u32(part + q * 32 + lane);
-        for (int i = rank; i < t.live; i += split) {
-          float v = 0.f;
-          for (int r = 0; r < split; ++r) v += ld_cluster_f32(map_to_cta(mine + i * BM * 4, r));
-          if (w_row < p.N) p.c[(int64_t)(t.row0 + i) * p.N + w_row] = __float2bfloat16_rn(v);
+        for (int i = rank; i < t.live; i += 4 * split) {      // four rows' sums on their way at a time
+          float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+          for (int r = 0; r < split; ++r) {
+            const uint32_t from = map_to_cta(mine, r);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (i + j * split < t.live) v[j] += ld_cluster_f32(from + (i + j * split) * BM * 4);
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (i + j * split < t.live && w_row < p.N) p.c[(int64_t)(t.row0 + i + j * split) * p.N + w_row] = __float2bfloat16_rn(v[j]);
         }
         __syncwarp();
         if (lane < split) mbar_arrive_cluster(map_to_cta(bar_pempty, lane));

@@ -39,8 +39,47 @@ __device__ __forceinline__ uint2 q128_pack8(const uint4& v, float m) {
                     q128_pack4(q128_lo(v.z) * m, q128_hi(v.z) * m, q128_lo(v.w) * m, q128_hi(v.w) * m));
 }
 
+__device__ __forceinline__ float q128_silu(float g) {       // to some 1e-7 and |g| roundings of the exponent
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(-1.4426950408889634f * g));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+  return g * r;
+}
+// largest magnitude of eight bf16, in both halves
+__device__ __forceinline__ uint32_t q128_max4(const uint4& v) {
+  const uint32_t m = q128_max(q128_max(q128_abs(v.x), q128_abs(v.y)), q128_max(q128_abs(v.z), q128_abs(v.w)));
+  return q128_max(m, __byte_perm(m, m, 0x1032));
+}
+// over sixteen lanes, for N blocks, two to a word
+template <int N>
+__device__ __forceinline__ void q128_max16(const uint32_t (&m)[N], uint32_t half, float (&amax)[N]) {
+#pragma unroll
+  for (int j = 0; j < N; j += 2) {
+    uint32_t two = j + 1 < N ? __byte_perm(m[j], m[j + 1 < N ? j + 1 : j], 0x5410) : m[j];
+#pragma unroll
+    for (int d = 8; d > 0; d >>= 1) two = q128_max(two, __shfl_xor_sync(half, two, d));
+    amax[j] = q128_lo(two);
+    if (j + 1 < N) amax[j + 1 < N ? j + 1 : j] = q128_hi(two);
+  }
+}
+// What N <= 8 blocks of sixteen lanes are multiplied by, from their maxima; returns, in lane 8 + j, block j's scale.  A division takes
+// as many instructions as the rest of a block: each lane does one, of either kind, instead of all.
+template <int N>
+__device__ __forceinline__ float q128_quotients(const float (&amax)[N], int lane16, uint32_t half, float (&inv)[N]) {
+  float a = amax[0];
+#pragma unroll
+  for (int j = 1; j < N; ++j) a = (lane16 & 7) == j ? amax[j] : a;
+  a = fmaxf(a, kAmaxFloor);
+  const bool scale = lane16 >= 8;
+  const float r = (scale ? a : kE4m3Max) / (scale ? kE4m3Max : a);
+#pragma unroll
+  for (int j = 0; j < N; ++j) inv[j] = __shfl_sync(half, r, j, 16);
+  return r;
+}
+
 // ---- rows -------------------------------------------------------------------------------------------------------------
-// Sixteen lanes take a block of 128 values, eight each (with GLU: of gate and up, interleaved, 32 bytes a lane).  Which rows:
+// Sixteen lanes take a block of 128 values, eight each (with GLU: of gate and up, interleaved, 32 bytes a lane), and blocks
+// that follow one another: all their loads are on their way before the first is looked at.  Which rows:
 //   list == null, naept == null   row i -> row i, i < n
 //   list                          row list[i] -> row list[i], i < min(n, *n_live)
 //   naept                         row i -> rows s_rev[naept[i]] .. s_rev[naept[i+1] - 1], i < n: a token's places
@@ -54,63 +93,88 @@ struct Rows128Args {
   float* s;
 };
 
-template <bool GLU>
-__global__ void __launch_bounds__(256) quant128_rows_kernel(const Rows128Args a) {
+template <bool GLU, int PER>
+__global__ void __launch_bounds__(256, PER == 4 ? 4 : 6) quant128_rows_kernel(const Rows128Args a) {
   const int kb = (a.K + 127) / 128;
-  const int64_t units = (a.list && a.n_live ? min((int64_t)*a.n_live, a.n) : a.n) * kb;
+  const int64_t n = a.list && a.n_live ? min((int64_t)*a.n_live, a.n) : a.n;
   const int lane16 = threadIdx.x & 15;
   const uint32_t half = 0xFFFFu << (threadIdx.x & 16);
-  for (int64_t u = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> 4; u < units; u += ((int64_t)gridDim.x * blockDim.x) >> 4) {
-    const int64_t i = u / kb;
-    const int b = (int)(u - i * kb);
-    const int64_t src = a.list ? a.list[i] : i;
+  const uint64_t u0 = ((blockIdx.x * (uint64_t)blockDim.x + threadIdx.x) >> 4) * PER;
+  // (a 32-bit quotient wherever it holds: the 64-bit one takes longer than a block's arithmetic)
+  int64_t i = u0 >> 32 ? (int64_t)(u0 / kb) : (int64_t)((uint32_t)u0 / (uint32_t)kb);
+  int b = (int)(u0 - (uint64_t)i * kb);
+  uint4 v[PER][GLU ? 2 : 1];
+  int64_t src[PER];
+  int blk[PER];
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    src[j] = i < n ? (a.list ? (int64_t)a.list[i] : i) : -1;
+    if (a.list && (src[j] < 0 || src[j] >= a.out_rows)) src[j] = -1;
+    blk[j] = b;
     const int col = b * 128 + lane16 * 8;
-    // K % 8 == 0: a lane's eight values are there or not
-    const bool in = col < a.K && (!a.list || (src >= 0 && src < a.out_rows));
-    uint2 out;
-    float amax;
-    if (GLU) {
-      float y[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] = 0.f;
-      if (in) {
-        const uint4* p = (const uint4*)((const uint16_t*)a.x + (src * a.K + col) * 2);
-        const uint4 v[2] = {p[0], p[1]};
-        const uint32_t* w = (const uint32_t*)v;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float g = q128_lo(w[j]), up = q128_hi(w[j]);
-          y[j] = g / (1.f + expf(-g)) * up;
-        }
+    v[j][0] = make_uint4(0, 0, 0, 0);
+    if (GLU) v[j][GLU ? 1 : 0] = make_uint4(0, 0, 0, 0);
+    if (src[j] >= 0 && col < a.K) {                       // K % 8 == 0: a lane's eight values are there or not
+      if (GLU) {
+        const uint4* p = (const uint4*)((const uint16_t*)a.x + (src[j] * a.K + col) * 2);
+        v[j][0] = __ldcs(p);
+        v[j][GLU ? 1 : 0] = __ldcs(p + 1);
+      } else {
+        v[j][0] = __ldcs((const uint4*)((const uint16_t*)a.x + src[j] * a.K + col));
       }
-      amax = kAmaxFloor;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(y[j]));
-#pragma unroll
-      for (int d = 8; d > 0; d >>= 1) amax = fmaxf(amax, __shfl_xor_sync(half, amax, d));
-      const float m = kE4m3Max / amax;
-      out = make_uint2(q128_pack4(y[0] * m, y[1] * m, y[2] * m, y[3] * m), q128_pack4(y[4] * m, y[5] * m, y[6] * m, y[7] * m));
-    } else {
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (in) v = *(const uint4*)((const uint16_t*)a.x + src * a.K + col);
-      uint32_t m2 = q128_max(q128_max(q128_abs(v.x), q128_abs(v.y)), q128_max(q128_abs(v.z), q128_abs(v.w)));
-#pragma unroll
-      for (int d = 8; d > 0; d >>= 1) m2 = q128_max(m2, __shfl_xor_sync(half, m2, d));
-      amax = q128_max_of(m2);
-      out = q128_pack8(v, kE4m3Max / amax);
     }
-    const float scale = amax / kE4m3Max;
-    if (a.naept) {
-      const int last = a.naept[i + 1];
-      for (int j = a.naept[i]; j < last; ++j) {
-        const int64_t dst = a.s_rev[j];
-        if (dst < 0 || dst >= a.out_rows) continue;
-        if (in) *(uint2*)(a.q + dst * q128_pitch(a.K) + col) = out;
-        if (lane16 == 0) a.s[dst * kb + b] = scale;
+    if (++b == kb) {
+      b = 0;
+      ++i;
+    }
+  }
+  float y[GLU ? PER : 1][8], amax[PER];
+  if (GLU) {
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const uint32_t* w = (const uint32_t*)v[j];
+      amax[j] = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        y[GLU ? j : 0][e] = q128_silu(q128_lo(w[e])) * q128_hi(w[e]);
+        amax[j] = fmaxf(amax[j], fabsf(y[GLU ? j : 0][e]));
       }
-    } else if (src >= 0 && src < a.out_rows) {
-      if (in) *(uint2*)(a.q + src * q128_pitch(a.K) + col) = out;
-      if (lane16 == 0) a.s[src * kb + b] = scale;
+#pragma unroll
+      for (int d = 8; d > 0; d >>= 1) amax[j] = fmaxf(amax[j], __shfl_xor_sync(half, amax[j], d));
+    }
+  } else {
+    uint32_t m[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) m[j] = q128_max4(v[j][0]);
+    q128_max16<PER>(m, half, amax);
+  }
+  float inv[PER];
+  const float scale = q128_quotients<PER>(amax, lane16, half, inv);
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const int64_t pitch = q128_pitch(a.K);
+    const int col = blk[j] * 128 + lane16 * 8;
+    const bool in = col < a.K, mine = lane16 == 8 + j;        // the lane that has this block's scale
+    if (src[j] < 0) continue;
+    uint2 out;
+    if (GLU) {
+      const float* f = y[GLU ? j : 0];
+      out = make_uint2(q128_pack4(f[0] * inv[j], f[1] * inv[j], f[2] * inv[j], f[3] * inv[j]),
+                       q128_pack4(f[4] * inv[j], f[5] * inv[j], f[6] * inv[j], f[7] * inv[j]));
+    } else {
+      out = q128_pack8(v[j][0], inv[j]);
+    }
+    if (a.naept) {
+      const int last = a.naept[src[j] + 1];
+      for (int t = a.naept[src[j]]; t < last; ++t) {
+        const int64_t dst = a.s_rev[t];
+        if (dst < 0 || dst >= a.out_rows) continue;
+        if (in) *(uint2*)(a.q + dst * pitch + col) = out;
+        if (mine) a.s[dst * kb + blk[j]] = scale;
+      }
+    } else {
+      if (in) *(uint2*)(a.q + src[j] * pitch + col) = out;
+      if (mine) a.s[src[j] * kb + blk[j]] = scale;
     }
   }
 }
@@ -167,17 +231,16 @@ __global__ void __launch_bounds__(256) quant128_tile_kernel(const Tile128Args a)
   }
   if (ROWS) {
     const uint32_t half = 0xFFFFu << (lane & 16);
+    uint32_t m[8];
+    float amax[8], inv[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      uint32_t m2 = q128_max(q128_max(q128_abs(v[i].x), q128_abs(v[i].y)), q128_max(q128_abs(v[i].z), q128_abs(v[i].w)));
+    for (int i = 0; i < 8; ++i) m[i] = q128_max4(v[i]);
+    q128_max16<8>(m, half, amax);
+    const float scale = q128_quotients<8>(amax, lane & 15, half, inv);
+    if ((lane & 8) && my_row + (lane & 7) < a.rows) a.s[(my_row + (lane & 7)) * kb + blockIdx.x] = scale;
 #pragma unroll
-      for (int d = 8; d > 0; d >>= 1) m2 = q128_max(m2, __shfl_xor_sync(half, m2, d));
-      const float amax = q128_max_of(m2);
-      if (my_row + i < a.rows) {
-        if (in_col) *(uint2*)(a.q + (my_row + i) * q128_pitch(a.K) + col) = q128_pack8(v[i], kE4m3Max / amax);
-        if ((lane & 15) == 0) a.s[(my_row + i) * kb + blockIdx.x] = amax / kE4m3Max;
-      }
-    }
+    for (int i = 0; i < 8; ++i)
+      if (in_col && my_row + i < a.rows) *(uint2*)(a.q + (my_row + i) * q128_pitch(a.K) + col) = q128_pack8(v[i], inv[i]);
   }
   if (COLS) {
     if (end <= row0) return;
@@ -260,9 +323,16 @@ static int quant128_check(const void* x, const void* q, const void* s, int64_t r
 static int launch_rows(const Rows128Args& a, bool glu, void* stream) {
   if (a.n == 0 || a.out_rows == 0) return SMOE_OK;
   const int64_t units = a.n * ((a.K + 127) / 128);
-  int64_t grid = (units + 15) / 16;
-  if (grid > 148 * 32) grid = 148 * 32;
-  auto kern = glu ? quant128_rows_kernel<true> : quant128_rows_kernel<false>;
+  // Several blocks each where that leaves every SM enough warps: four, or two where the activation's or a token's many rows need
+  // the registers.  8192 x 4096 one block 28.0 us, two 24.2, four 22.7; gated 32768 x 768 40, 25.2, 26.5; eight places a token 18.6,
+  // 18.4, 19.9.
+  const int most = glu || a.naept ? 2 : 4, per = units >= 148 * 64 * 4 ? most : 1;
+  const int64_t grid = (units + 16 * per - 1) / (16 * per);
+  if (grid >= (int64_t)1 << 31) return SMOE_ERR_SHAPE;
+  auto kern = glu        ? (per == 2 ? quant128_rows_kernel<true, 2> : quant128_rows_kernel<true, 1>)
+              : per == 4 ? quant128_rows_kernel<false, 4>
+              : per == 2 ? quant128_rows_kernel<false, 2>
+                         : quant128_rows_kernel<false, 1>;
   kern<<<(unsigned)grid, 256, 0, (cudaStream_t)stream>>>(a);
   return cudaGetLastError() == cudaSuccess ? SMOE_OK : SMOE_ERR_LAUNCH;
 }
