@@ -42,15 +42,19 @@ __device__ __forceinline__ void fail128(int* status, volatile int* host_word, in
 
 constexpr int kG128Segs = kMaxExperts2 + 1;        // the rows behind the last segment are one more
 
+constexpr int kG128N = 256;        // columns of a tile (128 with four buffers, weight gradient: 204 -> 259 us, more to do per block)
+
 struct Gemm128Smem {
-  static constexpr int A_BYTES = BM * BK, B_BYTES = 128 * BK;
+  static constexpr int BN = kG128N;
+  static constexpr int A_BYTES = BM * BK, B_BYTES = BN / 2 * BK;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES, STAGES = 5;
+  static constexpr int BUFS = 512 / BN;                     // TMEM buffers
   static constexpr int EPI_WARPS = 8;
   static constexpr int STG_TILE = 2048, STG_TILES = 3;      // output staging of a warp: 32 rows x 64 bytes
   static constexpr int STG_BYTES = STG_TILES * STG_TILE;
   // WGRAD128: scales of this CTA's 128 rows and of the 256 columns in a block, in a ring of their own, filled by a warp of its own:
   // every block reads new lines of them, and a register's worth of look-ahead does not cover HBM (measured: 1650 clocks a block)
-  static constexpr int SC_BYTES = (128 + 256) * 4, SC_SLOTS = 6;
+  static constexpr int SC_BYTES = (128 + BN) * 4, SC_SLOTS = 8;
   static constexpr int AUX_BYTES = 512 + 4 * (kG128Segs + 1) * 4;
   static constexpr int TOTAL = 1024 + STAGES * STAGE_BYTES + EPI_WARPS * STG_BYTES + SC_SLOTS * SC_BYTES + AUX_BYTES;
   // Two warpgroups of epilogue warps and one with the producer and the MMA issuer.  A thread of the former needs more than the 168
@@ -58,7 +62,7 @@ struct Gemm128Smem {
   static constexpr int THREADS = 32 * (EPI_WARPS + 4), EPI_REGS = 224, OTHER_REGS = 56;
   static constexpr uint32_t TX_BYTES = 2u * STAGE_BYTES;
   static_assert(TOTAL <= 227 * 1024, "shared memory budget");
-  static_assert((2 * STAGES + 4 + 2 * SC_SLOTS) * 8 <= 496, "barrier storage");
+  static_assert((2 * STAGES + 2 * BUFS + 2 * SC_SLOTS) * 8 <= 496, "barrier storage");
 };
 
 // tcgen05.mma kind::f8f6f4: e4m3 x e4m3 -> f32
@@ -165,19 +169,20 @@ struct Tile128 {
 template <int MODE>
 __device__ __forceinline__ Tile128 tile128(int tile, int rank, const Gemm128Params& p, const Segs128& s) {
   Tile128 t;
-  const int nt = (p.N + 255) / 256;
+  constexpr int BN = kG128N;
+  const int nt = (p.N + BN - 1) / BN;
   if (MODE == WGRAD128) {
     const int mt = (p.M + 255) / 256, per = mt * nt;
     t.e = tile / per;
     const int r = tile - t.e * per;
     t.m0 = (r / nt) * 256 + rank * 128;
-    t.n0 = (r % nt) * 256;
+    t.n0 = (r % nt) * BN;
     t.t0 = s.start[t.e] & ~127;          // segments start there; a copy has to start on 16 bytes in any case
     t.nkt = (s.live[t.e] - s.start[t.e] + 127) / 128;
     t.live = t.end = p.M;
   } else {
     const int pr = tile / nt;
-    t.n0 = (tile - pr * nt) * 256;
+    t.n0 = (tile - pr * nt) * BN;
     t.e = seg_of_tile(s.tiles, p.E + 1, pr);
     const int first = s.start[t.e] + (pr - s.tiles[t.e]) * 256;
     t.m0 = first + rank * 128;
@@ -228,12 +233,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Gemm128Smem::THREADS
 gemm128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                const __grid_constant__ CUtensorMap tmap_c, const Gemm128Params p) {
   using S = Gemm128Smem;
+  constexpr int BN = kG128N;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* epi = smem + S::STAGES * S::STAGE_BYTES;
   uint8_t* scales = epi + S::EPI_WARPS * S::STG_BYTES;
   uint8_t* aux = scales + S::SC_SLOTS * S::SC_BYTES;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(aux);            // full[S], empty[S], tfull[2], tempty[2], scfull[], scempty[]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(aux);            // full[S], empty[S], tfull[BUFS], tempty[BUFS], scfull[], scempty[]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(aux + 496);
   volatile int* s_abort = reinterpret_cast<volatile int*>(aux + 500);
   Segs128 segs;
@@ -245,8 +251,8 @@ gemm128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
   const uint32_t rank = cluster_ctarank();
   const int pair_id = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
   const uint32_t bar_full = smem_u32(bars), bar_empty = bar_full + 8 * S::STAGES;
-  const uint32_t bar_tfull = bar_empty + 8 * S::STAGES, bar_tempty = bar_tfull + 16;
-  const uint32_t bar_scfull = bar_tempty + 16, bar_scempty = bar_scfull + 8 * S::SC_SLOTS;
+  const uint32_t bar_tfull = bar_empty + 8 * S::STAGES, bar_tempty = bar_tfull + 8 * S::BUFS;
+  const uint32_t bar_scfull = bar_tempty + 8 * S::BUFS, bar_scempty = bar_scfull + 8 * S::SC_SLOTS;
 
   constexpr int PRODUCER = S::EPI_WARPS, ISSUER = S::EPI_WARPS + 1, SCALER = S::EPI_WARPS + 2;
   if (warp == 2) load_segs128(segs, p.efo, p.counts, p.E, p.rows, 256, false, lane);
@@ -255,7 +261,7 @@ gemm128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
       mbar_init(bar_full + 8 * s, 1);                     // leader's: its producer arms it, both CTAs' copies credit it
       mbar_init(bar_empty + 8 * s, 1);                    // one commit arrival per use, in each CTA
     }
-    for (int s = 0; s < 2; ++s) {
+    for (int s = 0; s < S::BUFS; ++s) {
       mbar_init(bar_tfull + 8 * s, 1);                    // commit arrival, in each CTA
       mbar_init(bar_tempty + 8 * s, 2 * S::EPI_WARPS);    // leader's: the epilogue warps of both CTAs
     }
@@ -277,7 +283,7 @@ gemm128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   const uint32_t smem_base = smem_u32(smem);
-  const int nt = (p.N + 255) / 256;
+  const int nt = (p.N + BN - 1) / BN;
   const int n_total = MODE == WGRAD128 ? p.E * ((p.M + 255) / 256) * nt : segs.tiles[p.E + 1] * nt;
 
   if (warp >= S::EPI_WARPS) {
@@ -292,7 +298,7 @@ gemm128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
     for (int tile = pair_id; tile < n_total && ok; tile += n_pairs) {
       const Tile128 t = tile128<MODE>(tile, rank, p, segs);
       const int nkt = __shfl_sync(0xffffffffu, t.nkt, 0), m0 = __shfl_sync(0xffffffffu, t.m0, 0);
-      const int n_row = __shfl_sync(0xffffffffu, t.n0, 0) + (int)rank * 128;
+      const int n_row = __shfl_sync(0xffffffffu, t.n0, 0) + (int)rank * (BN / 2);
       const int e = MODE == WGRAD128 ? 0 : __shfl_sync(0xffffffffu, t.e, 0), t0 = __shfl_sync(0xffffffffu, t.t0, 0);
       for (int k = 0; k < nkt; ++k) {
         ok = __all_sync(0xffffffffu, mbar_wait(bar_empty + 8 * stage, phase ^ 1));
@@ -313,7 +319,7 @@ gemm128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
     // ------------------------------------------------------------ MMA issuer (leader CTA only)
     if (rank == 0) {
       const bool b_mn = MODE == ROWS128 && p.b_mn;
-      const uint32_t idesc = make_idesc_f8(256, 256, false, b_mn);
+      const uint32_t idesc = make_idesc_f8(256, BN, false, b_mn);
       // operand descriptors: see make_desc_kmajor_sw128 / make_desc_mnmajor_sw128; a step of 32 along the reduction is 32 bytes
       // (K-major) or 32 rows of 128 bytes
       const uint32_t desc_hi = (1024u >> 4) | (1u << 14) | (2u << 29);
@@ -337,12 +343,12 @@ gemm128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
           if (elect_one()) {
 #pragma unroll
             for (int kb = 0; kb < BK / 32; ++kb)
-              mma_f8_pair_lo(tmem_base + as * 256, a_lo + 2 * kb, b_lo + b_step * kb, desc_hi, idesc, kb != 0);
+              mma_f8_pair_lo(tmem_base + as * BN, a_lo + 2 * kb, b_lo + b_step * kb, desc_hi, idesc, kb != 0);
             tc_commit_pair(bar_empty + 8 * stage, 3);
             tc_commit_pair(bar_tfull + 8 * as, 3);
           }
           if (++stage == S::STAGES) { stage = 0; phase ^= 1; }
-          if (++as == 2) { as = 0; aphase ^= 1; }
+          if (++as == S::BUFS) { as = 0; aphase ^= 1; }
         }
       }
       if (!ok && lane == 0) { *s_abort = 1; fail128(p.status, p.host_word, 402); }
@@ -356,7 +362,7 @@ gemm128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
       bool ok = true;
       for (int tile = pair_id; tile < n_total && ok; tile += n_pairs) {
         const Tile128 t = tile128<MODE>(tile, rank, p, segs);
-        const uint32_t a_bytes = max(min(128, p.M - t.m0), 0) * 4, b_bytes = min(256, p.N - t.n0) * 4;      // multiples of 32
+        const uint32_t a_bytes = max(min(128, p.M - t.m0), 0) * 4, b_bytes = min(BN, p.N - t.n0) * 4;      // multiples of 32
         for (int k = 0; k < t.nkt; ++k) {
           ok = mbar_wait(bar_scempty + 8 * slot, phase ^ 1);
           if (!ok) break;
@@ -412,22 +418,25 @@ gemm128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
       if (MODE == ROWS128 && t.nkt > 0) {
         const int row = t.m0 + q * 32 + lane;
         sa = p.a_s + (int64_t)(row < t.live ? row : 0) * p.a_kb;
-        sb = p.b_s + t.e * p.bs_e + (int64_t)min(t.n0 / 128 + half, (p.N - 1) / 128) * p.bs_n;
+        sb = p.b_s + t.e * p.bs_e + (int64_t)min((t.n0 + half * (BN / 2)) / 128, (p.N - 1) / 128) * p.bs_n;
         sa_next = *sa;
         sb_next = *sb;
       }
     };
     if (pair_id < n_total) begin(pair_id);
     for (int tile = pair_id; tile < n_total; tile += n_pairs) {
-      float acc[MODE == ROWS128 ? 128 : 1];               // [column]
-      F2 acc2[MODE == WGRAD128 ? 64 : 1];                 // [32 columns][16 rows][8 columns][row r4, row r4 + 8]: two columns
+      float acc[MODE == ROWS128 ? BN / 2 : 1];               // [column]
+      F2 acc2[MODE == WGRAD128 ? BN / 4 : 1];                 // [32 columns][16 rows][8 columns][row r4, row r4 + 8]: two columns
 #pragma unroll
-      for (int i = 0; i < (MODE == ROWS128 ? 128 : 0); ++i) acc[i] = 0.f;
+      for (int i = 0; i < (MODE == ROWS128 ? BN / 2 : 0); ++i) acc[i] = 0.f;
 #pragma unroll
-      for (int i = 0; i < (MODE == WGRAD128 ? 64 : 0); ++i) acc2[i] = f2(0.f, 0.f);
+      for (int i = 0; i < (MODE == WGRAD128 ? BN / 4 : 0); ++i) acc2[i] = f2(0.f, 0.f);
       const int r4 = lane >> 2, c2 = (lane & 3) * 2;
+      float fa[4];                                        // WGRAD128: scales of the rows r4 + 8 j; of two columns each
+      F2 s2[2][4];
+      bool have_scales = false, have_sums = false;
       for (int k = 0; k < t.nkt; ++k) {
-        const uint32_t src = tmem_base + ((uint32_t)(q * 32) << 16) + as * 256 + half * 128;
+        const uint32_t src = tmem_base + ((uint32_t)(q * 32) << 16) + as * BN + half * (BN / 2);
         if (MODE == ROWS128) {
           // A lane is a row, a register a column: one factor a thread and block, the row's scale times the weight's.
           const float f = sa_next * sb_next;
@@ -442,10 +451,10 @@ gemm128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
           uint32_t r[2][16];
           tmem_ld16(src, r[0]);
 #pragma unroll
-          for (int c = 0; c < 8; ++c) {
+          for (int c = 0; c < BN / 32; ++c) {
             tmem_ld_wait();
             tmem_arrived(r[c & 1]);
-            if (c < 7) tmem_ld16(src + (c + 1) * 16, r[(c + 1) & 1]);
+            if (c < BN / 32 - 1) tmem_ld16(src + (c + 1) * 16, r[(c + 1) & 1]);
             else release();
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc[c * 16 + i] = fmaf(__uint_as_float(r[c & 1][i]), f, acc[c * 16 + i]);
@@ -455,36 +464,49 @@ gemm128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
           // would read the scales of all 128 columns, 128 KB a block and SM out of shared memory; in the matrix layout a thread
           // has four rows and a quarter of the columns.  Two columns an instruction, which is half the issue (a load shape that
           // reads TMEM in half the time, 16x128b, pairs rows instead and needs more of it: 213 -> 227 us).
-          // A look at a barrier or at shared memory takes some 200 clocks beside the MMAs: both are asked early.
-          const float* sbk = reinterpret_cast<const float*>(scales + slot * S::SC_BYTES + 512) + half * 128 + c2;
-          F2 f[4], s2[2][4];
-          if (k == 0) {
+          // A look at a barrier or at shared memory takes some 200 clocks beside the MMAs, so that the next block's are asked for
+          // under this one's arithmetic: whether its sums and its scales are there, and then its first scales.
+          auto first_scales = [&] {
+            const float* sak = reinterpret_cast<const float*>(scales + slot * S::SC_BYTES) + q * 32 + r4;
+            const float* sbk = reinterpret_cast<const float*>(scales + slot * S::SC_BYTES + 512) + half * (BN / 2) + c2;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              fa[j] = sak[8 * j];
+              s2[0][j].v = *reinterpret_cast<const uint64_t*>(sbk + j * 8);
+            }
+          };
+          if (!have_scales) {
             ok = __all_sync(0xffffffffu, mbar_wait(bar_scfull + 8 * slot, scphase));
             if (!ok) break;
+            first_scales();
           }
-          const float* sak = reinterpret_cast<const float*>(scales + slot * S::SC_BYTES) + q * 32 + r4;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            f[j] = f2(sak[8 * j], sak[8 * j]);
-            s2[0][j].v = *reinterpret_cast<const uint64_t*>(sbk + j * 8);
+          if (!have_sums) {
+            ok = __all_sync(0xffffffffu, mbar_wait(bar_tfull + 8 * as, aphase));
+            if (!ok) break;
           }
-          ok = __all_sync(0xffffffffu, mbar_wait(bar_tfull + 8 * as, aphase));
-          if (!ok) break;
           tc_fence_after();
-          const int next_slot = slot + 1 == S::SC_SLOTS ? 0 : slot + 1;
-          const uint32_t next_phase = scphase ^ (next_slot == 0 ? 1u : 0u);
-          bool seen = true;
+          const float* sbk = reinterpret_cast<const float*>(scales + slot * S::SC_BYTES + 512) + half * (BN / 2) + c2;
+          const int next_slot = slot + 1 == S::SC_SLOTS ? 0 : slot + 1, next_as = as + 1 == S::BUFS ? 0 : as + 1;
+          const uint32_t next_phase = scphase ^ (next_slot == 0 ? 1u : 0u), next_aphase = aphase ^ (next_as == 0 ? 1u : 0u);
+          const bool more = k + 1 < t.nkt;
+          bool seen = false, summed = false;
+          F2 f[4];
 #pragma unroll
-          for (int c = 0; c < 8; ++c) {                   // 32 columns (c / 2) of 16 rows (c % 2)
+          for (int j = 0; j < 4; ++j) f[j] = f2(fa[j], fa[j]);
+#pragma unroll
+          for (int c = 0; c < BN / 32; ++c) {             // 32 columns (c / 2) of 16 rows (c % 2)
             F2 r[8];
             tmem_matrix16x32(src + ((uint32_t)((c & 1) * 16) << 16) + (c >> 1) * 32, r);
-            if (c == 7) release();
-            if ((c & 1) == 0 && c < 6) {
+            if (c == BN / 32 - 1) release();
+            if ((c & 1) == 0 && c < BN / 32 - 2) {
 #pragma unroll
               for (int g = 0; g < 4; ++g)
                 s2[((c >> 1) + 1) & 1][g].v = *reinterpret_cast<const uint64_t*>(sbk + ((c >> 1) + 1) * 32 + g * 8);
             }
-            if (c == 6 && k + 1 < t.nkt) seen = mbar_try_wait(bar_scfull + 8 * next_slot, next_phase);
+            if (c == BN / 32 - 2 && more) {
+              seen = mbar_try_wait(bar_scfull + 8 * next_slot, next_phase);
+              summed = mbar_try_wait(bar_tfull + 8 * next_as, next_aphase);
+            }
 #pragma unroll
             for (int j = 0; j < 8; ++j)
               acc2[c * 8 + j] = f2_fma(r[j] * s2[(c >> 1) & 1][j >> 1], f[(c & 1) * 2 + (j & 1)], acc2[c * 8 + j]);
@@ -493,23 +515,22 @@ gemm128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
           if (lane == 0) mbar_arrive(bar_scempty + 8 * slot);
           slot = next_slot;
           scphase = next_phase;
-          if (k + 1 < t.nkt && !__all_sync(0xffffffffu, seen)) {
-            ok = __all_sync(0xffffffffu, mbar_wait(bar_scfull + 8 * slot, scphase));
-            if (!ok) break;
-          }
+          have_scales = __all_sync(0xffffffffu, seen);
+          have_sums = __all_sync(0xffffffffu, summed);
+          if (have_scales) first_scales();
         }
-        if (++as == 2) { as = 0; aphase ^= 1; }
+        if (++as == S::BUFS) { as = 0; aphase ^= 1; }
       }
       if (!ok) break;
       // ---- out
-      const int row0 = t.m0 + q * 32, col0 = t.n0 + half * 128, end = t.end, e = t.e;
+      const int row0 = t.m0 + q * 32, col0 = t.n0 + half * (BN / 2), end = t.end, e = t.e;
       const bool row_in = row0 + lane < t.live;
       if (tile + n_pairs < n_total) begin(tile + n_pairs);
       if (row0 >= end) continue;                          // nothing of this warp's rows is stored
       if (MODE == ROWS128) {
         const bool whole = row0 + 32 <= end;
 #pragma unroll
-        for (int cc = 0; cc < 4; ++cc) {
+        for (int cc = 0; cc < BN / 64; ++cc) {
           const int col = col0 + cc * 32;
           if (col >= p.N) break;
           const uint32_t at = staging();
@@ -526,7 +547,7 @@ gemm128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
         }
       } else if (p.out_bf16) {
 #pragma unroll
-        for (int cc = 0; cc < 4; ++cc) {
+        for (int cc = 0; cc < BN / 64; ++cc) {
           if (col0 + cc * 32 >= p.N) break;
           const uint32_t at = staging();
 #pragma unroll
@@ -541,7 +562,7 @@ gemm128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
         }
       } else {
 #pragma unroll
-        for (int cc = 0; cc < 8; ++cc) {                  // 16 columns
+        for (int cc = 0; cc < BN / 32; ++cc) {            // 16 columns
           if (col0 + cc * 16 >= p.N) break;
           const uint32_t at = staging();
 #pragma unroll
