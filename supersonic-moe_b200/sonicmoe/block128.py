@@ -45,11 +45,12 @@ def _fp8_weight(weight, what):
 
 
 class _Block128Linear(torch.autograd.Function):
-    """x [rows,K]; weight bf16 [E,N,K] or [N,K], or None with (q, s) its quantised form."""
+    """x [rows,K]; weight bf16 [E,N,K] or [N,K], or None; `of` = (its quantised form or None twice, efo, counts, E, N, K)."""
 
     @staticmethod
-    def forward(ctx, x, weight, q, s, efo, counts, E, N, K):
-        dx, dw = ctx.needs_input_grad[:2]
+    def forward(ctx, x, weight, of):
+        q, s, efo, counts, E, N, K = of
+        dx, dw, _ = ctx.needs_input_grad
         flags = (ops.B128_QUANT_W if weight is not None else 0) | (ops.B128_DW if dw else 0)
         y, saved = ops.block128_linear(x, q if weight is None else weight.contiguous(), s, efo, counts, E, N, K, flags)
         ctx.save_for_backward(q, s, efo, counts, saved)
@@ -64,10 +65,10 @@ class _Block128Linear(torch.autograd.Function):
         w, main_grad = ctx.weight, None
         if w is not None:
             main_grad, base = _grad_target(w, w.shape)
-        dx, dw = ops.block128_linear_bwd(dy.contiguous(), q, s, efo, counts, saved, *ctx.of, main_grad)
+        dx, dw = ops.block128_linear_bwd(dy if dy.is_contiguous() else dy.contiguous(), q, s, efo, counts, saved, *ctx.of, main_grad)
         if main_grad is not None:
             _after_accumulate(base)
-        return dx, None if dw is None else dw.view(w.shape), None, None, None, None, None, None, None
+        return dx, None if dw is None else dw.view(w.shape), None
 
 
 def block128_linear(x: torch.Tensor, weight, efo: torch.Tensor | None = None, counts: torch.Tensor | None = None) -> torch.Tensor:
@@ -101,7 +102,7 @@ def block128_linear(x: torch.Tensor, weight, efo: torch.Tensor | None = None, co
     ops.check_segments(efo, counts, E, "block128_linear")
     rows = (x if x.ndim == 2 else x.reshape(-1, K)).contiguous()
     if torch.is_grad_enabled() and (x.requires_grad or (not pair and weight.requires_grad)):
-        y = _Block128Linear.apply(rows, weight, q, s, efo, counts, E, N, K)
+        y = _Block128Linear.apply(rows, weight, (q, s, efo, counts, E, N, K))
     elif pair:
         y = ops.block128_linear(rows, q, s, efo, counts, E, N, K, 0)[0]
     else:

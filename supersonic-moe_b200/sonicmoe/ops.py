@@ -783,19 +783,20 @@ def switch_loss_bwd(logits, grad, dloss):
 _current = torch._C._cuda_getDevice
 
 
-def _on_its_device(fn):
-    """Launch on the GPU of the first argument, which need not be the current one."""
+def _op(fn):
+    """As `_timed`, launched on the GPU of the first argument, which need not be the current one."""
     import functools
+    timed = _timed(fn)
 
     @functools.wraps(fn)
     def wrapper(x, *a, **k):
         d = x.get_device()
+        if d == _current():
+            return fn(x, *a, **k) if _recorder is None else timed(x, *a, **k)
         if d < 0:
             raise RuntimeError("sonicmoe kernels need CUDA tensors (no CPU fallback)")
-        if d == _current():
-            return fn(x, *a, **k)
         with torch.cuda.device(d):
-            return fn(x, *a, **k)
+            return timed(x, *a, **k)
     return wrapper
 
 
@@ -815,8 +816,7 @@ def _check_dense(what, *ts):
             raise RuntimeError("sonicmoe kernels need contiguous tensors")
 
 
-@_timed
-@_on_its_device
+@_op
 def group_routing(logits, K, bias=None, groups=1, top_groups=1, group_score=2, softmax=False, normalize=True, scale=1.0):
     """Router logits [T,E] (f32, bf16) -> (scores f32 [T,K], expert indices i32 [T,K]); see `group_limited_routing`."""
     _check_dense("group_routing", logits, bias)
@@ -833,8 +833,7 @@ def group_routing(logits, K, bias=None, groups=1, top_groups=1, group_score=2, s
     return scores, idx
 
 
-@_timed
-@_on_its_device
+@_op
 def group_routing_bwd(logits, idx, dscores, softmax=False, normalize=True, scale=1.0):
     """Gradient of the logits, in their type."""
     _check_dense("group_routing_bwd", logits, idx, dscores)
@@ -894,8 +893,7 @@ def check_segments(efo, counts, E, what):
         raise ValueError(f"{what}: counts is i32 [{E}], got {counts.dtype} {tuple(counts.shape)}")
 
 
-@_timed
-@_on_its_device
+@_op
 def quant128_rows(x, swiglu=False, rows_list=None, n_live=None):
     """bf16 [rows,K] -> (e4m3 bytes [rows,K], scales f32 [rows,K/128]).  `swiglu`: x is [rows,2K], gate and up interleaved, and
     silu(gate) * up is quantised.  `rows_list` i32, `n_live` i32 (device): only the first n_live rows listed."""
@@ -916,8 +914,7 @@ def quant128_rows(x, swiglu=False, rows_list=None, n_live=None):
     return q, s
 
 
-@_timed
-@_on_its_device
+@_op
 def quant128_rows_scatter(x, naept, s_rev, rows):
     """bf16 [T,K], the routing metadata's token offsets and places -> (e4m3 bytes [rows,K], scales [rows,K/128]) in expert-sorted
     order; rows without a token are left as they are."""
@@ -932,8 +929,7 @@ def quant128_rows_scatter(x, naept, s_rev, rows):
     return q, s
 
 
-@_timed
-@_on_its_device
+@_op
 def quant128_dual(x, efo=None, counts=None, with_rows=True):
     """bf16 [rows,K] -> (row form e4m3 [rows,K], scales [rows,K/128]; both None without `with_rows`; column form transposed, e4m3
     [K,rows], scales [rows/128,K]) from one read."""
@@ -949,8 +945,7 @@ def quant128_dual(x, efo=None, counts=None, with_rows=True):
     return q, s, qt, st
 
 
-@_timed
-@_on_its_device
+@_op
 def quant128_weight(w):
     """bf16 [E,N,K] -> (e4m3 bytes [E,N,K], scales f32 [E,N/128,K/128])."""
     _check_dense("quant128_weight", w)
@@ -963,7 +958,10 @@ def quant128_weight(w):
 
 def failure_words(device):
     """Addresses of the status word and of its host mirror (which a capture must not be the first to allocate)."""
-    if _dev_index(device) not in _posted and torch.cuda.is_current_stream_capturing():
+    m = _posted.get(device.index)
+    if m is not None:
+        return m[2:]
+    if torch.cuda.is_current_stream_capturing():
         return status_word(device).data_ptr(), None
     return status_pointers(device)
 
@@ -981,8 +979,7 @@ def _check_product(a_q, a_s, b_q, b_s, efo, counts, E, N, K, b_blocks, what):
         raise ValueError(f"{what}: the weights' scales are f32 {(E, *b_blocks)}, got {b_s.dtype} {tuple(b_s.shape)}")
 
 
-@_timed
-@_on_its_device
+@_op
 def gemm128_rows(a_q, a_s, b_q, b_s, efo=None, counts=None, b_mn=False, zero_rest=True):
     """a e4m3 [rows,K] by rows, b e4m3 [E,N,K] by blocks (`b_mn`: [E,K,N], the reduction over its rows) -> bf16 [rows,N]; rows behind a
     segment's live ones zero, or not written."""
@@ -998,8 +995,7 @@ def gemm128_rows(a_q, a_s, b_q, b_s, efo=None, counts=None, b_mn=False, zero_res
     return c
 
 
-@_timed
-@_on_its_device
+@_op
 def gemm128_few(a_q, a_s, b_q, b_s, efo=None, counts=None, live_rows=0):
     """`gemm128_rows` made for few rows per expert; rows that are not live are not written.  `live_rows`: an upper bound of theirs, if
     known."""
@@ -1014,8 +1010,7 @@ def gemm128_few(a_q, a_s, b_q, b_s, efo=None, counts=None, live_rows=0):
     return c
 
 
-@_timed
-@_on_its_device
+@_op
 def gemm128_wgrad(a_q, a_s, b_q, b_s, efo=None, counts=None, out=None, accumulate=False):
     """a e4m3 [M,rows], b e4m3 [N,rows], the column forms of `quant128_dual` -> bf16 [E,M,N], the products of each segment's live rows; or into `out` f32
     [E,M,N], overwritten or added to."""
@@ -1065,8 +1060,7 @@ def block128_bytes(rows, N, K, E, flags, which):
     return n
 
 
-@_timed
-@_on_its_device
+@_op
 def block128_linear(x, w, w_s, efo, counts, E, N, K, flags):
     """x bf16 [rows,K] and w (e4m3 with scales, or bf16 with B128_QUANT_W) -> (y bf16 [rows,N], arena for the backward pass or None)."""
     _check_same_gpu("block128_linear", x, w, w_s, efo, counts)
@@ -1080,8 +1074,7 @@ def block128_linear(x, w, w_s, efo, counts, E, N, K, flags):
     return y, saved
 
 
-@_timed
-@_on_its_device
+@_op
 def block128_linear_bwd(dy, w, w_s, efo, counts, saved, E, N, K, flags, main_grad=None):
     """dy bf16 [rows,N] -> (dx bf16 [rows,K] or None, dw bf16 [E,N,K] or None, where it is added to `main_grad` f32)."""
     rows = dy.shape[0]
@@ -1097,8 +1090,7 @@ def block128_linear_bwd(dy, w, w_s, efo, counts, saved, E, N, K, flags, main_gra
     return dx, (dw if main_grad is None else None)
 
 
-@_timed
-@_on_its_device
+@_op
 def block128_experts(x, idx, scores, w1, w1_s, w2, w2_s, E, I):
     """x bf16 [T,H], idx i32 and scores f32 [T,K], quantised weights -> bf16 [T,H]; see `sonicmoe.block128_experts`."""
     _check_same_gpu("block128_experts", x, idx, scores, w1, w1_s, w2, w2_s)

@@ -19,10 +19,10 @@ from .count_cumsum import count_cumsum
 
 class _GroupLimitedRouting(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, K, bias, groups, top_groups, group_score, softmax, normalize, scale):
-        scores, idx = ops.group_routing(logits, K, bias, groups, top_groups, group_score, softmax, normalize, scale)
+    def forward(ctx, logits, K, rule):
+        scores, idx = ops.group_routing(logits, K, *rule)
         ctx.save_for_backward(logits, idx)
-        ctx.rule = (softmax, normalize, scale)
+        ctx.rule = rule[4:]                                  # softmax, normalize, scale
         ctx.mark_non_differentiable(idx)
         return scores, idx
 
@@ -30,7 +30,9 @@ class _GroupLimitedRouting(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dscores, _didx):
         logits, idx = ctx.saved_tensors
-        return (ops.group_routing_bwd(logits, idx, dscores.float().contiguous(), *ctx.rule),) + (None,) * 8
+        if dscores.dtype != torch.float32 or not dscores.is_contiguous():
+            dscores = dscores.float().contiguous()
+        return ops.group_routing_bwd(logits, idx, dscores, *ctx.rule), None, None
 
 
 def group_limited_routing(router_logits: torch.Tensor, K: int, *, score: str = "sigmoid", bias: torch.Tensor | None = None,
@@ -62,11 +64,13 @@ def group_limited_routing(router_logits: torch.Tensor, K: int, *, score: str = "
     if bias is not None:
         if bias.shape != (E,):
             raise ValueError(f"bias {tuple(bias.shape)}: one value for each of {E} experts")
-        bias = bias.detach().float().contiguous()
+        if bias.dtype != torch.float32 or not bias.is_contiguous():
+            bias = bias.detach().float().contiguous()
     rule = (bias, groups, top_groups, group_score, score == "softmax", bool(normalize), float(scale))
-    if router_logits.requires_grad and torch.is_grad_enabled():
-        return _GroupLimitedRouting.apply(router_logits.contiguous(), K, *rule)
-    return ops.group_routing(router_logits.detach().contiguous(), K, *rule)
+    logits = router_logits if router_logits.is_contiguous() else router_logits.contiguous()
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _GroupLimitedRouting.apply(logits, K, rule)
+    return ops.group_routing(logits, K, *rule)
 
 
 def token_rounding_routing(router_logits: torch.Tensor, K: int, Mtile: int = 128, routing: str = "nr"):
