@@ -22,16 +22,16 @@ static int make_tmap128(CUtensorMap* m, const void* base, uint64_t depth, uint64
   return r == CUDA_SUCCESS ? SMOE_OK : SMOE_ERR_TMAP;
 }
 
-// The result [depth, rows, cols], box of 32 rows of 64 bytes
+// The result [depth, rows, cols], box of 32 rows of 128 bytes
 static int make_tmap128_out(CUtensorMap* m, void* base, bool bf16, uint64_t depth, uint64_t rows, uint64_t cols) {
   if (!load_encode()) return SMOE_ERR_DRIVER;
   const cuuint64_t es = bf16 ? 2 : 4;
   cuuint64_t extent[3] = {cols, rows, depth};
   cuuint64_t strides[2] = {cols * es, cols * rows * es};
-  cuuint32_t box[3] = {(cuuint32_t)(64 / es), 32, 1};
+  cuuint32_t box[3] = {(cuuint32_t)(128 / es), 32, 1};
   cuuint32_t estr[3] = {1, 1, 1};
   const CUresult r = g_encode(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, base, extent, strides,
-                              box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B,
+                              box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? SMOE_OK : SMOE_ERR_TMAP;
 }

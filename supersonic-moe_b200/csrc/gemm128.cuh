@@ -47,11 +47,13 @@ constexpr int kG128N = 256;        // columns of a tile (128 with four buffers, 
 struct Gemm128Smem {
   static constexpr int BN = kG128N;
   static constexpr int A_BYTES = BM * BK, B_BYTES = BN / 2 * BK;
-  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES, STAGES = 5;
+  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES, STAGES = 4;
   static constexpr int BUFS = 512 / BN;                     // TMEM buffers
   static constexpr int EPI_WARPS = 8;
-  static constexpr int STG_TILE = 2048, STG_TILES = 3;      // output staging of a warp: 32 rows x 64 bytes
-  static constexpr int STG_BYTES = STG_TILES * STG_TILE;
+  // Output staging of a warp: two tiles of 32 rows x 128 bytes, all of its bf16 columns, so that they pass through shared memory
+  // with one fence.  (Four passes of 64 bytes and a fifth ring stage: 3200 clocks between the last block of a tile and the next
+  // one's first, of which the MMAs have 1300 to do; 8192 x 4096 x 128 17.4 -> 15.4 us, x 8192 196 -> 200.)
+  static constexpr int STG_TILE = 4096, STG_BYTES = 2 * STG_TILE;
   // WGRAD128: scales of this CTA's 128 rows and of the 256 columns in a block, in a ring of their own, filled by a warp of its own:
   // every block reads new lines of them, and a register's worth of look-ahead does not cover HBM (measured: 1650 clocks a block)
   static constexpr int SC_BYTES = (128 + BN) * 4, SC_SLOTS = 8;
@@ -194,18 +196,16 @@ __device__ __forceinline__ Tile128 tile128(int tile, int rank, const Gemm128Para
   return t;
 }
 
-// A warp's staged 32 rows x 32 bf16 columns (16-byte pieces of a row at places xor (row / 2) % 4, the 64-byte TMA swizzle), where
-// not all rows are to be written: four lanes a row
+// A warp's staged 32 rows x 64 bf16 columns (16-byte pieces of a row at places xor row % 8, the 128-byte TMA swizzle), where not all
+// rows are to be written: eight lanes a row
 __device__ __forceinline__ void store_slab128(uint32_t stg, int lane, uint16_t* c, int N, int row0, int end, int col0) {
-  __syncwarp();
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = i * 8 + (lane >> 2), j = lane & 3, gr = row0 + r, gc = col0 + j * 8;
+  for (int i = 0; i < 8; ++i) {
+    const int r = i * 4 + (lane >> 3), j = lane & 7, gr = row0 + r, gc = col0 + j * 8;
     uint4 v;
-    ld_shared_v4(stg + r * 64 + ((j ^ ((r >> 1) & 3)) << 4), v.x, v.y, v.z, v.w);
+    ld_shared_v4(stg + r * 128 + ((j ^ (r & 7)) << 4), v.x, v.y, v.z, v.w);
     if (gr < end && gc < N) *reinterpret_cast<uint4*>(c + (int64_t)gr * N + gc) = v;
   }
-  __syncwarp();
 }
 __device__ __forceinline__ void tma_store_3d(const void* tmap, uint32_t src, int c0, int c1, int c2) {
   asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];"
@@ -384,23 +384,24 @@ gemm128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
     const int q = warp & 3, half = warp >> 2;
     const uint32_t tempty0 = map_to_cta(bar_tempty, 0);
     const uint32_t stg = smem_u32(epi) + warp * S::STG_BYTES;
-    int as = 0, slot = 0, buf = 0;
+    int as = 0, slot = 0;
     uint32_t aphase = 0, scphase = 0;
     bool ok = true;
-    // A staging tile is free again once the store before the last one has been read out of shared memory
-    auto staging = [&] {
-      if (lane == 0) bulk_wait_group_read<S::STG_TILES - 1>();
+    auto staging_free = [&] {                             // all that was staged before has been read
+      if (lane == 0) bulk_wait_group_read<0>();
       __syncwarp();
-      const uint32_t at = stg + buf * S::STG_TILE;
-      if (++buf == S::STG_TILES) buf = 0;
-      return at;
     };
-    auto staged = [&](uint32_t at, int col, int row, int e) {
+    // both staging tiles to columns col and col + cols on
+    auto staged = [&](int col, int cols, int row, int e) {
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
-        if (MODE == WGRAD128 && p.accumulate) tma_reduce_add_3d(&tmap_c, at, col, row, e);
-        else tma_store_3d(&tmap_c, at, col, row, e);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          if (col + u * cols >= p.N) break;
+          if (MODE == WGRAD128 && p.accumulate) tma_reduce_add_3d(&tmap_c, stg + u * S::STG_TILE, col + u * cols, row, e);
+          else tma_store_3d(&tmap_c, stg + u * S::STG_TILE, col + u * cols, row, e);
+        }
         bulk_commit_group();
       }
     };
@@ -409,22 +410,24 @@ gemm128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster_relaxed(tempty0 + 8 * as);
     };
-    Tile128 t{};
+    Tile128 t{}, next{};
     const float *sa = nullptr, *sb = nullptr;             // ROWS128: scales of a lane's row, of the columns
     float sa_next = 0.f, sb_next = 0.f;
-    // The next tile and its first scales are asked for before the results of the one before it are written
+    // The next tile and its first scales are asked for while the last block of the one before it is on its way
     auto begin = [&](int tile) {
-      t = tile128<MODE>(tile, rank, p, segs);
-      if (MODE == ROWS128 && t.nkt > 0) {
-        const int row = t.m0 + q * 32 + lane;
-        sa = p.a_s + (int64_t)(row < t.live ? row : 0) * p.a_kb;
-        sb = p.b_s + t.e * p.bs_e + (int64_t)min((t.n0 + half * (BN / 2)) / 128, (p.N - 1) / 128) * p.bs_n;
+      next = tile128<MODE>(tile, rank, p, segs);
+      if (MODE == ROWS128 && next.nkt > 0) {
+        const int row = next.m0 + q * 32 + lane;
+        sa = p.a_s + (int64_t)(row < next.live ? row : 0) * p.a_kb;
+        sb = p.b_s + next.e * p.bs_e + (int64_t)min((next.n0 + half * (BN / 2)) / 128, (p.N - 1) / 128) * p.bs_n;
         sa_next = *sa;
         sb_next = *sb;
       }
     };
     if (pair_id < n_total) begin(pair_id);
     for (int tile = pair_id; tile < n_total; tile += n_pairs) {
+      t = next;
+      if (t.nkt == 0 && tile + n_pairs < n_total) begin(tile + n_pairs);
       float acc[MODE == ROWS128 ? BN / 2 : 1];               // [column]
       F2 acc2[MODE == WGRAD128 ? BN / 4 : 1];                 // [32 columns][16 rows][8 columns][row r4, row r4 + 8]: two columns
 #pragma unroll
@@ -444,6 +447,8 @@ gemm128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
             sa_next = *++sa;
             sb += p.bs_k;
             sb_next = *sb;
+          } else if (tile + n_pairs < n_total) {
+            begin(tile + n_pairs);
           }
           ok = __all_sync(0xffffffffu, mbar_wait(bar_tfull + 8 * as, aphase));
           if (!ok) break;
@@ -485,6 +490,7 @@ gemm128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
             if (!ok) break;
           }
           tc_fence_after();
+          if (k + 1 == t.nkt && tile + n_pairs < n_total) begin(tile + n_pairs);
           const float* sbk = reinterpret_cast<const float*>(scales + slot * S::SC_BYTES + 512) + half * (BN / 2) + c2;
           const int next_slot = slot + 1 == S::SC_SLOTS ? 0 : slot + 1, next_as = as + 1 == S::BUFS ? 0 : as + 1;
           const uint32_t next_phase = scphase ^ (next_slot == 0 ? 1u : 0u), next_aphase = aphase ^ (next_as == 0 ? 1u : 0u);
@@ -523,57 +529,54 @@ gemm128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
       }
       if (!ok) break;
       // ---- out
-      const int row0 = t.m0 + q * 32, col0 = t.n0 + half * (BN / 2), end = t.end, e = t.e;
-      const bool row_in = row0 + lane < t.live;
-      if (tile + n_pairs < n_total) begin(tile + n_pairs);
-      if (row0 >= end) continue;                          // nothing of this warp's rows is stored
+      const int row0 = t.m0 + q * 32, col0 = t.n0 + half * (BN / 2);
+      if (row0 >= t.end) continue;                        // nothing of this warp's rows is stored
+      staging_free();
       if (MODE == ROWS128) {
-        const bool whole = row0 + 32 <= end;
+        const bool row_in = row0 + lane < t.live;
 #pragma unroll
-        for (int cc = 0; cc < BN / 64; ++cc) {
-          const int col = col0 + cc * 32;
-          if (col >= p.N) break;
-          const uint32_t at = staging();
+        for (int j = 0; j < 16; ++j) {
+          uint32_t w[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            uint32_t w[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              w[i] = row_in ? pack_bf16x2(acc[cc * 32 + 8 * j + 2 * i], acc[cc * 32 + 8 * j + 2 * i + 1]) : 0u;
-            st_shared_v4(at + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4), w[0], w[1], w[2], w[3]);
-          }
-          if (whole) staged(at, col, row0, 0);
-          else store_slab128(at, lane, reinterpret_cast<uint16_t*>(p.c), p.N, row0, end, col);
+          for (int i = 0; i < 4; ++i) w[i] = row_in ? pack_bf16x2(acc[8 * j + 2 * i], acc[8 * j + 2 * i + 1]) : 0u;
+          st_shared_v4(stg + (j >> 3) * S::STG_TILE + lane * 128 + (((j & 7) ^ (lane & 7)) << 4), w[0], w[1], w[2], w[3]);
+        }
+        if (row0 + 32 <= t.end) {
+          staged(col0, 64, row0, 0);
+        } else {
+          __syncwarp();
+          store_slab128(stg, lane, reinterpret_cast<uint16_t*>(p.c), p.N, row0, t.end, col0);
+          store_slab128(stg + S::STG_TILE, lane, reinterpret_cast<uint16_t*>(p.c), p.N, row0, t.end, col0 + 64);
+          __syncwarp();
         }
       } else if (p.out_bf16) {
 #pragma unroll
-        for (int cc = 0; cc < BN / 64; ++cc) {
-          if (col0 + cc * 32 >= p.N) break;
-          const uint32_t at = staging();
+        for (int cc = 0; cc < BN / 64; ++cc) {            // 32 columns
 #pragma unroll
           for (int j = 0; j < 4; ++j) {                   // rows r4 + 8 j
-            const int r = r4 + 8 * j;
 #pragma unroll
             for (int g = 0; g < 4; ++g)
-              st_shared_b32(at + r * 64 + ((g ^ ((r >> 1) & 3)) << 4) + c2 * 2,
+              st_shared_b32(stg + (cc >> 1) * S::STG_TILE + (r4 + 8 * j) * 128 + ((((cc & 1) * 4 + g) ^ r4) << 4) + c2 * 2,
                             pack_bf16x2(acc2[cc * 16 + (j >> 1) * 8 + g * 2 + (j & 1)]));
           }
-          staged(at, col0 + cc * 32, row0, e);
         }
+        staged(col0, 64, row0, t.e);
       } else {
 #pragma unroll
-        for (int cc = 0; cc < BN / 32; ++cc) {            // 16 columns
-          if (col0 + cc * 16 >= p.N) break;
-          const uint32_t at = staging();
+        for (int h = 0; h < 2; ++h) {                     // 64 columns
+          if (h) staging_free();
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int r = r4 + 8 * j;
+          for (int u = 0; u < 2; ++u) {                   // 32 columns
+            const int cc = h * 2 + u;
 #pragma unroll
-            for (int g = 0; g < 2; ++g)
-              st_shared_b64(at + r * 64 + (((g * 2 + (c2 >> 2)) ^ ((r >> 1) & 3)) << 4) + (c2 & 2) * 4,
-                            acc2[(cc >> 1) * 16 + (j >> 1) * 8 + ((cc & 1) * 2 + g) * 2 + (j & 1)]);
+            for (int j = 0; j < 4; ++j) {
+#pragma unroll
+              for (int g = 0; g < 4; ++g)
+                st_shared_b64(stg + u * S::STG_TILE + (r4 + 8 * j) * 128 + (((g * 2 + (c2 >> 2)) ^ r4) << 4) + (c2 & 2) * 4,
+                              acc2[cc * 16 + (j >> 1) * 8 + g * 2 + (j & 1)]);
+            }
           }
-          staged(at, col0 + cc * 16, row0, e);
+          staged(col0 + h * 64, 32, row0, t.e);
         }
       }
     }
