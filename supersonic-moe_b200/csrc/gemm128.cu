@@ -123,15 +123,16 @@ int smoe_gemm128_few(const void* a_fp8, const float* a_scales, const void* b_fp8
   int rc = check128(a_fp8, a_scales, b_fp8, b_scales, efo, counts, c_bf16, rows, N, K, E, status);
   if (rc || rows == 0) return rc;
   if (live_rows <= 0 || live_rows > rows) live_rows = rows;
-  CUtensorMap tw, tx;
+  CUtensorMap tw, tx16, tx64;
   rc = make_tmap128(&tw, b_fp8, E, N, K, 128, 3);
-  if (!rc) rc = make_tmap128(&tx, a_fp8, 1, rows, K, 16, 2);
+  if (!rc) rc = make_tmap128(&tx16, a_fp8, 1, rows, K, 16, 2);
+  if (!rc) rc = make_tmap128(&tx64, a_fp8, 1, rows, K, Few128Smem::NT, 2);
   if (rc) return rc;
   static bool attr_set[kMaxDevices] = {};
   if (!ensure_smem_attr(gemm128_few_kernel, Few128Smem::TOTAL, attr_set)) return SMOE_ERR_LAUNCH;
   const int sms = sm_count();
   const int64_t nw = up(N, 128), busy = live_rows < E ? live_rows : E;
-  const int64_t tiles = (live_rows / Few128Smem::NT + busy) * nw;       // as many as there can be
+  const int64_t tiles = (live_rows + (Few128Smem::NT - 1) * busy) / Few128Smem::NT * nw;       // as many as there can be
   int split = 1;
   while (split < 8 && tiles * split * 2 <= sms && split * 4 <= up(K, 128)) split *= 2;
   Few128Params p{(int)rows, (int)N, (int)K, (int)E, efo, counts, b_scales, a_scales, (__nv_bfloat16*)c_bf16, split, status,
@@ -149,7 +150,7 @@ int smoe_gemm128_few(const void* a_fp8, const float* a_scales, const void* b_fp8
   cfg.stream = (cudaStream_t)stream;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, gemm128_few_kernel, tw, tx, p) != cudaSuccess) return SMOE_ERR_LAUNCH;
+  if (cudaLaunchKernelEx(&cfg, gemm128_few_kernel, tw, tx16, tx64, p) != cudaSuccess) return SMOE_ERR_LAUNCH;
   return cudaGetLastError() == cudaSuccess ? SMOE_OK : SMOE_ERR_LAUNCH;
 }
 

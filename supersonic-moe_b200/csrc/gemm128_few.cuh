@@ -1,7 +1,7 @@
 // The product of gemm128.cuh for few rows per expert (single tokens, decoding): the weights are the M operand.
 //
 // Such a call is bound by the read of the weights.  A CTA computes 128 weight rows x up to 64 routed rows, so that each SM streams
-// weight tiles of its own; of the routed rows only as many 16-row pieces are fetched and multiplied as hold live ones.  The sum
+// weight tiles of its own; of the routed rows 16 or 64 are fetched and as many pieces of 16 multiplied as hold live ones.  The sum
 // of a block of 128 lies transposed in TMEM (lane = weight row, column = routed row) in one of eight buffers of 64 columns; the
 // epilogue warps scale it - one number a column, which every lane reads from shared memory - and keep 64 f32 sums a thread.
 //
@@ -79,7 +79,8 @@ __device__ __forceinline__ FewTile128 few_tile128(int tile, int nw, int E, const
 }
 
 __global__ void __launch_bounds__(Few128Smem::THREADS, 1)
-gemm128_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, const Few128Params p) {
+gemm128_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x16,
+                   const __grid_constant__ CUtensorMap tmap_x64, const Few128Params p) {
   using S = Few128Smem;
   constexpr int NT = S::NT;
   extern __shared__ uint8_t smem_raw[];
@@ -145,20 +146,23 @@ gemm128_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
     // ------------------------------------------------------------ producer
     if (lane == 0) {
       prefetch_tmap(&tmap_w);
-      prefetch_tmap(&tmap_x);
+      prefetch_tmap(&tmap_x16);
+      prefetch_tmap(&tmap_x64);
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
       for (int tile = group; tile < n_total && ok; tile += n_groups) {
         const FewTile128 t = few_tile128(tile, nw, p.E, segs);
-        const int pieces = (t.live + 15) / 16;
+        // 16 routed rows or all 64 (a copy takes this thread some 200 clocks to issue)
+        const CUtensorMap* tx = t.live <= 16 ? &tmap_x16 : &tmap_x64;
+        const uint32_t bytes = S::A_BYTES + (t.live <= 16 ? 16 : NT) * BK;
         for (int k = k0; k < k1; ++k) {
           ok = mbar_wait(bar_empty + 8 * stage, phase ^ 1);
           if (!ok) break;
           const uint32_t full = bar_full + 8 * stage, a_dst = smem_base + stage * S::STAGE_BYTES, b_dst = a_dst + S::A_BYTES;
-          mbar_expect_tx(full, S::A_BYTES + pieces * 16 * BK);
+          mbar_expect_tx(full, bytes);
           tma_load_3d(a_dst, &tmap_w, full, k * 128, t.w0, t.e);
-          for (int i = 0; i < pieces; ++i) tma_load_2d(b_dst + i * 16 * BK, &tmap_x, full, k * 128, t.row0 + i * 16);
+          tma_load_2d(b_dst, tx, full, k * 128, t.row0);
           if (++stage == S::STAGES) { stage = 0; phase ^= 1; }
         }
       }
@@ -339,18 +343,21 @@ gemm128_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
         ok = __all_sync(0xffffffffu, mbar_wait_cluster(bar_pfull, pphase));
         if (!ok) break;
         const uint32_t mine = smem_u32(part + q * 32 + lane);
-        for (int i = rank; i < t.live; i += 4 * split) {      // four rows' sums on their way at a time
-          float v[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 2
-          for (int r = 0; r < split; ++r) {
-            const uint32_t from = map_to_cta(mine, r);
+        // a stretch of the rows each, eight of them on their way from a CTA at a time
+        const int per = (t.live + split - 1) / split, last = min((rank + 1) * per, t.live);
+        for (int i = rank * per; i < last; i += 8) {
+          float v[8];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (i + j * split < t.live) v[j] += ld_cluster_f32(from + (i + j * split) * BM * 4);
+          for (int j = 0; j < 8; ++j) v[j] = 0.f;
+#pragma unroll 4
+          for (int r = 0; r < split; ++r) {
+            const uint32_t from = map_to_cta(mine, r) + i * BM * 4;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] += ld_cluster_f32(from + min(j, last - 1 - i) * BM * 4);
           }
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (i + j * split < t.live && w_row < p.N) p.c[(int64_t)(t.row0 + i + j * split) * p.N + w_row] = __float2bfloat16_rn(v[j]);
+          for (int j = 0; j < 8; ++j)
+            if (i + j < last && w_row < p.N) p.c[(int64_t)(t.row0 + i + j) * p.N + w_row] = __float2bfloat16_rn(v[j]);
         }
         __syncwarp();
         if (lane < split) mbar_arrive_cluster(map_to_cta(bar_pempty, lane));
