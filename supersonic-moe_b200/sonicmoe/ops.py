@@ -791,10 +791,10 @@ def _op(fn):
     @functools.wraps(fn)
     def wrapper(x, *a, **k):
         d = x.get_device()
-        if d == _current():
-            return fn(x, *a, **k) if _recorder is None else timed(x, *a, **k)
         if d < 0:
             raise RuntimeError("sonicmoe kernels need CUDA tensors (no CPU fallback)")
+        if d == _current():
+            return fn(x, *a, **k) if _recorder is None else timed(x, *a, **k)
         with torch.cuda.device(d):
             return timed(x, *a, **k)
     return wrapper

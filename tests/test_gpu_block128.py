@@ -436,3 +436,103 @@ def test_captured_on_another_stream_and_two_at_once(sonicmoe):
     torch.cuda.synchronize()
     for a, b in outs:
         assert torch.equal(a, want[1]) and torch.equal(b, lin[1])
+
+
+def test_gradients_asked_for_one_at_a_time_and_a_matrix_with_an_accumulator(sonicmoe):
+    x, w, dy = randn(70, 136, seed=1).to(DEV), randn(264, 136, seed=2).to(DEV), randn(70, 264, seed=3).to(DEV)
+    both = [t.clone().requires_grad_(True) for t in (x, w)]
+    sonicmoe.block128_linear(*both).backward(dy)
+    one = x.clone().requires_grad_(True)
+    sonicmoe.block128_linear(one, w).backward(dy)
+    other = w.clone().requires_grad_(True)
+    other.main_grad = torch.zeros(264, 136, device=DEV)
+    sonicmoe.block128_linear(x, other).backward(dy.T.contiguous().T)          # a gradient of other strides
+    assert torch.equal(one.grad, both[0].grad) and other.grad is None
+    assert torch.equal(other.main_grad.to(torch.bfloat16), both[1].grad)
+    other.main_grad = torch.zeros(264, 137, device=DEV)
+    with pytest.raises(ValueError):
+        sonicmoe.block128_linear(x, other).backward(dy)
+    y = sonicmoe.block128_linear(*both)
+    g, = torch.autograd.grad(y.sum(), both[0], create_graph=True)
+    with pytest.raises(RuntimeError):                          # no second derivative, and it says so
+        torch.autograd.grad(g.sum(), both[1])
+
+
+def test_segments_without_counts_and_tables_without_rows(sonicmoe):
+    efo, _, rows = table([128, 256, 0, 128])
+    x, w = randn(rows, 136, seed=1), randn(4, 128, 136, seed=2)
+    y = sonicmoe.block128_linear(x.to(DEV), w.to(DEV), efo.to(DEV))
+    ref = O.rows_product(O.deq_rows(*O.quant_rows(x)), O.deq_weight(*O.quant_weight(w)), efo, None)
+    near(y, ref, 136)
+    # nothing is routed here: zeros, and gradients of zeros
+    none = torch.zeros(4, dtype=torch.int32, device=DEV)
+    xd, wd = x.to(DEV).requires_grad_(True), w.to(DEV).requires_grad_(True)
+    for e, n in ((efo.to(DEV), none), (torch.zeros(5, dtype=torch.int32, device=DEV), none)):
+        y = sonicmoe.block128_linear(xd, wd, e, n)
+        gx, gw = torch.autograd.grad(y, (xd, wd), torch.ones_like(y))
+        assert (y == 0).all() and (gx == 0).all() and (gw == 0).all()
+    pairs = [sonicmoe.quantize_weight_block128(randn(*s, seed=4).to(DEV)) for s in ((4, 256, 136), (4, 136, 128))]
+    idx, sc = torch.full((9, 2), -1, dtype=torch.int32, device=DEV), torch.ones(9, 2, device=DEV)
+    out = sonicmoe.block128_experts(x[:9].to(DEV), idx, sc, *pairs)
+    assert out.shape == (9, 136) and (out == 0).all()
+    assert sonicmoe.block128_experts(x[:0].to(DEV), idx[:0], sc[:0], *pairs).shape == (0, 136)
+
+
+def test_offsets_beyond_32_bits(sonicmoe):
+    """Rows x columns, and experts x rows x columns, above 2^31: what lies at the end is what a small call gives."""
+    ops = sonicmoe.ops
+    rows, N, K = 300032, 8192, 128
+    g = torch.Generator(device=DEV).manual_seed(1)
+    x = torch.randn(rows, K, generator=g, device=DEV).to(torch.bfloat16)
+    w = torch.randn(1, N, K, generator=g, device=DEV).to(torch.bfloat16)
+    W = ops.quant128_weight(w)
+    y = ops.gemm128_rows(*ops.quant128_rows(x), *W)
+    end = slice(rows - 200, rows)
+    assert torch.equal(y[end], ops.gemm128_rows(*ops.quant128_rows(x[end].contiguous()), *W))
+    # y as the gradient that comes back: both forms, and a weight gradient over the last block alone
+    q, s, qt, st = ops.quant128_dual(y)
+    small = ops.quant128_dual(y[rows - 128:].contiguous())
+    assert torch.equal(q[rows - 128:], small[0]) and torch.equal(s[rows - 128:], small[1])
+    assert torch.equal(qt[:, rows - 128:], small[2]) and torch.equal(st[-1:], small[3])
+    xt = ops.quant128_dual(x, with_rows=False)[2:]
+    efo = torch.tensor([0, rows - 128, rows], dtype=torch.int32, device=DEV)
+    counts = torch.tensor([0, 128], dtype=torch.int32, device=DEV)
+    dw = ops.gemm128_wgrad(qt, st, *xt, efo, counts)
+    assert (dw[0] == 0).all()
+    assert torch.equal(dw[1:], ops.gemm128_wgrad(small[2], small[3], *ops.quant128_dual(x[rows - 128:].contiguous())[2:]))
+    dx = ops.gemm128_rows(q, s, *W, b_mn=True)
+    assert torch.equal(dx[rows - 128:], ops.gemm128_rows(small[0], small[1], *W, b_mn=True))
+    z = ops.quant128_rows(y, True)
+    assert torch.equal(z[0][rows - 128:], ops.quant128_rows(y[rows - 128:].contiguous(), True)[0])
+    del x, y, q, s, qt, st, xt, dx, z
+    E, N, K = 200, 4096, 2816
+    w = torch.empty(E, N, K, dtype=torch.bfloat16, device=DEV).normal_(generator=g)
+    W = ops.quant128_weight(w)
+    x = torch.randn(3, K, generator=g, device=DEV).to(torch.bfloat16)
+    X = ops.quant128_rows(x)
+    last = ops.gemm128_few(*X, *(t[E - 1:] for t in W))
+    assert torch.equal(W[0][E - 1:], ops.quant128_weight(w[E - 1:].contiguous())[0])
+    efo = torch.tensor([0] * E + [3], dtype=torch.int32, device=DEV)
+    counts = torch.tensor([0] * (E - 1) + [3], dtype=torch.int32, device=DEV)
+    far = ops.gemm128_few(*X, *W, efo, counts)                 # (the reduction may be divided otherwise: other roundings in f32)
+    ref, mag = O.rows_product(O.deq_rows(*(t.cpu().view(torch.float8_e4m3fn) if t.dtype == torch.uint8 else t.cpu() for t in X)),
+                              O.deq_weight(W[0][E - 1:].cpu().view(torch.float8_e4m3fn), W[1][E - 1:].cpu()), None, None)
+    tol = BF16 * ref.abs() + f32_tol(K, 22) * mag * (1 + BF16)
+    for got in (last, far, ops.gemm128_rows(*X, *W, efo, counts)):
+        assert ((got.cpu().double() - ref).abs() <= tol).all()
+
+
+def test_repeated_calls_give_the_same_bits(sonicmoe):
+    """No sum here depends on which block of threads came first."""
+    efo, cnt, rows = table([300, 0, 5, 700])
+    e, c = efo.to(DEV), cnt.to(DEV)
+    x, w, dy = randn(rows, 264, seed=1).to(DEV), randn(4, 520, 264, seed=2).to(DEV), randn(rows, 520, seed=3).to(DEV)
+    runs = []
+    for _ in range(3):
+        a, b = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+        y = sonicmoe.block128_linear(a, b, e, c)
+        y.backward(dy)
+        one = sonicmoe.block128_linear(x[:3], w[0])
+        runs.append((y.detach(), a.grad, b.grad, one))
+    for run in runs[1:]:
+        assert all(torch.equal(p, q) for p, q in zip(run, runs[0]))
