@@ -453,17 +453,28 @@ gemm128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
           ok = __all_sync(0xffffffffu, mbar_wait(bar_tfull + 8 * as, aphase));
           if (!ok) break;
           tc_fence_after();
-          uint32_t r[2][16];
-          tmem_ld16(src, r[0]);
+          // Half the columns, and the other half as each piece's registers come free: the buffer goes back to the MMAs when
+          // half of the arithmetic is done (one piece ahead: when seven eighths are, and 783 clocks a block instead of 752).
+          uint32_t r[4][16];
 #pragma unroll
-          for (int c = 0; c < BN / 32; ++c) {
-            tmem_ld_wait();
-            tmem_arrived(r[c & 1]);
-            if (c < BN / 32 - 1) tmem_ld16(src + (c + 1) * 16, r[(c + 1) & 1]);
-            else release();
+          for (int c = 0; c < 4; ++c) tmem_ld16(src + c * 16, r[c]);
+          tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 16; ++i) acc[c * 16 + i] = fmaf(__uint_as_float(r[c & 1][i]), f, acc[c * 16 + i]);
+          for (int c = 0; c < 4; ++c) tmem_arrived(r[c]);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[c * 16 + i] = fmaf(__uint_as_float(r[c][i]), f, acc[c * 16 + i]);
+            tmem_ld16(src + (c + 4) * 16, r[c]);
           }
+          tmem_ld_wait();
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_arrived(r[c]);
+          release();
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[64 + c * 16 + i] = fmaf(__uint_as_float(r[c][i]), f, acc[64 + c * 16 + i]);
         } else {
           // Both operands have a scale of their own in every block: two multiplications a value.  With a lane a row every lane
           // would read the scales of all 128 columns, 128 KB a block and SM out of shared memory; in the matrix layout a thread
