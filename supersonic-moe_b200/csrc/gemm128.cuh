@@ -107,18 +107,21 @@ __device__ __forceinline__ void tmem_arrived(uint32_t (&r)[16]) {
   asm volatile("" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
                "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]));
 }
-// 16 lanes x 32 columns, complete when it returns: thread t gets, of each 8 columns g, columns 2 (t % 4) and the next of lanes t / 4
-// (the pair r[2g]) and t / 4 + 8 (r[2g+1]).
-__device__ __forceinline__ void tmem_matrix16x32(uint32_t taddr, F2 (&r)[8]) {
+// 16 lanes x 32 columns: thread t gets, of each 8 columns g, columns 2 (t % 4) and the next of lanes t / 4 (r[4g], r[4g+1]) and
+// t / 4 + 8 (r[4g+2], r[4g+3]).
+__device__ __forceinline__ void tmem_ld_16x32(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
-      "{\n\t.reg .b32 t<16>;\n\t"
-      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {t0,t1,t2,t3,t4,t5,t6,t7,t8,t9,t10,t11,t12,t13,t14,t15}, [%8];\n\t"
-      "tcgen05.wait::ld.sync.aligned;\n\t"
-      "mov.b64 %0, {t0,t1};\n\tmov.b64 %1, {t2,t3};\n\tmov.b64 %2, {t4,t5};\n\tmov.b64 %3, {t6,t7};\n\t"
-      "mov.b64 %4, {t8,t9};\n\tmov.b64 %5, {t10,t11};\n\tmov.b64 %6, {t12,t13};\n\tmov.b64 %7, {t14,t15};\n\t}"
-      : "=l"(r[0].v), "=l"(r[1].v), "=l"(r[2].v), "=l"(r[3].v), "=l"(r[4].v), "=l"(r[5].v), "=l"(r[6].v), "=l"(r[7].v)
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr)
       : "memory");
+}
+__device__ __forceinline__ F2 f2_bits(uint32_t lo, uint32_t hi) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "r"(lo), "r"(hi));
+  return r;
 }
 
 // Segments from efo / counts, any values taken as they fit: 0 <= start <= end <= rows, start <= live end <= end
@@ -510,11 +513,16 @@ gemm128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
           F2 f[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) f[j] = f2(fa[j], fa[j]);
+          uint32_t r[2][16];
+          tmem_ld_16x32(src, r[0]);
 #pragma unroll
-          for (int c = 0; c < BN / 32; ++c) {             // 32 columns (c / 2) of 16 rows (c % 2)
-            F2 r[8];
-            tmem_matrix16x32(src + ((uint32_t)((c & 1) * 16) << 16) + (c >> 1) * 32, r);
-            if (c == BN / 32 - 1) release();
+          for (int c = 0; c < BN / 32; ++c) {             // 32 columns (c / 2) of 16 rows (c % 2), the next piece on its way
+            tmem_ld_wait();
+            tmem_arrived(r[c & 1]);
+            if (c < BN / 32 - 1)
+              tmem_ld_16x32(src + ((uint32_t)(((c + 1) & 1) * 16) << 16) + ((c + 1) >> 1) * 32, r[(c + 1) & 1]);
+            else
+              release();
             if ((c & 1) == 0 && c < BN / 32 - 2) {
 #pragma unroll
               for (int g = 0; g < 4; ++g)
@@ -526,7 +534,8 @@ gemm128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
             }
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-              acc2[c * 8 + j] = f2_fma(r[j] * s2[(c >> 1) & 1][j >> 1], f[(c & 1) * 2 + (j & 1)], acc2[c * 8 + j]);
+              acc2[c * 8 + j] = f2_fma(f2_bits(r[c & 1][2 * j], r[c & 1][2 * j + 1]) * s2[(c >> 1) & 1][j >> 1],
+                                       f[(c & 1) * 2 + (j & 1)], acc2[c * 8 + j]);
           }
           __syncwarp();
           if (lane == 0) mbar_arrive(bar_scempty + 8 * slot);
