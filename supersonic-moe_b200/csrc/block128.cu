@@ -3,6 +3,7 @@
 #include <cuda_runtime.h>
 
 #include "smoe_b200.h"
+#include "smoe_internal.h"
 
 namespace smoe {
 
@@ -185,7 +186,8 @@ int smoe_block128_experts(const void* x_bf16, const int32_t* idx, const float* s
                               s.scores, s.src_idx, s.counts, s.ws, stream));
   const bool few = few_rows128(T, E, K);
   auto product = [&](const void* a, const float* as, const void* w, const float* ws, void* c, int64_t N, int64_t Kr) {
-    return few ? smoe_gemm128_few(a, as, w, ws, s.efo, s.counts, c, s.rows, N, Kr, E, s.slots, status, pinned_host_word, stream)
+    // (offsets and counts were complete when the quantiser ahead of the product began)
+    return few ? gemm128_few(a, as, w, ws, s.efo, s.counts, c, s.rows, N, Kr, E, s.slots, status, pinned_host_word, true, stream)
                : smoe_gemm128_rows(a, as, w, ws, s.efo, s.counts, c, s.rows, N, Kr, E, 0, 0, status, pinned_host_word, stream);
   };
   SMOE_TRY(smoe_quant128_rows_scatter(x_bf16, T, H, s.naept, s.s_rev, s.rows, s.xq, s.xs, stream));

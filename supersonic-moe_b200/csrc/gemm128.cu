@@ -3,6 +3,7 @@
 #include "gemm128_few.cuh"
 #include "host.h"
 #include "smoe_b200.h"
+#include "smoe_internal.h"
 
 namespace smoe {
 
@@ -62,6 +63,45 @@ static int check128(const void* a, const float* a_s, const void* b, const float*
 
 static int64_t up(int64_t n, int64_t m) { return (n + m - 1) / m; }
 
+int gemm128_few(const void* a_fp8, const float* a_scales, const void* b_fp8, const float* b_scales, const int* efo, const int* counts,
+                void* c_bf16, int64_t rows, int64_t N, int64_t K, int64_t E, int64_t live_rows, int* status, int* pinned_host_word,
+                bool early, void* stream) {
+  int rc = check128(a_fp8, a_scales, b_fp8, b_scales, efo, counts, c_bf16, rows, N, K, E, status);
+  if (rc || rows == 0) return rc;
+  if (live_rows <= 0 || live_rows > rows) live_rows = rows;
+  CUtensorMap tw, tx16, tx64;
+  rc = make_tmap128(&tw, b_fp8, E, N, K, 128, 3);
+  if (!rc) rc = make_tmap128(&tx16, a_fp8, 1, rows, K, 16, 2);
+  if (!rc) rc = make_tmap128(&tx64, a_fp8, 1, rows, K, Few128Smem::NT, 2);
+  if (rc) return rc;
+  static bool attr_set[kMaxDevices] = {};
+  if (!ensure_smem_attr(gemm128_few_kernel, Few128Smem::TOTAL, attr_set)) return SMOE_ERR_LAUNCH;
+  const int sms = sm_count();
+  const int64_t nw = up(N, 128), busy = live_rows < E ? live_rows : E;
+  const int64_t tiles = (live_rows + (Few128Smem::NT - 1) * busy) / Few128Smem::NT * nw;       // as many as there can be
+  int split = 1;
+  while (split < 8 && tiles * split * 2 <= sms && split * 4 <= up(K, 128)) split *= 2;
+  Few128Params p{(int)rows, (int)N, (int)K, (int)E, efo, counts, b_scales, a_scales, (__nv_bfloat16*)c_bf16, split, status,
+                 pinned_host_word};
+  int64_t groups = sms / split;
+  if (tiles < groups) groups = tiles;
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)split;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(groups * split));
+  cfg.blockDim = dim3(Few128Smem::THREADS);
+  cfg.dynamicSmemBytes = Few128Smem::TOTAL;
+  cfg.stream = (cudaStream_t)stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = early ? 2 : 1;
+  if (cudaLaunchKernelEx(&cfg, gemm128_few_kernel, tw, tx16, tx64, p) != cudaSuccess) return SMOE_ERR_LAUNCH;
+  return cudaGetLastError() == cudaSuccess ? SMOE_OK : SMOE_ERR_LAUNCH;
+}
+
 }  // namespace smoe
 
 using namespace smoe;
@@ -120,38 +160,8 @@ int smoe_gemm128_wgrad(const void* a_fp8, const float* a_scales, const void* b_f
 int smoe_gemm128_few(const void* a_fp8, const float* a_scales, const void* b_fp8, const float* b_scales, const int32_t* efo,
                      const int32_t* counts, void* c_bf16, int64_t rows, int64_t N, int64_t K, int64_t E, int64_t live_rows,
                      int32_t* status, int32_t* pinned_host_word, void* stream) {
-  int rc = check128(a_fp8, a_scales, b_fp8, b_scales, efo, counts, c_bf16, rows, N, K, E, status);
-  if (rc || rows == 0) return rc;
-  if (live_rows <= 0 || live_rows > rows) live_rows = rows;
-  CUtensorMap tw, tx16, tx64;
-  rc = make_tmap128(&tw, b_fp8, E, N, K, 128, 3);
-  if (!rc) rc = make_tmap128(&tx16, a_fp8, 1, rows, K, 16, 2);
-  if (!rc) rc = make_tmap128(&tx64, a_fp8, 1, rows, K, Few128Smem::NT, 2);
-  if (rc) return rc;
-  static bool attr_set[kMaxDevices] = {};
-  if (!ensure_smem_attr(gemm128_few_kernel, Few128Smem::TOTAL, attr_set)) return SMOE_ERR_LAUNCH;
-  const int sms = sm_count();
-  const int64_t nw = up(N, 128), busy = live_rows < E ? live_rows : E;
-  const int64_t tiles = (live_rows + (Few128Smem::NT - 1) * busy) / Few128Smem::NT * nw;       // as many as there can be
-  int split = 1;
-  while (split < 8 && tiles * split * 2 <= sms && split * 4 <= up(K, 128)) split *= 2;
-  Few128Params p{(int)rows, (int)N, (int)K, (int)E, efo, counts, b_scales, a_scales, (__nv_bfloat16*)c_bf16, split, status,
-                 pinned_host_word};
-  int64_t groups = sms / split;
-  if (tiles < groups) groups = tiles;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = (unsigned)split;
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(groups * split));
-  cfg.blockDim = dim3(Few128Smem::THREADS);
-  cfg.dynamicSmemBytes = Few128Smem::TOTAL;
-  cfg.stream = (cudaStream_t)stream;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, gemm128_few_kernel, tw, tx16, tx64, p) != cudaSuccess) return SMOE_ERR_LAUNCH;
-  return cudaGetLastError() == cudaSuccess ? SMOE_OK : SMOE_ERR_LAUNCH;
+  return gemm128_few(a_fp8, a_scales, b_fp8, b_scales, efo, counts, c_bf16, rows, N, K, E, live_rows, status, pinned_host_word, false,
+                     stream);
 }
 
 }  // extern "C"

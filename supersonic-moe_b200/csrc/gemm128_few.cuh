@@ -7,6 +7,9 @@
 //
 // Where the weight tiles are too few to occupy the SMs a cluster of 2, 4 or 8 CTAs shares one: each takes a stretch of the
 // reduction, leaves its sums in its shared memory, and adds up a share of the columns from all of them, in rank order.
+//
+// Where its caller allows it (see gemm128_few) the kernel starts before the one before it in the stream has ended: until
+// wait_for_kernel_before it touches only offsets, counts and weights.
 #pragma once
 #include "gemm128.cuh"
 
@@ -97,6 +100,7 @@ gemm128_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
   segs.tiles = segs.live + kG128Segs + 1;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  next_kernel_may_start();
   const int split = p.split, rank = split > 1 ? (int)cluster_ctarank() : 0;
   const int group = blockIdx.x / split, n_groups = gridDim.x / split;
   const uint32_t bar_full = smem_u32(bars), bar_empty = bar_full + 8 * S::STAGES;
@@ -151,18 +155,28 @@ gemm128_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
+      // 16 routed rows or all 64 (a copy takes this thread some 200 clocks to issue)
+      auto weights = [&](const FewTile128& t, int k, int st) {
+        mbar_expect_tx(bar_full + 8 * st, S::A_BYTES + (t.live <= 16 ? 16 : NT) * BK);
+        tma_load_3d(smem_base + st * S::STAGE_BYTES, &tmap_w, bar_full + 8 * st, k * 128, t.w0, t.e);
+      };
+      // the weights of the first pass over the ring are asked for before the kernel that makes the routed rows has ended
+      const int early = group < n_total ? min(S::STAGES, blocks) : 0;
+      if (early) {
+        const FewTile128 t = few_tile128(group, nw, p.E, segs);
+        for (int i = 0; i < early; ++i) weights(t, k0 + i, i);
+      }
+      wait_for_kernel_before();
       for (int tile = group; tile < n_total && ok; tile += n_groups) {
         const FewTile128 t = few_tile128(tile, nw, p.E, segs);
-        // 16 routed rows or all 64 (a copy takes this thread some 200 clocks to issue)
-        const CUtensorMap* tx = t.live <= 16 ? &tmap_x16 : &tmap_x64;
-        const uint32_t bytes = S::A_BYTES + (t.live <= 16 ? 16 : NT) * BK;
         for (int k = k0; k < k1; ++k) {
-          ok = mbar_wait(bar_empty + 8 * stage, phase ^ 1);
-          if (!ok) break;
-          const uint32_t full = bar_full + 8 * stage, a_dst = smem_base + stage * S::STAGE_BYTES, b_dst = a_dst + S::A_BYTES;
-          mbar_expect_tx(full, bytes);
-          tma_load_3d(a_dst, &tmap_w, full, k * 128, t.w0, t.e);
-          tma_load_2d(b_dst, tx, full, k * 128, t.row0);
+          if (tile != group || k - k0 >= early) {
+            ok = mbar_wait(bar_empty + 8 * stage, phase ^ 1);
+            if (!ok) break;
+            weights(t, k, stage);
+          }
+          tma_load_2d(smem_base + stage * S::STAGE_BYTES + S::A_BYTES, t.live <= 16 ? &tmap_x16 : &tmap_x64, bar_full + 8 * stage,
+                      k * 128, t.row0);
           if (++stage == S::STAGES) { stage = 0; phase ^= 1; }
         }
       }
@@ -246,6 +260,7 @@ gemm128_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
       if (lane == 0) mbar_arrive(bar_sfull + 8 * slot);
       ++given;
     };
+    wait_for_kernel_before();                                 // every block, also one without tiles
     at_tile();
     float a0[G], a1[G], b0[G], b1[G];
     if (tile < n_total) {

@@ -8,6 +8,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "ptx.cuh"
 #include "smoe_b200.h"
 
 namespace smoe {
@@ -95,6 +96,7 @@ struct Rows128Args {
 
 template <bool GLU, int PER>
 __global__ void __launch_bounds__(256, PER == 4 ? 4 : 6) quant128_rows_kernel(const Rows128Args a) {
+  next_kernel_may_start();
   const int kb = (a.K + 127) / 128;
   const int64_t n = a.list && a.n_live ? min((int64_t)*a.n_live, a.n) : a.n;
   const int lane16 = threadIdx.x & 15;

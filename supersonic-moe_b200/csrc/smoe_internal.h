@@ -34,6 +34,10 @@ int gemm_gated_few(const void* x_sorted_fp8, const void* a_sf, const void* w1_fp
 int gemm_varlen_m_few(const void* a_fp8, const void* a_sf, const void* b_fp8, const void* b_sf, const int* efo,
                       const int* counts, void* c_bf16, int64_t rows, int64_t N, int64_t K, int64_t E, int* status, bool early,
                       void* stream);
+// smoe_gemm128_few, `early` as above
+int gemm128_few(const void* a_fp8, const float* a_scales, const void* b_fp8, const float* b_scales, const int* efo, const int* counts,
+                void* c_bf16, int64_t rows, int64_t N, int64_t K, int64_t E, int64_t live_rows, int* status, int* pinned_host_word,
+                bool early, void* stream);
 }  // namespace smoe
 #endif
 #endif /* SMOE_INTERNAL_H_ */
