@@ -142,9 +142,10 @@ int smoe_block128_linear(const void* x_bf16, const void* w, const float* w_scale
   }
   if (flags & SMOE_B128_DW) SMOE_TRY(smoe_quant128_dual(x_bf16, rows, K, efo, counts, E, f.xq, f.xs, sv.xc, sv.xcs, stream));
   else SMOE_TRY(smoe_quant128_rows(x_bf16, rows, K, 0, nullptr, nullptr, 0, f.xq, f.xs, stream));
+  // (segments and weights were complete when the quantiser ahead of the product began)
   if (!efo && rows <= kFewRows)
-    return smoe_gemm128_few(f.xq, f.xs, w, w_scales, efo, counts, y_bf16, rows, N, K, E, 0, status, pinned_host_word, stream);
-  return smoe_gemm128_rows(f.xq, f.xs, w, w_scales, efo, counts, y_bf16, rows, N, K, E, 0, 1, status, pinned_host_word, stream);
+    return gemm128_few(f.xq, f.xs, w, w_scales, efo, counts, y_bf16, rows, N, K, E, 0, status, pinned_host_word, true, stream);
+  return gemm128_rows(f.xq, f.xs, w, w_scales, efo, counts, y_bf16, rows, N, K, E, 0, 1, status, pinned_host_word, true, stream);
 }
 
 int smoe_block128_linear_bwd(const void* dy_bf16, const void* w_fp8, const float* w_scales, const int32_t* efo,
@@ -162,11 +163,11 @@ int smoe_block128_linear_bwd(const void* dy_bf16, const void* w_fp8, const float
   if (flags & SMOE_B128_DW) SMOE_TRY(smoe_quant128_dual(dy_bf16, rows, N, efo, counts, E, b.dq, b.ds, b.dc, b.dcs, stream));
   else if (flags & SMOE_B128_DX) SMOE_TRY(smoe_quant128_rows(dy_bf16, rows, N, 0, nullptr, nullptr, 0, b.dq, b.ds, stream));
   if (flags & SMOE_B128_DX)
-    SMOE_TRY(smoe_gemm128_rows(b.dq, b.ds, w_fp8, w_scales, efo, counts, dx_bf16, rows, K, N, E, 1, 1, status, pinned_host_word,
-                               stream));
+    SMOE_TRY(gemm128_rows(b.dq, b.ds, w_fp8, w_scales, efo, counts, dx_bf16, rows, K, N, E, 1, 1, status, pinned_host_word, true,
+                          stream));
   if (flags & SMOE_B128_DW)
-    SMOE_TRY(smoe_gemm128_wgrad(b.dc, b.dcs, sv.xc, sv.xcs, efo, counts, dw, N, K, rows, E, !dw_f32_accumulate, dw_f32_accumulate,
-                                status, pinned_host_word, stream));
+    SMOE_TRY(gemm128_wgrad(b.dc, b.dcs, sv.xc, sv.xcs, efo, counts, dw, N, K, rows, E, !dw_f32_accumulate, dw_f32_accumulate, status,
+                           pinned_host_word, (flags & SMOE_B128_DX) && rows > 0, stream));      // its operands were complete before dx began
   return SMOE_OK;
 }
 
@@ -188,7 +189,7 @@ int smoe_block128_experts(const void* x_bf16, const int32_t* idx, const float* s
   auto product = [&](const void* a, const float* as, const void* w, const float* ws, void* c, int64_t N, int64_t Kr) {
     // (offsets and counts were complete when the quantiser ahead of the product began)
     return few ? gemm128_few(a, as, w, ws, s.efo, s.counts, c, s.rows, N, Kr, E, s.slots, status, pinned_host_word, true, stream)
-               : smoe_gemm128_rows(a, as, w, ws, s.efo, s.counts, c, s.rows, N, Kr, E, 0, 0, status, pinned_host_word, stream);
+               : gemm128_rows(a, as, w, ws, s.efo, s.counts, c, s.rows, N, Kr, E, 0, 0, status, pinned_host_word, true, stream);
   };
   SMOE_TRY(smoe_quant128_rows_scatter(x_bf16, T, H, s.naept, s.s_rev, s.rows, s.xq, s.xs, stream));
   SMOE_TRY(product(s.xq, s.xs, w1_fp8, w1_scales, s.z, 2 * I, H));

@@ -39,14 +39,24 @@ static int make_tmap128_out(CUtensorMap* m, void* base, bool bf16, uint64_t dept
 
 template <int MODE>
 static int launch128(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, const Gemm128Params& p, int64_t tiles,
-                     cudaStream_t stream) {
+                     bool early, cudaStream_t stream) {
   static bool attr_set[kMaxDevices] = {};
   auto kern = gemm128_kernel<MODE>;
   if (!ensure_smem_attr(kern, Gemm128Smem::TOTAL, attr_set)) return SMOE_ERR_LAUNCH;
   int64_t pairs = sm_count() / 2;
   if (tiles < pairs) pairs = tiles;
   if (pairs <= 0) return SMOE_OK;
-  kern<<<(unsigned)(2 * pairs), Gemm128Smem::THREADS, Gemm128Smem::TOTAL, stream>>>(ta, tb, tc, p);
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(2 * pairs));
+  cfg.blockDim = dim3(Gemm128Smem::THREADS);
+  cfg.dynamicSmemBytes = Gemm128Smem::TOTAL;
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = early ? 1 : 0;
+  if (cudaLaunchKernelEx(&cfg, kern, ta, tb, tc, p) != cudaSuccess) return SMOE_ERR_LAUNCH;
   return cudaGetLastError() == cudaSuccess ? SMOE_OK : SMOE_ERR_LAUNCH;
 }
 
@@ -62,6 +72,55 @@ static int check128(const void* a, const float* a_s, const void* b, const float*
 }
 
 static int64_t up(int64_t n, int64_t m) { return (n + m - 1) / m; }
+
+int gemm128_rows(const void* a_fp8, const float* a_scales, const void* b_fp8, const float* b_scales, const int* efo, const int* counts,
+                 void* c_bf16, int64_t rows, int64_t N, int64_t K, int64_t E, int b_mn, int zero_rest, int* status,
+                 int* pinned_host_word, bool early, void* stream) {
+  int rc = check128(a_fp8, a_scales, b_fp8, b_scales, efo, counts, c_bf16, rows, N, K, E, status);
+  if (rc || rows == 0) return rc;
+  CUtensorMap ta, tb, tc;
+  rc = make_tmap128(&ta, a_fp8, 1, rows, K, 128, 2);
+  if (!rc) rc = make_tmap128_out(&tc, c_bf16, true, 1, rows, N);
+  if (!rc) rc = b_mn ? make_tmap128(&tb, b_fp8, E, K, N, 128, 3) : make_tmap128(&tb, b_fp8, E, N, K, 128, 3);
+  if (rc) return rc;
+  Gemm128Params p{};
+  p.rows = (int)rows; p.N = (int)N; p.K = (int)K; p.E = (int)E;
+  p.efo = efo; p.counts = counts; p.a_s = a_scales; p.b_s = b_scales;
+  const int64_t nb = up(N, 128), kb = up(K, 128);
+  p.a_kb = (int)kb;
+  p.bs_e = nb * kb;
+  p.bs_n = b_mn ? 1 : kb;
+  p.bs_k = b_mn ? (int)nb : 1;
+  p.b_mn = b_mn != 0; p.c = c_bf16; p.zero_rest = zero_rest != 0; p.status = status; p.host_word = pinned_host_word;
+  // every segment may end in a tile that is not full, and so may the rows behind the last
+  const int64_t tiles = efo ? (rows / 256 + E + 1) * up(N, 256) : up(rows, 256) * up(N, 256);
+  return launch128<ROWS128>(ta, tb, tc, p, tiles, early, (cudaStream_t)stream);
+}
+
+int gemm128_wgrad(const void* a_fp8, const float* a_scales, const void* b_fp8, const float* b_scales, const int* efo, const int* counts,
+                  void* c, int64_t M, int64_t N, int64_t rows, int64_t E, int out_bf16, int accumulate, int* status,
+                  int* pinned_host_word, bool independent, void* stream) {
+  int rc = check128(a_fp8, a_scales, b_fp8, b_scales, efo, counts, c, rows, N, M, E, status);
+  if (rc) return rc;
+  if (out_bf16 && accumulate) return SMOE_ERR_ARG;
+  if (rows == 0) {                                  // an empty sum
+    if (accumulate) return SMOE_OK;
+    if (!c) return SMOE_ERR_ARG;
+    return cudaMemsetAsync(c, 0, (size_t)(E * M * N) * (out_bf16 ? 2 : 4), (cudaStream_t)stream) == cudaSuccess ? SMOE_OK
+                                                                                                             : SMOE_ERR_LAUNCH;
+  }
+  CUtensorMap ta, tb, tc;
+  rc = make_tmap128(&ta, a_fp8, 1, M, rows, 128, 2);
+  if (!rc) rc = make_tmap128_out(&tc, c, out_bf16, E, M, N);
+  if (!rc) rc = make_tmap128(&tb, b_fp8, 1, N, rows, 128, 3);
+  if (rc) return rc;
+  Gemm128Params p{};
+  p.rows = (int)rows; p.M = (int)M; p.N = (int)N; p.E = (int)E;
+  p.efo = efo; p.counts = counts; p.a_s = a_scales; p.b_s = b_scales;
+  p.c = c; p.out_bf16 = out_bf16 != 0; p.accumulate = accumulate != 0; p.status = status;
+  p.host_word = pinned_host_word; p.independent = independent;
+  return launch128<WGRAD128>(ta, tb, tc, p, E * up(M, 256) * up(N, 256), independent, (cudaStream_t)stream);
+}
 
 int gemm128_few(const void* a_fp8, const float* a_scales, const void* b_fp8, const float* b_scales, const int* efo, const int* counts,
                 void* c_bf16, int64_t rows, int64_t N, int64_t K, int64_t E, int64_t live_rows, int* status, int* pinned_host_word,
@@ -111,50 +170,15 @@ extern "C" {
 int smoe_gemm128_rows(const void* a_fp8, const float* a_scales, const void* b_fp8, const float* b_scales, const int32_t* efo,
                       const int32_t* counts, void* c_bf16, int64_t rows, int64_t N, int64_t K, int64_t E, int b_mn,
                       int zero_rest, int32_t* status, int32_t* pinned_host_word, void* stream) {
-  int rc = check128(a_fp8, a_scales, b_fp8, b_scales, efo, counts, c_bf16, rows, N, K, E, status);
-  if (rc || rows == 0) return rc;
-  CUtensorMap ta, tb, tc;
-  rc = make_tmap128(&ta, a_fp8, 1, rows, K, 128, 2);
-  if (!rc) rc = make_tmap128_out(&tc, c_bf16, true, 1, rows, N);
-  if (!rc) rc = b_mn ? make_tmap128(&tb, b_fp8, E, K, N, 128, 3) : make_tmap128(&tb, b_fp8, E, N, K, 128, 3);
-  if (rc) return rc;
-  Gemm128Params p{};
-  p.rows = (int)rows; p.N = (int)N; p.K = (int)K; p.E = (int)E;
-  p.efo = efo; p.counts = counts; p.a_s = a_scales; p.b_s = b_scales;
-  const int64_t nb = up(N, 128), kb = up(K, 128);
-  p.a_kb = (int)kb;
-  p.bs_e = nb * kb;
-  p.bs_n = b_mn ? 1 : kb;
-  p.bs_k = b_mn ? (int)nb : 1;
-  p.b_mn = b_mn != 0; p.c = c_bf16; p.zero_rest = zero_rest != 0; p.status = status; p.host_word = pinned_host_word;
-  // every segment may end in a tile that is not full, and so may the rows behind the last
-  const int64_t tiles = efo ? (rows / 256 + E + 1) * up(N, 256) : up(rows, 256) * up(N, 256);
-  return launch128<ROWS128>(ta, tb, tc, p, tiles, (cudaStream_t)stream);
+  return gemm128_rows(a_fp8, a_scales, b_fp8, b_scales, efo, counts, c_bf16, rows, N, K, E, b_mn, zero_rest, status, pinned_host_word,
+                      false, stream);
 }
 
 int smoe_gemm128_wgrad(const void* a_fp8, const float* a_scales, const void* b_fp8, const float* b_scales, const int32_t* efo,
                        const int32_t* counts, void* c, int64_t M, int64_t N, int64_t rows, int64_t E, int out_bf16, int accumulate,
                        int32_t* status, int32_t* pinned_host_word, void* stream) {
-  int rc = check128(a_fp8, a_scales, b_fp8, b_scales, efo, counts, c, rows, N, M, E, status);
-  if (rc) return rc;
-  if (out_bf16 && accumulate) return SMOE_ERR_ARG;
-  if (rows == 0) {                                  // an empty sum
-    if (accumulate) return SMOE_OK;
-    if (!c) return SMOE_ERR_ARG;
-    return cudaMemsetAsync(c, 0, (size_t)(E * M * N) * (out_bf16 ? 2 : 4), (cudaStream_t)stream) == cudaSuccess ? SMOE_OK
-                                                                                                             : SMOE_ERR_LAUNCH;
-  }
-  CUtensorMap ta, tb, tc;
-  rc = make_tmap128(&ta, a_fp8, 1, M, rows, 128, 2);
-  if (!rc) rc = make_tmap128_out(&tc, c, out_bf16, E, M, N);
-  if (!rc) rc = make_tmap128(&tb, b_fp8, 1, N, rows, 128, 3);
-  if (rc) return rc;
-  Gemm128Params p{};
-  p.rows = (int)rows; p.M = (int)M; p.N = (int)N; p.E = (int)E;
-  p.efo = efo; p.counts = counts; p.a_s = a_scales; p.b_s = b_scales;
-  p.c = c; p.out_bf16 = out_bf16 != 0; p.accumulate = accumulate != 0; p.status = status;
-  p.host_word = pinned_host_word;
-  return launch128<WGRAD128>(ta, tb, tc, p, E * up(M, 256) * up(N, 256), (cudaStream_t)stream);
+  return gemm128_wgrad(a_fp8, a_scales, b_fp8, b_scales, efo, counts, c, M, N, rows, E, out_bf16, accumulate, status, pinned_host_word,
+                       false, stream);
 }
 
 int smoe_gemm128_few(const void* a_fp8, const float* a_scales, const void* b_fp8, const float* b_scales, const int32_t* efo,

@@ -26,6 +26,7 @@ struct Gemm128Params {
   int b_mn;
   void* c;                   // ROWS128: bf16 [rows, N]; WGRAD128: [E, M, N] f32 or bf16
   int out_bf16, accumulate;  // WGRAD128
+  int independent;           // of the kernel before in the stream: waited for at the end only
   int zero_rest;             // ROWS128: rows that are not live are written as zero (else left as they are)
   int* status;
   volatile int* host_word;   // pinned mirror of *status, or null
@@ -286,6 +287,9 @@ gemm128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   const uint32_t smem_base = smem_u32(smem);
+  // (so far offsets and counts alone have been read, which a caller that lets this kernel begin early vouches for)
+  if (!p.independent) wait_for_kernel_before();
+  next_kernel_may_start();                    // not earlier: an independent one counts on what this kernel has waited for
   const int nt = (p.N + BN - 1) / BN;
   const int n_total = MODE == WGRAD128 ? p.E * ((p.M + 255) / 256) * nt : segs.tiles[p.E + 1] * nt;
 
@@ -614,6 +618,7 @@ gemm128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
   cluster_sync_all();                         // the peer may still be signalling this CTA's barriers
   tc_fence_after();
   if (warp == ISSUER) tmem_dealloc2(tmem_base, 512);
+  if (p.independent) wait_for_kernel_before();
 }
 
 }  // namespace smoe

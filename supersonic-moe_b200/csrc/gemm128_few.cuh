@@ -100,7 +100,6 @@ gemm128_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
   segs.tiles = segs.live + kG128Segs + 1;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  next_kernel_may_start();
   const int split = p.split, rank = split > 1 ? (int)cluster_ctarank() : 0;
   const int group = blockIdx.x / split, n_groups = gridDim.x / split;
   const uint32_t bar_full = smem_u32(bars), bar_empty = bar_full + 8 * S::STAGES;
