@@ -104,10 +104,14 @@ static bool sizes128(int64_t rows, int64_t N, int64_t K, int64_t E) {
          K < (int64_t)1 << 24 && E > 0 && E <= 256;
 }
 
-// Rows of one projection up to which its weights are the wide operand of the product
+// Rows of one projection up to which its weights are the wide operand of the product: one tile of rows there, and more CTAs per
+// weight (us with / without at 16, 64 and 128 rows: 4096 x 4096 11 / 19, 14 / 19, 18 / 20; 16384 x 4096 17 / 22, 22 / 22, 36 / 23)
 constexpr int64_t kFewRows = 64;
-// Of routed experts: so few rows an expert that reading its weights bounds the product
-static bool few_rows128(int64_t T, int64_t E, int64_t K) { return T <= kFewRows || T * K <= 16 * E; }
+// Of routed experts: where an expert's rows, evenly routed, are 32 or fewer, or no expert can have more than one tile of them, reading
+// the weights bounds the product (up and down, us with / without, 128 experts of 2048 x 768: 8 rows 113 / 176, 32 rows 124 / 182,
+// 48 rows 133 / 185, 64 rows 185 / 186; 8 of 4096 x 2048: 44 / 60, 52 / 60, 58 / 62, 77 / 62).  Uneven routing leaves fewer weights
+// to read, and gives some experts a second tile.
+static bool few_rows128(int64_t T, int64_t E, int64_t K) { return T <= kFewRows || T * K <= 32 * E; }
 
 #define SMOE_TRY(call)          \
   do {                          \

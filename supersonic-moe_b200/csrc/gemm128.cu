@@ -138,8 +138,13 @@ int gemm128_few(const void* a_fp8, const float* a_scales, const void* b_fp8, con
   const int sms = sm_count();
   const int64_t nw = up(N, 128), busy = live_rows < E ? live_rows : E;
   const int64_t tiles = (live_rows + (Few128Smem::NT - 1) * busy) / Few128Smem::NT * nw;       // as many as there can be
+  // Few tiles are shared by clusters while each CTA keeps three blocks of a reduction of twelve or more (us at 16 rows with 1 / 2 / 4
+  // CTAs: 4096 x 4096 15.0 / 12.3 / 11.2, 2048 x 1536 8.2 / 8.4 / 7.7, 8192 x 2048 10.6 / 10.6 / -; 1024 x 1024 7.0 / 7.8 / 7.4,
+  // 2048 x 768 6.4 / 7.5 / 7.3).  Eight find room together on half of the SMs only, as they come from one part of the chip (with 8
+  // instead of 4: 1024 x 16384 16.4 -> 13.7, 2048 x 8192, on 128 SMs, 12.5 -> 21.1).
+  const int64_t kb = up(K, 128);
   int split = 1;
-  while (split < 8 && tiles * split * 2 <= sms && split * 4 <= up(K, 128)) split *= 2;
+  while (split < 8 && kb >= 12 && split * 6 <= kb && tiles * split * (split == 4 ? 4 : 2) <= sms) split *= 2;
   Few128Params p{(int)rows, (int)N, (int)K, (int)E, efo, counts, b_scales, a_scales, (__nv_bfloat16*)c_bf16, split, status,
                  pinned_host_word};
   int64_t groups = sms / split;

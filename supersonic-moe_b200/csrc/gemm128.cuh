@@ -167,6 +167,20 @@ __device__ __forceinline__ int seg_of_tile(const int* tiles, int segs, int t) { 
   return lo;
 }
 
+// the same by a whole warp: independent reads, where a search would wait for one after the other (each some 200 clocks beside the MMAs)
+__device__ __forceinline__ int seg_of_tile_warp(const int* tiles, int segs, int t) {
+  const int lane = threadIdx.x & 31;
+  int n = 0;
+  for (int e0 = 0; e0 < segs; e0 += 128) {
+    int first[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) first[j] = tiles[min(e0 + 32 * j + lane, segs) + 1];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) n += __popc(__ballot_sync(0xffffffffu, e0 + 32 * j + lane < segs && first[j] <= t));
+  }
+  return n;
+}
+
 struct Tile128 {
   int e, m0, n0;             // m0: first row of this CTA's 128
   int t0, nkt;               // WGRAD128: first row of the reduction (ROWS128: 0); blocks of 128
@@ -189,7 +203,7 @@ __device__ __forceinline__ Tile128 tile128(int tile, int rank, const Gemm128Para
   } else {
     const int pr = tile / nt;
     t.n0 = (tile - pr * nt) * BN;
-    t.e = seg_of_tile(s.tiles, p.E + 1, pr);
+    t.e = seg_of_tile_warp(s.tiles, p.E, pr);               // (E: the rows behind the last)
     const int first = s.start[t.e] + (pr - s.tiles[t.e]) * 256;
     t.m0 = first + rank * 128;
     t.t0 = 0;
