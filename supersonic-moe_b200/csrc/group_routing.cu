@@ -476,10 +476,16 @@ group_routing_bwd_kernel(const L* __restrict__ logits, const int* __restrict__ i
   }
   int sel = lane < K ? idx[r * K + lane] : -1;
   if (sel >= E) sel = -1;
-  float s = 0.f, g = 0.f;
+  float s = 0.f, g = 0.f, slope = 0.f;                   // slope: s (1 - s) of a sigmoid
   if (sel >= 0) {
     const float x = gr_logit(row, sel);
-    s = softmax ? expf(x - top) * inv : 1.f / (1.f + expf(-x));
+    if (softmax) {
+      s = expf(x - top) * inv;
+    } else {
+      s = 1.f / (1.f + expf(-x));
+      const float t = expf(-fabsf(x));
+      slope = t / ((1.f + t) * (1.f + t));
+    }
     g = scale * dscores[r * K + lane];
   }
   float total = s, dot = g * s;
@@ -487,17 +493,20 @@ group_routing_bwd_kernel(const L* __restrict__ logits, const int* __restrict__ i
     total += __shfl_xor_sync(kAll, total, d);
     dot += __shfl_xor_sync(kAll, dot, d);
   }
-  float ds = g;
+  float ds = g, all = dot;                               // all: sum_j ds_j s_j
   if (normalize) {
+    // g_k / D - dot / D^2 = (sum_j s_j (g_k - g_j) + 1e-20 g_k) / D^2, and sum_j ds_j s_j = 1e-20 dot / D^2: where the g are alike (one
+    // expert a token) the left sides are differences of rounded equals
     total += kGrEps;
-    ds = (g - dot / total) / total;
+    float diff = kGrEps * g;
+    for (int j = 0; j < K; ++j) diff = fmaf(__shfl_sync(kAll, s, j), g - __shfl_sync(kAll, g, j), diff);
+    ds = diff / total / total;
+    all = kGrEps * dot / total / total;
   }
-  float all = ds * s;                                    // sum_j ds_j s_j
-  for (int d = 16; d > 0; d >>= 1) all += __shfl_xor_sync(kAll, all, d);
   for (int e = lane; e < E; e += 32)
     gr_store(out, e, softmax && top != -INFINITY ? -all * (expf(gr_logit(row, e) - top) * inv) : 0.f);
   __syncwarp();
-  if (sel >= 0) gr_store(out, sel, softmax ? s * (ds - all) : ds * s * (1.f - s));
+  if (sel >= 0) gr_store(out, sel, softmax ? s * (ds - all) : ds * slope);
 }
 
 }  // namespace smoe

@@ -161,3 +161,23 @@ def test_no_tokens_and_replays(sonicmoe):
     graph.replay()
     want = call(sonicmoe, x, 4, bias, groups=8, top_groups=2)
     assert torch.equal(idx, want[1]) and torch.equal(scores, want[0])
+
+
+@pytest.mark.parametrize("softmax", [False, True])
+@pytest.mark.parametrize("K", [1, 4])
+def test_gradient_of_normalised_weights_that_cannot_move(sonicmoe, softmax, K):
+    """One weight, or all with the same gradient g: their sum does not move, and what is left is 1e-20 g_k / D^2 of each score."""
+    x = randn(33, 24, 7).to(DEV).requires_grad_(True)
+    scores, idx = call(sonicmoe, x, K, softmax=softmax, scale=2.0)
+    grad, = torch.autograd.grad(scores, x, torch.full_like(scores, 1.5))
+    s = G.all_scores(x.detach().cpu().double(), softmax)
+    at = idx.cpu().long()
+    sk = s.gather(1, at)
+    D = sk.sum(-1, keepdim=True)                              # (1e-20 more is no other number)
+    ds = torch.zeros_like(s).scatter_(1, at, (1e-20 * 3.0 / D ** 2).expand(-1, K))
+    if softmax:
+        parts = s * ds, s * (ds * s).sum(-1, keepdim=True)
+        want, mag = parts[0] - parts[1], parts[0] + parts[1]
+    else:
+        want = mag = ds * s * (1 - s)
+    assert ((grad.cpu().double() - want).abs() <= SCORE_TOL * mag + 1e-37).all()
