@@ -540,7 +540,7 @@ int smoe_block128_linear_bwd(const void* dy_bf16, const void* w_fp8, const float
                              int64_t N, int64_t K, int64_t E, int flags, int dw_f32_accumulate, int32_t* status,
                              int32_t* pinned_host_word, void* stream);
 /* SwiGLU experts on routed tokens, inference, in one call: out[t,:] = sum_k scores[t,k] W2[e] (silu(gate) * up) with gate / up
- * interleaved in W1[e] x[t], e = idx[t,k] (valid iff 0 <= e < E, a token's distinct).  w1 [E,2I,H], w2 [E,H,I] with their scales.
+ * interleaved in W1[e] x[t], e = idx[t,k] (valid iff 0 <= e < E; an expert named twice by a token counts twice).  w1 [E,2I,H], w2 [E,H,I] with their scales.
  * scratch: smoe_block128_experts_bytes bytes, 256-byte aligned (-1 for sizes that are not taken; K <= 16). */
 int64_t smoe_block128_experts_bytes(int64_t T, int64_t H, int64_t I, int64_t E, int64_t K);
 int smoe_block128_experts(const void* x_bf16, const int32_t* idx, const float* scores, const void* w1_fp8, const float* w1_scales,

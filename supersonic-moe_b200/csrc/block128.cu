@@ -78,7 +78,7 @@ struct Experts128 {           // everything between the tokens and their sums
   int64_t bytes;
   Experts128(int64_t T, int64_t H, int64_t I, int64_t E, int64_t K, void* base) {
     Arena128 m(base);
-    slots = T * (K < E ? K : E);
+    slots = T * K;
     rows = blocks128(slots) * 128 + E * 128;
     efo = m.ints(E + 1);
     x_gather = m.ints(rows);
@@ -187,7 +187,8 @@ int smoe_block128_experts(const void* x_bf16, const int32_t* idx, const float* s
   if (T == 0) return SMOE_OK;
   if (!x_bf16 || !idx || !scores || !out_bf16 || !scratch) return SMOE_ERR_ARG;
   const Experts128 s(T, H, I, E, K, scratch);
-  SMOE_TRY(smoe_topk_metadata(idx, scores, T, K, E, 128, s.slots, s.rows, 0, 0, s.efo, s.x_gather, s.s_scatter, s.s_rev, s.naept,
+  // (a token's places in the order of its slots: one for each, also where two name one expert)
+  SMOE_TRY(smoe_topk_metadata(idx, scores, T, K, E, 128, s.slots, s.rows, 1, 0, s.efo, s.x_gather, s.s_scatter, s.s_rev, s.naept,
                               s.scores, s.src_idx, s.counts, s.ws, stream));
   const bool few = few_rows128(T, E, K);
   auto product = [&](const void* a, const float* as, const void* w, const float* ws, void* c, int64_t N, int64_t Kr) {

@@ -125,13 +125,15 @@ struct Layout {
   int limit;       // expert-sorted positions at or beyond it are not published
   int tot_p;       // padded rows
   int real_TK;     // entries that are published, naept[N]
+  int entries;     // token-major entries that are written: real_TK, and more where a row names an expert twice
   bool cut;
 };
 
 // s_efo / s_base [E+1]: padded and unpadded offsets from counts(e); the whole block takes part, `first`: this block writes efo
 // and, of a cut pass, naept[N]
-template <typename C>
-__device__ Layout block_layout(const TopkOut& o, C counts, int* s_efo, int* s_base, int* s_warp, bool first) {
+// valid(): entries that idx holds, at most TK_alloc
+template <typename C, typename V>
+__device__ Layout block_layout(const TopkOut& o, C counts, V valid, int* s_efo, int* s_base, int* s_warp, bool first) {
   Layout l;
   const int E = o.E, alignment = o.alignment;
   l.tot_p = block_excl_scan(
@@ -165,6 +167,7 @@ __device__ Layout block_layout(const TopkOut& o, C counts, int* s_efo, int* s_ba
     l.real_TK = min(fit, o.TK_alloc);
     if (first && threadIdx.x == 0) o.naept[o.N] = l.real_TK;
   }
+  l.entries = l.cut ? l.real_TK : max(valid(), l.real_TK);
   return l;
 }
 
@@ -244,8 +247,8 @@ __device__ __forceinline__ void fill_pads(const TopkOut& o, const Layout& l, con
     o.x_gather[pos] = 0;
     o.s_scatter[pos] = sentinel || pos < l.tot_p ? l.real_TK : pos;
   }
-  for (int i = l.real_TK + gtid; i < o.TKp_alloc; i += nthreads) o.scores[i] = 0.f;
-  for (int i = l.real_TK + gtid; i < o.TK_alloc; i += nthreads) {
+  for (int i = l.entries + gtid; i < o.TKp_alloc; i += nthreads) o.scores[i] = 0.f;
+  for (int i = l.entries + gtid; i < o.TK_alloc; i += nthreads) {
     o.s_rev[i] = 0;
     o.src_idx[i] = 0;
   }
@@ -260,7 +263,8 @@ scatter_fill_kernel(const TopkOut o, const uint32_t* __restrict__ mask, const in
   int* s_base = s_mem + (o.E + 1);   // [E+1] unpadded offsets
   int* s_warp = s_base + (o.E + 1);  // [33]
   const int* counts = o.counts;
-  const Layout l = block_layout(o, [&](int e) { return counts[e]; }, s_efo, s_base, s_warp, blockIdx.x == 0);
+  const Layout l = block_layout(
+      o, [&](int e) { return counts[e]; }, [&] { return o.naept[o.N]; }, s_efo, s_base, s_warp, blockIdx.x == 0);
   if ((int)blockIdx.x < scatter_blocks) {
     const int unit = blockIdx.x * ((int)blockDim.x / (32 * KP)) + (threadIdx.x >> 5) / KP;
     scatter_unit<KP>(
@@ -360,7 +364,8 @@ metadata_cluster_kernel(const TopkOut o) {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");      // this CTA has read the others' shared memory
   if (rank == 0 && tid == 0) o.naept[o.N] = min(all_entries, o.TK_alloc);    // (a cut pass writes it again, below)
   __syncthreads();
-  const Layout l = block_layout(o, [&](int e) { return s_tot[e]; }, s_efo, s_base, s_warp, rank == 0);
+  const Layout l = block_layout(
+      o, [&](int e) { return s_tot[e]; }, [&] { return min(all_entries, o.TK_alloc); }, s_efo, s_base, s_warp, rank == 0);
   constexpr int UPB = kMetaThreads / (32 * KP);              // units of a pass over the block
   for (int ub = 0; ub < nu; ub += UPB) {
     const int lu = ub + (tid >> 5) / KP;

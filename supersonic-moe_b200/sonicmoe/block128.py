@@ -114,7 +114,7 @@ def block128_experts(x: torch.Tensor, topk_indices: torch.Tensor, topk_scores: t
     """SwiGLU experts on routed tokens, inference: out[t] = sum_k scores[t,k] W2[e] (silu(gate) * up), gate and up the interleaved rows
     of W1[e] x[t], e = indices[t,k].
 
-    x bf16 [T,H]; topk_indices [T,K] (-1: no expert in this slot; a token's experts distinct), topk_scores [T,K];
+    x bf16 [T,H]; topk_indices [T,K] (-1: no expert in this slot; one that a token names twice counts twice), topk_scores [T,K];
     w1_fp8, w2_fp8: pairs of `quantize_weight_block128` of W1 [E,2I,H] and W2 [E,H,I].  Returns bf16 [T,H].  Both products leave
     bf16; what lies between is quantised in blocks of 128 like x.  No gradient flows."""
     if x.ndim != 2 or x.dtype != torch.bfloat16:

@@ -356,6 +356,22 @@ def test_experts(sonicmoe, T, E, K, H, I):
     assert (out - free).norm() / free.norm() <= 3 * 2.0 ** -4
 
 
+@pytest.mark.parametrize("T,E,K", [(1, 4, 3), (5, 2, 6), (40, 8, 3), (2100, 16, 4)])
+def test_experts_named_twice_count_twice(sonicmoe, T, E, K):
+    H, I = 256, 128
+    x, w1, w2 = randn(T, H, seed=1), randn(E, 2 * I, H, seed=2, scale=H ** -0.5), randn(E, H, I, seed=3, scale=I ** -0.5)
+    g = torch.Generator().manual_seed(T)
+    idx = torch.randint(-1, E, (T, K), generator=g, dtype=torch.int32)
+    idx[-1] = E - 1                                            # the last token: one expert in every slot
+    scores = torch.rand(T, K, generator=g)
+    p1, p2 = (sonicmoe.quantize_weight_block128(w.to(DEV)) for w in (w1, w2))
+    out = sonicmoe.block128_experts(x.to(DEV), idx.to(DEV), scores.to(DEV), p1, p2).cpu().double()
+    ref = experts_reference(x, idx, scores, *(O.deq_weight(*O.quant_weight(w)) for w in (w1, w2)))
+    # as in test_experts, by token: e4m3 values may be half a step off, 2^-4, and the norm is over 256 of them
+    assert ((out - ref).norm(dim=1) <= 2.0 ** -4 * ref.norm(dim=1)).all()
+    assert (out[(idx < 0).all(1)] == 0).all()
+
+
 def test_router_and_experts_in_one_step(sonicmoe):
     """Route, sort, two products with an activation between them, weighted sum; outputs and all gradients against the same step in
     f32 on the values that the operators see, and the inference chain against it."""
