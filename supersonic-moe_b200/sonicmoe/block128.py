@@ -16,16 +16,22 @@ from .functional import _after_accumulate, _grad_target
 _E4M3 = torch.float8_e4m3fn
 
 
+def _dense(t: torch.Tensor) -> torch.Tensor:
+    """Contiguous, from a 16-byte boundary on (a view into a larger buffer need not be)."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 def quantize_rows_block128(x: torch.Tensor, swiglu: bool = False):
     """bf16 [rows,K] -> (e4m3 [rows,K], scales f32 [rows,ceil(K/128)]).  `swiglu`: x is [rows,2K] with gate and up interleaved (what an
     up-projection leaves) and silu(gate) * up is what is quantised, without leaving the chip in between."""
-    q, s = ops.quant128_rows(x.contiguous(), swiglu)
+    q, s = ops.quant128_rows(_dense(x), swiglu)
     return q.view(_E4M3), s
 
 
 def quantize_weight_block128(w: torch.Tensor):
     """bf16 [E,N,K] (or [N,K]) -> (e4m3 of that shape, scales f32 [E,ceil(N/128),ceil(K/128)])."""
-    q, s = ops.quant128_weight(w.detach().contiguous().view(-1, *w.shape[-2:]))
+    q, s = ops.quant128_weight(_dense(w.detach()).view(-1, *w.shape[-2:]))
     return (q.view(_E4M3), s) if w.ndim == 3 else (q[0].view(_E4M3), s[0])
 
 
@@ -52,7 +58,7 @@ class _Block128Linear(torch.autograd.Function):
         q, s, efo, counts, E, N, K = of
         dx, dw, _ = ctx.needs_input_grad
         flags = (ops.B128_QUANT_W if weight is not None else 0) | (ops.B128_DW if dw else 0)
-        y, saved = ops.block128_linear(x, q if weight is None else weight.contiguous(), s, efo, counts, E, N, K, flags)
+        y, saved = ops.block128_linear(x, q if weight is None else _dense(weight), s, efo, counts, E, N, K, flags)
         ctx.save_for_backward(q, s, efo, counts, saved)
         ctx.of = (E, N, K, flags | (ops.B128_DX if dx else 0))
         ctx.weight = weight if dw else None
@@ -65,7 +71,7 @@ class _Block128Linear(torch.autograd.Function):
         w, main_grad = ctx.weight, None
         if w is not None:
             main_grad, base = _grad_target(w, w.shape)
-        dx, dw = ops.block128_linear_bwd(dy if dy.is_contiguous() else dy.contiguous(), q, s, efo, counts, saved, *ctx.of, main_grad)
+        dx, dw = ops.block128_linear_bwd(_dense(dy), q, s, efo, counts, saved, *ctx.of, main_grad)
         if main_grad is not None:
             _after_accumulate(base)
         return dx, None if dw is None else dw.view(w.shape), None
@@ -100,13 +106,13 @@ def block128_linear(x: torch.Tensor, weight, efo: torch.Tensor | None = None, co
     if efo is not None and x.ndim != 2:
         raise ValueError("block128_linear: x is [rows,K] where efo is given")
     ops.check_segments(efo, counts, E, "block128_linear")
-    rows = (x if x.ndim == 2 else x.reshape(-1, K)).contiguous()
+    rows = _dense(x if x.ndim == 2 else x.reshape(-1, K))
     if torch.is_grad_enabled() and (x.requires_grad or (not pair and weight.requires_grad)):
         y = _Block128Linear.apply(rows, weight, (q, s, efo, counts, E, N, K))
     elif pair:
         y = ops.block128_linear(rows, q, s, efo, counts, E, N, K, 0)[0]
     else:
-        y = ops.block128_linear(rows, weight.contiguous(), None, efo, counts, E, N, K, ops.B128_QUANT_W)[0]
+        y = ops.block128_linear(rows, _dense(weight), None, efo, counts, E, N, K, ops.B128_QUANT_W)[0]
     return y if x.ndim == 2 else y.view(*x.shape[:-1], N)
 
 
@@ -129,5 +135,5 @@ def block128_experts(x: torch.Tensor, topk_indices: torch.Tensor, topk_scores: t
         raise ValueError(f"block128_experts: indices {tuple(topk_indices.shape)} and scores {tuple(topk_scores.shape)} of {T} tokens")
     if T == 0 or topk_indices.shape[1] == 0:
         return torch.zeros_like(x)
-    return ops.block128_experts(x.detach().contiguous(), topk_indices.to(torch.int32).contiguous(),
+    return ops.block128_experts(_dense(x.detach()), topk_indices.to(torch.int32).contiguous(),
                                 topk_scores.detach().float().contiguous(), q1, s1, q2, s2, E, I)

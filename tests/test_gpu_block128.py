@@ -552,3 +552,27 @@ def test_repeated_calls_give_the_same_bits(sonicmoe):
         runs.append((y.detach(), a.grad, b.grad, one))
     for run in runs[1:]:
         assert all(torch.equal(p, q) for p, q in zip(run, runs[0]))
+
+
+def test_views_that_begin_off_a_boundary(sonicmoe):
+    """Tensors inside a larger buffer, gradients too, give what copies of them give."""
+    def off(t):
+        buf = torch.zeros(t.numel() + 3, dtype=t.dtype, device=DEV)
+        v = buf[3:].view(t.shape)
+        v.copy_(t)
+        assert v.data_ptr() % 16
+        return v
+
+    x, w, dy = randn(70, 264).to(DEV), randn(1, 136, 264, seed=1).to(DEV), randn(70, 136, seed=2).to(DEV)
+    got = []
+    for f in (lambda t: t, off):
+        a, b = f(x).requires_grad_(True), f(w).requires_grad_(True)
+        y = sonicmoe.block128_linear(a, b)
+        got.append([y.detach(), *torch.autograd.grad(y, (a, b), f(dy)), *sonicmoe.quantize_rows_block128(a.detach()),
+                    *sonicmoe.quantize_weight_block128(b)])
+    for u, v in zip(*got):
+        assert torch.equal(u.float(), v.float())
+    w1, w2 = (sonicmoe.quantize_weight_block128(randn(4, *s, seed=3).to(DEV)) for s in ((256, 264), (264, 128)))
+    scores, idx = torch.rand(70, 4, device=DEV).topk(2)
+    a, b = (sonicmoe.block128_experts(f(x), idx.int(), scores, w1, w2) for f in (lambda t: t, off))
+    assert torch.equal(a, b)
