@@ -148,8 +148,9 @@ int smoe_block128_linear(const void* x_bf16, const void* w, const float* w_scale
   else SMOE_TRY(smoe_quant128_rows(x_bf16, rows, K, 0, nullptr, nullptr, 0, f.xq, f.xs, stream));
   // (segments and weights were complete when the quantiser ahead of the product began)
   if (!efo && rows <= kFewRows)
-    return gemm128_few(f.xq, f.xs, w, w_scales, efo, counts, y_bf16, rows, N, K, E, 0, status, pinned_host_word, true, stream);
-  return gemm128_rows(f.xq, f.xs, w, w_scales, efo, counts, y_bf16, rows, N, K, E, 0, 1, status, pinned_host_word, true, stream);
+    return gemm128_few(f.xq, f.xs, w, w_scales, efo, counts, y_bf16, rows, N, K, E, 0, 0, status, pinned_host_word, true, false,
+                       stream);
+  return gemm128_rows(f.xq, f.xs, w, w_scales, efo, counts, y_bf16, rows, N, K, E, 0, 1, 0, status, pinned_host_word, true, stream);
 }
 
 int smoe_block128_linear_bwd(const void* dy_bf16, const void* w_fp8, const float* w_scales, const int32_t* efo,
@@ -167,7 +168,7 @@ int smoe_block128_linear_bwd(const void* dy_bf16, const void* w_fp8, const float
   if (flags & SMOE_B128_DW) SMOE_TRY(smoe_quant128_dual(dy_bf16, rows, N, efo, counts, E, b.dq, b.ds, b.dc, b.dcs, stream));
   else if (flags & SMOE_B128_DX) SMOE_TRY(smoe_quant128_rows(dy_bf16, rows, N, 0, nullptr, nullptr, 0, b.dq, b.ds, stream));
   if (flags & SMOE_B128_DX)
-    SMOE_TRY(gemm128_rows(b.dq, b.ds, w_fp8, w_scales, efo, counts, dx_bf16, rows, K, N, E, 1, 1, status, pinned_host_word, true,
+    SMOE_TRY(gemm128_rows(b.dq, b.ds, w_fp8, w_scales, efo, counts, dx_bf16, rows, K, N, E, 1, 1, 0, status, pinned_host_word, true,
                           stream));
   if (flags & SMOE_B128_DW)
     SMOE_TRY(gemm128_wgrad(b.dc, b.dcs, sv.xc, sv.xcs, efo, counts, dw, N, K, rows, E, !dw_f32_accumulate, dw_f32_accumulate, status,
@@ -193,8 +194,13 @@ int smoe_block128_experts(const void* x_bf16, const int32_t* idx, const float* s
   const bool few = few_rows128(T, E, K);
   auto product = [&](const void* a, const float* as, const void* w, const float* ws, void* c, int64_t N, int64_t Kr) {
     // (offsets and counts were complete when the quantiser ahead of the product began)
-    return few ? gemm128_few(a, as, w, ws, s.efo, s.counts, c, s.rows, N, Kr, E, s.slots, status, pinned_host_word, true, stream)
-               : gemm128_rows(a, as, w, ws, s.efo, s.counts, c, s.rows, N, Kr, E, 0, 0, status, pinned_host_word, true, stream);
+    if (few)
+      return gemm128_few(a, as, w, ws, s.efo, s.counts, c, s.rows, N, Kr, E, s.slots, 0, status, pinned_host_word, true, false, stream);
+    const int rc = gemm128_rows(a, as, w, ws, s.efo, s.counts, c, s.rows, N, Kr, E, 0, 0, kFewRows, status, pinned_host_word, true, stream);
+    // What is left of an expert after tiles of 256 rows, beside the last of those: its operands were complete when they began
+    return rc ? rc
+              : gemm128_few(a, as, w, ws, s.efo, s.counts, c, s.rows, N, Kr, E, s.slots, 256, status, pinned_host_word, false, true,
+                            stream);
   };
   SMOE_TRY(smoe_quant128_rows_scatter(x_bf16, T, H, s.naept, s.s_rev, s.rows, s.xq, s.xs, stream));
   SMOE_TRY(product(s.xq, s.xs, w1_fp8, w1_scales, s.z, 2 * I, H));

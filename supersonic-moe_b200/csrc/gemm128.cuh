@@ -28,6 +28,7 @@ struct Gemm128Params {
   int out_bf16, accumulate;  // WGRAD128
   int independent;           // of the kernel before in the stream: waited for at the end only
   int zero_rest;             // ROWS128: rows that are not live are written as zero (else left as they are)
+  int skip;                  // ROWS128, without zero_rest: the last tile of a segment is left out if it has no more live rows than these
   int* status;
   volatile int* host_word;   // pinned mirror of *status, or null
 };
@@ -130,23 +131,29 @@ struct Segs128 {
   int *start, *live, *tiles;       // [segs + 1] starts; [segs] ends of the live rows; [segs + 1] row tiles before
 };
 // one warp; segment `E` holds the rows behind the last one, none of them live
+//   skip      what is left of a segment after its full tiles makes a tile only if it is more than `skip` rows
+//   rest_of   tiles are the rests alone, of segments cut into pieces of `rest_of` rows, that fit one tile
 __device__ __forceinline__ void load_segs128(const Segs128& s, const int* efo, const int* counts, int E, int rows, int tile_rows,
-                                             bool live_only, int lane) {
+                                             bool live_only, int skip, int rest_of, int lane) {
   for (int e = lane; e <= E; e += 32) s.start[e] = efo ? min(max(efo[e], 0), rows) : (e == 0 ? 0 : rows);
   if (lane == 0) s.start[E + 1] = rows;
   __syncwarp();
   int run = 0;
   for (int e0 = 0; e0 <= E; e0 += 32) {
     const int e = e0 + lane;
-    int n = 0;
+    int n = 0, rest0 = 0;
     if (e <= E) {
       const int a = s.start[e], end = s.start[e + 1];
       int live = e == E ? a : end;
       if (e < E && counts) live = min(end, a + min(max(counts[e], 0), rows));
       s.live[e] = max(live, a);
       n = max((live_only ? s.live[e] : end) - a, 0);
-      n = (n + tile_rows - 1) / tile_rows;
+      const int rest = n % (rest_of ? rest_of : tile_rows);
+      rest0 = a + n - rest;
+      n = rest_of ? rest > 0 && rest <= tile_rows : n / tile_rows + (rest > skip);
     }
+    __syncwarp();                                         // the starts have been read
+    if (rest_of && e <= E) s.start[e] = rest0;
     int inc = n;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -273,7 +280,7 @@ gemm128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
   const uint32_t bar_scfull = bar_tempty + 8 * S::BUFS, bar_scempty = bar_scfull + 8 * S::SC_SLOTS;
 
   constexpr int PRODUCER = S::EPI_WARPS, ISSUER = S::EPI_WARPS + 1, SCALER = S::EPI_WARPS + 2;
-  if (warp == 2) load_segs128(segs, p.efo, p.counts, p.E, p.rows, 256, false, lane);
+  if (warp == 2) load_segs128(segs, p.efo, p.counts, p.E, p.rows, 256, MODE == ROWS128 && !p.zero_rest, p.skip, 0, lane);
   if (threadIdx.x == 0) {
     for (int s = 0; s < S::STAGES; ++s) {
       mbar_init(bar_full + 8 * s, 1);                     // leader's: its producer arms it, both CTAs' copies credit it

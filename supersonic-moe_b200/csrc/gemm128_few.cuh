@@ -21,6 +21,8 @@ struct Few128Params {
   const float *w_s, *x_s;    // [E, N/128, K/128], [rows, K/128]
   __nv_bfloat16* c;          // [rows, N], live rows only are written
   int split;                 // CTAs of a cluster
+  int rest_of;               // see load_segs128
+  int independent;           // of the kernel before in the stream: waited for at the end only
   int* status;
   volatile int* host_word;
 };
@@ -107,7 +109,7 @@ gemm128_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
   const uint32_t bar_pfull = bar_tempty + 8 * S::ACC, bar_pempty = bar_pfull + 8;
   const uint32_t bar_sfull = bar_pempty + 8, bar_sempty = bar_sfull + 8 * S::SX_SLOTS;
 
-  if (warp == 2) load_segs128(segs, p.efo, p.counts, p.E, p.rows, NT, true, lane);
+  if (warp == 2) load_segs128(segs, p.efo, p.counts, p.E, p.rows, NT, true, 0, p.rest_of, lane);
   if (threadIdx.x == 0) {
     for (int s = 0; s < S::STAGES; ++s) {
       mbar_init(bar_full + 8 * s, 1);
@@ -165,7 +167,7 @@ gemm128_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
         const FewTile128 t = few_tile128(group, nw, p.E, segs);
         for (int i = 0; i < early; ++i) weights(t, k0 + i, i);
       }
-      wait_for_kernel_before();
+      if (!p.independent) wait_for_kernel_before();
       for (int tile = group; tile < n_total && ok; tile += n_groups) {
         const FewTile128 t = few_tile128(tile, nw, p.E, segs);
         for (int k = k0; k < k1; ++k) {
@@ -259,7 +261,7 @@ gemm128_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
       if (lane == 0) mbar_arrive(bar_sfull + 8 * slot);
       ++given;
     };
-    wait_for_kernel_before();                                 // every block, also one without tiles
+    if (!p.independent) wait_for_kernel_before();             // every block, also one without tiles
     at_tile();
     float a0[G], a1[G], b0[G], b1[G];
     if (tile < n_total) {
@@ -392,6 +394,7 @@ gemm128_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
   if (split > 1) cluster_sync_all();          // the others may still read this CTA's sums
   tc_fence_after();
   if (warp == 1) tmem_dealloc(tmem_base, 512);
+  if (p.independent) wait_for_kernel_before();
 }
 
 }  // namespace smoe

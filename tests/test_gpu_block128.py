@@ -372,6 +372,23 @@ def test_experts_named_twice_count_twice(sonicmoe, T, E, K):
     assert (out[(idx < 0).all(1)] == 0).all()
 
 
+@pytest.mark.parametrize("T,E,K", [(1000, 16, 4), (1500, 128, 8), (300, 5, 2)])
+def test_experts_of_very_different_loads(sonicmoe, T, E, K):
+    """Full tiles, long and short rests of them, experts of a few rows and of none, each token against its reference."""
+    H, I = 264, 136
+    x, w1, w2 = randn(T, H, seed=1), randn(E, 2 * I, H, seed=2, scale=H ** -0.5), randn(E, H, I, seed=3, scale=I ** -0.5)
+    g = torch.Generator().manual_seed(T)
+    logits = torch.randn(T, E, generator=g) + 1.5 * torch.randn(E, generator=g)
+    logits[:, 1] = -100.0
+    scores, idx = logits.softmax(-1).topk(K)
+    p1, p2 = (sonicmoe.quantize_weight_block128(w.to(DEV)) for w in (w1, w2))
+    out = sonicmoe.block128_experts(x.to(DEV), idx.int().to(DEV), scores.to(DEV), p1, p2).cpu().double()
+    n = torch.bincount(idx.flatten(), minlength=E)
+    assert n[1] == 0 and ((n % 256 > 0) & (n % 256 <= 64)).any() and (n % 256 > 64).any()
+    ref = experts_reference(x, idx, scores, *(O.deq_weight(*O.quant_weight(w)) for w in (w1, w2)))
+    assert ((out - ref).norm(dim=1) <= 2.0 ** -4 * ref.norm(dim=1)).all()      # as above
+
+
 def test_router_and_experts_in_one_step(sonicmoe):
     """Route, sort, two products with an activation between them, weighted sum; outputs and all gradients against the same step in
     f32 on the values that the operators see, and the inference chain against it."""
