@@ -107,10 +107,12 @@ static bool sizes128(int64_t rows, int64_t N, int64_t K, int64_t E) {
 // Rows of one projection up to which its weights are the wide operand of the product: one tile of rows there, and more CTAs per
 // weight (us with / without at 16, 64 and 128 rows: 4096 x 4096 11 / 19, 14 / 19, 18 / 20; 16384 x 4096 17 / 22, 22 / 22, 36 / 23)
 constexpr int64_t kFewRows = 64;
-// Of routed experts: where an expert's rows, evenly routed, are 32 or fewer, or no expert can have more than one tile of them, reading
-// the weights bounds the product (up and down, us with / without, 128 experts of 2048 x 768: 8 rows 113 / 176, 32 rows 124 / 182,
-// 48 rows 133 / 185, 64 rows 185 / 186; 8 of 4096 x 2048: 44 / 60, 52 / 60, 58 / 62, 77 / 62).  Uneven routing leaves fewer weights
-// to read, and gives some experts a second tile.
+// Of routed experts: where an expert's rows, evenly routed, are 32 or fewer, or none can have more than one tile of them, reading the
+// weights bounds the products, and all of them are of few rows.  Elsewhere tiles of 256 rows, and for the rest of an expert, if that
+// is 64 rows or fewer, the product for few rows.  (us of a call, all of few rows / tiles and rests, 128 experts of 2048 x 768: 16
+// rows an expert 133 / 142, 32 143 / 152, 64 208 / 194, 128 319 / 237; very unevenly routed, most rows at a few experts, 85 / 83,
+// 115 / 103, 184 / 141; 8 of 4096 x 2048: 63 / 70, 67 / 73, 92 / 87, 134 / 89, unevenly 55 / 64, 71 / 86, 83 / 79.  4096 tokens x 8
+// over the 128, tiles alone 329, with rests 333; unevenly 453 and 403.)
 static bool few_rows128(int64_t T, int64_t E, int64_t K) { return T <= kFewRows || T * K <= 32 * E; }
 
 #define SMOE_TRY(call)          \
@@ -148,9 +150,9 @@ int smoe_block128_linear(const void* x_bf16, const void* w, const float* w_scale
   else SMOE_TRY(smoe_quant128_rows(x_bf16, rows, K, 0, nullptr, nullptr, 0, f.xq, f.xs, stream));
   // (segments and weights were complete when the quantiser ahead of the product began)
   if (!efo && rows <= kFewRows)
-    return gemm128_few(f.xq, f.xs, w, w_scales, efo, counts, y_bf16, rows, N, K, E, 0, 0, status, pinned_host_word, true, false,
+    return gemm128_few(f.xq, f.xs, w, w_scales, efo, counts, y_bf16, rows, N, K, E, 0, false, status, pinned_host_word, true, false,
                        stream);
-  return gemm128_rows(f.xq, f.xs, w, w_scales, efo, counts, y_bf16, rows, N, K, E, 0, 1, 0, status, pinned_host_word, true, stream);
+  return gemm128_rows(f.xq, f.xs, w, w_scales, efo, counts, y_bf16, rows, N, K, E, 0, 1, false, status, pinned_host_word, true, stream);
 }
 
 int smoe_block128_linear_bwd(const void* dy_bf16, const void* w_fp8, const float* w_scales, const int32_t* efo,
@@ -168,7 +170,7 @@ int smoe_block128_linear_bwd(const void* dy_bf16, const void* w_fp8, const float
   if (flags & SMOE_B128_DW) SMOE_TRY(smoe_quant128_dual(dy_bf16, rows, N, efo, counts, E, b.dq, b.ds, b.dc, b.dcs, stream));
   else if (flags & SMOE_B128_DX) SMOE_TRY(smoe_quant128_rows(dy_bf16, rows, N, 0, nullptr, nullptr, 0, b.dq, b.ds, stream));
   if (flags & SMOE_B128_DX)
-    SMOE_TRY(gemm128_rows(b.dq, b.ds, w_fp8, w_scales, efo, counts, dx_bf16, rows, K, N, E, 1, 1, 0, status, pinned_host_word, true,
+    SMOE_TRY(gemm128_rows(b.dq, b.ds, w_fp8, w_scales, efo, counts, dx_bf16, rows, K, N, E, 1, 1, false, status, pinned_host_word, true,
                           stream));
   if (flags & SMOE_B128_DW)
     SMOE_TRY(gemm128_wgrad(b.dc, b.dcs, sv.xc, sv.xcs, efo, counts, dw, N, K, rows, E, !dw_f32_accumulate, dw_f32_accumulate, status,
@@ -195,11 +197,11 @@ int smoe_block128_experts(const void* x_bf16, const int32_t* idx, const float* s
   auto product = [&](const void* a, const float* as, const void* w, const float* ws, void* c, int64_t N, int64_t Kr) {
     // (offsets and counts were complete when the quantiser ahead of the product began)
     if (few)
-      return gemm128_few(a, as, w, ws, s.efo, s.counts, c, s.rows, N, Kr, E, s.slots, 0, status, pinned_host_word, true, false, stream);
-    const int rc = gemm128_rows(a, as, w, ws, s.efo, s.counts, c, s.rows, N, Kr, E, 0, 0, kFewRows, status, pinned_host_word, true, stream);
+      return gemm128_few(a, as, w, ws, s.efo, s.counts, c, s.rows, N, Kr, E, s.slots, false, status, pinned_host_word, true, false, stream);
+    const int rc = gemm128_rows(a, as, w, ws, s.efo, s.counts, c, s.rows, N, Kr, E, 0, 0, true, status, pinned_host_word, true, stream);
     // What is left of an expert after tiles of 256 rows, beside the last of those: its operands were complete when they began
     return rc ? rc
-              : gemm128_few(a, as, w, ws, s.efo, s.counts, c, s.rows, N, Kr, E, s.slots, 256, status, pinned_host_word, false, true,
+              : gemm128_few(a, as, w, ws, s.efo, s.counts, c, s.rows, N, Kr, E, s.slots, true, status, pinned_host_word, false, true,
                             stream);
   };
   SMOE_TRY(smoe_quant128_rows_scatter(x_bf16, T, H, s.naept, s.s_rev, s.rows, s.xq, s.xs, stream));

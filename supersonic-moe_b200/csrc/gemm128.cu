@@ -74,7 +74,7 @@ static int check128(const void* a, const float* a_s, const void* b, const float*
 static int64_t up(int64_t n, int64_t m) { return (n + m - 1) / m; }
 
 int gemm128_rows(const void* a_fp8, const float* a_scales, const void* b_fp8, const float* b_scales, const int* efo, const int* counts,
-                 void* c_bf16, int64_t rows, int64_t N, int64_t K, int64_t E, int b_mn, int zero_rest, int skip, int* status,
+                 void* c_bf16, int64_t rows, int64_t N, int64_t K, int64_t E, int b_mn, int zero_rest, bool without_rests, int* status,
                  int* pinned_host_word, bool early, void* stream) {
   int rc = check128(a_fp8, a_scales, b_fp8, b_scales, efo, counts, c_bf16, rows, N, K, E, status);
   if (rc || rows == 0) return rc;
@@ -91,7 +91,7 @@ int gemm128_rows(const void* a_fp8, const float* a_scales, const void* b_fp8, co
   p.bs_e = nb * kb;
   p.bs_n = b_mn ? 1 : kb;
   p.bs_k = b_mn ? (int)nb : 1;
-  p.b_mn = b_mn != 0; p.c = c_bf16; p.zero_rest = zero_rest != 0; p.skip = skip; p.status = status; p.host_word = pinned_host_word;
+  p.b_mn = b_mn != 0; p.c = c_bf16; p.zero_rest = without_rests ? -Few128Smem::NT : zero_rest != 0; p.status = status; p.host_word = pinned_host_word;
   // every segment may end in a tile that is not full, and so may the rows behind the last
   const int64_t tiles = efo ? (rows / 256 + E + 1) * up(N, 256) : up(rows, 256) * up(N, 256);
   return launch128<ROWS128>(ta, tb, tc, p, tiles, early, (cudaStream_t)stream);
@@ -123,7 +123,7 @@ int gemm128_wgrad(const void* a_fp8, const float* a_scales, const void* b_fp8, c
 }
 
 int gemm128_few(const void* a_fp8, const float* a_scales, const void* b_fp8, const float* b_scales, const int* efo, const int* counts,
-                void* c_bf16, int64_t rows, int64_t N, int64_t K, int64_t E, int64_t live_rows, int rest_of, int* status,
+                void* c_bf16, int64_t rows, int64_t N, int64_t K, int64_t E, int64_t live_rows, bool rests, int* status,
                 int* pinned_host_word, bool early, bool independent, void* stream) {
   int rc = check128(a_fp8, a_scales, b_fp8, b_scales, efo, counts, c_bf16, rows, N, K, E, status);
   if (rc || rows == 0) return rc;
@@ -137,7 +137,7 @@ int gemm128_few(const void* a_fp8, const float* a_scales, const void* b_fp8, con
   if (!ensure_smem_attr(gemm128_few_kernel, Few128Smem::TOTAL, attr_set)) return SMOE_ERR_LAUNCH;
   const int sms = sm_count();
   const int64_t nw = up(N, 128), busy = live_rows < E ? live_rows : E;
-  const int64_t tiles = (rest_of ? busy : (live_rows + (Few128Smem::NT - 1) * busy) / Few128Smem::NT) * nw;      // as many as there can be
+  const int64_t tiles = (rests ? busy : (live_rows + (Few128Smem::NT - 1) * busy) / Few128Smem::NT) * nw;      // as many as there can be
   // Few tiles are shared by clusters while each CTA keeps three blocks of a reduction of twelve or more (us at 16 rows with 1 / 2 / 4
   // CTAs: 4096 x 4096 15.0 / 12.3 / 11.2, 2048 x 1536 8.2 / 8.4 / 7.7, 8192 x 2048 10.6 / 10.6 / -; 1024 x 1024 7.0 / 7.8 / 7.4,
   // 2048 x 768 6.4 / 7.5 / 7.3).  Eight find room together on half of the SMs only, as they come from one part of the chip (with 8
@@ -145,7 +145,7 @@ int gemm128_few(const void* a_fp8, const float* a_scales, const void* b_fp8, con
   const int64_t kb = up(K, 128);
   int split = 1;
   while (split < 8 && kb >= 12 && split * 6 <= kb && tiles * split * (split == 4 ? 4 : 2) <= sms) split *= 2;
-  Few128Params p{(int)rows, (int)N, (int)K, (int)E, efo, counts, b_scales, a_scales, (__nv_bfloat16*)c_bf16, split, rest_of,
+  Few128Params p{(int)rows, (int)N, (int)K, (int)E, efo, counts, b_scales, a_scales, (__nv_bfloat16*)c_bf16, split, rests ? 256 : 0,
                  independent, status, pinned_host_word};
   int64_t groups = sms / split;
   if (tiles < groups) groups = tiles;
@@ -175,7 +175,7 @@ extern "C" {
 int smoe_gemm128_rows(const void* a_fp8, const float* a_scales, const void* b_fp8, const float* b_scales, const int32_t* efo,
                       const int32_t* counts, void* c_bf16, int64_t rows, int64_t N, int64_t K, int64_t E, int b_mn,
                       int zero_rest, int32_t* status, int32_t* pinned_host_word, void* stream) {
-  return gemm128_rows(a_fp8, a_scales, b_fp8, b_scales, efo, counts, c_bf16, rows, N, K, E, b_mn, zero_rest, 0, status,
+  return gemm128_rows(a_fp8, a_scales, b_fp8, b_scales, efo, counts, c_bf16, rows, N, K, E, b_mn, zero_rest, false, status,
                       pinned_host_word, false, stream);
 }
 
@@ -189,7 +189,7 @@ int smoe_gemm128_wgrad(const void* a_fp8, const float* a_scales, const void* b_f
 int smoe_gemm128_few(const void* a_fp8, const float* a_scales, const void* b_fp8, const float* b_scales, const int32_t* efo,
                      const int32_t* counts, void* c_bf16, int64_t rows, int64_t N, int64_t K, int64_t E, int64_t live_rows,
                      int32_t* status, int32_t* pinned_host_word, void* stream) {
-  return gemm128_few(a_fp8, a_scales, b_fp8, b_scales, efo, counts, c_bf16, rows, N, K, E, live_rows, 0, status, pinned_host_word,
+  return gemm128_few(a_fp8, a_scales, b_fp8, b_scales, efo, counts, c_bf16, rows, N, K, E, live_rows, false, status, pinned_host_word,
                      false, false, stream);
 }
 

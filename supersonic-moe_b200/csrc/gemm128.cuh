@@ -5,8 +5,11 @@
 //
 // f32 scales are not what the block-scaled MMA takes (powers of two, 32 wide), so the plain e4m3 MMA sums one block of 128 at a
 // time into TMEM and the epilogue warps add it, scaled, to sums that stay in their registers: 128 f32 a thread, 256 x 256 outputs
-// a CTA pair.  Two TMEM buffers of 256 columns: the MMAs of one block (512 clocks) run while the block before is read out (256
-// clocks of TMEM reads, half as many of packed multiply-adds).
+// a CTA pair.  Two TMEM buffers of 256 columns: the MMAs of one block run while the block before is read out and added up.
+//   What bounds it: by rows, shared memory, out of which the MMAs of a block (512 clocks of arithmetic) read their operands in some
+//   640; a block takes 750, and a tile some 3400 clocks beside its blocks.  8192 x 4096 x 4096 123 us (2.2 PFLOP/s), 16384 x 4096 x
+//   2048 over 8 experts 133, its dx 128.  The weight gradient: the arithmetic of the epilogue, where a value has two scales of its
+//   own in every block; the same size 191 us (1.4 PFLOP/s), added to f32 221.
 //   B [E, N, K] is read K-major, or with b_mn as [E, K, N] as it lies: the gradient of the rows needs no transposed weights.
 //   Both operands of the weight gradient lie [dim, rows].
 #pragma once
@@ -27,8 +30,8 @@ struct Gemm128Params {
   void* c;                   // ROWS128: bf16 [rows, N]; WGRAD128: [E, M, N] f32 or bf16
   int out_bf16, accumulate;  // WGRAD128
   int independent;           // of the kernel before in the stream: waited for at the end only
-  int zero_rest;             // ROWS128: rows that are not live are written as zero (else left as they are)
-  int skip;                  // ROWS128, without zero_rest: the last tile of a segment is left out if it has no more live rows than these
+  int zero_rest;             // ROWS128: rows that are not live are written as zero (else left as they are; if it is below zero, the
+                             // last tile of a segment is left out where it has no more live rows than - zero_rest)
   int* status;
   volatile int* host_word;   // pinned mirror of *status, or null
 };
@@ -70,8 +73,8 @@ struct Gemm128Smem {
 };
 
 // tcgen05.mma kind::f8f6f4: e4m3 x e4m3 -> f32
-__host__ __device__ constexpr uint32_t make_idesc_f8(int M, int N, bool a_mn, bool b_mn) {
-  return (1u << 4) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+__host__ __device__ constexpr uint32_t make_idesc_f8(int M, int N, bool b_mn) {
+  return (1u << 4) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 __device__ __forceinline__ void mma_f8_pair_lo(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t desc_hi, uint32_t idesc,
                                                uint32_t accumulate) {
@@ -132,7 +135,8 @@ struct Segs128 {
 };
 // one warp; segment `E` holds the rows behind the last one, none of them live
 //   skip      what is left of a segment after its full tiles makes a tile only if it is more than `skip` rows
-//   rest_of   tiles are the rests alone, of segments cut into pieces of `rest_of` rows, that fit one tile
+//   rest_of   (RESTS) if not 0, tiles are the rests alone, of segments cut into pieces of `rest_of` rows, that fit one tile
+template <bool RESTS>
 __device__ __forceinline__ void load_segs128(const Segs128& s, const int* efo, const int* counts, int E, int rows, int tile_rows,
                                              bool live_only, int skip, int rest_of, int lane) {
   for (int e = lane; e <= E; e += 32) s.start[e] = efo ? min(max(efo[e], 0), rows) : (e == 0 ? 0 : rows);
@@ -148,12 +152,18 @@ __device__ __forceinline__ void load_segs128(const Segs128& s, const int* efo, c
       if (e < E && counts) live = min(end, a + min(max(counts[e], 0), rows));
       s.live[e] = max(live, a);
       n = max((live_only ? s.live[e] : end) - a, 0);
-      const int rest = n % (rest_of ? rest_of : tile_rows);
-      rest0 = a + n - rest;
-      n = rest_of ? rest > 0 && rest <= tile_rows : n / tile_rows + (rest > skip);
+      if (RESTS && rest_of) {
+        const int rest = n % rest_of;
+        rest0 = a + n - rest;
+        n = rest > 0 && rest <= tile_rows;
+      } else {
+        n = (n + tile_rows - 1 - skip) / tile_rows;
+      }
     }
-    __syncwarp();                                         // the starts have been read
-    if (rest_of && e <= E) s.start[e] = rest0;
+    if (RESTS) {
+      __syncwarp();                                       // the starts have been read
+      if (rest_of && e <= E) s.start[e] = rest0;
+    }
     int inc = n;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -215,7 +225,7 @@ __device__ __forceinline__ Tile128 tile128(int tile, int rank, const Gemm128Para
     t.m0 = first + rank * 128;
     t.t0 = 0;
     t.live = s.live[t.e];
-    t.end = p.zero_rest ? s.start[t.e + 1] : t.live;
+    t.end = p.zero_rest > 0 ? s.start[t.e + 1] : t.live;
     t.nkt = first < t.live ? (p.K + 127) / 128 : 0;
   }
   return t;
@@ -280,7 +290,7 @@ gemm128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
   const uint32_t bar_scfull = bar_tempty + 8 * S::BUFS, bar_scempty = bar_scfull + 8 * S::SC_SLOTS;
 
   constexpr int PRODUCER = S::EPI_WARPS, ISSUER = S::EPI_WARPS + 1, SCALER = S::EPI_WARPS + 2;
-  if (warp == 2) load_segs128(segs, p.efo, p.counts, p.E, p.rows, 256, MODE == ROWS128 && !p.zero_rest, p.skip, 0, lane);
+  if (warp == 2) load_segs128<false>(segs, p.efo, p.counts, p.E, p.rows, 256, MODE == ROWS128 && p.zero_rest <= 0, MODE == ROWS128 ? -min(p.zero_rest, 0) : 0, 0, lane);
   if (threadIdx.x == 0) {
     for (int s = 0; s < S::STAGES; ++s) {
       mbar_init(bar_full + 8 * s, 1);                     // leader's: its producer arms it, both CTAs' copies credit it
@@ -347,7 +357,7 @@ gemm128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
     // ------------------------------------------------------------ MMA issuer (leader CTA only)
     if (rank == 0) {
       const bool b_mn = MODE == ROWS128 && p.b_mn;
-      const uint32_t idesc = make_idesc_f8(256, BN, false, b_mn);
+      const uint32_t idesc = make_idesc_f8(256, BN, b_mn);
       // operand descriptors: see make_desc_kmajor_sw128 / make_desc_mnmajor_sw128; a step of 32 along the reduction is 32 bytes
       // (K-major) or 32 rows of 128 bytes
       const uint32_t desc_hi = (1024u >> 4) | (1u << 14) | (2u << 29);

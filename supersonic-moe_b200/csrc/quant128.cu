@@ -3,7 +3,8 @@
 //   a = max(max |x| of the block, 2^-100),  scale = a / 448,  q = e4m3(x * (448 / a)),  each step rounded once in f32
 //
 // (the multiplier is the rounded quotient 448 / a, so that a block costs one division more and not one for each value).  NaN is
-// no magnitude: it stays NaN in the payload and leaves its block's scale alone.  All three are bound by HBM: one read, one write.
+// no magnitude: it stays NaN in the payload and leaves its block's scale alone.  Rows and weights are bound by HBM, one read, one
+// write: 8192 x 4096 rows 22.7 us (4.5 TB/s), weights 8 x 4096 x 2048 34 us (5.9 TB/s).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -185,8 +186,9 @@ __global__ void __launch_bounds__(256, PER == 4 ? 4 : 6) quant128_rows_kernel(co
 // A block holds a tile in registers (eight rows of eight values a thread) and takes from it what is asked for: a scale a row, a
 // scale a column, or one for all.  ROWS and COLS from one read is what a training step needs of an activation and of a
 // gradient: the row form feeds the products over columns, the column form the weight gradient, whose sum runs over rows.
-// The column form leaves transposed: the tensor core reads 8-bit operands whose reduction is not contiguous at half the rate out of
-// shared memory (the weight gradient's MMAs: 950 clocks a block against 650).
+// The column form leaves transposed: a copy of the weight gradient's operands then starts on 16 bytes wherever a segment does, and the
+// reduction is contiguous, which the MMAs read out of shared memory in 650 clocks a block (950 otherwise; the epilogue hides either).
+// Bound by the issue of instructions (72 % of the slots, 3.8 TB/s of HBM): 16384 x 4096 to both forms 58 us, 41 at the copy rate.
 //   efo, counts (column form): rows of a segment behind its live ones count as zero and leave zero; tiles without live rows stay
 //   unwritten
 struct Tile128Args {

@@ -35,15 +35,16 @@ int gemm_varlen_m_few(const void* a_fp8, const void* a_sf, const void* b_fp8, co
                       const int* counts, void* c_bf16, int64_t rows, int64_t N, int64_t K, int64_t E, int* status, bool early,
                       void* stream);
 // The block-128 products as the calls that launch a whole pass make them.  `early` as above, for efo, counts and (few rows) weights;
-// `independent`: the kernel neither reads nor writes what the one before it does, and only ends after it.
+// `independent`: the kernel reads nothing that the one before it writes, writes elsewhere, and only ends after it.  `without_rests` (rows
+// that are not live are left) / `rests`: see load_segs128; the two share a product.
 int gemm128_rows(const void* a_fp8, const float* a_scales, const void* b_fp8, const float* b_scales, const int* efo, const int* counts,
-                 void* c_bf16, int64_t rows, int64_t N, int64_t K, int64_t E, int b_mn, int zero_rest, int skip, int* status,
+                 void* c_bf16, int64_t rows, int64_t N, int64_t K, int64_t E, int b_mn, int zero_rest, bool without_rests, int* status,
                  int* pinned_host_word, bool early, void* stream);
 int gemm128_wgrad(const void* a_fp8, const float* a_scales, const void* b_fp8, const float* b_scales, const int* efo, const int* counts,
                   void* c, int64_t M, int64_t N, int64_t rows, int64_t E, int out_bf16, int accumulate, int* status,
                   int* pinned_host_word, bool independent, void* stream);
 int gemm128_few(const void* a_fp8, const float* a_scales, const void* b_fp8, const float* b_scales, const int* efo, const int* counts,
-                void* c_bf16, int64_t rows, int64_t N, int64_t K, int64_t E, int64_t live_rows, int rest_of, int* status,
+                void* c_bf16, int64_t rows, int64_t N, int64_t K, int64_t E, int64_t live_rows, bool rests, int* status,
                 int* pinned_host_word, bool early, bool independent, void* stream);
 }  // namespace smoe
 #endif
