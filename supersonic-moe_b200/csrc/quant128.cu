@@ -41,7 +41,9 @@ __device__ __forceinline__ uint2 q128_pack8(const uint4& v, float m) {
                     q128_pack4(q128_lo(v.z) * m, q128_hi(v.z) * m, q128_lo(v.w) * m, q128_hi(v.w) * m));
 }
 
-__device__ __forceinline__ float q128_silu(float g) {       // to some 1e-7 and |g| roundings of the exponent
+// To some 1e-7 and |g| roundings of the exponent: of 12.6 M e4m3 values 18.8 fall to another side of a step than in 64 bits (mean of
+// eight batches), with expf and the quotient 17.8, and 32768 x 768 take 31 us instead of 25.
+__device__ __forceinline__ float q128_silu(float g) {
   float e, r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(-1.4426950408889634f * g));
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
