@@ -367,8 +367,11 @@ gemm128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
       int stage = 0, as = 0;
       uint32_t phase = 0, aphase = 0;
       bool ok = true;
+      auto blocks_of = [&](int tile) { return tile < n_total ? __shfl_sync(0xffffffffu, tile128<MODE>(tile, 0, p, segs).nkt, 0) : 0; };
+      int next_nkt = blocks_of(pair_id);
       for (int tile = pair_id; tile < n_total && ok; tile += n_pairs) {
-        const int nkt = __shfl_sync(0xffffffffu, tile128<MODE>(tile, 0, p, segs).nkt, 0);
+        const int nkt = next_nkt;
+        if (nkt == 0) next_nkt = blocks_of(tile + n_pairs);
         for (int k = 0; k < nkt; ++k) {
           // (the operands first: they are there long before the buffer is, and a look at a barrier takes some 200 clocks while the
           // MMAs read shared memory)
@@ -387,6 +390,7 @@ gemm128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
           }
           if (++stage == S::STAGES) { stage = 0; phase ^= 1; }
           if (++as == S::BUFS) { as = 0; aphase ^= 1; }
+          if (k == 0) next_nkt = blocks_of(tile + n_pairs);       // (some 700 clocks, under this tile's MMAs)
         }
       }
       if (!ok && lane == 0) { *s_abort = 1; fail128(p.status, p.host_word, 402); }
