@@ -593,3 +593,51 @@ def test_views_that_begin_off_a_boundary(sonicmoe):
     scores, idx = torch.rand(70, 4, device=DEV).topk(2)
     a, b = (sonicmoe.block128_experts(f(x), idx.int(), scores, w1, w2) for f in (lambda t: t, off))
     assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_a_captured_training_step(sonicmoe, accumulate):
+    """Router, projection and all gradients from one graph, replayed on new values, one replay after another."""
+    efo, counts, rows = table([300, 0, 129, 70])
+    e, n = efo.to(DEV), counts.to(DEV)
+    make = lambda seed: (randn(rows, 264, seed=seed), randn(4, 136, 264, seed=seed + 1), randn(rows, 136, seed=seed + 2),
+                         torch.randn(65, 16, generator=torch.Generator().manual_seed(seed + 3)))
+
+    def step(x, w, dy, logits):
+        y = sonicmoe.block128_linear(x, w, e, n)
+        scores, idx = sonicmoe.group_limited_routing(logits, 3, groups=4, top_groups=2)
+        # (with a main_grad w's gradient goes there on the way, and None comes back)
+        grads = torch.autograd.grad((y, scores), (x, logits, w), (dy, scores.detach() * 2 + 1), allow_unused=True)
+        return [y.detach(), scores.detach(), idx, *(g for g in grads if g is not None)]
+
+    def leaves(seed):
+        x, w, dy, logits = (t.to(DEV) for t in make(seed))
+        x, w, logits = (t.requires_grad_(True) for t in (x, w, logits))
+        if accumulate:
+            w.main_grad = torch.zeros(4, 136, 264, device=DEV)
+        return x, w, dy, logits
+
+    wants = []
+    for seed in (10, 20):
+        t = leaves(seed)
+        wants.append([v.clone() for v in step(*t)] + ([t[1].main_grad.clone()] if accumulate else []))
+    static = leaves(30)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step(*static)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step(*static)
+    for seed, want in zip((10, 20), wants):
+        with torch.no_grad():
+            for a, b in zip(static, make(seed)):
+                a.copy_(b)
+            if accumulate:
+                static[1].main_grad.zero_()
+        graph.replay()
+        graph.replay()
+        got = list(outs) + ([static[1].main_grad / 2] if accumulate else [])      # added twice: x + x is exact
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+    sonicmoe.ops.check_status(DEV)
