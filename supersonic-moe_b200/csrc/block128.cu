@@ -2,6 +2,7 @@
 // and routed SwiGLU experts.  The kernels of small problems end before a caller has issued them one by one.
 #include <cuda_runtime.h>
 
+#include "host.h"
 #include "smoe_b200.h"
 #include "smoe_internal.h"
 
@@ -104,16 +105,22 @@ static bool sizes128(int64_t rows, int64_t N, int64_t K, int64_t E) {
          K < (int64_t)1 << 24 && E > 0 && E <= 256;
 }
 
-// Rows of one projection up to which its weights are the wide operand of the product: one tile of rows there, and more CTAs per
-// weight (us with / without at 16, 64 and 128 rows: 4096 x 4096 11 / 19, 14 / 19, 18 / 20; 16384 x 4096 17 / 22, 22 / 22, 36 / 23)
+// The weights are the wide operand of a product of so few rows that they make one tile
 constexpr int64_t kFewRows = 64;
+// One projection: also where tiles of 128 weight rows x 64 leave half of the SMs or more, which then share the tiles' reductions (us
+// with / without, at 64, 128 and 256 rows: 4096 x 4096 13.5 / 19.5, 17.6 / 20.5, 21.3 / 20.5; 1024 x 4096 10 / 19, 12 / 19, 12.5 / 19;
+// 2048 x 8192 16 / 33, 17 / 34, 24 / 34, at 384 35.0 / 34.0; 8192 x 2048 13.8 / 13.4, 14.2 / 14.2, 20.5 / 14.2; 16384 x 4096 at 16, 64
+// and 128: 17 / 22, 22 / 22, 36 / 23).
+static bool few_rows128(int64_t rows, int64_t N) {
+  return rows <= kFewRows || (rows + kFewRows - 1) / kFewRows * blocks128(N) * 2 <= sm_count();
+}
 // Of routed experts: where an expert's rows, evenly routed, are 32 or fewer, or none can have more than one tile of them, reading the
 // weights bounds the products, and all of them are of few rows.  Elsewhere tiles of 256 rows, and for the rest of an expert, if that
 // is 64 rows or fewer, the product for few rows.  (us of a call, all of few rows / tiles and rests, 128 experts of 2048 x 768: 16
 // rows an expert 133 / 142, 32 143 / 152, 64 208 / 194, 128 319 / 237; very unevenly routed, most rows at a few experts, 85 / 83,
 // 115 / 103, 184 / 141; 8 of 4096 x 2048: 63 / 70, 67 / 73, 92 / 87, 134 / 89, unevenly 55 / 64, 71 / 86, 83 / 79.  4096 tokens x 8
 // over the 128, tiles alone 329, with rests 333; unevenly 453 and 403.)
-static bool few_rows128(int64_t T, int64_t E, int64_t K) { return T <= kFewRows || T * K <= 32 * E; }
+static bool few_experts128(int64_t T, int64_t E, int64_t K) { return T <= kFewRows || T * K <= 32 * E; }
 
 #define SMOE_TRY(call)          \
   do {                          \
@@ -149,7 +156,7 @@ int smoe_block128_linear(const void* x_bf16, const void* w, const float* w_scale
   if (flags & SMOE_B128_DW) SMOE_TRY(smoe_quant128_dual(x_bf16, rows, K, efo, counts, E, f.xq, f.xs, sv.xc, sv.xcs, stream));
   else SMOE_TRY(smoe_quant128_rows(x_bf16, rows, K, 0, nullptr, nullptr, 0, f.xq, f.xs, stream));
   // (segments and weights were complete when the quantiser ahead of the product began)
-  if (!efo && rows <= kFewRows)
+  if (!efo && few_rows128(rows, N))
     return gemm128_few(f.xq, f.xs, w, w_scales, efo, counts, y_bf16, rows, N, K, E, 0, false, status, pinned_host_word, true, false,
                        stream);
   return gemm128_rows(f.xq, f.xs, w, w_scales, efo, counts, y_bf16, rows, N, K, E, 0, 1, false, status, pinned_host_word, true, stream);
@@ -193,7 +200,7 @@ int smoe_block128_experts(const void* x_bf16, const int32_t* idx, const float* s
   // (a token's places in the order of its slots: one for each, also where two name one expert)
   SMOE_TRY(smoe_topk_metadata(idx, scores, T, K, E, 128, s.slots, s.rows, 1, 0, s.efo, s.x_gather, s.s_scatter, s.s_rev, s.naept,
                               s.scores, s.src_idx, s.counts, s.ws, stream));
-  const bool few = few_rows128(T, E, K);
+  const bool few = few_experts128(T, E, K);
   auto product = [&](const void* a, const float* as, const void* w, const float* ws, void* c, int64_t N, int64_t Kr) {
     // (offsets and counts were complete when the quantiser ahead of the product began)
     if (few)
