@@ -497,13 +497,15 @@ group_routing_bwd_kernel(const L* __restrict__ logits, const int* __restrict__ i
   }
   float ds = g, all = dot;                               // all: sum_j ds_j s_j
   if (normalize) {
-    // g_k / D - dot / D^2 = (sum_j s_j (g_k - g_j) + 1e-20 g_k) / D^2, and sum_j ds_j s_j = 1e-20 dot / D^2: where the g are alike (one
-    // expert a token) the left sides are differences of rounded equals
+    // g_k / D - dot / D^2 = (sum_j s_j (g_k - g_j) + eps g_k) / D^2, and sum_j ds_j s_j = eps dot / D^2, with eps what the 1e-20 adds to
+    // the f32 sum: where the g are alike (one expert a token) the left sides are differences of rounded equals
+    const float sum = total;
     total += kGrEps;
-    float diff = kGrEps * g;
+    const float eps = total - sum;
+    float diff = eps * g;
     for (int j = 0; j < K; ++j) diff = fmaf(__shfl_sync(kAll, s, j), g - __shfl_sync(kAll, g, j), diff);
     ds = diff / total / total;
-    all = kGrEps * dot / total / total;
+    all = eps * dot / total / total;
   }
   for (int e = lane; e < E; e += 32)
     gr_store(out, e, softmax && top != -INFINITY ? -all * (expf(gr_logit(row, e) - top) * inv) : 0.f);

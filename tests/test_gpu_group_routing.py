@@ -166,18 +166,21 @@ def test_no_tokens_and_replays(sonicmoe):
 @pytest.mark.parametrize("softmax", [False, True])
 @pytest.mark.parametrize("K", [1, 4])
 def test_gradient_of_normalised_weights_that_cannot_move(sonicmoe, softmax, K):
-    """One weight, or all with the same gradient g: their sum does not move, and what is left is 1e-20 g_k / D^2 of each score."""
+    """One weight, or all with the same gradient: their sum does not move (1e-20 is no part of these sums in f32)."""
     x = randn(33, 24, 7).to(DEV).requires_grad_(True)
-    scores, idx = call(sonicmoe, x, K, softmax=softmax, scale=2.0)
+    scores, _ = call(sonicmoe, x, K, softmax=softmax, scale=2.0)
     grad, = torch.autograd.grad(scores, x, torch.full_like(scores, 1.5))
-    s = G.all_scores(x.detach().cpu().double(), softmax)
-    at = idx.cpu().long()
-    sk = s.gather(1, at)
-    D = sk.sum(-1, keepdim=True)                              # (1e-20 more is no other number)
-    ds = torch.zeros_like(s).scatter_(1, at, (1e-20 * 3.0 / D ** 2).expand(-1, K))
-    if softmax:
-        parts = s * ds, s * (ds * s).sum(-1, keepdim=True)
-        want, mag = parts[0] - parts[1], parts[0] + parts[1]
-    else:
-        want = mag = ds * s * (1 - s)
-    assert ((grad.cpu().double() - want).abs() <= SCORE_TOL * mag + 1e-37).all()
+    assert (grad == 0).all()
+
+
+def test_gradient_where_the_sum_is_as_small_as_what_is_added_to_it(sonicmoe):
+    """s / (s + 1e-20) with s about 1e-20: 1e-20 g s (1 - s) / (s + 1e-20)^2 at the expert chosen."""
+    x = (randn(40, 24, 8) - 46.0).to(DEV).requires_grad_(True)
+    scores, idx = call(sonicmoe, x, 1)
+    grad, = torch.autograd.grad(scores, x, torch.full_like(scores, 1.5))
+    s = torch.sigmoid(x.detach().cpu().double())
+    want = torch.zeros_like(s).scatter_(1, idx.cpu().long(), 1.5)
+    want = want * 1e-20 * s * (1 - s) / (s + 1e-20) ** 2
+    assert want.abs().max() > 0.1
+    # exp of 46 +- 6: its argument's rounding is 2^-24 of at most 52, and the score enters three times
+    assert ((grad.cpu().double() - want).abs() <= (3 * 52 + 64) * 2.0 ** -24 * want).all()
