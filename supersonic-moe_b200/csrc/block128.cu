@@ -211,9 +211,9 @@ int smoe_block128_experts(const void* x_bf16, const int32_t* idx, const float* s
               : gemm128_few(a, as, w, ws, s.efo, s.counts, c, s.rows, N, Kr, E, s.slots, true, status, pinned_host_word, false, true,
                             stream);
   };
-  SMOE_TRY(smoe_quant128_rows_scatter(x_bf16, T, H, s.naept, s.s_rev, s.rows, s.xq, s.xs, stream));
+  SMOE_TRY(quant128_rows_scatter(x_bf16, T, H, s.naept, s.s_rev, s.rows, s.xq, s.xs, true, stream));
   SMOE_TRY(product(s.xq, s.xs, w1_fp8, w1_scales, s.z, 2 * I, H));
-  SMOE_TRY(smoe_quant128_rows(s.z, s.rows, I, 1, s.s_rev, s.naept + T, s.slots, s.yq, s.ys, stream));
+  SMOE_TRY(quant128_rows(s.z, s.rows, I, 1, s.s_rev, s.naept + T, s.slots, s.yq, s.ys, true, stream));
   SMOE_TRY(product(s.yq, s.ys, w2_fp8, w2_scales, s.o, H, I));
   return smoe_combine(s.o, s.s_rev, s.naept, s.scores, out_bf16, T, H, stream);
 }

@@ -140,6 +140,7 @@ gemm128_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   const uint32_t smem_base = smem_u32(smem);
+  next_kernel_may_start();                    // (which waits for this one's end before it touches anything)
   const int nw = (p.N + BM - 1) / BM, nkt = (p.K + 127) / 128;
   const int n_total = segs.tiles[p.E] * nw;
   const int k0 = rank * nkt / split, k1 = (rank + 1) * nkt / split;        // split <= nkt: nobody is without

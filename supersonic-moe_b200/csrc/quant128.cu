@@ -11,6 +11,7 @@
 
 #include "ptx.cuh"
 #include "smoe_b200.h"
+#include "smoe_internal.h"
 
 namespace smoe {
 
@@ -99,6 +100,7 @@ struct Rows128Args {
 
 template <bool GLU, int PER>
 __global__ void __launch_bounds__(256, PER == 4 ? 4 : 6) quant128_rows_kernel(const Rows128Args a) {
+  wait_for_kernel_before();                               // (a launch of `chained`; the next one counts on it)
   next_kernel_may_start();
   const int kb = (a.K + 127) / 128;
   const int64_t n = a.list && a.n_live ? min((int64_t)*a.n_live, a.n) : a.n;
@@ -326,7 +328,7 @@ static int quant128_check(const void* x, const void* q, const void* s, int64_t r
   return SMOE_OK;
 }
 
-static int launch_rows(const Rows128Args& a, bool glu, void* stream) {
+static int launch_rows(const Rows128Args& a, bool glu, bool chained, void* stream) {
   if (a.n == 0 || a.out_rows == 0) return SMOE_OK;
   const int64_t units = a.n * ((a.K + 127) / 128);
   // Several blocks each where that leaves every SM enough warps: four, or two where the activation's or a token's many rows need
@@ -339,8 +341,36 @@ static int launch_rows(const Rows128Args& a, bool glu, void* stream) {
               : per == 4 ? quant128_rows_kernel<false, 4>
               : per == 2 ? quant128_rows_kernel<false, 2>
                          : quant128_rows_kernel<false, 1>;
-  kern<<<(unsigned)grid, 256, 0, (cudaStream_t)stream>>>(a);
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(256);
+  cfg.stream = (cudaStream_t)stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = chained ? 1 : 0;
+  if (cudaLaunchKernelEx(&cfg, kern, a) != cudaSuccess) return SMOE_ERR_LAUNCH;
   return cudaGetLastError() == cudaSuccess ? SMOE_OK : SMOE_ERR_LAUNCH;
+}
+
+int quant128_rows(const void* x_bf16, int64_t rows, int64_t K, int swiglu, const int* list, const int* n_live, int64_t n_list, void* q,
+                  float* scales, bool chained, void* stream) {
+  const int rc = quant128_check(x_bf16, q, scales, rows, K);
+  if (rc) return rc;
+  if (list && (n_list < 0 || !n_live)) return SMOE_ERR_ARG;
+  Rows128Args a{x_bf16, list ? n_list : rows, rows, (int)K, list, n_live, nullptr, nullptr, (uint8_t*)q, scales};
+  return launch_rows(a, swiglu != 0, chained, stream);
+}
+
+int quant128_rows_scatter(const void* x_bf16, int64_t T, int64_t K, const int* naept, const int* s_rev, int64_t rows, void* q,
+                          float* scales, bool chained, void* stream) {
+  const int rc = quant128_check(x_bf16, q, scales, rows, K);
+  if (rc) return rc;
+  if (T < 0 || T >= (int64_t)1 << 31) return SMOE_ERR_SHAPE;
+  if (T > 0 && rows > 0 && (!naept || !s_rev)) return SMOE_ERR_ARG;
+  Rows128Args a{x_bf16, T, rows, (int)K, nullptr, nullptr, naept, s_rev, (uint8_t*)q, scales};
+  return launch_rows(a, false, chained, stream);
 }
 
 }  // namespace smoe
@@ -351,21 +381,12 @@ extern "C" {
 
 int smoe_quant128_rows(const void* x_bf16, int64_t rows, int64_t K, int swiglu, const int32_t* list, const int32_t* n_live,
                        int64_t n_list, void* q, float* scales, void* stream) {
-  const int rc = quant128_check(x_bf16, q, scales, rows, K);
-  if (rc) return rc;
-  if (list && (n_list < 0 || !n_live)) return SMOE_ERR_ARG;
-  Rows128Args a{x_bf16, list ? n_list : rows, rows, (int)K, list, n_live, nullptr, nullptr, (uint8_t*)q, scales};
-  return launch_rows(a, swiglu != 0, stream);
+  return quant128_rows(x_bf16, rows, K, swiglu, list, n_live, n_list, q, scales, false, stream);
 }
 
 int smoe_quant128_rows_scatter(const void* x_bf16, int64_t T, int64_t K, const int32_t* naept, const int32_t* s_rev, int64_t rows,
                                void* q, float* scales, void* stream) {
-  const int rc = quant128_check(x_bf16, q, scales, rows, K);
-  if (rc) return rc;
-  if (T < 0 || T >= (int64_t)1 << 31) return SMOE_ERR_SHAPE;
-  if (T > 0 && rows > 0 && (!naept || !s_rev)) return SMOE_ERR_ARG;
-  Rows128Args a{x_bf16, T, rows, (int)K, nullptr, nullptr, naept, s_rev, (uint8_t*)q, scales};
-  return launch_rows(a, false, stream);
+  return quant128_rows_scatter(x_bf16, T, K, naept, s_rev, rows, q, scales, false, stream);
 }
 
 int smoe_quant128_dual(const void* x_bf16, int64_t rows, int64_t K, const int32_t* efo, const int32_t* counts, int64_t E, void* q,

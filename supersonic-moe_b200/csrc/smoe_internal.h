@@ -37,6 +37,11 @@ int gemm_varlen_m_few(const void* a_fp8, const void* a_sf, const void* b_fp8, co
 // The block-128 products as the calls that launch a whole pass make them.  `early` as above, for efo, counts and (few rows) weights;
 // `independent`: the kernel reads nothing that the one before it writes, writes elsewhere, and only ends after it.  `without_rests` (rows
 // that are not live are left) / `rests`: see load_segs128; the two share a product.
+// The quantisers, `chained`: launched while the kernel before them ends, which they wait for before anything else.
+int quant128_rows(const void* x_bf16, int64_t rows, int64_t K, int swiglu, const int* list, const int* n_live, int64_t n_list, void* q,
+                  float* scales, bool chained, void* stream);
+int quant128_rows_scatter(const void* x_bf16, int64_t T, int64_t K, const int* naept, const int* s_rev, int64_t rows, void* q,
+                          float* scales, bool chained, void* stream);
 int gemm128_rows(const void* a_fp8, const float* a_scales, const void* b_fp8, const float* b_scales, const int* efo, const int* counts,
                  void* c_bf16, int64_t rows, int64_t N, int64_t K, int64_t E, int b_mn, int zero_rest, bool without_rests, int* status,
                  int* pinned_host_word, bool early, void* stream);
