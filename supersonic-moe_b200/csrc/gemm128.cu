@@ -91,7 +91,8 @@ int gemm128_rows(const void* a_fp8, const float* a_scales, const void* b_fp8, co
   p.bs_e = nb * kb;
   p.bs_n = b_mn ? 1 : kb;
   p.bs_k = b_mn ? (int)nb : 1;
-  p.b_mn = b_mn != 0; p.c = c_bf16; p.zero_rest = without_rests ? -Few128Smem::NT : zero_rest != 0; p.status = status; p.host_word = pinned_host_word;
+  p.b_mn = b_mn != 0; p.c = c_bf16; p.zero_rest = without_rests ? -Few128Smem::NT : zero_rest != 0;
+  p.status = status; p.host_word = pinned_host_word;
   // every segment may end in a tile that is not full, and so may the rows behind the last
   const int64_t tiles = efo ? (rows / 256 + E + 1) * up(N, 256) : up(rows, 256) * up(N, 256);
   return launch128<ROWS128>(ta, tb, tc, p, tiles, early, (cudaStream_t)stream);

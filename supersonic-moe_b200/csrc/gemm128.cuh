@@ -290,7 +290,9 @@ gemm128_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
   const uint32_t bar_scfull = bar_tempty + 8 * S::BUFS, bar_scempty = bar_scfull + 8 * S::SC_SLOTS;
 
   constexpr int PRODUCER = S::EPI_WARPS, ISSUER = S::EPI_WARPS + 1, SCALER = S::EPI_WARPS + 2;
-  if (warp == 2) load_segs128<false>(segs, p.efo, p.counts, p.E, p.rows, 256, MODE == ROWS128 && p.zero_rest <= 0, MODE == ROWS128 ? -min(p.zero_rest, 0) : 0, 0, lane);
+  if (warp == 2)
+    load_segs128<false>(segs, p.efo, p.counts, p.E, p.rows, 256, MODE == ROWS128 && p.zero_rest <= 0,
+                        MODE == ROWS128 ? -min(p.zero_rest, 0) : 0, 0, lane);
   if (threadIdx.x == 0) {
     for (int s = 0; s < S::STAGES; ++s) {
       mbar_init(bar_full + 8 * s, 1);                     // leader's: its producer arms it, both CTAs' copies credit it
