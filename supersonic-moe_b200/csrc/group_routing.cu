@@ -343,7 +343,8 @@ __global__ void __launch_bounds__(32 * gr_warps(PER)) group_routing_kernel(const
     if (scores_rank) c[i] = (a.softmax ? gr_exp(x[i] - top) * factor : gr_inverse(1.f + gr_exp(-x[i]))) + bias[i];
     const float o = (a.bias ? c[i] : x[i]) + 0.f;             // zeros of either sign are one value
     key[i] = x[i] == -INFINITY ? 0u : o == o ? gr_key(o) : 1u;
-    if (GROUPS) c[i] = x[i] == -INFINITY ? -INFINITY : c[i] == c[i] ? c[i] : -FLT_MAX;
+    // (as gr_rank: NaN and what a bias of -inf leaves are the lowest of numbers, only a closed expert is none)
+    if (GROUPS) c[i] = x[i] == -INFINITY ? -INFINITY : fmaxf(c[i], -FLT_MAX);
   }
   bool sure = true;                                           // the order so far is beyond doubt
   if (GROUPS) {
