@@ -57,3 +57,30 @@ def test_groups_of_one_expert_or_none_that_its_bias_leaves(sonicmoe, E, groups, 
         bias[2 * n + 1::2] = off                              # and half of the others
         for top in (1, groups // 2, groups - 1):
             same_choice(sonicmoe, logits, min(3, top * n), bias, groups, top, group_score, softmax)
+
+
+@pytest.mark.parametrize("E,groups", TABLES)
+@pytest.mark.parametrize("a", [10.0, 100.0, 1e4])
+@pytest.mark.parametrize("softmax", [False, True])
+def test_two_large_biases_that_cancel_in_a_group(sonicmoe, E, groups, a, softmax):
+    """The scores' sum is near 1 but was rounded at the size of the biases.  Logits in steps of what that rounding is."""
+    n, g = E // groups, torch.Generator().manual_seed(int(a) + E)
+    bias = torch.full((groups, n), -a)
+    bias[:, 0] = a
+    wide = E if softmax else 1                                # a softmax score is 1 / E here
+    logits = torch.randint(0, 16, (200, E), generator=g) * (a * 2.0 ** -24 * wide)
+    for top in (1, groups // 2):
+        same_choice(sonicmoe, logits, min(2, top * n), bias.flatten(), groups, top, 2, softmax)
+
+
+def test_the_least_kept_group_need_not_be_the_one_in_doubt(sonicmoe):
+    """Biases of 1e4 that cancel in one group alone, which ranks just ahead of or behind groups without any; also the two scores whose
+    rounded sums stand the other way round than the sums."""
+    bias = torch.tensor([1e4, -1e4, 0.0, 0, 0, 0, 0, 0])
+    g = torch.Generator().manual_seed(1)
+    logits = torch.randint(0, 64, (300, 8), generator=g) * 2.0 ** -14
+    for top in (1, 2, 3):
+        same_choice(sonicmoe, logits, 2, bias, 4, top, 2, False)
+    s = torch.tensor([[0.5003, 0.5, 0.5001, 0.5]], dtype=torch.float64)
+    x = torch.log(s / (1 - s)).float()
+    same_choice(sonicmoe, x, 1, bias[:4], 2, 1, 2, False)
