@@ -385,15 +385,17 @@ __global__ void __launch_bounds__(32 * gr_warps(PER)) group_routing_kernel(const
     }
     const bool in = lane < a.groups && ahead < a.top_groups;
     const uint32_t kept = __ballot_sync(kAll, in);
-    if (scores_rank) {
-      // Each group's score may be off by what its terms were rounded by, and those may cancel: the least of those kept, less its
-      // own error, against the largest left out, with its own.  (A closed one is kept only where no open one stays out.)
-      const bool two = a.group_score > 1 && q != -INFINITY;
-      const float off = gr_near(slack, 2.f * (fabsf(p) + (two ? fabsf(q) : 0.f)));
-      const uint32_t least = gr_min(in ? gr_key(fmaxf(score - off, -INFINITY)) : kAll);       // fmaxf: no NaN of infinities
-      // (a sum that overflows is one of two lowest numbers, and lies below every other)
-      const uint32_t most = gr_max(in || g_key == 0 ? 0u : gr_key(score == -INFINITY ? -3.4e38f : score + off));
-      if (most) sure = gr_unkey(least) > gr_unkey(most);
+    // Each group's score may be off by what its terms were rounded by, and those may cancel: the least of those kept, less its own
+    // error, against the largest left out, with its own.  (A closed one is kept only where no open one stays out.)  Logits are
+    // exact, but the lowest of them is what stands for NaN.
+    const bool two = a.group_score > 1 && q != -INFINITY;
+    const float off = scores_rank ? gr_near(slack, 2.f * (fabsf(p) + (two ? fabsf(q) : 0.f))) : 0.f;
+    const uint32_t least = gr_min(in ? gr_key(fmaxf(score - off, -INFINITY)) : kAll);         // fmaxf: no NaN of infinities
+    // (a sum that overflows is one of two lowest numbers, and lies below every other)
+    const uint32_t most = gr_max(in || g_key == 0 ? 0u : gr_key(score == -INFINITY ? -3.4e38f : score + off));
+    if (most) {
+      const float lo = gr_unkey(least);
+      sure = lo > gr_unkey(most) || (!scores_rank && lo > -FLT_MAX);
     }
     if (a.group_lanes) {
       const bool stay = (kept >> (lane / a.group_lanes)) & 1;

@@ -84,3 +84,16 @@ def test_the_least_kept_group_need_not_be_the_one_in_doubt(sonicmoe):
     s = torch.tensor([[0.5003, 0.5, 0.5001, 0.5]], dtype=torch.float64)
     x = torch.log(s / (1 - s)).float()
     same_choice(sonicmoe, x, 1, bias[:4], 2, 1, 2, False)
+
+
+@pytest.mark.parametrize("E,groups", TABLES)
+def test_a_group_of_nan_behind_one_of_the_lowest_logits(sonicmoe, E, groups):
+    """Without a bias groups of one score rank by their logits, and NaN is below every number."""
+    n = E // groups
+    logits = torch.full((4, E), -math.inf)
+    logits[0, :n], logits[0, 2 * n:3 * n] = math.nan, LOWEST
+    logits[1, n:2 * n], logits[1, :n] = math.nan, LOWEST
+    logits[2, :2 * n] = math.nan
+    logits[3, -1], logits[3, 0] = LOWEST, math.nan
+    for group_score in (1, 2):
+        same_choice(sonicmoe, logits, 1, None, groups, 1, group_score, False)
