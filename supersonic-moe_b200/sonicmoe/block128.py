@@ -31,6 +31,8 @@ def quantize_rows_block128(x: torch.Tensor, swiglu: bool = False):
 
 def quantize_weight_block128(w: torch.Tensor):
     """bf16 [E,N,K] (or [N,K]) -> (e4m3 of that shape, scales f32 [E,ceil(N/128),ceil(K/128)])."""
+    if w.ndim not in (2, 3):
+        raise ValueError(f"quantize_weight_block128: the weight is bf16 [E,N,K] or [N,K], got {w.dtype} {tuple(w.shape)}")
     q, s = ops.quant128_weight(_dense(w.detach()).view(-1, *w.shape[-2:]))
     return (q.view(_E4M3), s) if w.ndim == 3 else (q[0].view(_E4M3), s[0])
 
