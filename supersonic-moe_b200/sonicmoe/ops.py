@@ -862,8 +862,8 @@ def _payload(like, *shape):
 
 
 def check_payload(q, what):
-    """e4m3 rows as the quantisers leave them: dense, each on a 16-byte boundary."""
-    if q.element_size() != 1:
+    """e4m3 rows (or their bytes) as the quantisers leave them: dense, each on a 16-byte boundary."""
+    if q.dtype not in (torch.float8_e4m3fn, _U8):
         raise ValueError(f"{what}: the payload is e4m3, got {q.dtype}")
     if q.shape[-1] % 16 == 0 and q.is_contiguous():
         return
