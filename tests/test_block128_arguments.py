@@ -12,7 +12,7 @@ def sonicmoe(built_library):
 def test_a_weight_has_two_or_three_dimensions(sonicmoe):
     for shape in ((2, 3, 16, 64), (1, 1, 16, 64), (64,), ()):
         with pytest.raises(ValueError, match=r"\[E,N,K\]"):
-            sonicmoe.quantize_weight_block128(torch.zeros(*shape, dtype=torch.bfloat16))
+            sonicmoe.quantize_weight_block128(torch.zeros(shape, dtype=torch.bfloat16))
 
 
 def test_a_payload_of_another_type_is_no_e4m3(sonicmoe):
