@@ -489,7 +489,9 @@ int smoe_group_routing_bwd(const void* logits, int bf16, const int32_t* idx, con
  * No counterpart in the reference, whose scales are ue8m0 per 1x32.  Activations carry a scale for each row and 128 columns
  * (1x128), weights one for each 128 x 128, the operands of a weight gradient one for each column and 128 rows.  A block's scale is
  * a / 448 and its payload e4m3(x * (448 / a)), a = max(max |x|, 2^-100), f32 throughout.
- * Payload rows lie ceil(cols / 16) * 16 bytes apart; scales are dense.  Sizes are multiples of 8; payloads start on 16 bytes.
+ * Payload rows lie ceil(cols / 16) * 16 bytes apart; scales are dense.  Sizes are multiples of 8; payloads start on 16 bytes, the
+ * scales of the three products too.  The calls that launch a whole pass take a weight's scales from any 4 bytes on (an expert's part
+ * of a stacked tensor).
  * Segments: efo [E+1] ascending multiples of 128 as smoe_topk_metadata leaves them, counts [E] live rows at a segment's start (null:
  * all); efo null: one segment (E = 1) of all rows. */
 

@@ -63,11 +63,13 @@ static int launch128(const CUtensorMap& ta, const CUtensorMap& tb, const CUtenso
 static bool size128(int64_t n) { return n > 0 && n % 8 == 0 && n < (int64_t)1 << 24; }
 
 static int check128(const void* a, const float* a_s, const void* b, const float* b_s, const int* efo, const int* counts, const void* c,
-                    int64_t rows, int64_t N, int64_t K, int64_t E, const int* status) {
+                    int64_t rows, int64_t N, int64_t K, int64_t E, const int* status, bool bulk_scales) {
   if (rows < 0 || rows >= (int64_t)1 << 31 || !size128(N) || !size128(K) || E <= 0 || E > kMaxExperts2) return SMOE_ERR_SHAPE;
   if (!efo && (E != 1 || counts)) return SMOE_ERR_ARG;
   if (!status || (rows > 0 && (!a || !a_s || !b || !b_s || !c))) return SMOE_ERR_ARG;
-  if (((uintptr_t)a | (uintptr_t)b | (uintptr_t)c | (uintptr_t)a_s | (uintptr_t)b_s) & 15) return SMOE_ERR_ALIGN;
+  if (((uintptr_t)a | (uintptr_t)b | (uintptr_t)c) & 15) return SMOE_ERR_ALIGN;
+  // the weight gradient copies scales in bulk; the products by rows read them one by one, from wherever an expert's begin
+  if (((uintptr_t)a_s | (uintptr_t)b_s) & (bulk_scales ? 15 : 3)) return SMOE_ERR_ALIGN;
   return SMOE_OK;
 }
 
@@ -76,7 +78,7 @@ static int64_t up(int64_t n, int64_t m) { return (n + m - 1) / m; }
 int gemm128_rows(const void* a_fp8, const float* a_scales, const void* b_fp8, const float* b_scales, const int* efo, const int* counts,
                  void* c_bf16, int64_t rows, int64_t N, int64_t K, int64_t E, int b_mn, int zero_rest, bool without_rests, int* status,
                  int* pinned_host_word, bool early, void* stream) {
-  int rc = check128(a_fp8, a_scales, b_fp8, b_scales, efo, counts, c_bf16, rows, N, K, E, status);
+  int rc = check128(a_fp8, a_scales, b_fp8, b_scales, efo, counts, c_bf16, rows, N, K, E, status, false);
   if (rc || rows == 0) return rc;
   CUtensorMap ta, tb, tc;
   rc = make_tmap128(&ta, a_fp8, 1, rows, K, 128, 2);
@@ -101,7 +103,7 @@ int gemm128_rows(const void* a_fp8, const float* a_scales, const void* b_fp8, co
 int gemm128_wgrad(const void* a_fp8, const float* a_scales, const void* b_fp8, const float* b_scales, const int* efo, const int* counts,
                   void* c, int64_t M, int64_t N, int64_t rows, int64_t E, int out_bf16, int accumulate, int* status,
                   int* pinned_host_word, bool independent, void* stream) {
-  int rc = check128(a_fp8, a_scales, b_fp8, b_scales, efo, counts, c, rows, N, M, E, status);
+  int rc = check128(a_fp8, a_scales, b_fp8, b_scales, efo, counts, c, rows, N, M, E, status, true);
   if (rc) return rc;
   if (out_bf16 && accumulate) return SMOE_ERR_ARG;
   if (rows == 0) {                                  // an empty sum
@@ -126,7 +128,7 @@ int gemm128_wgrad(const void* a_fp8, const float* a_scales, const void* b_fp8, c
 int gemm128_few(const void* a_fp8, const float* a_scales, const void* b_fp8, const float* b_scales, const int* efo, const int* counts,
                 void* c_bf16, int64_t rows, int64_t N, int64_t K, int64_t E, int64_t live_rows, bool rests, int* status,
                 int* pinned_host_word, bool early, bool independent, void* stream) {
-  int rc = check128(a_fp8, a_scales, b_fp8, b_scales, efo, counts, c_bf16, rows, N, K, E, status);
+  int rc = check128(a_fp8, a_scales, b_fp8, b_scales, efo, counts, c_bf16, rows, N, K, E, status, false);
   if (rc || rows == 0) return rc;
   if (live_rows <= 0 || live_rows > rows) live_rows = rows;
   CUtensorMap tw, tx16, tx64;
@@ -171,11 +173,15 @@ int gemm128_few(const void* a_fp8, const float* a_scales, const void* b_fp8, con
 
 using namespace smoe;
 
+static bool on16(const void* p, const void* q) { return (((uintptr_t)p | (uintptr_t)q) & 15) == 0; }
+
 extern "C" {
 
+// (by themselves, the products ask the same of all their operands)
 int smoe_gemm128_rows(const void* a_fp8, const float* a_scales, const void* b_fp8, const float* b_scales, const int32_t* efo,
                       const int32_t* counts, void* c_bf16, int64_t rows, int64_t N, int64_t K, int64_t E, int b_mn,
                       int zero_rest, int32_t* status, int32_t* pinned_host_word, void* stream) {
+  if (!on16(a_scales, b_scales)) return SMOE_ERR_ALIGN;
   return gemm128_rows(a_fp8, a_scales, b_fp8, b_scales, efo, counts, c_bf16, rows, N, K, E, b_mn, zero_rest, false, status,
                       pinned_host_word, false, stream);
 }
@@ -190,6 +196,7 @@ int smoe_gemm128_wgrad(const void* a_fp8, const float* a_scales, const void* b_f
 int smoe_gemm128_few(const void* a_fp8, const float* a_scales, const void* b_fp8, const float* b_scales, const int32_t* efo,
                      const int32_t* counts, void* c_bf16, int64_t rows, int64_t N, int64_t K, int64_t E, int64_t live_rows,
                      int32_t* status, int32_t* pinned_host_word, void* stream) {
+  if (!on16(a_scales, b_scales)) return SMOE_ERR_ALIGN;
   return gemm128_few(a_fp8, a_scales, b_fp8, b_scales, efo, counts, c_bf16, rows, N, K, E, live_rows, false, status, pinned_host_word,
                      false, false, stream);
 }

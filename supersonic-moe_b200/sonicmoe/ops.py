@@ -956,6 +956,11 @@ def quant128_weight(w):
     return q, s
 
 
+def _on16(t):
+    """From a 16-byte boundary on (an expert's scales inside a stacked tensor need not be)."""
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 def failure_words(device):
     """Addresses of the status word and of its host mirror (which a capture must not be the first to allocate)."""
     m = _posted.get(device.index)
@@ -989,6 +994,7 @@ def gemm128_rows(a_q, a_s, b_q, b_s, efo=None, counts=None, b_mn=False, zero_res
     E, N = b_q.shape[0], b_q.shape[2 if b_mn else 1]
     nb, kb = _blocks128(N), _blocks128(K)
     _check_product(a_q, a_s, b_q, b_s, efo, counts, E, N, K, (kb, nb) if b_mn else (nb, kb), "gemm128_rows")
+    a_s, b_s = _on16(a_s), _on16(b_s)
     c = a_s.new_empty((rows, N), dtype=torch.bfloat16)
     check(lib.smoe_gemm128_rows(a_q.data_ptr(), a_s.data_ptr(), b_q.data_ptr(), b_s.data_ptr(), _p(efo), _p(counts), c.data_ptr(),
                                 rows, N, K, E, b_mn, zero_rest, *failure_words(a_q.device), _stream()), "gemm128_rows")
@@ -1004,6 +1010,7 @@ def gemm128_few(a_q, a_s, b_q, b_s, efo=None, counts=None, live_rows=0):
     rows, K = a_q.shape
     E, N = b_q.shape[:2]
     _check_product(a_q, a_s, b_q, b_s, efo, counts, E, N, K, (_blocks128(N), _blocks128(K)), "gemm128_few")
+    a_s, b_s = _on16(a_s), _on16(b_s)
     c = a_s.new_empty((rows, N), dtype=torch.bfloat16)
     check(lib.smoe_gemm128_few(a_q.data_ptr(), a_s.data_ptr(), b_q.data_ptr(), b_s.data_ptr(), _p(efo), _p(counts), c.data_ptr(),
                                rows, N, K, E, live_rows, *failure_words(a_q.device), _stream()), "gemm128_few")
@@ -1028,6 +1035,7 @@ def gemm128_wgrad(a_q, a_s, b_q, b_s, efo=None, counts=None, out=None, accumulat
     for s, n in ((a_s, M), (b_s, N)):
         if s.dtype != torch.float32 or s.shape != (rb, n) or not s.is_contiguous():
             raise ValueError(f"gemm128_wgrad: scales are f32 [{rb},{n}], got {s.dtype} {tuple(s.shape)}")
+    a_s, b_s = _on16(a_s), _on16(b_s)
     if out is None:
         if accumulate:
             raise ValueError("gemm128_wgrad: nothing to accumulate into")

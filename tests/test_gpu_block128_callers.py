@@ -1,0 +1,87 @@
+"""Block-128 operators on what callers hold: parts of stacked checkpoints, accumulators inside a flat buffer, a first call that is being
+captured, bounds that were too low."""
+import pytest
+import torch
+
+from oracle import block128 as O
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF16 = 2.0 ** -8                     # half a step of bf16, relative
+
+
+@pytest.fixture(scope="module")
+def sonicmoe():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    import sonicmoe as m
+    yield m
+    torch.cuda.synchronize()
+    m.ops.check_status(DEV)
+
+
+def f32_tol(K):
+    """Roundings of a sum of K products in f32 by blocks of 128, whatever their order, relative to the sum of the terms' magnitudes;
+    twice 2^-24 each, for an adder that cuts instead of rounding."""
+    return (min(K, 128) + -(-K // 128) + 4) * 2.0 ** -23
+
+
+def randn(*shape, seed=0, scale=1.0):
+    return (torch.randn(*shape, generator=torch.Generator().manual_seed(seed)) * scale).to(torch.bfloat16)
+
+
+def table(counts):
+    efo = torch.zeros(len(counts) + 1, dtype=torch.int32)
+    efo[1:] = torch.tensor([-(-c // 128) * 128 for c in counts]).cumsum(0)
+    return efo, torch.tensor(counts, dtype=torch.int32), int(efo[-1])
+
+
+@pytest.mark.parametrize("N,K", [(384, 384), (520, 328), (328, 1400)])
+def test_parts_of_stacked_weights(sonicmoe, N, K):
+    """An odd number of scales a matrix: every expert's but the first start off a 16-byte boundary."""
+    E, rows = 5, 200
+    x, w, dy = randn(rows, K, seed=1), randn(E, N, K, seed=2), randn(rows, N, seed=3)
+    q, s = sonicmoe.quantize_weight_block128(w.to(DEV))
+    xs = x.to(DEV)
+    for e in (1, 2, 3):
+        assert s[e].data_ptr() % 16
+        for n in (1, 70, rows):                               # the kernel for few rows, and tiles
+            got, want = [], []
+            for part, out in (((q[e], s[e]), got), ((q[e], s[e].clone()), want)):
+                a = xs[:n].clone().requires_grad_(True)
+                y = sonicmoe.block128_linear(a, part)
+                out += [y.detach(), *torch.autograd.grad(y, a, dy[:n].to(DEV))]
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+    efo, counts, n = table([130, 0, 40])
+    x = randn(n, K, seed=4).to(DEV)
+    y = sonicmoe.block128_linear(x, (q[1:4], s[1:4]), efo.to(DEV), counts.to(DEV))
+    assert torch.equal(y, sonicmoe.block128_linear(x, (q[1:4], s[1:4].clone()), efo.to(DEV), counts.to(DEV)))
+
+
+@pytest.mark.parametrize("T", [3, 200])
+def test_an_expert_parallel_rank_of_stacked_layers(sonicmoe, T):
+    E, H, I, K = 6, 384, 192, 2                               # 3 x 3 and 3 x 2 scales an expert
+    w1 = sonicmoe.quantize_weight_block128(randn(E, 2 * I, H, seed=1, scale=H ** -0.5).to(DEV))
+    w2 = sonicmoe.quantize_weight_block128(randn(E, H, I, seed=2, scale=I ** -0.5).to(DEV))
+    x = randn(T, H, seed=3).to(DEV)
+    scores, idx = torch.rand(T, 3, generator=torch.Generator().manual_seed(4)).topk(K)
+    part = [tuple(t[3:] for t in w) for w in (w1, w2)]
+    assert part[0][1].data_ptr() % 16 and part[1][1].data_ptr() % 16
+    a = sonicmoe.block128_experts(x, idx.int().to(DEV), scores.to(DEV), *part)
+    b = sonicmoe.block128_experts(x, idx.int().to(DEV), scores.to(DEV), *(tuple(t.clone() for t in w) for w in part))
+    assert torch.equal(a, b)
+
+
+def test_kernel_by_kernel_on_scales_off_a_boundary(sonicmoe):
+    ops = sonicmoe.ops
+    off = lambda t: torch.cat([t.new_zeros(1), t.flatten()])[1:].view(t.shape)
+    xq, xs = ops.quant128_rows(randn(70, 264).to(DEV))
+    wq, ws = ops.quant128_weight(randn(1, 136, 264, seed=1).to(DEV))
+    dq, ds = ops.quant128_rows(randn(70, 136, seed=2).to(DEV))
+    col = [ops.quant128_dual(randn(70, n, seed=3).to(DEV), with_rows=False)[2:] for n in (136, 264)]
+    assert off(xs).data_ptr() % 16 and off(ws).data_ptr() % 16
+    for f in (ops.gemm128_rows, ops.gemm128_few):
+        assert torch.equal(f(xq, off(xs), wq, off(ws)), f(xq, xs, wq, ws))
+    assert torch.equal(ops.gemm128_rows(dq, off(ds), wq, off(ws), b_mn=True), ops.gemm128_rows(dq, ds, wq, ws, b_mn=True))
+    (a, s), (b, t) = col
+    assert torch.equal(ops.gemm128_wgrad(a, off(s), b, off(t)), ops.gemm128_wgrad(a, s, b, t))
