@@ -1089,13 +1089,22 @@ def block128_linear_bwd(dy, w, w_s, efo, counts, saved, E, N, K, flags, main_gra
     dx = dy.new_empty((rows, K)) if flags & B128_DX else None
     dw = None
     if flags & B128_DW:
-        dw = dy.new_empty((E, N, K)) if main_grad is None else main_grad
-        _check_same_gpu("block128_linear", dy, dw)
+        _check_same_gpu("block128_linear", dy, main_grad)
+        if main_grad is None:
+            dw = dy.new_empty((E, N, K))
+        elif main_grad.data_ptr() % 16 == 0:
+            dw = main_grad
+        else:                                    # what is added leaves in pieces that start on 16 bytes
+            dw = dy.new_zeros((E, N, K), dtype=torch.float32)
     scratch = dy.new_empty(block128_bytes(rows, N, K, E, flags, 2), dtype=_U8)
     check(lib.smoe_block128_linear_bwd(dy.data_ptr(), _p(w), _p(w_s), _p(efo), _p(counts), _p(saved), scratch.data_ptr(), _p(dx),
                                        _p(dw), rows, N, K, E, flags, main_grad is not None, *failure_words(dy.device), _stream()),
           "block128_linear_bwd")
-    return dx, (dw if main_grad is None else None)
+    if main_grad is None:
+        return dx, dw
+    if dw is not None and dw is not main_grad:
+        main_grad.add_(dw.view(main_grad.shape))
+    return dx, None
 
 
 @_op

@@ -85,3 +85,24 @@ def test_kernel_by_kernel_on_scales_off_a_boundary(sonicmoe):
     assert torch.equal(ops.gemm128_rows(dq, off(ds), wq, off(ws), b_mn=True), ops.gemm128_rows(dq, ds, wq, ws, b_mn=True))
     (a, s), (b, t) = col
     assert torch.equal(ops.gemm128_wgrad(a, off(s), b, off(t)), ops.gemm128_wgrad(a, s, b, t))
+
+
+def test_an_accumulator_inside_a_flat_buffer(sonicmoe):
+    """A main_grad that starts at any element is added to like one that starts on a boundary."""
+    E, N, K = 2, 136, 264
+    efo, counts, rows = table([130, 70])
+    x, dy = randn(rows, K, seed=1).to(DEV), randn(rows, N, seed=2).to(DEV)
+    start = torch.randn(E, N, K, generator=torch.Generator().manual_seed(3)).to(DEV)
+    got = []
+    for pad in (0, 1):
+        w = randn(E, N, K, seed=4).to(DEV).requires_grad_(True)
+        flat = torch.full((E * N * K + 9,), 5.0, device=DEV)
+        w.main_grad = flat[pad:pad + E * N * K].view(E, N, K)
+        w.main_grad.copy_(start)
+        a = x.clone().requires_grad_(True)
+        sonicmoe.block128_linear(a, w, efo.to(DEV), counts.to(DEV)).backward(dy)
+        assert w.grad is None and (flat[:pad] == 5).all() and (flat[pad + E * N * K:] == 5).all()
+        got.append((w.main_grad.clone(), a.grad))
+    assert w.main_grad.data_ptr() % 16
+    assert torch.equal(got[0][1], got[1][1])
+    assert torch.equal(got[0][0], got[1][0])
