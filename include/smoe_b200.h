@@ -413,6 +413,11 @@ int smoe_ds_slots(const float* ds_partial, int64_t partials, int64_t rows, const
  * would queue behind bulk transfers.  No counterpart in the reference, whose kernels report nothing. */
 int smoe_status_post(const int32_t* status, int32_t* pinned_host_word, void* stream);
 
+/* Sets how stream captures in progress restrict this thread's calls (cudaStreamCaptureMode: 0 global, 1 thread-local, 2 relaxed) and
+ * returns what it was, -1 on an error.  A status word and its mirror are allocated under 2, on a stream of their own: they belong to
+ * no graph, although the first call may be one that is captured. */
+int smoe_exchange_capture_mode(int mode);
+
 /* top-K of each row of logits [T,E] (f32) and softmax over the K selected values.
  * Replaces _softmax_topk_fwd (sonicmoe/functional/forward.py:217-236, topk_softmax.py). */
 int smoe_topk_softmax(const float* logits, int64_t T, int64_t E, int64_t K, float* scores, int32_t* idx, void* stream);

@@ -381,6 +381,12 @@ int smoe_ds_slots(const float* ds_partial, int64_t partials, int64_t rows, const
   return cudaGetLastError() == cudaSuccess ? SMOE_OK : SMOE_ERR_LAUNCH;
 }
 
+int smoe_exchange_capture_mode(int mode) {
+  if (mode < cudaStreamCaptureModeGlobal || mode > cudaStreamCaptureModeRelaxed) return -1;
+  cudaStreamCaptureMode m = (cudaStreamCaptureMode)mode;
+  return cudaThreadExchangeStreamCaptureMode(&m) == cudaSuccess ? (int)m : -1;
+}
+
 int smoe_status_post(const int32_t* status, int32_t* pinned_host_word, void* stream) {
   if (!status || !pinned_host_word) return SMOE_ERR_ARG;
   status_post_kernel<<<1, 1, 0, (cudaStream_t)stream>>>(status, pinned_host_word);

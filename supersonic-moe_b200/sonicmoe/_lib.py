@@ -87,6 +87,7 @@ SIGNATURES = {
     "smoe_switch_loss_workspace": (_L, [_L]),
     "smoe_switch_loss": (_I, [_P, _I, _P, _L, _L, _P, _P, _P, _P]),
     "smoe_switch_loss_bwd": (_I, [_P, _I, _P, _P, _L, _L, _P, _P]),
+    "smoe_exchange_capture_mode": (_I, [_I]),
     "smoe_group_routing": (_I, [_P, _I, _P, _L, _L, _L, _L, _L, _I, _I, _I, _F, _P, _P, _P]),
     "smoe_group_routing_bwd": (_I, [_P, _I, _P, _P, _L, _L, _L, _I, _I, _F, _P, _P]),
     "smoe_quant128_rows": (_I, [_P, _L, _L, _I, _P, _P, _L, _P, _P, _P]),

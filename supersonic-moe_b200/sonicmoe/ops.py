@@ -4,6 +4,7 @@ there is no CPU path.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 
 import torch
@@ -78,11 +79,30 @@ def _dev_index(device) -> int:
     return d.index if d.index is not None else torch.cuda.current_device()
 
 
+@contextlib.contextmanager
+def _beside_capture(key):
+    """Allocations and launches in here are part of no graph, whatever the current stream is being captured into, and complete at
+    the end."""
+    before = lib.smoe_exchange_capture_mode(2)       # relaxed: a capture in progress does not forbid this thread to allocate
+    try:
+        while True:                                  # (streams come round again: not one that is being captured)
+            side = torch.cuda.Stream(key)
+            with torch.cuda.stream(side):
+                if not torch.cuda.is_current_stream_capturing():
+                    yield
+                    side.synchronize()
+                    return
+    finally:
+        if before >= 0:
+            lib.smoe_exchange_capture_mode(before)
+
+
 def status_word(device) -> torch.Tensor:
     """Per-device int32 word the GEMM kernels write a failure code into (0 = ok)."""
     key = _dev_index(device)
     if key not in _status:
-        _status[key] = torch.zeros(1, dtype=_I32, device=torch.device("cuda", key))
+        with _beside_capture(key):                   # in a graph's pool, replays would zero it
+            _status.setdefault(key, torch.zeros(1, dtype=_I32, device=torch.device("cuda", key)))
     return _status[key]
 
 
@@ -110,8 +130,10 @@ _posted = {}     # device index -> (pinned int32[1] mirror of the device status 
 def _mirror(key):
     m = _posted.get(key)
     if m is None:
-        host = torch.zeros(1, dtype=_I32).pin_memory()
-        m = _posted[key] = (host, ctypes.c_int32.from_address(host.data_ptr()), status_word(key).data_ptr(), host.data_ptr())
+        word = status_word(key).data_ptr()
+        with _beside_capture(key):
+            host = torch.zeros(1, dtype=_I32).pin_memory()
+        m = _posted.setdefault(key, (host, ctypes.c_int32.from_address(host.data_ptr()), word, host.data_ptr()))
     return m
 
 
@@ -962,13 +984,9 @@ def _on16(t):
 
 
 def failure_words(device):
-    """Addresses of the status word and of its host mirror (which a capture must not be the first to allocate)."""
+    """Addresses of the status word and of its host mirror."""
     m = _posted.get(device.index)
-    if m is not None:
-        return m[2:]
-    if torch.cuda.is_current_stream_capturing():
-        return status_word(device).data_ptr(), None
-    return status_pointers(device)
+    return m[2:] if m is not None else status_pointers(device)
 
 
 def _check_product(a_q, a_s, b_q, b_s, efo, counts, E, N, K, b_blocks, what):

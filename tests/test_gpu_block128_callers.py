@@ -1,5 +1,9 @@
 """Block-128 operators on what callers hold: parts of stacked checkpoints, accumulators inside a flat buffer, a first call that is being
 captured, bounds that were too low."""
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -8,6 +12,7 @@ from oracle import block128 as O
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
 BF16 = 2.0 ** -8                     # half a step of bf16, relative
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 @pytest.fixture(scope="module")
@@ -106,3 +111,41 @@ def test_an_accumulator_inside_a_flat_buffer(sonicmoe):
     assert w.main_grad.data_ptr() % 16
     assert torch.equal(got[0][1], got[1][1])
     assert torch.equal(got[0][0], got[1][0])
+
+
+CAPTURED_FIRST = """
+import sys
+import torch
+sys.path[:0] = [{root!r}, {root!r} + "/supersonic-moe_b200"]
+import sonicmoe
+x = torch.randn(40, 256, device="cuda").bfloat16()
+w = torch.randn(136, 256, device="cuda").bfloat16()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y = sonicmoe.block128_linear(x, w)
+    word, host = sonicmoe.ops.failure_words(x.device)
+status = sonicmoe.ops.status_word("cuda")
+assert status.data_ptr() == word and host
+assert int(status.item()) == 0, "before the first replay"
+status.fill_(503)
+graph.replay()
+torch.cuda.synchronize()
+assert int(status.item()) == 503, "a replay took a recorded failure back"
+status.zero_()
+assert torch.equal(y, sonicmoe.block128_linear(x, w))
+assert sonicmoe.ops.failure_words(x.device) == (word, host)
+sonicmoe.ops._posted[0][1].value = 502
+try:
+    sonicmoe.block128_linear(x, w)
+    raise SystemExit("a failure that a replay posted did not surface")
+except RuntimeError as e:
+    assert "502" in str(e)
+sonicmoe.ops.check_status("cuda")
+print("captured first: ok")
+"""
+
+
+def test_the_first_call_of_a_process_is_captured(sonicmoe):
+    """The word that kernels report failures in is no part of the graph, and the host sees it from a replay too."""
+    run = subprocess.run([sys.executable, "-c", CAPTURED_FIRST.format(root=ROOT)], capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and "captured first: ok" in run.stdout, run.stderr[-2000:]
