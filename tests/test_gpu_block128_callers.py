@@ -113,6 +113,53 @@ def test_an_accumulator_inside_a_flat_buffer(sonicmoe):
     assert torch.equal(got[0][0], got[1][0])
 
 
+def test_more_rows_than_a_few_row_product_was_told(sonicmoe):
+    """`live_rows` only divides the work: told too few, clusters of CTAs that share a tile's reduction take several tiles each."""
+    ops = sonicmoe.ops
+    counts = [70, 0, 129, 64, 1, 200]
+    efo, cnt, rows = table(counts)
+    live = O.live_rows(efo, cnt, rows)
+    # blocks of the reduction and weight tiles for clusters of 2, of 4 and of 8 where one row is expected on some 148 SMs
+    for N, K in ((5120, 1536), (4608, 1536), (1000, 6152)):
+        x, w = randn(rows, K, seed=N), randn(len(counts), N, K, seed=K)
+        xq, xs = ops.quant128_rows(x.to(DEV))
+        wq, ws = ops.quant128_weight(w.to(DEV))
+        y = ops.gemm128_few(xq, xs, wq, ws, efo.to(DEV), cnt.to(DEV), live_rows=1)
+        again = ops.gemm128_few(xq, xs, wq, ws, efo.to(DEV), cnt.to(DEV), live_rows=1)
+        assert torch.equal(y[live.to(DEV)], again[live.to(DEV)])
+        ref, mag = O.rows_product(O.deq_rows(*O.quant_rows(x)), O.deq_weight(*O.quant_weight(w)), efo, cnt)
+        err = (y.cpu().double() - ref).abs()
+        assert (err <= BF16 * ref.abs() + f32_tol(K) * mag * (1 + BF16))[live].all()
+    ops.check_status(DEV)
+
+
+def test_live_rows_of_products_that_leave_the_others(sonicmoe):
+    """Every live row is written, with the product, where tiles are laid over live rows only."""
+    ops = sonicmoe.ops
+    from sonicmoe._lib import check, lib
+    N, K = 264, 256
+    for counts in ([3, 0, 70, 128], [257, 1, 0, 64], [0, 0, 513, 128]):
+        efo, cnt, rows = table(counts)
+        x, w = randn(rows, K), randn(4, N, K, seed=1)
+        xq, xs = ops.quant128_rows(x.to(DEV))
+        wq, ws = ops.quant128_weight(w.to(DEV))
+        ref, mag = O.rows_product(O.deq_rows(*O.quant_rows(x)), O.deq_weight(*O.quant_weight(w)), efo, cnt)
+        live = O.live_rows(efo, cnt, rows)
+        e, n = efo.to(DEV), cnt.to(DEV)
+        for few in (True, False):
+            c = torch.full((rows, N), float("nan"), dtype=torch.bfloat16, device=DEV)
+            P = lambda t: t.data_ptr()
+            head = (P(xq), P(xs), P(wq), P(ws), P(e), P(n), P(c), rows, N, K, 4)
+            tail = (P(ops.status_word(DEV)), None, torch.cuda.current_stream().cuda_stream)
+            if few:
+                check(lib.smoe_gemm128_few(*head, 0, *tail), "few")
+            else:
+                check(lib.smoe_gemm128_rows(*head, 0, 0, *tail), "rows")
+            c = c.cpu()
+            assert torch.isnan(c[~live]).all()
+            assert ((c.double() - ref).abs() <= BF16 * ref.abs() + f32_tol(K) * mag * (1 + BF16))[live].all()
+
+
 CAPTURED_FIRST = """
 import sys
 import torch
