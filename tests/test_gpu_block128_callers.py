@@ -196,3 +196,27 @@ def test_the_first_call_of_a_process_is_captured(sonicmoe):
     """The word that kernels report failures in is no part of the graph, and the host sees it from a replay too."""
     run = subprocess.run([sys.executable, "-c", CAPTURED_FIRST.format(root=ROOT)], capture_output=True, text=True, timeout=300)
     assert run.returncode == 0 and "captured first: ok" in run.stdout, run.stderr[-2000:]
+
+
+def test_router_of_groups_into_the_layer(sonicmoe):
+    """The router's tables are what the layer takes: its outputs and gradients are those of the same tables handed over as leaves."""
+    T, E, K, H, I = 256, 8, 2, 256, 128
+    x, w1, w2 = randn(T, H, seed=1).to(DEV), randn(E, 2 * I, H, seed=2, scale=H ** -0.5), randn(E, H, I, seed=3, scale=I ** -0.5)
+    logits = torch.randn(T, E, generator=torch.Generator().manual_seed(4))
+    logits[-9:] = -torch.inf                                  # a padded batch
+    dy = randn(T, H, seed=5).to(DEV)
+    outs = []
+    for leaves in (False, True):
+        a, b, c = (t.to(DEV).clone().requires_grad_(True) for t in (x, w1, w2))
+        ld = logits.to(DEV).requires_grad_(True)
+        scores, idx = sonicmoe.group_limited_routing(ld, K, groups=4, top_groups=2, scale=1.5)
+        s = scores.detach().requires_grad_(True) if leaves else scores
+        out = sonicmoe.run_sonic_moe(a, idx, s, K, E, b, c, fp8=True)
+        out.backward(dy)
+        if leaves:
+            ld.grad, = torch.autograd.grad(scores, ld, s.grad)
+        outs.append((out.detach(), a.grad, b.grad, c.grad, ld.grad))
+    for u, v in zip(*outs):
+        assert torch.isfinite(u).all() and torch.equal(u, v)
+    assert (outs[0][0][-9:] == 0).all() and (outs[0][1][-9:] == 0).all() and (outs[0][4][-9:] == 0).all()
+    assert outs[0][4].abs().max() > 0
