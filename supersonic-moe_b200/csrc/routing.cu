@@ -211,7 +211,7 @@ __device__ __forceinline__ void scatter_unit(const TopkOut& o, const Layout& l, 
 #pragma unroll
     for (int j = 0; j < KP; ++j) {
       const int ej = __shfl_sync(0xffffffffu, e, rw * KP + j);
-      rank += (ej >= 0 && ej < e) ? 1 : 0;
+      rank += (ej >= 0 && (ej < e || (ej == e && j < k))) ? 1 : 0;      // (an expert named twice: an entry for each slot)
     }
   } else {
     rank = __popc(ball & ((1u << lane) - 1u)) - __popc(ball & ((1u << (rw * KP)) - 1u));
