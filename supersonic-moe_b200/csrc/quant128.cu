@@ -9,6 +9,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "host.h"
 #include "ptx.cuh"
 #include "smoe_b200.h"
 #include "smoe_internal.h"
@@ -334,7 +335,7 @@ static int launch_rows(const Rows128Args& a, bool glu, bool chained, void* strea
   // Several blocks each where that leaves every SM enough warps: four, or two where the activation's or a token's many rows need
   // the registers.  8192 x 4096 one block 28.0 us, two 24.2, four 22.7; gated 32768 x 768 40, 25.2, 26.5; eight places a token 18.6,
   // 18.4, 19.9.
-  const int most = glu || a.naept ? 2 : 4, per = units >= 148 * 64 * 4 ? most : 1;
+  const int most = glu || a.naept ? 2 : 4, per = units >= (int64_t)sm_count() * 64 * 4 ? most : 1;
   const int64_t grid = (units + 16 * per - 1) / (16 * per);
   if (grid >= (int64_t)1 << 31) return SMOE_ERR_SHAPE;
   auto kern = glu        ? (per == 2 ? quant128_rows_kernel<true, 2> : quant128_rows_kernel<true, 1>)
