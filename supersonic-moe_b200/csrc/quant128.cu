@@ -43,8 +43,8 @@ __device__ __forceinline__ uint2 q128_pack8(const uint4& v, float m) {
                     q128_pack4(q128_lo(v.z) * m, q128_hi(v.z) * m, q128_lo(v.w) * m, q128_hi(v.w) * m));
 }
 
-// To some 1e-7 and |g| roundings of the exponent: of 12.6 M e4m3 values 18.8 fall to another side of a step than in 64 bits (mean of
-// eight batches), with expf and the quotient 17.8, and 32768 x 768 take 31 us instead of 25.
+// To some 4e-7, and 8e-8 |g| more where g is negative (its exponential's argument is rounded).  What that may decide is decided by
+// q128_gated_again.
 __device__ __forceinline__ float q128_silu(float g) {
   float e, r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(-1.4426950408889634f * g));
@@ -83,6 +83,61 @@ __device__ __forceinline__ float q128_quotients(const float (&amax)[N], int lane
   return r;
 }
 
+// An activation's payload must not depend on how an exponential was rounded.  A value and its block's maximum are off by a unit or
+// two of the last place of f32 (more than kQ128Near for g below -16 or so); where that leaves a value within kQ128Near of the border
+// between two e4m3 values (three in 200,000), it and the maximum are made again in 64 bits.  Of 150 M values none is another than in
+// 64 bits then, with 4 in place of 8 one, without it 226.  It takes 16384 x 768 from 13.5 to 16.9 us, 512 x 768 from 2.4 to 3.7: half
+// for the look at every value, half for the last such block, of code that no cache holds.  (Borders below the least normal value,
+// 2^-6 of a maximum of 448, are not looked for.)
+constexpr uint32_t kQ128Near = 8;
+__device__ __forceinline__ uint32_t q128_from_border(float v) {      // below 2 * kQ128Near << 12: near one
+  return (__float_as_uint(v) << 12) + 0x80000000u + (kQ128Near << 12);
+}
+// One block of sixteen lanes: eight values of a lane, gate and up from p on (none: null) -> payload, and the scale's bits
+__device__ __noinline__ uint3 q128_gated_again(const uint4* p, uint32_t half) {
+  uint32_t w[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  if (p) {
+    *(uint4*)w = p[0];
+    *(uint4*)(w + 4) = p[1];
+  }
+  float y[8], rest[8], amax = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    y[e] = q128_silu(q128_lo(w[e])) * q128_hi(w[e]);
+    rest[e] = 0.f;
+    amax = fmaxf(amax, fabsf(y[e]));
+  }
+  for (int d = 8; d > 0; d >>= 1) amax = fmaxf(amax, __shfl_xor_sync(half, amax, d));
+  const float first = kE4m3Max / fmaxf(amax, kAmaxFloor), least = amax * (1.f - 1e-5f);
+  uint32_t todo = 0;                                      // near a border, or what may be the largest
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    todo |= q128_from_border(y[e] * first) < 2 * kQ128Near << 12 || fabsf(y[e]) >= least ? 1u << e : 0u;
+  while (__any_sync(half, todo)) {                        // lanes do theirs at the same time: once, mostly
+    const int at = __ffs(todo) - 1;
+    uint32_t word = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) word = e == at ? w[e] : word;
+    const double g = q128_lo(word), v = g / (1.0 + exp(-g)) * q128_hi(word);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e == at) {
+        y[e] = (float)v;
+        rest[e] = (float)(v - y[e]);
+      }
+    todo &= todo - 1;
+  }
+  amax = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(y[e]));
+  for (int d = 8; d > 0; d >>= 1) amax = fmaxf(amax, __shfl_xor_sync(half, amax, d));
+  amax = fmaxf(amax, kAmaxFloor);
+  const float inv = kE4m3Max / amax;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) y[e] = fmaf(y[e], inv, rest[e] * inv);
+  return make_uint3(q128_pack4(y[0], y[1], y[2], y[3]), q128_pack4(y[4], y[5], y[6], y[7]), __float_as_uint(amax / kE4m3Max));
+}
+
 // ---- rows -------------------------------------------------------------------------------------------------------------
 // Sixteen lanes take a block of 128 values, eight each (with GLU: of gate and up, interleaved, 32 bytes a lane), and blocks
 // that follow one another: all their loads are on their way before the first is looked at.  Which rows:
@@ -100,7 +155,7 @@ struct Rows128Args {
 };
 
 template <bool GLU, int PER>
-__global__ void __launch_bounds__(256, PER == 4 ? 4 : 6) quant128_rows_kernel(const Rows128Args a) {
+__global__ void __launch_bounds__(256, PER == 4 ? 4 : GLU ? 5 : 6) quant128_rows_kernel(const Rows128Args a) {
   wait_for_kernel_before();                               // (a launch of `chained`; the next one counts on it)
   next_kernel_may_start();
   const int kb = (a.K + 127) / 128;
@@ -158,20 +213,27 @@ __global__ void __launch_bounds__(256, PER == 4 ? 4 : 6) quant128_rows_kernel(co
   }
   float inv[PER];
   const float scale = q128_quotients<PER>(amax, lane16, half, inv);
+  uint32_t again = 0;                                     // GLU: blocks to be done again
+  const int64_t pitch = q128_pitch(a.K);
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
-    const int64_t pitch = q128_pitch(a.K);
     const int col = blk[j] * 128 + lane16 * 8;
     const bool in = col < a.K, mine = lane16 == 8 + j;        // the lane that has this block's scale
-    if (src[j] < 0) continue;
     uint2 out;
     if (GLU) {
-      const float* f = y[GLU ? j : 0];
-      out = make_uint2(q128_pack4(f[0] * inv[j], f[1] * inv[j], f[2] * inv[j], f[3] * inv[j]),
-                       q128_pack4(f[4] * inv[j], f[5] * inv[j], f[6] * inv[j], f[7] * inv[j]));
+      float f[8];
+      uint32_t near = 0xFFFFFFFFu;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        f[e] = y[GLU ? j : 0][e] * inv[j];
+        near = min(near, q128_from_border(f[e]));
+      }
+      again |= near < 2 * kQ128Near << 12 ? 1u << j : 0u;
+      out = make_uint2(q128_pack4(f[0], f[1], f[2], f[3]), q128_pack4(f[4], f[5], f[6], f[7]));
     } else {
       out = q128_pack8(v[j][0], inv[j]);
     }
+    if (src[j] < 0) continue;
     if (a.naept) {
       const int last = a.naept[src[j] + 1];
       for (int t = a.naept[src[j]]; t < last; ++t) {
@@ -183,6 +245,17 @@ __global__ void __launch_bounds__(256, PER == 4 ? 4 : 6) quant128_rows_kernel(co
     } else {
       if (in) *(uint2*)(a.q + src[j] * pitch + col) = out;
       if (mine) a.s[src[j] * kb + blk[j]] = scale;
+    }
+  }
+  if (GLU && __any_sync(0xffffffffu, again != 0)) {
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      if (!__any_sync(half, again >> j & 1)) continue;
+      const int col = blk[j] * 128 + lane16 * 8;
+      const bool in = src[j] >= 0 && col < a.K;
+      const uint3 out = q128_gated_again(in ? (const uint4*)((const uint16_t*)a.x + (src[j] * a.K + col) * 2) : nullptr, half);
+      if (in) *(uint2*)(a.q + src[j] * pitch + col) = make_uint2(out.x, out.y);
+      if (src[j] >= 0 && lane16 == 8 + j) a.s[src[j] * kb + blk[j]] = __uint_as_float(out.z);
     }
   }
 }
