@@ -86,56 +86,39 @@ __device__ __forceinline__ float q128_quotients(const float (&amax)[N], int lane
 // An activation's payload must not depend on how an exponential was rounded.  A value and its block's maximum are off by a unit or
 // two of the last place of f32 (more than kQ128Near for g below -16 or so); where that leaves a value within kQ128Near of the border
 // between two e4m3 values (three in 200,000), it and the maximum are made again in 64 bits.  Of 150 M values none is another than in
-// 64 bits then, with 4 in place of 8 one, without it 226.  It takes 16384 x 768 from 13.5 to 16.9 us, 512 x 768 from 2.4 to 3.7: half
-// for the look at every value, half for the last such block, of code that no cache holds.  (Borders below the least normal value,
-// 2^-6 of a maximum of 448, are not looked for.)
+// 64 bits then, with 4 in place of 8 one, without it 226.  It takes 16384 x 768 from 13.4 to 16.5 us, 512 x 768 from 2.4 to 3.4: half
+// for the look at every value, half for the last warp with such a block, whose code no cache holds.  (Borders below the least normal
+// value, 2^-6 of a maximum of 448, are not looked for.)
 constexpr uint32_t kQ128Near = 8;
 __device__ __forceinline__ uint32_t q128_from_border(float v) {      // below 2 * kQ128Near << 12: near one
   return (__float_as_uint(v) << 12) + 0x80000000u + (kQ128Near << 12);
 }
-// One block of sixteen lanes: eight values of a lane, gate and up from p on (none: null) -> payload, and the scale's bits
-__device__ __noinline__ uint3 q128_gated_again(const uint4* p, uint32_t half) {
-  uint32_t w[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-  if (p) {
-    *(uint4*)w = p[0];
-    *(uint4*)(w + 4) = p[1];
+__device__ __noinline__ double q128_gated64(uint32_t w) {
+  const double g = q128_lo(w);
+  return g / (1.0 + exp(-g)) * q128_hi(w);
+}
+// A block of sixteen lanes: words, q: gate and up, and the payload, of a lane's eight values; which: those that may be the largest, and
+// << 8 those near a border.  The payload of the others stands: none of them is near one.
+__device__ __noinline__ void q128_gated_again(const uint32_t* words, uint8_t* q, float* scale, uint32_t which, uint32_t half) {
+  uint32_t near = which >> 8;
+  const uint32_t first = near & (0u - near);
+  double mine = 0.0;
+  float a = kAmaxFloor;
+  for (uint32_t todo = (which & 0xFF) | first; __any_sync(half, todo); todo &= todo - 1) {      // lanes side by side: once, mostly
+    const uint32_t bit = todo & (0u - todo);
+    const double v = todo ? q128_gated64(words[__ffs(todo) - 1]) : 0.0;
+    if (which & 0xFF & bit) a = fmaxf(a, (float)fabs(v));
+    if (bit == first) mine = v;
   }
-  float y[8], rest[8], amax = 0.f;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    y[e] = q128_silu(q128_lo(w[e])) * q128_hi(w[e]);
-    rest[e] = 0.f;
-    amax = fmaxf(amax, fabsf(y[e]));
+  for (int d = 8; d > 0; d >>= 1) a = fmaxf(a, __shfl_xor_sync(half, a, d));
+  const float inv = kE4m3Max / a;
+  if (scale) *scale = a / kE4m3Max;
+  while (near) {
+    const int at = __ffs(near) - 1;
+    q[at] = (uint8_t)q128_pack4((float)(mine * inv), 0.f, 0.f, 0.f);
+    near &= near - 1;
+    if (near) mine = q128_gated64(words[__ffs(near) - 1]);
   }
-  for (int d = 8; d > 0; d >>= 1) amax = fmaxf(amax, __shfl_xor_sync(half, amax, d));
-  const float first = kE4m3Max / fmaxf(amax, kAmaxFloor), least = amax * (1.f - 1e-5f);
-  uint32_t todo = 0;                                      // near a border, or what may be the largest
-#pragma unroll
-  for (int e = 0; e < 8; ++e)
-    todo |= q128_from_border(y[e] * first) < 2 * kQ128Near << 12 || fabsf(y[e]) >= least ? 1u << e : 0u;
-  while (__any_sync(half, todo)) {                        // lanes do theirs at the same time: once, mostly
-    const int at = __ffs(todo) - 1;
-    uint32_t word = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) word = e == at ? w[e] : word;
-    const double g = q128_lo(word), v = g / (1.0 + exp(-g)) * q128_hi(word);
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (e == at) {
-        y[e] = (float)v;
-        rest[e] = (float)(v - y[e]);
-      }
-    todo &= todo - 1;
-  }
-  amax = 0.f;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(y[e]));
-  for (int d = 8; d > 0; d >>= 1) amax = fmaxf(amax, __shfl_xor_sync(half, amax, d));
-  amax = fmaxf(amax, kAmaxFloor);
-  const float inv = kE4m3Max / amax;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) y[e] = fmaf(y[e], inv, rest[e] * inv);
-  return make_uint3(q128_pack4(y[0], y[1], y[2], y[3]), q128_pack4(y[4], y[5], y[6], y[7]), __float_as_uint(amax / kE4m3Max));
 }
 
 // ---- rows -------------------------------------------------------------------------------------------------------------
@@ -213,23 +196,42 @@ __global__ void __launch_bounds__(256, PER == 4 ? 4 : GLU ? 5 : 6) quant128_rows
   }
   float inv[PER];
   const float scale = q128_quotients<PER>(amax, lane16, half, inv);
-  uint32_t again = 0;                                     // GLU: blocks to be done again
   const int64_t pitch = q128_pitch(a.K);
+  uint2 gated[GLU ? PER : 1];
+  uint32_t again = 0;                                     // GLU: values of each block to be made again, see q128_gated_again
+  if (GLU) {
+    uint32_t near = 0xFFFFFFFFu;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      float f[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        f[e] = y[GLU ? j : 0][e] * inv[j];
+        near = min(near, q128_from_border(f[e]));
+      }
+      gated[GLU ? j : 0] = make_uint2(q128_pack4(f[0], f[1], f[2], f[3]), q128_pack4(f[4], f[5], f[6], f[7]));
+    }
+    if (__any_sync(0xffffffffu, near < 2 * kQ128Near << 12)) {
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        uint32_t top = 0, by = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float x = y[GLU ? j : 0][e];
+          top |= fabsf(x) >= amax[j] * (1.f - 1e-5f) ? 1u << e : 0u;
+          by |= q128_from_border(x * inv[j]) < 2 * kQ128Near << 12 ? 1u << e : 0u;
+        }
+        if (__any_sync(half, by)) again |= (by << 8 | top) << (16 * j);
+      }
+    }
+  }
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
     const int col = blk[j] * 128 + lane16 * 8;
     const bool in = col < a.K, mine = lane16 == 8 + j;        // the lane that has this block's scale
     uint2 out;
     if (GLU) {
-      float f[8];
-      uint32_t near = 0xFFFFFFFFu;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        f[e] = y[GLU ? j : 0][e] * inv[j];
-        near = min(near, q128_from_border(f[e]));
-      }
-      again |= near < 2 * kQ128Near << 12 ? 1u << j : 0u;
-      out = make_uint2(q128_pack4(f[0], f[1], f[2], f[3]), q128_pack4(f[4], f[5], f[6], f[7]));
+      out = gated[GLU ? j : 0];
     } else {
       out = q128_pack8(v[j][0], inv[j]);
     }
@@ -247,15 +249,14 @@ __global__ void __launch_bounds__(256, PER == 4 ? 4 : GLU ? 5 : 6) quant128_rows
       if (mine) a.s[src[j] * kb + blk[j]] = scale;
     }
   }
-  if (GLU && __any_sync(0xffffffffu, again != 0)) {
+  if (GLU && __any_sync(0xffffffffu, again)) {
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-      if (!__any_sync(half, again >> j & 1)) continue;
-      const int col = blk[j] * 128 + lane16 * 8;
-      const bool in = src[j] >= 0 && col < a.K;
-      const uint3 out = q128_gated_again(in ? (const uint4*)((const uint16_t*)a.x + (src[j] * a.K + col) * 2) : nullptr, half);
-      if (in) *(uint2*)(a.q + src[j] * pitch + col) = make_uint2(out.x, out.y);
-      if (src[j] >= 0 && lane16 == 8 + j) a.s[src[j] * kb + blk[j]] = __uint_as_float(out.z);
+      const uint32_t which = again >> (16 * j) & 0xFFFF;
+      if (!__any_sync(half, which)) continue;
+      const int64_t at = blk[j] * 128 + lane16 * 8;            // (lanes beyond the columns ask for nothing)
+      q128_gated_again((const uint32_t*)a.x + src[j] * a.K + at, a.q + src[j] * pitch + at,
+                       lane16 == 8 + j ? a.s + src[j] * kb + blk[j] : nullptr, which, half);
     }
   }
 }
@@ -406,8 +407,8 @@ static int launch_rows(const Rows128Args& a, bool glu, bool chained, void* strea
   if (a.n == 0 || a.out_rows == 0) return SMOE_OK;
   const int64_t units = a.n * ((a.K + 127) / 128);
   // Several blocks each where that leaves every SM enough warps: four, or two where the activation's or a token's many rows need
-  // the registers.  8192 x 4096 one block 28.0 us, two 24.2, four 22.7; gated 32768 x 768 40, 25.2, 26.5; eight places a token 18.6,
-  // 18.4, 19.9.
+  // the registers.  8192 x 4096 one block 28.0 us, two 24.2, four 22.7; gated 32768 x 768 40, 25.2, 26.5 (two with q128_gated_again
+  // 28.9); eight places a token 18.6, 18.4, 19.9.
   const int most = glu || a.naept ? 2 : 4, per = units >= (int64_t)sm_count() * 64 * 4 ? most : 1;
   const int64_t grid = (units + 16 * per - 1) / (16 * per);
   if (grid >= (int64_t)1 << 31) return SMOE_ERR_SHAPE;
