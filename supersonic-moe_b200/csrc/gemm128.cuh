@@ -8,8 +8,9 @@
 // a CTA pair.  Two TMEM buffers of 256 columns: the MMAs of one block run while the block before is read out and added up.
 //   What bounds it: by rows, shared memory, out of which the MMAs of a block (512 clocks of arithmetic) read their operands in some
 //   640; a block takes 750, and a tile some 3400 clocks beside its blocks.  8192 x 4096 x 4096 123 us (2.2 PFLOP/s), 16384 x 4096 x
-//   2048 over 8 experts 133, its dx 128.  The weight gradient: the arithmetic of the epilogue, where a value has two scales of its
-//   own in every block; the same size 191 us (1.4 PFLOP/s), added to f32 221.
+//   2048 over 8 experts 133, its dx 128.  The weight gradient: the epilogue's latencies, where a value has two scales of its own in
+//   every block: two warps a scheduler, 0.7 of them eligible, no pipe more than half busy (issue 47 %, FMA 47, TMEM 47, MMA 34); the
+//   same size 191 us (1.4 PFLOP/s), added to f32 221.
 //   B [E, N, K] is read K-major, or with b_mn as [E, K, N] as it lies: the gradient of the rows needs no transposed weights.
 //   Both operands of the weight gradient lie [dim, rows].
 #pragma once

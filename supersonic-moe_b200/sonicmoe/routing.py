@@ -1,5 +1,6 @@
 """Routers beside the layer's own softmax top-k: `group_limited_routing` makes the [T,K] tables that `run_sonic_moe` and
-`block128_experts` take, `token_rounding_routing` (score, token, expert) pair lists for `moe_general_routing_inputs`.
+`block128_experts` take (up to 16 experts a token, of 256 there), `token_rounding_routing` (score, token, expert) pair lists for
+`moe_general_routing_inputs`.
 
 `token_rounding_routing` restates the token-rounding router of the reference's benchmark
 (benchmarks/moe-token-rounding.py:139-181): a token-choice top-K pass fixes each expert's load, the load is rounded
@@ -48,7 +49,9 @@ def group_limited_routing(router_logits: torch.Tensor, K: int, *, score: str = "
 
     A logit of -inf closes its expert; a row with fewer than K open experts ends in slots of index -1 and score 0 (the layer's
     mark of a slot without an expert), so that a padded token is a row of -inf.  NaN ranks lowest.  The selection is that of 64-bit
-    arithmetic: it does not depend on how an exponential is rounded.  E <= 1024, K <= 32, groups <= 32."""
+    arithmetic: it does not depend on how an exponential is rounded.  A bias of -inf makes its expert the last choice, and one of
+    two best experts that has it its group, without closing them.  E <= 1024, K <= 32, groups <= 32 (the layer and
+    `block128_experts` take tables of K <= 16, the latter of E <= 256)."""
     if score not in ("sigmoid", "softmax"):
         raise ValueError(f"score={score!r}: 'sigmoid' or 'softmax'")
     if router_logits.ndim != 2 or router_logits.dtype not in (torch.float32, torch.bfloat16):
