@@ -501,7 +501,8 @@ int smoe_group_routing_bwd(const void* logits, int bf16, const int32_t* idx, con
  * all); efo null: one segment (E = 1) of all rows. */
 
 /* x bf16 [rows,K] -> q [rows,K], scales [rows, K/128].  swiglu: x is [rows,2K], gate / up interleaved, and what is quantised is
- * silu(gate) * up (f32).  list != null: only the rows list[i], i < min(n_list, *n_live), are read and written. */
+ * silu(gate) * up, whose payload is that of 64-bit arithmetic (below 2^-6 of a maximum of 448, or with gates below -16, a value may be
+ * a step off) and whose scale is off by a few roundings of f32.  list != null: only the rows list[i], i < min(n_list, *n_live), are read and written. */
 int smoe_quant128_rows(const void* x_bf16, int64_t rows, int64_t K, int swiglu, const int32_t* list, const int32_t* n_live,
                        int64_t n_list, void* q, float* scales, void* stream);
 /* x bf16 [T,K]: row t, quantised once, to the rows s_rev[naept[t]] .. s_rev[naept[t+1] - 1] of q [rows,K], scales [rows, K/128]. */

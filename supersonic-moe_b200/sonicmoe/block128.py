@@ -25,7 +25,7 @@ def _dense(t: torch.Tensor) -> torch.Tensor:
 def quantize_rows_block128(x: torch.Tensor, swiglu: bool = False):
     """bf16 [rows,K] -> (e4m3 [rows,K], scales f32 [rows,ceil(K/128)]).  `swiglu`: x is [rows,2K] with gate and up interleaved (what an
     up-projection leaves) and silu(gate) * up is what is quantised, without leaving the chip in between; the payload is that of
-    64-bit arithmetic."""
+    64-bit arithmetic (but for e4m3's subnormals, and gates below -16)."""
     q, s = ops.quant128_rows(_dense(x), swiglu)
     return q.view(_E4M3), s
 
@@ -126,7 +126,7 @@ def block128_experts(x: torch.Tensor, topk_indices: torch.Tensor, topk_scores: t
     x bf16 [T,H]; topk_indices [T,K] (-1: no expert in this slot; one that a token names twice counts twice), topk_scores [T,K];
     w1_fp8, w2_fp8: pairs of `quantize_weight_block128` of W1 [E,2I,H] and W2 [E,H,I], E <= 256, K <= 16 (a checkpoint that holds gate and
     up as two matrices has other blocks than W1: it is put together in bf16 and quantised).  Returns bf16 [T,H].  Both products
-    leave bf16; what lies between is quantised in blocks of 128 like x, its payload that of 64-bit arithmetic.  No gradient flows."""
+    leave bf16; what lies between is quantised in blocks of 128 like x, as `quantize_rows_block128` does it.  No gradient flows."""
     if x.ndim != 2 or x.dtype != torch.bfloat16:
         raise ValueError(f"block128_experts: x is bf16 [T,H], got {x.dtype} {tuple(x.shape)}")
     ops.poll_status(x.device)
