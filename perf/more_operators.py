@@ -176,6 +176,14 @@ def _norm(st, f):
     return h, r, hf * r * st["weight"].detach().to(f)
 
 
+def _bf16(v):
+    """The bf16 nearest to each f64, without a stop in f32 that may turn a value beside a border into one on it."""
+    f = v.float()
+    bits = f.view(torch.int32)
+    side = (v.abs() - f.double().abs()).sign().int()
+    return torch.where((bits & 0xFFFF) == 0x8000, bits + side, bits).view(torch.float32).to(torch.bfloat16)
+
+
 def _norm_train(st, f):
     h, r, y = _norm(st, f)
     hf, dy = h.to(f), st["dy"].to(f)
@@ -246,7 +254,7 @@ def _plain(st):
         return out + ([] if st["residual"] is None else [h])
     if kind == "norm_quant":
         h, _, y = _norm(st, torch.float64)                      # which side of a border between two bf16 a value lies on
-        y = y.to(torch.bfloat16)
+        y = _bf16(y)
         return [*_payload(y, case["scales"])] + ([y] if case["rows_too"] else []) + ([] if st["residual"] is None else [h])
     if kind == "grouped":
         return [_grouped(st, f, False)[0].to(torch.bfloat16)]
@@ -356,7 +364,9 @@ def exact(case, seed):
             dh = (g - unit * along) / length
             out += [dh if st["dh"] is None else dh + st["dh"].double(), torch.einsum("th,th->h", st["dy"].double(), unit)]
         if kind == "norm_quant":
-            y = out.pop().to(torch.bfloat16).double()                # the definition quantises bf16 rows
+            v = out.pop()                                            # the definition quantises bf16 rows: 8 bits of v, rounded once
+            step = torch.ldexp(torch.ones_like(v), torch.frexp(v).exponent.clamp(min=-125) - 8)
+            y = torch.round(v / step) * step
             size = 32 if case["scales"] == "mx" else 128
             q, scales = torch.empty_like(y), []
             for a in range(0, H, size):
