@@ -555,6 +555,41 @@ int smoe_block128_experts(const void* x_bf16, const int32_t* idx, const float* s
                           const void* w2_fp8, const float* w2_scales, void* out_bf16, void* scratch, int64_t T, int64_t H,
                           int64_t I, int64_t E, int64_t K, int32_t* status, int32_t* pinned_host_word, void* stream);
 
+/* ---- the norm in front of the experts -------------------------------------------
+ * No counterpart in the reference, whose layer begins behind it.
+ * h = x + residual, held in the residual's type (without one h = x and nothing is written); r = 1 / sqrt(mean(h^2) + eps), one a
+ * row; y = h r w.  x, y bf16 or f32 [T,H], rows of x ldx values apart; residual, h of x's type or f32, rows of the residual ldr
+ * apart; w bf16 or f32 [H]; rstd f64 [T] or null.  H <= 16384.  The mean and r are f64, and bf16 results those of 64 bits.
+ * scale_kind 1 (x bf16, H % 32 == 0): of y, q e4m3 [T,H] and scales u8 [T,H/32] as smoe_quant_rows makes them; 2 (x bf16, H % 8 == 0): q, rows
+ * ceil(H/16)*16 bytes apart, and scales f32 [T,ceil(H/128)] as smoe_quant128_rows does; y may then be null. */
+int smoe_rms_norm(const void* x, int x_f32, int64_t ldx, const void* residual, int residual_f32, int64_t ldr, const void* w, int w_f32,
+                  int64_t T, int64_t H, double eps, void* y, void* h, double* rstd, int scale_kind, void* q, void* scales,
+                  void* stream);
+/* g = dy w, dh' = r (g - h r^2 mean(g h)) + dh: to dx (x's type) and, where h is f32 and x bf16, dres (f32); dw = the sum over rows of
+ * dy h r, bf16 or f32, or added to f32.  dy of x's type [T,H], h rows ldh apart, dh of h's type [T,H] or null.  dx, dres, dw may be
+ * null.  workspace: smoe_rms_norm_bwd_workspace bytes where dw is wanted (-1 for sizes that are not taken). */
+int64_t smoe_rms_norm_bwd_workspace(int64_t T, int64_t H);
+int smoe_rms_norm_bwd(const void* dy, int x_f32, const void* h, int h_f32, int64_t ldh, const void* w, int w_f32, const double* rstd,
+                      const void* dh, int64_t T, int64_t H, void* dx, void* dres, void* dw, int dw_f32, int dw_accumulate,
+                      void* workspace, void* stream);
+
+/* ---- the norm of the gradients, and their clipping ------------------------------
+ * No counterpart in the reference, which leaves both to its host framework.
+ * list: `count` tensors of numel values in HOST memory, read before the call returns; grad and out are device memory, f32 (!= 0) or
+ * bf16; out == grad scales in place, otherwise they do not overlap.  norm = sqrt(sum of all squares), f32 in device memory. */
+typedef struct {
+  const void* grad;
+  void* out;                 /* smoe_gradient_norm: not looked at */
+  int64_t numel;
+  int32_t grad_f32, out_f32;
+} smoe_gradient;
+int64_t smoe_gradient_workspace(int64_t count);
+int smoe_gradient_norm(const smoe_gradient* list, int64_t count, float* norm, void* workspace, void* stream);
+/* out = grad * min(1, max_norm / (n + 1e-6)), n the norm, which also goes to `norm`; or *given_norm, if that is not null (norm and
+ * workspace may then be null).  In place and with a factor of 1 nothing is written. */
+int smoe_gradient_clip(const smoe_gradient* list, int64_t count, double max_norm, const float* given_norm, float* norm, void* workspace,
+                       void* stream);
+
 #ifdef __cplusplus
 }
 #endif

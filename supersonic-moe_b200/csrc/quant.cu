@@ -10,41 +10,13 @@
 #include <stdint.h>
 
 #include "ptx.cuh"
+#include "quant_groups.cuh"
 #include "smoe_b200.h"
 
 namespace smoe {
 
-__device__ __forceinline__ int q_e8m0_of(float amax) {
-  const int bits = __float_as_int(amax);
-  const int bexp = (bits >> 23) & 0xFF;
-  const int e = bexp - 8 + ((bits & 0x7FFFFF) > 0x600000 ? 1 : 0);
-  return bexp > 0 ? max(e, 0) : 0;
-}
-__device__ __forceinline__ float q_scale_of(int e8m0) {
-  return __int_as_float(min(max(254 - e8m0, 1), 254) << 23);
-}
-__device__ __forceinline__ uint32_t q_pack4(float a, float b, float c, float d) {
-  uint16_t lo, hi;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
-  return (uint32_t)lo | ((uint32_t)hi << 16);
-}
-__device__ __forceinline__ void bf16x8_to_f32(const uint4& v, float (&f)[8]) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    f[2 * i] = __uint_as_float(w[i] << 16);
-    f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-  }
-}
 __device__ __forceinline__ size_t isa_offset(size_t row, size_t g, size_t k_tiles) {
   return ((row >> 7) * k_tiles + (g >> 2)) * 512 + (row & 31) * 16 + ((row & 127) >> 5) * 4 + (g & 3);
-}
-
-__device__ __forceinline__ uint32_t q_max_bf16x2(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
 }
 
 // max of the magnitudes of two bf16 pairs, element by element; the sign bits are those of the product

@@ -12,13 +12,11 @@
 
 #include "host.h"
 #include "ptx.cuh"
+#include "quant_groups.cuh"
 #include "smoe_b200.h"
 #include "smoe_internal.h"
 
 namespace smoe {
-
-constexpr float kE4m3Max = 448.f;
-constexpr float kAmaxFloor = 7.888609052210118e-31f;      // 2^-100: 448 / a stays finite, a / 448 normal
 
 __device__ __forceinline__ uint32_t q128_pack4(float a, float b, float c, float d) {
   uint16_t lo, hi;

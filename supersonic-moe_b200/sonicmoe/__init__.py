@@ -28,7 +28,9 @@ from .functional import (  # noqa: F401
     moe_TC_softmax_topk_layer,
     precompute_weight_fp8,
 )
+from .gradients import clip_gradients, gradient_norm  # noqa: F401
 from .interface import run_sonic_moe  # noqa: F401
 from .moe import MoE  # noqa: F401
+from .norm import NormQuantized, rms_norm, rms_norm_quantized  # noqa: F401
 from .quack_utils import pack_blockscaled_1x32_scales  # noqa: F401
 from .routing import group_limited_routing, token_rounding_routing  # noqa: F401

@@ -7,12 +7,12 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_float, c_int, c_int64, c_void_p
+from ctypes import c_double, c_float, c_int, c_int64, c_void_p
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libsmoe_b200.so")
 
-_P, _I, _L, _F = c_void_p, c_int, c_int64, c_float
+_P, _I, _L, _F, _D = c_void_p, c_int, c_int64, c_float, c_double
 
 
 class LayerArgs(ctypes.Structure):
@@ -102,6 +102,12 @@ SIGNATURES = {
     "smoe_block128_linear_bwd": (_I, [_P] * 9 + [_L] * 4 + [_I, _I, _P, _P, _P]),
     "smoe_block128_experts_bytes": (_L, [_L] * 5),
     "smoe_block128_experts": (_I, [_P] * 9 + [_L] * 5 + [_P, _P, _P]),
+    "smoe_rms_norm": (_I, [_P, _I, _L, _P, _I, _L, _P, _I, _L, _L, _D, _P, _P, _P, _I, _P, _P, _P]),
+    "smoe_rms_norm_bwd_workspace": (_L, [_L, _L]),
+    "smoe_rms_norm_bwd": (_I, [_P, _I, _P, _I, _L, _P, _I, _P, _P, _L, _L, _P, _P, _P, _I, _I, _P, _P]),
+    "smoe_gradient_workspace": (_L, [_L]),
+    "smoe_gradient_norm": (_I, [_P, _L, _P, _P, _P]),
+    "smoe_gradient_clip": (_I, [_P, _L, _D, _P, _P, _P, _P]),
 }
 
 # exported for the library's own tests only (csrc/smoe_internal.h); not product ABI
