@@ -555,6 +555,22 @@ int smoe_block128_experts(const void* x_bf16, const int32_t* idx, const float* s
                           const void* w2_fp8, const float* w2_scales, void* out_bf16, void* scratch, int64_t T, int64_t H,
                           int64_t I, int64_t E, int64_t K, int32_t* status, int32_t* pinned_host_word, void* stream);
 
+/* ---- products of bf16 rows grouped by expert -------------------------------------
+ * In the precision of the weights, beside the 8-bit products above; segments begin and end at any row.
+ * efo [E+1] ascending first rows, counts [E] live rows at a segment's start (null: all); efo null: one segment (E = 1) of all rows.
+ * Rows that are not live, those before the first and behind the last segment among them, are never part of a result.  f32 sums.
+ * N, K and the distances between rows (ldx, ldy, in values) are multiples of 8, tensors start on 16 bytes, E <= 256. */
+
+/* y[r,:] = x[r,:] . w[e(r)]^T, bf16 [rows,N]: x [rows,K], w [E,N,K], or w_transposed [E,K,N] (the gradient of the rows reads the weights as
+ * they lie); rows that are not live become zero.  pinned_host_word (may be null) receives a failure code at once. */
+int smoe_grouped_rows(const void* x_bf16, int64_t ldx, const void* w_bf16, int w_transposed, const int32_t* efo, const int32_t* counts,
+                      void* y_bf16, int64_t rows, int64_t N, int64_t K, int64_t E, int32_t* status, int32_t* pinned_host_word,
+                      void* stream);
+/* dw[e] (N x K) = the sum over e's live rows of dy[r,:]^T x[r,:]: f32, added to dw or stored, or rounded to bf16. */
+int smoe_grouped_wgrad(const void* dy_bf16, int64_t ldy, const void* x_bf16, int64_t ldx, const int32_t* efo, const int32_t* counts,
+                       void* dw, int64_t N, int64_t K, int64_t rows, int64_t E, int out_bf16, int accumulate, int32_t* status,
+                       int32_t* pinned_host_word, void* stream);
+
 /* ---- the norm in front of the experts -------------------------------------------
  * No counterpart in the reference, whose layer begins behind it.
  * h = x + residual, held in the residual's type (without one h = x and nothing is written); r = 1 / sqrt(mean(h^2) + eps), one a

@@ -47,29 +47,6 @@ struct Few128Smem {
   static_assert((2 * STAGES + 2 * ACC + 2 + 2 * SX_SLOTS) * 8 <= kFewBars, "barrier storage");
 };
 
-// as mbar_wait, for data that other CTAs of the cluster left before they arrived
-__device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity) {
-  const uint64_t t0 = globaltimer_ns();
-  uint32_t spins = 0;
-  while (true) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity), "r"(kTryWaitHintNs)
-        : "memory");
-    if (ok) return true;
-    if ((++spins & 0x3ff) == 0 && globaltimer_ns() - t0 > kWaitLimitNs) return false;
-  }
-}
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
-}
-
 struct FewTile128 {
   int e, w0, row0, live;     // live: 1 .. NT
 };

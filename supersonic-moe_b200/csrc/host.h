@@ -11,7 +11,15 @@ namespace smoe {
 inline PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
 inline std::once_flag g_encode_once;
 
+// The encoder wants a current context, which a thread that has launched nothing yet (autograd's, whose first call is a product) lacks
+inline void bind_context() {
+  static thread_local int bound = -1;
+  int dev = 0;
+  if (cudaGetDevice(&dev) == cudaSuccess && dev != bound && cudaSetDevice(dev) == cudaSuccess) bound = dev;
+}
+
 inline bool load_encode() {
+  bind_context();
   std::call_once(g_encode_once, [] {
     void* fn = nullptr;
     cudaDriverEntryPointQueryResult qres;

@@ -29,6 +29,7 @@ from .functional import (  # noqa: F401
     precompute_weight_fp8,
 )
 from .gradients import clip_gradients, gradient_norm  # noqa: F401
+from .grouped import grouped_linear  # noqa: F401
 from .interface import run_sonic_moe  # noqa: F401
 from .moe import MoE  # noqa: F401
 from .norm import NormQuantized, rms_norm, rms_norm_quantized  # noqa: F401

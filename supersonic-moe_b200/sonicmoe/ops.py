@@ -1144,6 +1144,50 @@ def block128_experts(x, idx, scores, w1, w1_s, w2, w2_s, E, I):
     return out
 
 
+# ---------------------------------------------------------------- products of bf16 rows grouped by expert
+def _check_grouped(efo, counts, E, N, K, what):
+    check_segments(efo, counts, E, what)
+    if N <= 0 or K <= 0 or N % 8 or K % 8 or not 1 <= E <= 256:
+        raise ValueError(f"{what}: {E} experts of {N} x {K}: sizes are multiples of 8, 1 to 256 experts")
+
+
+def _ld(t):
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+@_op
+def grouped_rows(x, w, efo=None, counts=None, transposed=False):
+    """x bf16 [rows,K] (rows any multiple of 8 values apart, from a 16-byte boundary on), w bf16 [E,N,K], or `transposed` [E,K,N] -> bf16
+    [rows,N], zero where a row is not live."""
+    _check_same_gpu("grouped_rows", x, w, efo, counts)
+    rows, K = x.shape
+    E, N = w.shape[0], w.shape[2 if transposed else 1]
+    y = x.new_empty((rows, N))
+    check(lib.smoe_grouped_rows(x.data_ptr(), _ld(x), w.data_ptr(), transposed, _p(efo), _p(counts), y.data_ptr(), rows, N, K, E,
+                                *failure_words(x.device), _stream()), "grouped_rows")
+    return y
+
+
+@_op
+def grouped_wgrad(dy, x, efo, counts, E, main_grad=None):
+    """dy bf16 [rows,N], x bf16 [rows,K] (as above) -> bf16 [E,N,K], or None where it is added to `main_grad` f32."""
+    _check_same_gpu("grouped_wgrad", dy, x, efo, counts, main_grad)
+    (rows, N), K = dy.shape, x.shape[1]
+    if main_grad is None:
+        dw = dy.new_empty((E, N, K))
+    elif main_grad.data_ptr() % 16 == 0:
+        dw = main_grad
+    else:                                        # what is added leaves in pieces that start on 16 bytes
+        dw = dy.new_zeros((E, N, K), dtype=_F32)
+    check(lib.smoe_grouped_wgrad(dy.data_ptr(), _ld(dy), x.data_ptr(), _ld(x), _p(efo), _p(counts), dw.data_ptr(), N, K, rows, E,
+                                 main_grad is None, main_grad is not None, *failure_words(dy.device), _stream()), "grouped_wgrad")
+    if main_grad is None:
+        return dw
+    if dw is not main_grad:
+        main_grad.add_(dw.view(main_grad.shape))
+    return None
+
+
 # ---------------------------------------------------------------- the norm in front of the experts
 NORM_SCALES = {None: 0, "mx": 1, "block128": 2}
 NORM_MAX_H = 16384
