@@ -3,11 +3,13 @@
     python supersonic-moe_b200/build.py [--force] [--verbose]
 
 The library lands next to the Python package (sonicmoe/libsmoe_b200.so) and is
-loaded with ctypes; it links nothing but the CUDA runtime.
+loaded with ctypes; it links nothing but the CUDA runtime.  Beside it lies
+sonicmoe/_host.so, which calls it on torch tensors (csrc/host_torch.cpp).
 """
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -16,6 +18,8 @@ OUT = os.path.join(HERE, "sonicmoe", "libsmoe_b200.so")
 SOURCES = ["routing.cu", "quant.cu", "combine.cu", "glu.cu", "ep_plan.cu", "ep_peer.cu", "gemm.cu", "layer.cu",
            "group_routing.cu", "quant128.cu", "gemm128.cu", "block128.cu",
            "norm.cu", "grad_norm.cu", "grouped.cu"]
+HOST_SOURCE = os.path.join(CSRC, "host_torch.cpp")
+HOST_OUT = os.path.join(HERE, "sonicmoe", "_host.so")
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", "-I", INCLUDE, "-I", CSRC]
 
@@ -25,6 +29,17 @@ def _stale(target, deps):
         return True
     t = os.path.getmtime(target)
     return any(os.path.getmtime(d) > t for d in deps)
+
+
+def _host_command():
+    import torch
+    at = os.path.dirname(torch.__file__)
+    return ([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+            + [a for i in (INCLUDE, os.path.join(at, "include"), os.path.join(at, "include", "torch", "csrc", "api", "include"),
+                           sysconfig.get_paths()["include"], "/usr/local/cuda/include") for a in ("-I", i)]
+            + [HOST_SOURCE, "-o", HOST_OUT, "-L", os.path.dirname(OUT), "-lsmoe_b200", "-L", os.path.join(at, "lib"), "-ltorch_python",
+               "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"])
 
 
 def build(force=False, verbose=False):
@@ -50,6 +65,8 @@ def build(force=False, verbose=False):
     if force or procs or _stale(OUT, objs):
         cmd = [nvcc, "-shared", "-o", OUT] + objs + ["-lcudart"]
         subprocess.check_call(cmd)
+    if force or _stale(HOST_OUT, [HOST_SOURCE, headers[-1]]):
+        subprocess.check_call(_host_command())
     return OUT
 
 

@@ -1,0 +1,401 @@
+// The host side of the operators around the experts, on torch tensors: outputs from the caching allocator, the current stream, autograd
+// nodes.  What Python and ctypes take for it is longer than the kernels of a small batch, or than the look at a list of a few hundred
+// gradients (us a call through Python / here: one decoded token's norm 21 / 13, norm with its backward pass 114 / 70, the norm of 300
+// gradients 205 / 29).  The kernels are those of the C ABI; nothing here computes.
+#include <ATen/core/Tensor.h>
+#include <ATen/ops/empty.h>
+#include <ATen/ops/empty_like.h>
+#include <ATen/ops/zeros.h>
+#include <ATen/ops/zeros_like.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/utils/pybind.h>
+
+#include <algorithm>
+#include <optional>
+#include <string>
+#include <tuple>
+#include <vector>
+
+#include "smoe_b200.h"
+
+namespace py = pybind11;
+using at::Tensor;
+using Maybe = std::optional<Tensor>;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+namespace {
+
+constexpr int64_t kMxGroup = 32, kBlock = 128;
+
+void check(int rc, const char* what) {
+  static const char* const names[] = {"SMOE_OK",       "SMOE_ERR_SHAPE",  "SMOE_ERR_ALIGN", "SMOE_ERR_DRIVER",
+                                      "SMOE_ERR_TMAP", "SMOE_ERR_LAUNCH", "SMOE_ERR_ARG"};
+  TORCH_CHECK(rc == 0, what, " failed: ", rc > 0 && rc < 7 ? names[rc] : "an unknown error");
+}
+// (numbers go into messages as text: the formatting of a stream clashes with that of libstdc++ inside torch's own libraries)
+std::string text(at::IntArrayRef v) {
+  std::string s = "[";
+  for (size_t i = 0; i < v.size(); ++i) s += (i ? ", " : "") + std::to_string(v[i]);
+  return s + "]";
+}
+bool f32(const Tensor& t) { return t.scalar_type() == at::kFloat; }
+void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+Tensor of(const Maybe& t) { return t ? *t : Tensor(); }
+int64_t distance(const Tensor& rows) { return rows.size(0) > 1 ? rows.stride(0) : rows.size(1); }
+
+void* stream() { return c10::cuda::getCurrentCUDAStream().stream(); }
+
+void same_gpu(const char* what, const Tensor& first, std::initializer_list<const Tensor*> others) {
+  TORCH_CHECK(first.is_cuda(), "sonicmoe kernels need CUDA tensors (no CPU fallback)");
+  for (const Tensor* t : others)
+    TORCH_CHECK(!t->defined() || t->device() == first.device(), what, ": tensors on different devices (", first.device().str(), " and ",
+                t->device().str(), ")");
+}
+
+// Gradients of gradients that could be differentiated again are not: their use raises
+variable_list once_only(const variable_list& in, variable_list out) {
+  if (!at::GradMode::is_enabled() ||
+      std::none_of(in.begin(), in.end(), [](const Tensor& t) { return t.defined() && t.requires_grad(); }))
+    return out;
+  const auto error = std::make_shared<torch::autograd::DelayedError>("trying to differentiate twice a function whose gradients cannot be",
+                                                                     (int64_t)out.size());
+  for (Tensor& t : out)
+    if (t.defined()) t = t.detach().set_requires_grad(true);
+  return (*error)(std::move(out));
+}
+
+// ---------------------------------------------------------------- the norm in front of the experts
+struct Norm {
+  Tensor y, h, q, s, r;
+};
+
+// x [T,H], rows any distance apart; kind: see smoe_rms_norm
+Norm norm(const Tensor& x, const Tensor& w, const Tensor& residual, double eps, int kind, bool with_y, bool keep) {
+  same_gpu("rms_norm", x, {&w, &residual});
+  const c10::cuda::CUDAGuard guard(x.device());
+  const int64_t T = x.size(0), H = x.size(1);
+  const auto o = x.options().requires_grad(false);
+  Norm n;
+  if (with_y || !kind) n.y = at::empty({T, H}, o);
+  if (residual.defined()) n.h = at::empty({T, H}, residual.options().requires_grad(false));
+  if (keep) n.r = at::empty({T}, o.dtype(at::kDouble));
+  if (kind == 1) {
+    n.q = at::empty({T, H}, o.dtype(at::kFloat8_e4m3fn));
+    n.s = at::empty({T, H / kMxGroup}, o.dtype(at::kByte));
+  } else if (kind == 2) {
+    n.q = at::empty({T, (H + 15) / 16 * 16}, o.dtype(at::kFloat8_e4m3fn));
+    if (H % 16) n.q = n.q.narrow(1, 0, H);
+    n.s = at::empty({T, (H + kBlock - 1) / kBlock}, o.dtype(at::kFloat));
+  }
+  check(smoe_rms_norm(x.data_ptr(), f32(x), distance(x), ptr(residual), residual.defined() && f32(residual),
+                      residual.defined() ? distance(residual) : H, w.data_ptr(), f32(w), T, H, eps, ptr(n.y), ptr(n.h),
+                      (double*)ptr(n.r), kind, ptr(n.q), ptr(n.s), stream()),
+        "rms_norm");
+  return n;
+}
+
+// -> gradients of x, of the residual where its type is another, of the weight
+std::tuple<Tensor, Tensor, Tensor> norm_backward(const Tensor& dy, const Tensor& h, const Tensor& w, const Tensor& r, const Tensor& dh,
+                                                 bool want_x, bool want_res, bool want_w, const Tensor& main_grad) {
+  same_gpu("rms_norm_bwd", dy, {&h, &w, &r, &dh, &main_grad});
+  const c10::cuda::CUDAGuard guard(dy.device());
+  const int64_t T = dy.size(0), H = dy.size(1);
+  const auto o = dy.options().requires_grad(false);
+  Tensor gx, gr, gw, ws;
+  if (want_x) gx = at::empty({T, H}, o);
+  if (want_res) gr = at::empty({T, H}, o.dtype(h.scalar_type()));
+  if (want_w) {
+    gw = main_grad.defined() ? main_grad : at::empty({H}, o.dtype(w.scalar_type()));
+    ws = at::empty({smoe_rms_norm_bwd_workspace(T, H)}, o.dtype(at::kByte));
+  }
+  check(smoe_rms_norm_bwd(dy.data_ptr(), f32(dy), h.data_ptr(), f32(h), distance(h), w.data_ptr(), f32(w), (const double*)r.data_ptr(),
+                          ptr(dh), T, H, ptr(gx), ptr(gr), ptr(gw), want_w && f32(gw), main_grad.defined(), ptr(ws), stream()),
+        "rms_norm_bwd");
+  return {gx, gr, main_grad.defined() ? Tensor() : gw};
+}
+
+struct NormNode : torch::autograd::Function<NormNode> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Maybe& residual, double eps, int64_t kind) {
+    const Tensor res = of(residual);
+    const Norm n = norm(x, w, res, eps, (int)kind, true, true);
+    ctx->save_for_backward({res.defined() ? n.h : x, w, n.r});
+    ctx->saved_data["added"] = res.defined();
+    ctx->saved_data["apart"] = res.defined() && res.scalar_type() != x.scalar_type();
+    ctx->saved_data["type"] = (int64_t)x.scalar_type();
+    ctx->set_materialize_grads(false);
+    variable_list out = {n.y};
+    if (res.defined()) out.push_back(n.h);
+    if (kind) {
+      out.push_back(n.q);
+      out.push_back(n.s);
+      ctx->mark_non_differentiable({n.q, n.s});
+    }
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &h = saved[0], &w = saved[1], &r = saved[2];
+    const bool apart = ctx->saved_data["apart"].toBool();
+    // (a call without a residual has no second gradient: what stands there is a payload's, and undefined)
+    const Tensor dy = grads[0], dh = grads.size() % 2 == 0 ? grads[1] : Tensor();
+    const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
+    const bool need_r = ctx->saved_data["added"].toBool() && ctx->needs_input_grad(2);      // (a tensor that is not there has no place)
+    Tensor gx, gr, gw;
+    if (!dy.defined()) {                                 // only the sum was used
+      if (need_x && dh.defined()) gx = dh.to((at::ScalarType)ctx->saved_data["type"].toInt());
+      if (need_r) gr = dh;
+      if (need_w) gw = at::zeros_like(w);
+    } else {
+      std::tie(gx, gr, gw) = norm_backward(dy.contiguous(), h, w, r, dh.defined() ? dh.contiguous() : dh,
+                                           need_x || (need_r && !apart), need_r && apart, need_w, Tensor());
+      if (need_r && !apart) gr = gx;
+      if (!need_x) gx = Tensor();
+    }
+    return once_only(grads, {gx, gw, gr, Tensor(), Tensor()});
+  }
+};
+
+// ---------------------------------------------------------------- products of bf16 rows grouped by expert
+struct Words {                                           // see failure_words in ops.py
+  int64_t status, host;
+};
+
+Tensor grouped_rows(const Tensor& x, const Tensor& w, const Tensor& efo, const Tensor& counts, bool transposed, Words at) {
+  same_gpu("grouped_rows", x, {&w, &efo, &counts});
+  const c10::cuda::CUDAGuard guard(x.device());
+  const int64_t rows = x.size(0), K = x.size(1), E = w.size(0), N = w.size(transposed ? 2 : 1);
+  Tensor y = at::empty({rows, N}, x.options().requires_grad(false));
+  check(smoe_grouped_rows(x.data_ptr(), distance(x), w.data_ptr(), transposed, (const int32_t*)ptr(efo), (const int32_t*)ptr(counts),
+                          y.data_ptr(), rows, N, K, E, (int32_t*)at.status, (int32_t*)at.host, stream()),
+        "grouped_rows");
+  return y;
+}
+
+// -> bf16 [E,N,K], or an undefined tensor where it was added to main_grad
+Tensor grouped_wgrad(const Tensor& dy, const Tensor& x, const Tensor& efo, const Tensor& counts, int64_t E, const Tensor& main_grad,
+                     Words at) {
+  same_gpu("grouped_wgrad", dy, {&x, &efo, &counts, &main_grad});
+  const c10::cuda::CUDAGuard guard(dy.device());
+  const int64_t rows = dy.size(0), N = dy.size(1), K = x.size(1);
+  const auto o = dy.options().requires_grad(false);
+  const bool add = main_grad.defined();
+  // (what is added leaves in pieces that start on 16 bytes)
+  const bool direct = add && (uintptr_t)main_grad.data_ptr() % 16 == 0;
+  Tensor dw = direct ? main_grad : add ? at::zeros({E, N, K}, o.dtype(at::kFloat)) : at::empty({E, N, K}, o);
+  check(smoe_grouped_wgrad(dy.data_ptr(), distance(dy), x.data_ptr(), distance(x), (const int32_t*)ptr(efo), (const int32_t*)ptr(counts),
+                           dw.data_ptr(), N, K, rows, E, !add, add, (int32_t*)at.status, (int32_t*)at.host, stream()),
+        "grouped_wgrad");
+  if (!add) return dw;
+  if (!direct) Tensor(main_grad).add_(dw.view(main_grad.sizes()));
+  return Tensor();
+}
+
+// as the copy engine can read them: rows a multiple of 16 bytes apart and from a 16-byte boundary on
+bool rows_lie(const Tensor& t) {
+  return t.stride(1) == 1 && (uintptr_t)t.data_ptr() % 16 == 0 &&
+         (t.size(0) <= 1 || (t.stride(0) >= t.size(1) && t.stride(0) % 8 == 0));
+}
+Tensor dense(const Tensor& t) {
+  const Tensor d = t.contiguous();
+  return (uintptr_t)d.data_ptr() % 16 == 0 ? d : d.clone();
+}
+
+struct GroupedNode : torch::autograd::Function<GroupedNode> {
+  // x [rows,K] as rows_lie, w [E,N,K] or [N,K]
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Maybe& efo, const Maybe& counts, int64_t status,
+                               int64_t host) {
+    const Tensor wd = dense(w);
+    const Tensor w3 = wd.dim() == 3 ? wd : wd.unsqueeze(0);
+    const Tensor e = of(efo), c = of(counts);
+    Tensor y = grouped_rows(x, w3, e, c, false, {status, host});
+    // (the weight itself where it is read as it lies: autograd then sees a change in place between the passes)
+    ctx->save_for_backward({ctx->needs_input_grad(1) ? x : Tensor(), ctx->needs_input_grad(0) ? (wd.data_ptr() == w.data_ptr() ? w : wd) : Tensor(),
+                            e, c});
+    ctx->saved_data["shape"] = w3.sizes().vec();
+    ctx->saved_data["dims"] = w.dim();
+    ctx->saved_data["status"] = status;
+    ctx->saved_data["host"] = host;
+    return {y};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const auto shape = ctx->saved_data["shape"].toIntVector();
+    const Words at{ctx->saved_data["status"].toInt(), ctx->saved_data["host"].toInt()};
+    const Tensor dy = rows_lie(grads[0]) ? grads[0] : dense(grads[0]);
+    Tensor dx, dw;
+    if (ctx->needs_input_grad(0) && saved[1].defined()) dx = grouped_rows(dy, saved[1].view(shape), saved[2], saved[3], true, at);
+    if (ctx->needs_input_grad(1) && saved[0].defined()) {
+      dw = grouped_wgrad(dy, saved[0], saved[2], saved[3], shape[0], Tensor(), at);
+      if (ctx->saved_data["dims"].toInt() == 2) dw = dw.squeeze(0);
+    }
+    return once_only(grads, {dx, dw, Tensor(), Tensor(), Tensor(), Tensor()});
+  }
+};
+
+// ---------------------------------------------------------------- the norm of the gradients
+// Gradient tensors of parameters (main_grad before grad; those with neither left out), tensors as they are
+std::vector<Tensor> gradients(const py::handle items, const char* what) {
+  static PyObject* const parameter = py::object(py::module_::import("torch.nn").attr("Parameter")).release().ptr();
+  std::vector<Tensor> out;
+  auto take = [&](PyObject* o) {
+    if (Py_TYPE(o) != (PyTypeObject*)THPVariableClass && PyObject_IsInstance(o, parameter) == 1) {
+      py::object g = py::getattr(o, "main_grad", py::none());
+      if (g.is_none()) {
+        const Tensor& own = THPVariable_Unpack(o).grad();
+        if (own.defined()) out.push_back(own);
+        return;
+      }
+      TORCH_CHECK_TYPE(THPVariable_Check(g.ptr()), what, ": main_grad is no tensor");
+      out.push_back(THPVariable_Unpack(g.ptr()));
+      return;
+    }
+    TORCH_CHECK_TYPE(THPVariable_Check(o), what, ": gradients are tensors or parameters, got ", Py_TYPE(o)->tp_name);
+    out.push_back(THPVariable_Unpack(o));
+  };
+  if (THPVariable_Check(items.ptr())) take(items.ptr());
+  else
+    for (const py::handle h : py::iter(items)) take(h.ptr());
+  TORCH_CHECK_VALUE(!out.empty(), what, ": no gradients");
+  return out;
+}
+
+bool taken(at::ScalarType t) { return t == at::kFloat || t == at::kBFloat16; }
+
+// One GPU, f32 or bf16; whatever does not lie densely is copied, and the copies kept
+std::vector<smoe_gradient> table(std::vector<Tensor>& grads, const std::vector<Tensor>* outs, const char* what) {
+  const auto device = grads[0].device();
+  std::vector<smoe_gradient> t(grads.size());
+  for (size_t i = 0; i < grads.size(); ++i) {
+    const Tensor& o = outs ? (*outs)[i] : grads[i];
+    TORCH_CHECK_VALUE(taken(grads[i].scalar_type()) && taken(o.scalar_type()), what, ": gradients are f32 or bf16, got ",
+                      at::toString(grads[i].scalar_type()), outs ? " into another type or that" : "");
+    TORCH_CHECK(grads[i].device() == device && o.device() == device, what, ": tensors on different devices (", device.str(), ", ",
+                grads[i].device().str(), " and ", o.device().str(), ")");
+    if (!grads[i].is_contiguous()) grads[i] = grads[i].contiguous();
+    void* const at = grads[i].data_ptr();
+    t[i] = {at, outs ? o.data_ptr() : at, grads[i].numel(), f32(grads[i]), f32(o)};
+  }
+  return t;
+}
+
+void on_gpu(const Tensor& t) { TORCH_CHECK(t.is_cuda(), "sonicmoe kernels need CUDA tensors (no CPU fallback)"); }
+Tensor gradient_workspace(const Tensor& like, size_t n) {
+  return at::empty({smoe_gradient_workspace((int64_t)n)}, at::TensorOptions().device(like.device()).dtype(at::kByte));
+}
+Tensor gradient_scalar(const Tensor& like) { return at::empty({}, at::TensorOptions().device(like.device()).dtype(at::kFloat)); }
+
+Tensor gradient_norm(const py::object& items) {
+  auto grads = gradients(items, "gradient_norm");
+  const auto t = table(grads, nullptr, "gradient_norm");
+  on_gpu(grads[0]);
+  const c10::cuda::CUDAGuard guard(grads[0].device());
+  Tensor n = gradient_scalar(grads[0]), ws = gradient_workspace(grads[0], t.size());
+  check(smoe_gradient_norm(t.data(), (int64_t)t.size(), (float*)n.data_ptr(), ws.data_ptr(), stream()), "gradient_norm");
+  return n;
+}
+
+// starts of what holds values, each once
+void once(const std::vector<smoe_gradient>& t, const char* which) {
+  std::vector<const void*> at;
+  at.reserve(t.size());
+  for (const auto& g : t)
+    if (g.numel) at.push_back(g.out);
+  std::sort(at.begin(), at.end());
+  TORCH_CHECK_VALUE(std::adjacent_find(at.begin(), at.end()) == at.end(), "clip_gradients: one of the ", which, " is given twice");
+}
+
+void written(const std::vector<Tensor>& ts) {            // autograd sees that they are others now
+  for (const Tensor& t : ts)
+    if (!t.is_inference()) torch::autograd::impl::bump_version(t);
+}
+
+Tensor clip_gradients(const py::object& items, double max_norm, const Maybe& given, const py::object& out) {
+  TORCH_CHECK_VALUE(max_norm >= 0, "clip_gradients: max_norm=", std::to_string(max_norm));
+  auto grads = gradients(items, "clip_gradients");
+  const Tensor norm = of(given);
+  TORCH_CHECK_VALUE(!norm.defined() || (norm.numel() == 1 && f32(norm) && norm.device() == grads[0].device()),
+                    "clip_gradients: the norm is one f32 on ", grads[0].device().str());
+  const std::vector<Tensor> before = grads;
+  std::vector<Tensor> outs;
+  if (!out.is_none()) {
+    for (const py::handle h : py::iter(out)) {
+      TORCH_CHECK_TYPE(THPVariable_Check(h.ptr()), "clip_gradients: outputs are tensors");
+      outs.push_back(THPVariable_Unpack(h.ptr()));
+    }
+    TORCH_CHECK_VALUE(outs.size() == grads.size(), "clip_gradients: ", std::to_string(outs.size()), " outputs for ",
+                      std::to_string(grads.size()), " gradients");
+    for (size_t i = 0; i < outs.size(); ++i)
+      TORCH_CHECK_VALUE(outs[i].sizes() == grads[i].sizes() && outs[i].is_contiguous(),
+                        "clip_gradients: outputs are contiguous and of their gradients' shapes, got ", text(outs[i].sizes()), " for ",
+                        text(grads[i].sizes()));
+  }
+  const auto t = table(grads, out.is_none() ? nullptr : &outs, "clip_gradients");
+  once(t, out.is_none() ? "gradients" : "outputs");
+  if (!out.is_none()) {
+    std::vector<std::pair<const void*, size_t>> at;
+    at.reserve(t.size());
+    for (size_t i = 0; i < t.size(); ++i)
+      if (t[i].numel) at.emplace_back(t[i].grad, i);
+    std::sort(at.begin(), at.end());
+    for (size_t i = 0; i < t.size(); ++i) {
+      if (!t[i].numel) continue;
+      for (auto g = std::lower_bound(at.begin(), at.end(), std::make_pair((const void*)t[i].out, (size_t)0));
+           g != at.end() && g->first == t[i].out; ++g)
+        TORCH_CHECK_VALUE(g->second == i && t[i].grad_f32 == t[i].out_f32, "clip_gradients: an output lies where another gradient does");
+    }
+  }
+  on_gpu(grads[0]);
+  const c10::cuda::CUDAGuard guard(grads[0].device());
+  Tensor n = norm, ws;
+  if (!norm.defined()) {
+    n = gradient_scalar(grads[0]);
+    ws = gradient_workspace(grads[0], t.size());
+  }
+  check(smoe_gradient_clip(t.data(), (int64_t)t.size(), max_norm, (const float*)ptr(norm), norm.defined() ? nullptr : (float*)n.data_ptr(),
+                           ptr(ws), stream()),
+        "clip_gradients");
+  if (out.is_none()) {
+    for (size_t i = 0; i < grads.size(); ++i)
+      if (!grads[i].is_same(before[i])) before[i].detach().copy_(grads[i]);
+    written(before);
+  } else {
+    written(outs);
+  }
+  return n;
+}
+
+}  // namespace
+
+PYBIND11_MODULE(_host, m) {
+  m.def("rms_norm", [](const Tensor& x, const Tensor& w, const Maybe& residual, double eps, int kind, bool with_y, bool keep) {
+    const Norm n = norm(x, w, of(residual), eps, kind, with_y, keep);
+    auto some = [](const Tensor& t) { return t.defined() ? Maybe(t) : Maybe(); };
+    return std::make_tuple(some(n.y), some(n.h), some(n.q), some(n.s), some(n.r));
+  });
+  m.def("rms_norm_bwd", [](const Tensor& dy, const Tensor& h, const Tensor& w, const Tensor& r, const Maybe& dh, bool want_x, bool want_res,
+                           bool want_w, const Maybe& main_grad) {
+    const auto [gx, gr, gw] = norm_backward(dy, h, w, r, of(dh), want_x, want_res, want_w, of(main_grad));
+    auto some = [](const Tensor& t) { return t.defined() ? Maybe(t) : Maybe(); };
+    return std::make_tuple(some(gx), some(gr), some(gw));
+  });
+  m.def("rms_norm_grad", [](const Tensor& x, const Tensor& w, const Maybe& residual, double eps, int64_t kind) {
+    return NormNode::apply(x, w, residual, eps, kind);
+  });
+  m.def("grouped_rows", [](const Tensor& x, const Tensor& w, const Maybe& efo, const Maybe& counts, bool transposed, int64_t status,
+                           int64_t host) { return grouped_rows(x, w, of(efo), of(counts), transposed, {status, host}); });
+  m.def("grouped_wgrad", [](const Tensor& dy, const Tensor& x, const Maybe& efo, const Maybe& counts, int64_t E, const Maybe& main_grad,
+                            int64_t status, int64_t host) {
+    const Tensor dw = grouped_wgrad(dy, x, of(efo), of(counts), E, of(main_grad), {status, host});
+    return dw.defined() ? Maybe(dw) : Maybe();
+  });
+  m.def("grouped_linear_grad", [](const Tensor& x, const Tensor& w, const Maybe& efo, const Maybe& counts, int64_t status, int64_t host) {
+    return GroupedNode::apply(x, w, efo, counts, status, host)[0];
+  });
+  m.def("gradient_norm", &gradient_norm);
+  m.def("clip_gradients", &clip_gradients);
+}

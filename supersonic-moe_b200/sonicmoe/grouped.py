@@ -6,8 +6,8 @@ from __future__ import annotations
 import torch
 from torch.autograd.function import once_differentiable
 
-from . import ops
-from .functional import _after_accumulate, _grad_target
+from . import _host, ops
+from .functional import _after_accumulate, _base_of, _grad_target
 
 
 def _rows16(t: torch.Tensor) -> torch.Tensor:
@@ -24,7 +24,8 @@ def _weight16(w: torch.Tensor) -> torch.Tensor:
 
 
 class _GroupedLinear(torch.autograd.Function):
-    """x [rows,K], weight bf16 [E,N,K] or [N,K]."""
+    """x [rows,K], weight bf16 [E,N,K] or [N,K] that accumulates into its `main_grad`.  (Others have their node in
+    csrc/host_torch.cpp.)"""
 
     @staticmethod
     def forward(ctx, x, weight, efo, counts):
@@ -77,11 +78,14 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, efo: torch.Tensor | No
         raise ValueError(f"{what}: x has {x.shape[-1]} columns, the weight {K}")
     if efo is not None and x.ndim != 2:
         raise ValueError(f"{what}: x is [rows,K] where efo is given")
-    ops._check_grouped(efo, counts, E, N, K, what)
+    ops.check_grouped(efo, counts, E, N, K, what)
     ops.poll_status(x.device)                 # a device-side failure of an earlier call surfaces here, without a sync
     rows = _rows16(x if x.ndim == 2 else x.reshape(-1, K))
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
-        y = _GroupedLinear.apply(rows, weight, efo, counts)
+        if ops._recorder is not None or (weight.requires_grad and getattr(_base_of(weight), "main_grad", None) is not None):
+            y = _GroupedLinear.apply(rows, weight, efo, counts)
+        else:
+            y = _host.grouped_linear_grad(rows, weight, efo, counts, *ops.failure_words(rows.device))
     else:
         w = _weight16(weight)
         y = ops.grouped_rows(rows, w if w.ndim == 3 else w[None], efo, counts)

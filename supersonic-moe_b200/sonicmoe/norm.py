@@ -9,10 +9,9 @@ from typing import NamedTuple
 import torch
 from torch.autograd.function import once_differentiable
 
-from . import ops
-from .functional import _after_accumulate, _grad_target
+from . import _host, ops
+from .functional import _after_accumulate, _base_of, _grad_target
 
-_E4M3 = torch.float8_e4m3fn
 _TYPES = (torch.bfloat16, torch.float32)
 
 
@@ -32,7 +31,8 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 
 
 class _RmsNorm(torch.autograd.Function):
-    """x, residual [rows,H] (residual or None), weight [H] -> y, h, payload, scales, each None where there is none."""
+    """x, residual [rows,H] (residual or None), weight [H] -> y, h, payload, scales, each None where there is none: for a weight that
+    accumulates into its `main_grad`.  (Others have their node in csrc/host_torch.cpp.)"""
 
     @staticmethod
     def forward(ctx, x, weight, residual, eps, scales):
@@ -83,6 +83,15 @@ def _needs_grad(*ts):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
 
 
+def _differentiable(rows, w, res, eps, scales):
+    """y, h, payload, scales."""
+    if ops._recorder is not None or (w.requires_grad and getattr(_base_of(w), "main_grad", None) is not None):
+        return _RmsNorm.apply(rows, w, res, eps, scales)
+    out = _host.rms_norm_grad(rows, w, res, eps, ops.NORM_SCALES[scales])
+    h = out[1] if res is not None else None
+    return (out[0], h, out[-2], out[-1]) if scales else (out[0], h, None, None)
+
+
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, *, eps: float = 1e-6):
     """y = h / sqrt(mean(h^2) + eps) * weight over the last dimension, h = x, or x + residual; returns y, with a residual (y, h).
 
@@ -95,7 +104,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | Non
     w = _checked(x, weight, residual, eps, "rms_norm", _TYPES)
     rows, res = _rows(x), None if residual is None else _rows(residual)
     if _needs_grad(x, weight, residual):
-        y, h = _RmsNorm.apply(rows, w, res, eps, None)[:2]
+        y, h = _differentiable(rows, w, res, eps, None)[:2]
     else:
         y, h = ops.rms_norm(rows, w, res, eps)[:2]
     y = y if x.ndim == 2 else y.view(x.shape)
@@ -124,10 +133,9 @@ def rms_norm_quantized(x: torch.Tensor, weight: torch.Tensor, residual: torch.Te
     if _needs_grad(x, weight, residual):
         if not with_output:
             raise ValueError("rms_norm_quantized: no gradient flows through the payload; with_output=True gives the rows it flows through")
-        y, h, q, s = _RmsNorm.apply(rows, w, res, eps, scales)
+        y, h, q, s = _differentiable(rows, w, res, eps, scales)
     else:
         y, h, q, s, _ = ops.rms_norm(rows, w, res, eps, scales, with_output)
-    q = q.view(_E4M3)
     if x.ndim != 2:
         lead = x.shape[:-1]
         q, s = q.unflatten(0, lead) if lead else q[0], s.unflatten(0, lead) if lead else s[0]

@@ -6,11 +6,11 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
-from array import array
 
 import torch
 
-from ._lib import check, lib
+from ._lib import check, lib  # (loads the library that _host calls)
+from . import _host
 
 _U8 = torch.uint8
 _I32 = torch.int32
@@ -1145,143 +1145,44 @@ def block128_experts(x, idx, scores, w1, w1_s, w2, w2_s, E, I):
 
 
 # ---------------------------------------------------------------- products of bf16 rows grouped by expert
-def _check_grouped(efo, counts, E, N, K, what):
+def check_grouped(efo, counts, E, N, K, what):
     check_segments(efo, counts, E, what)
     if N <= 0 or K <= 0 or N % 8 or K % 8 or not 1 <= E <= 256:
         raise ValueError(f"{what}: {E} experts of {N} x {K}: sizes are multiples of 8, 1 to 256 experts")
 
 
-def _ld(t):
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-
-@_op
+@_timed
 def grouped_rows(x, w, efo=None, counts=None, transposed=False):
     """x bf16 [rows,K] (rows any multiple of 8 values apart, from a 16-byte boundary on), w bf16 [E,N,K], or `transposed` [E,K,N] -> bf16
     [rows,N], zero where a row is not live."""
-    _check_same_gpu("grouped_rows", x, w, efo, counts)
-    rows, K = x.shape
-    E, N = w.shape[0], w.shape[2 if transposed else 1]
-    y = x.new_empty((rows, N))
-    check(lib.smoe_grouped_rows(x.data_ptr(), _ld(x), w.data_ptr(), transposed, _p(efo), _p(counts), y.data_ptr(), rows, N, K, E,
-                                *failure_words(x.device), _stream()), "grouped_rows")
-    return y
+    return _host.grouped_rows(x, w, efo, counts, transposed, *failure_words(x.device))
 
 
-@_op
+@_timed
 def grouped_wgrad(dy, x, efo, counts, E, main_grad=None):
     """dy bf16 [rows,N], x bf16 [rows,K] (as above) -> bf16 [E,N,K], or None where it is added to `main_grad` f32."""
-    _check_same_gpu("grouped_wgrad", dy, x, efo, counts, main_grad)
-    (rows, N), K = dy.shape, x.shape[1]
-    if main_grad is None:
-        dw = dy.new_empty((E, N, K))
-    elif main_grad.data_ptr() % 16 == 0:
-        dw = main_grad
-    else:                                        # what is added leaves in pieces that start on 16 bytes
-        dw = dy.new_zeros((E, N, K), dtype=_F32)
-    check(lib.smoe_grouped_wgrad(dy.data_ptr(), _ld(dy), x.data_ptr(), _ld(x), _p(efo), _p(counts), dw.data_ptr(), N, K, rows, E,
-                                 main_grad is None, main_grad is not None, *failure_words(dy.device), _stream()), "grouped_wgrad")
-    if main_grad is None:
-        return dw
-    if dw is not main_grad:
-        main_grad.add_(dw.view(main_grad.shape))
-    return None
+    return _host.grouped_wgrad(dy, x, efo, counts, E, main_grad, *failure_words(dy.device))
 
 
 # ---------------------------------------------------------------- the norm in front of the experts
 NORM_SCALES = {None: 0, "mx": 1, "block128": 2}
 NORM_MAX_H = 16384
-_F32 = torch.float32
 
 
-@_op
+@_timed
 def rms_norm(x, w, residual=None, eps=1e-6, scales=None, with_y=True, keep=False):
     """x bf16 / f32 [T,H] (rows any distance apart), w bf16 / f32 [H], residual of x's type or f32 [T,H] -> (y or None, h or None, payload
     or None, scales or None, reciprocal norms f64 [T] with `keep`, else None); see `sonicmoe.rms_norm_quantized`."""
-    _check_same_gpu("rms_norm", x, w, residual)
-    T, H = x.shape
-    kind = NORM_SCALES[scales]
-    x32, w32 = x.dtype is _F32, w.dtype is _F32
-    y = x.new_empty((T, H)) if with_y or not kind else None
-    h = residual.new_empty((T, H)) if residual is not None else None
-    r = x.new_empty(T, dtype=torch.float64) if keep else None
-    q = s = None
-    if kind == 1:
-        q, s = x.new_empty((T, H), dtype=_U8), x.new_empty((T, H // 32), dtype=_U8)
-    elif kind == 2:
-        q, s = _payload(x, T, H), x.new_empty((T, _blocks128(H)), dtype=_F32)
-    check(lib.smoe_rms_norm(x.data_ptr(), x32, x.stride(0) if T > 1 else H, _p(residual),
-                            residual is not None and residual.dtype is _F32, residual.stride(0) if residual is not None and T > 1 else H,
-                            w.data_ptr(), w32, T, H, eps, _p(y), _p(h), _p(r), kind, _p(q), _p(s), _stream()), "rms_norm")
-    return y, h, q, s, r
+    return _host.rms_norm(x, w, residual, eps, NORM_SCALES[scales], with_y, keep)
 
 
-@_op
+@_timed
 def rms_norm_bwd(dy, h, w, rstd, dh=None, dx=True, dres=False, dw=True, main_grad=None):
     """Gradients of `rms_norm`: dy of x's type [T,H], h [T,H] (rows any distance apart), dh of h's type or None -> (dx of x's type, dres of h's
     type where that is another, dw of w's type); each None where it is not wanted, dw where it is added to `main_grad` f32."""
-    _check_same_gpu("rms_norm", dy, h, w, rstd, dh, main_grad)
-    T, H = dy.shape
-    gx = torch.empty_like(dy) if dx else None
-    gr = h.new_empty((T, H)) if dres else None
-    gw = (main_grad if main_grad is not None else torch.empty_like(w)) if dw else None
-    ws = dy.new_empty(lib.smoe_rms_norm_bwd_workspace(T, H), dtype=_U8) if dw else None
-    check(lib.smoe_rms_norm_bwd(dy.data_ptr(), dy.dtype is _F32, h.data_ptr(), h.dtype is _F32, h.stride(0) if T > 1 else H, w.data_ptr(),
-                                w.dtype is _F32, rstd.data_ptr(), _p(dh), T, H, _p(gx), _p(gr), _p(gw),
-                                gw is not None and gw.dtype is _F32, main_grad is not None, _p(ws), _stream()), "rms_norm_bwd")
-    return gx, gr, None if main_grad is not None else gw
+    return _host.rms_norm_bwd(dy, h, w, rstd, dh, dx, dres, dw, main_grad)
 
 
 # ---------------------------------------------------------------- the norm of the gradients
-def _gradient_list(grads, outs, what):
-    """The table of smoe_gradient that the C side reads; everything on one GPU, contiguous, f32 or bf16."""
-    dev = grads[0].get_device()
-    if dev < 0:
-        raise RuntimeError("sonicmoe kernels need CUDA tensors (no CPU fallback)")
-    table, bf16 = [], torch.bfloat16
-    for g, o in zip(grads, grads if outs is None else outs):
-        t, u = g.dtype, o.dtype
-        if (t is not _F32 and t is not bf16) or (u is not _F32 and u is not bf16):
-            raise ValueError(f"{what}: gradients are f32 or bf16, got {t}" + ("" if outs is None else f" into {u}"))
-        if g.get_device() != dev or o.get_device() != dev:
-            raise RuntimeError(f"{what}: tensors on different devices ({grads[0].device}, {g.device} and {o.device})")
-        table += (g.data_ptr(), o.data_ptr(), g.numel(), (t is _F32) | (u is _F32) << 32)
-    return array("q", table)
-
-
-def _on(device, fn, *a):
-    if device == _current():
-        return fn(*a)
-    with torch.cuda.device(device):
-        return fn(*a)
-
-
-@_timed
-def gradient_norm(grads):
-    """Contiguous f32 or bf16 tensors -> f32 []: the root of the sum of their squares."""
-    table = _gradient_list(grads, None, "gradient_norm")
-
-    def run():
-        norm, ws = _norm_and_workspace(grads)
-        check(lib.smoe_gradient_norm(table.buffer_info()[0], len(grads), norm.data_ptr(), ws.data_ptr(), _stream()), "gradient_norm")
-        return norm
-    return _on(grads[0].get_device(), run)
-
-
-def _norm_and_workspace(grads):
-    d = grads[0].device
-    return torch.empty((), dtype=_F32, device=d), torch.empty(lib.smoe_gradient_workspace(len(grads)), dtype=_U8, device=d)
-
-
-@_timed
-def gradient_clip(grads, max_norm, norm=None, outs=None):
-    """Contiguous f32 or bf16 tensors times min(1, max_norm / (their norm + 1e-6)), in place or to `outs`; `norm` f32 []: instead of theirs.
-    Returns the norm."""
-    table = _gradient_list(grads, outs, "gradient_clip")
-
-    def run():
-        n, ws = (norm, None) if norm is not None else _norm_and_workspace(grads)
-        check(lib.smoe_gradient_clip(table.buffer_info()[0], len(grads), max_norm, _p(norm), None if norm is not None else n.data_ptr(),
-                                     _p(ws), _stream()), "gradient_clip")
-        return n
-    return _on(grads[0].get_device(), run)
+gradient_norm = _timed(_host.gradient_norm)
+gradient_clip = _timed(_host.clip_gradients)

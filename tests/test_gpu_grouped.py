@@ -219,6 +219,16 @@ def test_a_weight_changed_between_the_passes_is_noticed(sonicmoe):
         y.backward(torch.ones_like(y))
 
 
+def test_gradients_are_not_differentiated_again(sonicmoe):
+    for main_grad in (False, True):
+        x, w, dy = (t.requires_grad_(True) for t in (randn(40, 72), randn(80, 72), randn(40, 80)))
+        if main_grad:
+            w.main_grad = torch.zeros(80, 72, device=DEV)
+        dx, = torch.autograd.grad(sonicmoe.grouped_linear(x, w), x, dy, create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiate"):
+            dx.sum().backward()
+
+
 def test_the_hook_of_a_parameter_with_main_grad(sonicmoe):
     p = torch.nn.Parameter(randn(2, 72, 136))
     p.main_grad = torch.zeros(2, 72, 136, device=DEV)

@@ -193,6 +193,17 @@ def test_gradients_one_at_a_time_and_of_the_sum_alone(sonicmoe):
     assert torch.equal(gx.cpu(), dh.to(BF)) and torch.equal(gr.cpu(), dh) and not gw.any()
 
 
+def test_gradients_are_not_differentiated_again(sonicmoe):
+    x, w, _, dy, _ = make(5, 136, F32, None, F32, seed=5)
+    for main_grad in (False, True):
+        gx, gw, gdy = (t.requires_grad_(True) for t in on(x, w, dy))
+        if main_grad:
+            gw.main_grad = torch.zeros(136, device=DEV)
+        dx, = torch.autograd.grad(sonicmoe.rms_norm(gx, gw), gx, gdy, create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiate"):
+            dx.sum().backward()
+
+
 def test_gradients_against_differences(sonicmoe):
     x, w, _, dy, _ = make(4, 96, F32, None, F32, seed=6)
     x = x / x.norm(dim=1, keepdim=True) * 10
