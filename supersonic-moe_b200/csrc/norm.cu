@@ -19,153 +19,180 @@ namespace smoe {
 constexpr int kNormMaxH = 16384;
 constexpr int kNormMaxWarps = 16;
 
+// ---- pairs of f32 in one instruction (round to nearest, as the scalar forms)
+struct P2 {
+  uint64_t v;
+};
+__device__ __forceinline__ P2 p2(float x, float y) {
+  P2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 p2_get(P2 a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
+  return r;
+}
+__device__ __forceinline__ P2 operator*(P2 a, P2 b) {
+  P2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ P2 operator+(P2 a, P2 b) {
+  P2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ P2 p2_fma(P2 a, P2 b, P2 c) {
+  P2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+
 template <bool F32>
 struct NormVec;                          // eight values of a row
 template <>
 struct NormVec<false> {
-  uint4 v;
+  uint32_t w[4];
   __device__ __forceinline__ void load(const void* base, int64_t at) {
-    v = *reinterpret_cast<const uint4*>((const uint16_t*)base + at);
+    const uint4 v = *reinterpret_cast<const uint4*>((const uint16_t*)base + at);
+    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
   }
-  __device__ __forceinline__ void load_some(const void* base, int64_t at, int n) {
+  // value i from at + i * step, the first n of them
+  __device__ __forceinline__ void load_some(const void* base, int64_t at, int n, int step) {
     const uint16_t* p = (const uint16_t*)base + at;
-    uint32_t w[8];
+    uint32_t u[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = i < n ? p[i] : 0u;
-    v = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
+    for (int i = 0; i < 8; ++i) u[i] = i < n ? p[i * step] : 0u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = u[2 * i] | u[2 * i + 1] << 16;
   }
-  __device__ __forceinline__ void get(float (&f)[8]) const { bf16x8_to_f32(v, f); }
-  __device__ __forceinline__ void set(const float (&f)[8]) {
-    v = make_uint4(q_bf16x2(f[0], f[1]), q_bf16x2(f[2], f[3]), q_bf16x2(f[4], f[5]), q_bf16x2(f[6], f[7]));
+  __device__ __forceinline__ P2 pair(int i) const { return p2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u)); }
+  __device__ __forceinline__ void set(int i, P2 v) {
+    const float2 f = p2_get(v);
+    w[i] = q_bf16x2(f.x, f.y);
   }
-  __device__ __forceinline__ void clear() { v = make_uint4(0, 0, 0, 0); }
-  __device__ __forceinline__ void store(void* base, int64_t at) const { *reinterpret_cast<uint4*>((uint16_t*)base + at) = v; }
-  __device__ __forceinline__ void store_some(void* base, int64_t at, int n) const {
+  __device__ __forceinline__ void clear() { w[0] = w[1] = w[2] = w[3] = 0u; }
+  // what follows from the values is made anew, here and not ahead of a loop
+  __device__ __forceinline__ void anew() { asm volatile("" : "+r"(w[0]), "+r"(w[1]), "+r"(w[2]), "+r"(w[3])); }
+  __device__ __forceinline__ void store(void* base, int64_t at) const {
+    *reinterpret_cast<uint4*>((uint16_t*)base + at) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  __device__ __forceinline__ void store_some(void* base, int64_t at, int n, int step) const {
     uint16_t* p = (uint16_t*)base + at;
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (i < n) p[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+      if (i < n) p[i * step] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
   }
 };
 template <>
 struct NormVec<true> {
-  float4 a, b;
+  float f[8];
   __device__ __forceinline__ void load(const void* base, int64_t at) {
     const float4* p = reinterpret_cast<const float4*>((const float*)base + at);
-    a = p[0];
-    b = p[1];
-  }
-  __device__ __forceinline__ void load_some(const void* base, int64_t at, int n) {
-    const float* p = (const float*)base + at;
-    float f[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = i < n ? p[i] : 0.f;
-    set(f);
-  }
-  __device__ __forceinline__ void get(float (&f)[8]) const {
+    const float4 a = p[0], b = p[1];
     f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
     f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
   }
-  __device__ __forceinline__ void set(const float (&f)[8]) {
-    a = make_float4(f[0], f[1], f[2], f[3]);
-    b = make_float4(f[4], f[5], f[6], f[7]);
+  __device__ __forceinline__ void load_some(const void* base, int64_t at, int n, int step) {
+    const float* p = (const float*)base + at;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = i < n ? p[i * step] : 0.f;
   }
-  __device__ __forceinline__ void clear() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
+  __device__ __forceinline__ P2 pair(int i) const { return p2(f[2 * i], f[2 * i + 1]); }
+  __device__ __forceinline__ void set(int i, P2 v) {
+    const float2 x = p2_get(v);
+    f[2 * i] = x.x;
+    f[2 * i + 1] = x.y;
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = 0.f;
+  }
+  __device__ __forceinline__ void anew() {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) asm volatile("" : "+f"(f[i]));
+  }
   __device__ __forceinline__ void store(void* base, int64_t at) const {
     float4* p = reinterpret_cast<float4*>((float*)base + at);
-    p[0] = a;
-    p[1] = b;
+    p[0] = make_float4(f[0], f[1], f[2], f[3]);
+    p[1] = make_float4(f[4], f[5], f[6], f[7]);
   }
-  __device__ __forceinline__ void store_some(void* base, int64_t at, int n) const {
-    float f[8];
-    get(f);
+  __device__ __forceinline__ void store_some(void* base, int64_t at, int n, int step) const {
     float* p = (float*)base + at;
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (i < n) p[i] = f[i];
+      if (i < n) p[i * step] = f[i];
   }
 };
 
-// A thread's pieces of a row: piece c is eight columns from (c * threads + t) * 8 on, t the thread among the row's.  `vec`: rows and
-// columns allow 16 bytes at a time (then H % 8 == 0 and a piece is there or not).
-template <bool F32, int NC>
-__device__ __forceinline__ void norm_load(NormVec<F32> (&v)[NC], const void* base, int64_t row_at, int t, int threads, int H, bool vec) {
-  if (vec) {
+// A row's columns among the `threads` threads of it, of which this one is t.  H a multiple of 8: piece c of a thread is eight columns
+// from (c * threads + t) * 8 on, with VEC by 16 bytes of every tensor.  Else its values are `threads` columns apart, so that the loads
+// of a warp lie side by side (eight neighbours a thread: T=1003, H=1001 in f32, forward and backward 30 us instead of 14).  Kernels of
+// their own: what the loads one by one keep in registers over a row leaves too few for the others.
+template <bool VEC>
+struct NormRow {
+  int t, threads, H;
+  bool apart;
+  __device__ __forceinline__ int col(int c) const { return !VEC && apart ? c * 8 * threads + t : (c * threads + t) * 8; }
+  __device__ __forceinline__ int step() const { return !VEC && apart ? threads : 1; }
+  __device__ __forceinline__ int left(int col) const {      // values of a piece that exist
+    return apart ? (H - col + threads - 1) / threads : H - col;
+  }
+  template <bool F32, int NC>
+  __device__ __forceinline__ void load(NormVec<F32> (&v)[NC], const void* base, int64_t row_at) const {
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      const int col = (c * threads + t) * 8;
-      v[c].clear();
-      if (col < H) v[c].load(base, row_at + col);
-    }
-  } else {
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      const int col = (c * threads + t) * 8;
-      v[c].load_some(base, row_at + col, H - col);
+      const int at = col(c);
+      if (VEC) {
+        v[c].clear();
+        if (at < H) v[c].load(base, row_at + at);
+      } else {
+        v[c].load_some(base, row_at + at, left(at), step());
+      }
     }
   }
-}
-template <bool F32, int NC>
-__device__ __forceinline__ void norm_store(const NormVec<F32> (&v)[NC], void* base, int64_t row_at, int t, int threads, int H,
-                                           bool vec) {
-#pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    const int col = (c * threads + t) * 8;
-    if (vec) {
-      if (col < H) v[c].store(base, row_at + col);
+  template <bool F32>
+  __device__ __forceinline__ void store(const NormVec<F32>& v, void* base, int64_t row_at, int c) const {
+    const int at = col(c);
+    if (VEC) {
+      if (at < H) v.store(base, row_at + at);
     } else {
-      v[c].store_some(base, row_at + col, H - col);
+      v.store_some(base, row_at + at, left(at), step());
     }
-  }
-}
-// the weight, of either type
-template <int NC>
-struct NormWeight {
-  NormVec<true> v[NC];                   // bf16: the first half of a piece's registers
-  __device__ __forceinline__ void load(const void* w, bool f32, int t, int threads, int H, bool vec) {
-    if (f32) {
-      norm_load<true, NC>(v, w, 0, t, threads, H, vec);
-    } else {
-      NormVec<false> b[NC];
-      norm_load<false, NC>(b, w, 0, t, threads, H, vec);
-#pragma unroll
-      for (int c = 0; c < NC; ++c)
-        v[c].a = make_float4(__uint_as_float(b[c].v.x), __uint_as_float(b[c].v.y), __uint_as_float(b[c].v.z),
-                             __uint_as_float(b[c].v.w));
-    }
-  }
-  __device__ __forceinline__ void get(int c, bool f32, float (&f)[8]) const {
-    if (f32) v[c].get(f);
-    else bf16x8_to_f32(make_uint4(__float_as_uint(v[c].a.x), __float_as_uint(v[c].a.y), __float_as_uint(v[c].a.z),
-                                  __float_as_uint(v[c].a.w)), f);
   }
 };
 
-// over the warps of a row (one row a block if there are several), in one order
+// over the warps of a row, in one order; `group` of the block's rows it is, each with sums and a barrier of its own
 template <typename T>
-__device__ __forceinline__ T norm_sum(T s, int warps, T* shared) {
+__device__ __forceinline__ T norm_sum(T s, int warps, int group, T* shared) {
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
   if (warps == 1) return s;
   if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = s;
-  __syncthreads();
-  s = shared[0];
-  for (int i = 1; i < warps; ++i) s += shared[i];
+  asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(warps * 32) : "memory");
+  shared += group * warps;
+  s = shared[0] + shared[1];                            // (a power of two)
+  for (int i = 2; i < warps; i += 2) s += shared[i] + shared[i + 1];
   return s;
 }
 
-// 1 / sqrt(v): the f32 approximation and one step of Newton's method, which leaves some 2^-44
+// 1 / sqrt(v): the f32 approximation and one step of Newton's method, which leaves some 2^-43; v is brought into the range of f32
 __device__ __forceinline__ double norm_rsqrt(double v) {
-  if (v > 1e-30 && v < 1e30) {
-    const double r = rsqrtf((float)v);
-    return r * (1.5 - 0.5 * v * r * r);
-  }
-  return 1.0 / sqrt(v);
+  const double scale = v < 1e-30 ? 0x1p200 : v > 1e30 ? 0x1p-200 : 1.0, back = v < 1e-30 ? 0x1p100 : v > 1e30 ? 0x1p-100 : 1.0;
+  v *= scale;
+  const float r = rsqrtf((float)v);
+  if (!(r > 0.f && r < __int_as_float(0x7f800000))) return r;      // of 0, infinity, NaN
+  return (double)r * (1.5 - 0.5 * v * r * r) * back;
 }
 
-// h r w in f32 is off by three roundings, each up to one unit of the last place
+// h r w in f32 is off by three roundings (r, two products), each up to one unit of the last place
 constexpr uint32_t kNormNear = 4;
+__device__ __forceinline__ uint32_t norm_min_u16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("min.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
 // f32 that rounds to the bf16 nearest to d: a tie of f32 that is none of f64 is moved off
 __device__ __forceinline__ float norm_for_bf16(double d) {
   float f = (float)d;
@@ -181,7 +208,7 @@ struct NormArgs {
   const void *x, *res, *w;
   int64_t ldx, ldr, T;
   int H, warps, rows;                    // warps of a row, rows of a block
-  int w_f32, vec_x, vec_r, vec_w, vec_y, vec_h;
+  int w_f32, vec, apart;                 // vec: see NormRow
   double eps, inv_H;
   void *y, *h;                           // null: not written
   double* rstd;
@@ -192,123 +219,146 @@ struct NormArgs {
 
 enum NormQuant : int { NORM_PLAIN = 0, NORM_MX = 1, NORM_BLOCK128 = 2 };
 
-// RES: 0 none, 1 of x's type, 2 f32 (beside bf16)
-template <bool XF32, int RES, int QUANT, int NC>
-__global__ void __launch_bounds__(32 * kNormMaxWarps) rms_norm_kernel(const NormArgs a) {
+// RES: 0 none, 1 of x's type, 2 f32 (beside bf16).  A block stays and takes rows in turn, several at a time, each by threads of its own;
+// a row's loads leave before the one ahead of it is added up.
+template <bool XF32, int RES, int QUANT, int NC, bool WF32, bool VEC>
+__global__ void __launch_bounds__(NC == 2 ? 256 : 512, NC == 2 ? 3 : 1) rms_norm_kernel(const NormArgs a) {
   constexpr bool HF32 = XF32 || RES == 2;
-  __shared__ double sums[kNormMaxWarps];
+  constexpr bool AHEAD = VEC && !HF32;                  // (rows in f32 would need more registers)
+  __shared__ double sums[2][kNormMaxWarps];
   const int lane = threadIdx.x & 31;
-  const int threads = a.warps * 32, t = a.warps == 1 ? lane : (int)threadIdx.x;
-  const int64_t row = a.warps == 1 ? (int64_t)blockIdx.x * a.rows + (threadIdx.x >> 5) : (int64_t)blockIdx.x;
-  if (row >= a.T) return;                               // a whole warp, and only where rows are of one warp
+  const int group = threadIdx.x / (a.warps * 32);
+  const NormRow<VEC> at{(int)threadIdx.x - group * a.warps * 32, a.warps * 32, a.H, QUANT == NORM_PLAIN && a.apart};
+  const int64_t stride = (int64_t)gridDim.x * a.rows;
+  int64_t row = (int64_t)blockIdx.x * a.rows + group;
+  if (row >= a.T) return;                               // all threads of the row
+  NormVec<XF32> x[NC];
+  NormVec<HF32> res[RES ? NC : 1];
+  auto ask = [&](int64_t of) {
+    if (of >= a.T) return;
+    at.load(x, a.x, of * a.ldx);
+    if constexpr (RES != 0) at.load(res, a.res, of * a.ldr);
+  };
+  if (AHEAD) ask(row);
+  NormVec<WF32> w[NC];
+  at.load(w, a.w, 0);
+  int turn = 0;
+  for (; row < a.T; row += stride) {
+  if (!AHEAD) ask(row);
   NormVec<HF32> h[NC];
-  if constexpr (RES == 0) {
-    norm_load<HF32, NC>(h, a.x, row * a.ldx, t, threads, a.H, a.vec_x);
-  } else {
-    NormVec<XF32> x[NC];
-    norm_load<XF32, NC>(x, a.x, row * a.ldx, t, threads, a.H, a.vec_x);
-    norm_load<HF32, NC>(h, a.res, row * a.ldr, t, threads, a.H, a.vec_r);
 #pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      float p[8], r[8];
-      x[c].get(p);
-      h[c].get(r);
+  for (int c = 0; c < NC; ++c) {
+    if constexpr (RES == 0) {
+      h[c] = x[c];
+    } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) r[i] += p[i];
-      h[c].set(r);
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (!HF32) asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(h[c].w[i]) : "r"(x[c].w[i]), "r"(res[c].w[i]));
+        else h[c].set(i, x[c].pair(i) + res[c].pair(i));
+      }
     }
   }
-  NormWeight<NC> w;
-  w.load(a.w, a.w_f32, t, threads, a.H, a.vec_w);
-  if constexpr (RES != 0) norm_store<HF32, NC>(h, a.h, row * a.H, t, threads, a.H, a.vec_h);
+  if (AHEAD) ask(row + stride);
+  if constexpr (RES != 0) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) at.store(h[c], a.h, row * a.H, c);
+  }
   double s0 = 0.0, s1 = 0.0;
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
-    float f[8];
-    h[c].get(f);
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-      const double p = f[i], q = f[i + 1];
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = p2_get(h[c].pair(i));
+      const double p = f.x, q = f.y;
       s0 = fma(p, p, s0);
       s1 = fma(q, q, s1);
     }
   }
-  const double r64 = norm_rsqrt(norm_sum<double>(s0 + s1, a.warps, sums) * a.inv_H + a.eps);
+  const double r64 = norm_rsqrt(norm_sum<double>(s0 + s1, a.warps, group, sums[turn]) * a.inv_H + a.eps);
+  turn ^= 1;                                            // the next row's sums do not wait for this one's readers
   const float r = (float)r64;
-  if (a.rstd && t == 0) a.rstd[row] = r64;
+  if (a.rstd && at.t == 0) a.rstd[row] = r64;
   const bool far = !(r64 > 1e-30 && r64 < 1e30);        // r in f32 would not have its full precision
+  const P2 r2 = p2(r, r);
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
-    const int col = (c * threads + t) * 8;
-    float f[8], g[8], v[8];
-    h[c].get(f);
-    w.get(c, a.w_f32, g);
+    const int col = at.col(c);
+    P2 v[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = f[i] * r * g[i];
+    for (int i = 0; i < 4; ++i) v[i] = h[c].pair(i) * r2 * w[c].pair(i);
     if constexpr (XF32) {
-      if (far) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = (float)((double)f[i] * r64 * (double)g[i]);
-      }
       NormVec<true> y;
-      y.set(v);
-      if (a.vec_y) {
-        if (col < a.H) y.store(a.y, row * a.H + col);
-      } else {
-        y.store_some(a.y, row * a.H + col, a.H - col);
-      }
-    } else {
-      uint32_t near = 0xFFFFFFFFu;                      // least distances above a border less kNormNear, of the even and the odd values
 #pragma unroll
-      for (int i = 0; i < 8; i += 2)
-        near = __viaddmin_u16x2(__byte_perm(__float_as_uint(v[i]), __float_as_uint(v[i + 1]), 0x5410),
-                                (0x8000u + kNormNear) * 0x10001u, near);
-      if ((near & 0xFFFFu) <= 2 * kNormNear || (near >> 16) <= 2 * kNormNear || far) {
+      for (int i = 0; i < 4; ++i) y.set(i, v[i]);
+      if (far) {
+        NormVec<HF32> hc = h[c];
+        NormVec<WF32> wc = w[c];
+        hc.anew();
+        wc.anew();
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = norm_for_bf16((double)f[i] * r64 * (double)g[i]);
-      }
-      NormVec<false> y;
-      y.set(v);
-      if (QUANT == NORM_PLAIN || a.y) {
-        if (a.vec_y) {
-          if (col < a.H) y.store(a.y, row * a.H + col);
-        } else {
-          y.store_some(a.y, row * a.H + col, a.H - col);
+        for (int i = 0; i < 8; ++i) {
+          const float2 f = p2_get(hc.pair(i >> 1)), g = p2_get(wc.pair(i >> 1));
+          y.f[i] = (float)((double)(i & 1 ? f.y : f.x) * r64 * (double)(i & 1 ? g.y : g.x));
         }
       }
+      at.store(y, a.y, row * a.H, c);
+    } else {
+      // least distances above a border less kNormNear, of the even and the odd values (a carry makes an odd one's one more)
+      uint32_t near = 0xFFFFFFFFu;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = p2_get(v[i]);
+        near = norm_min_u16x2(near, __byte_perm(__float_as_uint(f.x), __float_as_uint(f.y), 0x5410) + (0x8000u + kNormNear) * 0x10001u);
+      }
+      if ((near & 0xFFFFu) <= 2 * kNormNear || near < (2 * kNormNear + 2) << 16 || far) {
+        // (anew: what is f64 of these values here would otherwise be kept from the sum of squares, and the weights' over all rows)
+        NormVec<HF32> hc = h[c];
+        NormVec<WF32> wc = w[c];
+        hc.anew();
+        wc.anew();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 f = p2_get(hc.pair(i)), g = p2_get(wc.pair(i));
+          v[i] = p2(norm_for_bf16((double)f.x * r64 * (double)g.x), norm_for_bf16((double)f.y * r64 * (double)g.y));
+        }
+      }
+      NormVec<false> y;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y.set(i, v[i]);
+      if (QUANT == NORM_PLAIN || a.y) at.store(y, a.y, row * a.H, c);
       if constexpr (QUANT == NORM_MX) {                 // four lanes a group
-        uint32_t m = q_max_bf16x2(q_max_bf16x2(q_abs_bf16x2(y.v.x), q_abs_bf16x2(y.v.y)),
-                                  q_max_bf16x2(q_abs_bf16x2(y.v.z), q_abs_bf16x2(y.v.w)));
-        m = q_max_bf16x2(m, __shfl_xor_sync(0xffffffffu, m, 1));
-        m = q_max_bf16x2(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        uint32_t m = q_max_abs_bf16x2(q_max_abs_bf16x2(y.w[0], y.w[1]), q_max_abs_bf16x2(y.w[2], y.w[3]));
+        m = q_max_abs_bf16x2(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = q_max_abs_bf16x2(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        m &= 0x7FFF7FFFu;
         const int e = q_e8m0_of(fmaxf(fmaxf(0.f, __uint_as_float(m << 16)), __uint_as_float(m & 0xFFFF0000u)));
-        const float qs = q_scale_of(e);
-        float b[8];
-        y.get(b);
+        const uint32_t qs = (__float_as_uint(q_scale_of(e)) >> 16) * 0x10001u;      // a power of two is a bf16
         if (col < a.H) {
           *reinterpret_cast<uint2*>(a.q + row * a.pitch + col) =
-              make_uint2(q_pack4(b[0] * qs, b[1] * qs, b[2] * qs, b[3] * qs), q_pack4(b[4] * qs, b[5] * qs, b[6] * qs, b[7] * qs));
+              make_uint2(q_pack4_scaled(y.w[0], y.w[1], qs, qs), q_pack4_scaled(y.w[2], y.w[3], qs, qs));
           if ((lane & 3) == 0) ((uint8_t*)a.s)[row * (a.H >> 5) + (col >> 5)] = (uint8_t)e;
         }
       }
       if constexpr (QUANT == NORM_BLOCK128) {           // sixteen
-        uint32_t m = q_max_bf16x2(q_max_bf16x2(q_abs_bf16x2(y.v.x), q_abs_bf16x2(y.v.y)),
-                                  q_max_bf16x2(q_abs_bf16x2(y.v.z), q_abs_bf16x2(y.v.w)));
+        uint32_t m = q_max_abs_bf16x2(q_max_abs_bf16x2(y.w[0], y.w[1]), q_max_abs_bf16x2(y.w[2], y.w[3]));
 #pragma unroll
-        for (int d = 1; d < 16; d <<= 1) m = q_max_bf16x2(m, __shfl_xor_sync(0xffffffffu, m, d));
+        for (int d = 1; d < 16; d <<= 1) m = q_max_abs_bf16x2(m, __shfl_xor_sync(0xffffffffu, m, d));
+        m &= 0x7FFF7FFFu;
         const float amax = fmaxf(fmaxf(__uint_as_float(m << 16), __uint_as_float(m & 0xFFFF0000u)), kAmaxFloor);
         // one division a lane, of either kind
-        const float quotient = (lane & 1) ? kE4m3Max / amax : amax / kE4m3Max;
+        const float quotient = ((lane & 1) ? kE4m3Max : amax) / ((lane & 1) ? amax : kE4m3Max);
         const float qs = __shfl_sync(0xffffffffu, quotient, lane | 1);
-        float b[8];
-        y.get(b);
+        float2 b[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) b[i] = p2_get(y.pair(i) * p2(qs, qs));
         if (col < a.H) {
           *reinterpret_cast<uint2*>(a.q + row * a.pitch + col) =
-              make_uint2(q_pack4(b[0] * qs, b[1] * qs, b[2] * qs, b[3] * qs), q_pack4(b[4] * qs, b[5] * qs, b[6] * qs, b[7] * qs));
+              make_uint2(q_pack4(b[0].x, b[0].y, b[1].x, b[1].y), q_pack4(b[2].x, b[2].y, b[3].x, b[3].y));
           if ((lane & 15) == 0) ((float*)a.s)[row * ((a.H + 127) >> 7) + (col >> 7)] = quotient;
         }
       }
     }
+  }
   }
 }
 
@@ -318,147 +368,158 @@ struct NormBwdArgs {
   const double* rstd;
   int64_t ldh, T;
   int H, warps, rows;
-  int w_f32, vec_dy, vec_h, vec_w, vec_dh, vec_dx, vec_dres;
+  int w_f32, vec, apart;
   void *dx, *dres;                       // null: not wanted
   float* part;                           // [blocks * flushes, H], null: no gradient of the weight
   int flushes;
 };
 
-// Rows that a block adds up in one f32 sum of a column; the sums of sums are f64
+// Rows that a thread adds up in one f32 sum of a column; the sums of sums are f64
 constexpr int kNormRun = 256;
 
-// dx of x's type, dres of h's (where the two types differ; else dx serves both)
-template <bool XF32, bool HF32, int NC>
-__global__ void __launch_bounds__(32 * kNormMaxWarps) rms_norm_bwd_kernel(const NormBwdArgs a) {
-  extern __shared__ float columns[];                    // [rows, H] where a block has several rows at a time
+// dx of x's type, dres of h's (where the two types differ; else dx serves both).  A block stays and takes rows in turn, several at a
+// time, each by threads of its own, which keep their columns' part of dw in registers.
+template <bool XF32, bool HF32, int NC, bool WF32, bool VEC>
+__global__ void __launch_bounds__(32 * kNormMaxWarps, 1) rms_norm_bwd_kernel(const NormBwdArgs a) {
+  extern __shared__ float columns[];                    // [rows, H]
   __shared__ float sums[2][kNormMaxWarps];
-  const int lane = threadIdx.x & 31;
-  const int threads = a.warps * 32, t = a.warps == 1 ? lane : (int)threadIdx.x;
-  const int group = a.warps == 1 ? threadIdx.x >> 5 : 0;
-  const int64_t step = (int64_t)gridDim.x * a.rows;
-  NormWeight<NC> w;
-  w.load(a.w, a.w_f32, t, threads, a.H, a.vec_w);
-  float dw[NC][8];
+  const int group = threadIdx.x / (a.warps * 32);
+  const NormRow<VEC> at{(int)threadIdx.x - group * a.warps * 32, a.warps * 32, a.H, a.apart != 0};
+  const int64_t stride = (int64_t)gridDim.x * a.rows;
+  NormVec<WF32> w[NC];
+  at.load(w, a.w, 0);
+  P2 dw[NC][4];
 #pragma unroll
   for (int c = 0; c < NC; ++c)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) dw[c][i] = 0.f;
+    for (int i = 0; i < 4; ++i) dw[c][i] = p2(0.f, 0.f);
   const float inv_H = 1.f / a.H;
   int turn = 0;
   int64_t row = (int64_t)blockIdx.x * a.rows + group;
+  // A row's loads leave before the one ahead of it is added up, which by then is held as h r and g.  (Four pieces a thread: neither, for
+  // want of registers.)
+  constexpr bool AHEAD = NC == 2;
+  NormVec<XF32> dy[NC];
+  NormVec<HF32> h[NC], dh[NC], next_dh[AHEAD ? NC : 1];
+  double next_r = 1.0;
+  auto ask = [&](int64_t of) {
+    if (of >= a.T) return;
+    at.load(dy, a.dy, of * a.H);
+    at.load(h, a.h, of * a.ldh);
+    if constexpr (AHEAD) {
+      if (a.dh) at.load(next_dh, a.dh, of * a.H);
+    } else {
+      if (a.dh) at.load(dh, a.dh, of * a.H);
+    }
+    next_r = a.rstd[of];
+  };
+  if (AHEAD) ask(row);
   for (int flush = 0; flush < a.flushes; ++flush) {
-    for (int n = 0; n < kNormRun && row < a.T; ++n, row += step) {
-      NormVec<XF32> dy[NC];
-      NormVec<HF32> h[NC], dh[NC];
-      norm_load<XF32, NC>(dy, a.dy, row * a.H, t, threads, a.H, a.vec_dy);
-      norm_load<HF32, NC>(h, a.h, row * a.ldh, t, threads, a.H, a.vec_h);
-      if (a.dh) norm_load<HF32, NC>(dh, a.dh, row * a.H, t, threads, a.H, a.vec_dh);
+    for (int n = 0; n < kNormRun && row < a.T; ++n, row += stride) {
+      if (!AHEAD) ask(row);
       // r as a product of two f32, the first a power of two, so that rows of very large or very small values keep their precision
-      const double r64 = a.rstd[row];
+      const double r64 = next_r;
       const float pre = r64 < 1e-30 ? 0x1p-64f : r64 > 1e30 ? 0x1p64f : 1.f;
       const float r = (float)(r64 / pre);
-      float s = 0.f;
+      const P2 pre2 = p2(pre, pre), r2 = p2(r, r);
+      P2 s2 = p2(0.f, 0.f), hr[AHEAD ? NC : 1][4], g[AHEAD ? NC : 1][4];
 #pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        float fy[8], fh[8], fw[8];
-        dy[c].get(fy);
-        h[c].get(fh);
-        w.get(c, a.w_f32, fw);
+      for (int c = 0; c < NC; ++c)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float hr = fh[i] * pre * r;
-          s = fmaf(fy[i] * fw[i], hr, s);
-          dw[c][i] = fmaf(fy[i], hr, dw[c][i]);
+        for (int i = 0; i < 4; ++i) {
+          const P2 d = dy[c].pair(i), u = h[c].pair(i) * pre2 * r2, v = d * w[c].pair(i);
+          s2 = p2_fma(v, u, s2);
+          dw[c][i] = p2_fma(d, u, dw[c][i]);
+          if constexpr (AHEAD) {
+            hr[c][i] = u;
+            g[c][i] = v;
+          }
         }
+      if constexpr (AHEAD) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c) dh[c] = next_dh[c];
+        ask(row + stride);
       }
-      s = norm_sum<float>(s, a.warps, sums[turn]) * inv_H;
+      const float2 both = p2_get(s2);
+      const float s = norm_sum<float>(both.x + both.y, a.warps, group, sums[turn]) * -inv_H;
       turn ^= 1;                                        // the next row's sums do not wait for this one's readers
+      const P2 minus = p2(s, s);
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
-        const int col = (c * threads + t) * 8;
-        float fy[8], fh[8], fw[8], d[8];
-        dy[c].get(fy);
-        h[c].get(fh);
-        w.get(c, a.w_f32, fw);
+        P2 d[4];
+        if constexpr (!AHEAD) {
+          dy[c].anew();
+          h[c].anew();
+        }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) d[i] = fmaf(-(fh[i] * pre * r), s, fy[i] * fw[i]) * r * pre;
-        if (a.dh) {
-          float e[8];
-          dh[c].get(e);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) d[i] += e[i];
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (AHEAD) d[i] = p2_fma(hr[c][i], minus, g[c][i]);
+          else d[i] = p2_fma(h[c].pair(i) * pre2 * r2, minus, dy[c].pair(i) * w[c].pair(i));
+          d[i] = d[i] * r2 * pre2;
+          if (a.dh) d[i] = d[i] + dh[c].pair(i);
         }
         if (a.dx) {
           NormVec<XF32> o;
-          o.set(d);
-          if (a.vec_dx) {
-            if (col < a.H) o.store(a.dx, row * a.H + col);
-          } else {
-            o.store_some(a.dx, row * a.H + col, a.H - col);
-          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o.set(i, d[i]);
+          at.store(o, a.dx, row * a.H, c);
         }
         if constexpr (XF32 != HF32) {
           if (a.dres) {
             NormVec<HF32> o;
-            o.set(d);
-            if (a.vec_dres) {
-              if (col < a.H) o.store(a.dres, row * a.H + col);
-            } else {
-              o.store_some(a.dres, row * a.H + col, a.H - col);
-            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o.set(i, d[i]);
+            at.store(o, a.dres, row * a.H, c);
           }
         }
       }
     }
     if (!a.part) continue;
     float* part = a.part + ((int64_t)blockIdx.x * a.flushes + flush) * a.H;
+    float* mine = a.rows > 1 ? columns + group * a.H : part;
+    if (a.rows > 1) __syncthreads();                    // the flush before has been read
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int col = at.col(c) + i * at.step();
+        const float2 v = p2_get(dw[c][i >> 1]);
+        if (col < a.H) mine[col] = i & 1 ? v.y : v.x;
+      }
     if (a.rows > 1) {                                   // the block's rows first
-      __syncthreads();
-#pragma unroll
-      for (int c = 0; c < NC; ++c)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int col = (c * threads + t) * 8 + i;
-          if (col < a.H) columns[group * a.H + col] = dw[c][i];
-        }
       __syncthreads();
       for (int col = threadIdx.x; col < a.H; col += blockDim.x) {
         float v = columns[col];
-        for (int g = 1; g < a.rows; ++g) v += columns[g * a.H + col];
+        for (int k = 1; k < a.rows; ++k) v += columns[k * a.H + col];
         part[col] = v;
       }
-    } else {
-#pragma unroll
-      for (int c = 0; c < NC; ++c)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int col = (c * threads + t) * 8 + i;
-          if (col < a.H) part[col] = dw[c][i];
-        }
     }
 #pragma unroll
     for (int c = 0; c < NC; ++c)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) dw[c][i] = 0.f;
+      for (int i = 0; i < 4; ++i) dw[c][i] = p2(0.f, 0.f);
   }
 }
 
 // dw[col] (+)= the sum of its column, 32 columns a block
-__global__ void __launch_bounds__(256) rms_norm_dw_kernel(const float* __restrict__ part, int64_t n, int H, void* dw, int f32,
-                                                          int accumulate) {
-  __shared__ double sums[8][32];
+constexpr int kNormSumWarps = 32;
+__global__ void __launch_bounds__(32 * kNormSumWarps) rms_norm_dw_kernel(const float* __restrict__ part, int64_t n, int H, void* dw,
+                                                                         int f32, int accumulate) {
+  __shared__ double sums[kNormSumWarps][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int col = blockIdx.x * 32 + lane;
+  int col = blockIdx.x * 32 + lane;
   double s = 0.0;
   if (col < H) {
 #pragma unroll 8
-    for (int64_t i = warp; i < n; i += 8) s += part[i * H + col];
+    for (int64_t i = warp; i < n; i += kNormSumWarps) s += part[i * H + col];
   }
   sums[warp][lane] = s;
   __syncthreads();
-  if (warp || col >= H) return;
+  col = blockIdx.x * 32 + warp;                         // a warp a column
+  s = sums[lane][warp];
 #pragma unroll
-  for (int i = 1; i < 8; ++i) s += sums[i][lane];
+  for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+  if (lane || col >= H) return;
   if (f32) {
     float* p = (float*)dw + col;
     *p = accumulate ? (float)(*p + s) : (float)s;
@@ -468,27 +529,43 @@ __global__ void __launch_bounds__(256) rms_norm_dw_kernel(const float* __restric
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------
+// Warps of a row of `nc` pieces a thread, and rows a block has at a time
 struct NormShape {
-  int warps, rows, nc;
-  explicit NormShape(int H) {
-    nc = H > kNormMaxWarps * 512 ? 4 : 2;
+  int warps, rows;
+  NormShape(int H, int nc, int block_warps) {
     warps = 1;
     while (warps * 32 * 8 * nc < H) warps *= 2;
-    rows = warps == 1 ? 8 : 1;
+    rows = warps < block_warps ? block_warps / warps : 1;
   }
   int threads() const { return 32 * warps * rows; }
 };
+static int norm_pieces(int H) { return H > 4096 ? 4 : 2; }
+static NormShape norm_forward_shape(int H) { return NormShape(H, norm_pieces(H), 8); }
+static int norm_bwd_pieces(int H) { return H > kNormMaxWarps * 512 ? 4 : 2; }
+static NormShape norm_bwd_shape(int H) { return NormShape(H, norm_bwd_pieces(H), kNormMaxWarps); }
 
+// rows of it can be read by 16 bytes (null: there are none)
 static bool norm_vec(const void* p, bool f32, int64_t ld, int64_t H) {
+  if (!p) return H % 8 == 0;
   return ((uintptr_t)p & 15) == 0 && H % 8 == 0 && ld % (f32 ? 4 : 8) == 0;
 }
 
+template <bool XF32, int RES, int QUANT, int NC>
+static cudaError_t norm_launch_pieces(const NormArgs& a, const NormShape& sh, cudaStream_t stream) {
+  const int64_t all = (a.T + sh.rows - 1) / sh.rows, most = (int64_t)sm_count() * (NC == 2 ? 3 : 512 / sh.threads());
+  const unsigned blocks = (unsigned)(all < most ? all : most);
+  if (a.vec) {
+    if (a.w_f32) rms_norm_kernel<XF32, RES, QUANT, NC, true, true><<<blocks, sh.threads(), 0, stream>>>(a);
+    else rms_norm_kernel<XF32, RES, QUANT, NC, false, true><<<blocks, sh.threads(), 0, stream>>>(a);
+  } else {
+    if (a.w_f32) rms_norm_kernel<XF32, RES, QUANT, NC, true, false><<<blocks, sh.threads(), 0, stream>>>(a);
+    else rms_norm_kernel<XF32, RES, QUANT, NC, false, false><<<blocks, sh.threads(), 0, stream>>>(a);
+  }
+  return cudaGetLastError();
+}
 template <bool XF32, int RES, int QUANT>
 static cudaError_t norm_launch(const NormArgs& a, const NormShape& sh, cudaStream_t stream) {
-  const unsigned blocks = (unsigned)((a.T + sh.rows - 1) / sh.rows);
-  if (sh.nc == 2) rms_norm_kernel<XF32, RES, QUANT, 2><<<blocks, sh.threads(), 0, stream>>>(a);
-  else rms_norm_kernel<XF32, RES, QUANT, 4><<<blocks, sh.threads(), 0, stream>>>(a);
-  return cudaGetLastError();
+  return norm_pieces(a.H) == 2 ? norm_launch_pieces<XF32, RES, QUANT, 2>(a, sh, stream) : norm_launch_pieces<XF32, RES, QUANT, 4>(a, sh, stream);
 }
 template <int RES>
 static cudaError_t norm_launch_bf16(const NormArgs& a, const NormShape& sh, int quant, cudaStream_t stream) {
@@ -499,13 +576,24 @@ static cudaError_t norm_launch_bf16(const NormArgs& a, const NormShape& sh, int 
 
 template <bool XF32, bool HF32, int NC>
 static int norm_bwd_launch(const NormBwdArgs& a, const NormShape& sh, int blocks, cudaStream_t stream) {
-  const size_t smem = sh.rows > 1 && a.part ? (size_t)sh.rows * a.H * 4 : 0;       // at most 8 x 512 x 4 bytes
-  rms_norm_bwd_kernel<XF32, HF32, NC><<<blocks, sh.threads(), smem, stream>>>(a);
+  const size_t smem = sh.rows > 1 && a.part ? (size_t)sh.rows * a.H * 4 : 0;       // at most 16 x 512 x 4 bytes
+  if (a.vec) {
+    if (a.w_f32) rms_norm_bwd_kernel<XF32, HF32, NC, true, true><<<blocks, sh.threads(), smem, stream>>>(a);
+    else rms_norm_bwd_kernel<XF32, HF32, NC, false, true><<<blocks, sh.threads(), smem, stream>>>(a);
+  } else {
+    if (a.w_f32) rms_norm_bwd_kernel<XF32, HF32, NC, true, false><<<blocks, sh.threads(), smem, stream>>>(a);
+    else rms_norm_bwd_kernel<XF32, HF32, NC, false, false><<<blocks, sh.threads(), smem, stream>>>(a);
+  }
   return cudaGetLastError() == cudaSuccess ? SMOE_OK : SMOE_ERR_LAUNCH;
+}
+template <bool XF32, bool HF32>
+static int norm_bwd_launch_any(const NormBwdArgs& a, const NormShape& sh, int blocks, cudaStream_t stream) {
+  return norm_bwd_pieces(a.H) == 2 ? norm_bwd_launch<XF32, HF32, 2>(a, sh, blocks, stream)
+                                   : norm_bwd_launch<XF32, HF32, 4>(a, sh, blocks, stream);
 }
 
 static int norm_bwd_blocks(int64_t T, const NormShape& sh) {
-  const int64_t most = (int64_t)sm_count() * (1024 / sh.threads()), all = (T + sh.rows - 1) / sh.rows;
+  const int64_t most = sm_count(), all = (T + sh.rows - 1) / sh.rows;
   return (int)(all < most ? all : most);
 }
 static int norm_flushes(int64_t T, const NormShape& sh, int blocks) {
@@ -529,16 +617,13 @@ int smoe_rms_norm(const void* x, int x_f32, int64_t ldx, const void* residual, i
   if (T == 0) return SMOE_OK;
   if (!x || !w || (residual && !h) || (scale_kind ? !q || !scales : !y)) return SMOE_ERR_ARG;
   if (scale_kind && (uintptr_t)q & 15) return SMOE_ERR_ALIGN;
-  const NormShape sh((int)H);
+  const NormShape sh = norm_forward_shape((int)H);
   NormArgs a{};
   a.x = x; a.res = residual; a.w = w; a.ldx = ldx; a.ldr = ldr; a.T = T; a.H = (int)H;
-  a.warps = sh.warps; a.rows = sh.rows; a.w_f32 = w_f32 != 0; a.eps = eps; a.inv_H = 1.0 / (double)H;
+  a.warps = sh.warps; a.rows = sh.rows; a.w_f32 = w_f32 != 0; a.apart = H % 8 != 0; a.eps = eps; a.inv_H = 1.0 / (double)H;
   const bool h_f32 = x_f32 || (residual && residual_f32);
-  a.vec_x = norm_vec(x, x_f32, ldx, H);
-  a.vec_r = norm_vec(residual, h_f32, ldr, H);
-  a.vec_w = norm_vec(w, w_f32, H, H);
-  a.vec_y = norm_vec(y, x_f32, H, H);
-  a.vec_h = norm_vec(h, h_f32, H, H);
+  a.vec = norm_vec(x, x_f32, ldx, H) && norm_vec(residual, h_f32, ldr, H) && norm_vec(w, w_f32, H, H) && norm_vec(y, x_f32, H, H) &&
+          norm_vec(h, h_f32, H, H);
   a.y = y; a.h = h; a.rstd = rstd; a.q = (uint8_t*)q; a.s = scales; a.pitch = (H + 15) / 16 * 16;
   const cudaStream_t st = (cudaStream_t)stream;
   cudaError_t rc;
@@ -551,7 +636,7 @@ int smoe_rms_norm(const void* x, int x_f32, int64_t ldx, const void* residual, i
 int64_t smoe_rms_norm_bwd_workspace(int64_t T, int64_t H) {
   if (!norm_sizes(T, H)) return -1;
   if (T == 0) return 0;
-  const NormShape sh((int)H);
+  const NormShape sh = norm_bwd_shape((int)H);
   const int blocks = norm_bwd_blocks(T, sh);
   return (int64_t)blocks * norm_flushes(T, sh, blocks) * H * 4;
 }
@@ -567,26 +652,21 @@ int smoe_rms_norm_bwd(const void* dy, int x_f32, const void* h, int h_f32, int64
     return cudaMemsetAsync(dw, 0, (size_t)H * (dw_f32 ? 4 : 2), st) == cudaSuccess ? SMOE_OK : SMOE_ERR_LAUNCH;
   }
   if (!dy || !h || !w || !rstd || (dw && !workspace)) return SMOE_ERR_ARG;
-  const NormShape sh((int)H);
+  const NormShape sh = norm_bwd_shape((int)H);
   const int blocks = norm_bwd_blocks(T, sh);
   NormBwdArgs a{};
   a.dy = dy; a.h = h; a.w = w; a.dh = dh; a.rstd = rstd; a.ldh = ldh; a.T = T; a.H = (int)H;
-  a.warps = sh.warps; a.rows = sh.rows; a.w_f32 = w_f32 != 0;
-  a.vec_dy = norm_vec(dy, x_f32, H, H);
-  a.vec_h = norm_vec(h, h_f32, ldh, H);
-  a.vec_w = norm_vec(w, w_f32, H, H);
-  a.vec_dh = norm_vec(dh, h_f32, H, H);
-  a.vec_dx = norm_vec(dx, x_f32, H, H);
-  a.vec_dres = norm_vec(dres, h_f32, H, H);
+  a.warps = sh.warps; a.rows = sh.rows; a.w_f32 = w_f32 != 0; a.apart = H % 8 != 0;
+  a.vec = norm_vec(dy, x_f32, H, H) && norm_vec(h, h_f32, ldh, H) && norm_vec(w, w_f32, H, H) && norm_vec(dh, h_f32, H, H) &&
+          norm_vec(dx, x_f32, H, H) && norm_vec(dres, h_f32, H, H);
   a.dx = dx; a.dres = dres;
   a.part = dw ? (float*)workspace : nullptr;
   a.flushes = norm_flushes(T, sh, blocks);
   int rc;
-  if (x_f32) rc = sh.nc == 2 ? norm_bwd_launch<true, true, 2>(a, sh, blocks, st) : norm_bwd_launch<true, true, 4>(a, sh, blocks, st);
-  else if (h_f32) rc = sh.nc == 2 ? norm_bwd_launch<false, true, 2>(a, sh, blocks, st) : norm_bwd_launch<false, true, 4>(a, sh, blocks, st);
-  else rc = sh.nc == 2 ? norm_bwd_launch<false, false, 2>(a, sh, blocks, st) : norm_bwd_launch<false, false, 4>(a, sh, blocks, st);
+  if (x_f32) rc = norm_bwd_launch_any<true, true>(a, sh, blocks, st);
+  else rc = h_f32 ? norm_bwd_launch_any<false, true>(a, sh, blocks, st) : norm_bwd_launch_any<false, false>(a, sh, blocks, st);
   if (rc || !dw) return rc;
-  rms_norm_dw_kernel<<<(unsigned)((H + 31) / 32), 256, 0, st>>>((const float*)workspace, (int64_t)blocks * a.flushes, (int)H, dw,
+  rms_norm_dw_kernel<<<(unsigned)((H + 31) / 32), 32 * kNormSumWarps, 0, st>>>((const float*)workspace, (int64_t)blocks * a.flushes, (int)H, dw,
                                                                dw_f32 != 0, dw_accumulate != 0);
   return cudaGetLastError() == cudaSuccess ? SMOE_OK : SMOE_ERR_LAUNCH;
 }

@@ -19,12 +19,6 @@ __device__ __forceinline__ size_t isa_offset(size_t row, size_t g, size_t k_tile
   return ((row >> 7) * k_tiles + (g >> 2)) * 512 + (row & 31) * 16 + ((row & 127) >> 5) * 4 + (g & 3);
 }
 
-// max of the magnitudes of two bf16 pairs, element by element; the sign bits are those of the product
-__device__ __forceinline__ uint32_t q_max_abs_bf16x2(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("max.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
 // q_e8m0_of of two magnitudes, as bf16 pairs: the exponent after rounding up a mantissa above 0x60, less 8, not below 0
 __device__ __forceinline__ uint32_t q_e8m0x2(uint32_t m) {
   const uint32_t e = ((m + 0x001F001Fu) >> 7) & 0x01FF01FFu;
@@ -34,22 +28,6 @@ __device__ __forceinline__ uint32_t q_e8m0x2(uint32_t m) {
 }
 // and their scales, 2^(127 - e) as bf16; e <= 247, the exponent of infinity: every maximum starts from 0 and drops NaN
 __device__ __forceinline__ uint32_t q_scalex2(uint32_t e2) { return (0x00FE00FEu - e2) << 7; }
-// A bf16 pair times a pair of powers of two, in f32: exact, one instruction a value where unpacking and multiplying take two, and
-// on another pipe than the conversions; adding -0 keeps the sign of a zero
-__device__ __forceinline__ float2 q_scaled(uint32_t w, uint32_t qs) {
-  float2 r;
-  asm("{\n\t.reg .b16 a, b, c, d;\n\t"
-      "mov.b32 {a, b}, %2;\n\tmov.b32 {c, d}, %3;\n\t"
-      "fma.rn.f32.bf16 %0, a, c, %4;\n\tfma.rn.f32.bf16 %1, b, d, %4;\n\t}"
-      : "=f"(r.x), "=f"(r.y) : "r"(w), "r"(qs), "f"(-0.0f));
-  return r;
-}
-// four bf16 values of a row, each with its scale -> four e4m3 bytes
-__device__ __forceinline__ uint32_t q_pack4_scaled(uint32_t a, uint32_t b, uint32_t qa, uint32_t qb) {
-  const float2 x = q_scaled(a, qa), y = q_scaled(b, qb);
-  return q_pack4(x.x, x.y, y.x, y.y);
-}
-
 // --------------------------------------------------------------------- rows
 // One warp per row; a lane owns 8 consecutive values, 4 lanes form a group.
 __global__ void __launch_bounds__(256)

@@ -35,7 +35,27 @@ __device__ __forceinline__ uint32_t q_max_bf16x2(uint32_t a, uint32_t b) {
   asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
-__device__ __forceinline__ uint32_t q_abs_bf16x2(uint32_t w) { return w & 0x7FFF7FFFu; }
+// max of the magnitudes of two bf16 pairs, element by element; the sign bits are those of the product
+__device__ __forceinline__ uint32_t q_max_abs_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// A bf16 pair times a pair of powers of two, in f32: exact, one instruction a value where unpacking and multiplying take two, and
+// on another pipe than the conversions; adding -0 keeps the sign of a zero
+__device__ __forceinline__ float2 q_scaled(uint32_t w, uint32_t qs) {
+  float2 r;
+  asm("{\n\t.reg .b16 a, b, c, d;\n\t"
+      "mov.b32 {a, b}, %2;\n\tmov.b32 {c, d}, %3;\n\t"
+      "fma.rn.f32.bf16 %0, a, c, %4;\n\tfma.rn.f32.bf16 %1, b, d, %4;\n\t}"
+      : "=f"(r.x), "=f"(r.y) : "r"(w), "r"(qs), "f"(-0.0f));
+  return r;
+}
+// four bf16 values of a row, each with its scale -> four e4m3 bytes
+__device__ __forceinline__ uint32_t q_pack4_scaled(uint32_t a, uint32_t b, uint32_t qa, uint32_t qb) {
+  const float2 x = q_scaled(a, qa), y = q_scaled(b, qb);
+  return q_pack4(x.x, x.y, y.x, y.y);
+}
 __device__ __forceinline__ uint32_t q_bf16x2(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
