@@ -152,7 +152,6 @@ gemm16_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
   const uint32_t bar_tfull = bar_fixed + 8 * S::STAGES, bar_tempty = bar_tfull + 8 * S::BUFS;
 
   constexpr int PRODUCER = S::EPI_WARPS, ISSUER = S::EPI_WARPS + 1, FIXER = S::EPI_WARPS + 2;
-  if (warp == 2) load_segs128<false>(segs, p.efo, p.counts, p.E, p.rows, 256, true, 0, 0, lane);
   if (threadIdx.x == 0) {
     for (int s = 0; s < S::STAGES; ++s) {
       mbar_init(bar_full + 8 * s, 1);                     // leader's: its producer arms it, both CTAs' copies credit it
@@ -172,6 +171,9 @@ gemm16_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
     tmem_alloc2(smem_u32(tmem_slot), 512);
     tmem_relinquish2();
   }
+  wait_for_kernel_before();                   // so far nothing in memory has been touched
+  next_kernel_may_start();
+  if (warp == 2) load_segs128<false>(segs, p.efo, p.counts, p.E, p.rows, 256, true, 0, 0, lane);
   tc_fence_before();
   __syncthreads();
   cluster_sync_all();

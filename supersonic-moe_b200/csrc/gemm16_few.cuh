@@ -86,7 +86,6 @@ gemm16_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
   const uint32_t bar_tfull = bar_empty + 8 * S::STAGES, bar_tempty = bar_tfull + 8 * S::ACC;
   const uint32_t bar_pfull = bar_tempty + 8 * S::ACC, bar_pempty = bar_pfull + 8;
 
-  if (warp == 2) load_segs128<false>(segs, p.efo, p.counts, p.E, p.rows, NT, true, 0, 0, lane);
   if (threadIdx.x == 0) {
     for (int s = 0; s < S::STAGES; ++s) {
       mbar_init(bar_full + 8 * s, 1);
@@ -106,6 +105,9 @@ gemm16_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
     tmem_alloc(smem_u32(tmem_slot), S::ACC * NT);
     tmem_relinquish();
   }
+  wait_for_kernel_before();                   // so far nothing in memory has been touched
+  next_kernel_may_start();
+  if (warp == 2) load_segs128<false>(segs, p.efo, p.counts, p.E, p.rows, NT, true, 0, 0, lane);
   tc_fence_before();
   __syncthreads();
   if (split > 1) cluster_sync_all();

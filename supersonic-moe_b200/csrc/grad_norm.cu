@@ -10,6 +10,7 @@
 #include <stdint.h>
 
 #include "host.h"
+#include "ptx.cuh"
 #include "quant_groups.cuh"
 #include "smoe_b200.h"
 
@@ -107,6 +108,7 @@ template <int N>
 __global__ void __launch_bounds__(kGradThreads, kGradBlocks)
 grad_squares_kernel(const __grid_constant__ GradList<N> l, double* __restrict__ partial) {
   __shared__ double sums[kGradThreads / 32];
+  next_kernel_may_start();                   // (which waits for this one's end)
   double s = 0.0;
   const int pieces = l.first[l.count];
   for (int piece = blockIdx.x; piece < pieces; piece += gridDim.x) {
@@ -151,6 +153,7 @@ __device__ __forceinline__ double grad_total(const double* __restrict__ partial,
 
 __global__ void __launch_bounds__(kGradThreads) grad_norm_kernel(const double* __restrict__ partial, int n, float* norm) {
   __shared__ double sums[kGradThreads / 32];
+  wait_for_kernel_before();
   const double s = grad_total(partial, n, sums);
   if (threadIdx.x == 0) *norm = (float)sqrt(s);
 }
@@ -161,6 +164,7 @@ __global__ void __launch_bounds__(kGradThreads, kGradBlocks)
 grad_scale_kernel(const __grid_constant__ GradList<N> l, const double* __restrict__ partial, int n_partial,
                   const float* __restrict__ given, double max_norm, float* norm) {
   __shared__ double sums[kGradThreads / 32];
+  wait_for_kernel_before();
   const double total = given ? (double)*given : sqrt(grad_total(partial, n_partial, sums));
   if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)total;
   const double ratio = max_norm / (total + 1e-6);
@@ -251,8 +255,10 @@ template <int N>
 static cudaError_t grad_launch(const GradCall& c, int64_t from, int64_t to, int blocks, bool scale, int at) {
   GradList<N> l;
   grad_fill(l, c.list, from, to, c.chunk);
-  if (scale) grad_scale_kernel<N><<<blocks, kGradThreads, 0, c.stream>>>(l, c.partial, at, c.given, c.max_norm, from == 0 ? c.norm : nullptr);
-  else grad_squares_kernel<N><<<blocks, kGradThreads, 0, c.stream>>>(l, c.partial + at);
+  if (scale)
+    return launch_early(grad_scale_kernel<N>, blocks, kGradThreads, 0, 0, c.stream, l, (const double*)c.partial, at, c.given, c.max_norm,
+                        from == 0 ? c.norm : nullptr);
+  grad_squares_kernel<N><<<blocks, kGradThreads, 0, c.stream>>>(l, c.partial + at);
   return cudaGetLastError();
 }
 // All launches of one kind; returns the partial sums there are, or -1.  `scale`: from the last tensors on, with `n` sums.
@@ -304,8 +310,8 @@ int smoe_gradient_norm(const smoe_gradient* list, int64_t count, float* norm, vo
   const GradCall c{list, count, grad_chunk(total), (double*)workspace, nullptr, 0.0, norm, (cudaStream_t)stream};
   const int n = grad_launches(c, false, 0);
   if (n < 0) return SMOE_ERR_LAUNCH;
-  grad_norm_kernel<<<1, kGradThreads, 0, c.stream>>>(c.partial, n, norm);
-  return cudaGetLastError() == cudaSuccess ? SMOE_OK : SMOE_ERR_LAUNCH;
+  return launch_early(grad_norm_kernel, 1, kGradThreads, 0, 0, c.stream, (const double*)c.partial, n, norm) == cudaSuccess ? SMOE_OK
+                                                                                                                   : SMOE_ERR_LAUNCH;
 }
 
 int smoe_gradient_clip(const smoe_gradient* list, int64_t count, double max_norm, const float* given_norm, float* norm, void* workspace,

@@ -56,8 +56,9 @@ static int launch16(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensor
   if (!ensure_smem_attr(kern, Gemm16Smem::TOTAL, attr_set)) return SMOE_ERR_LAUNCH;
   int64_t pairs = sm_count() / 2;
   if (tiles < pairs) pairs = tiles;
-  kern<<<(unsigned)(2 * pairs), Gemm16Smem::THREADS, Gemm16Smem::TOTAL, stream>>>(ta, tb, tc, p);
-  return cudaGetLastError() == cudaSuccess ? SMOE_OK : SMOE_ERR_LAUNCH;
+  return launch_early(kern, (unsigned)(2 * pairs), Gemm16Smem::THREADS, Gemm16Smem::TOTAL, 0, stream, ta, tb, tc, p) == cudaSuccess
+             ? SMOE_OK
+             : SMOE_ERR_LAUNCH;
 }
 
 static bool few_rows16(int64_t rows, int64_t E) { return rows <= Few16Smem::NT || rows <= 32 * E; }
@@ -80,19 +81,10 @@ static int few16(const void* x, int64_t ldx, const void* w, const int* efo, cons
   Few16Params p{(int)rows, (int)N, (int)K, (int)E, efo, counts, w_mn, (__nv_bfloat16*)y, split, status, host_word};
   int64_t groups = sms / split;
   if (tiles < groups) groups = tiles;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = (unsigned)split;
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(groups * split));
-  cfg.blockDim = dim3(Few16Smem::THREADS);
-  cfg.dynamicSmemBytes = Few16Smem::TOTAL;
-  cfg.stream = stream;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, gemm16_few_kernel, tw, tx16, tx64, p) != cudaSuccess) return SMOE_ERR_LAUNCH;
-  return cudaGetLastError() == cudaSuccess ? SMOE_OK : SMOE_ERR_LAUNCH;
+  return launch_early(gemm16_few_kernel, (unsigned)(groups * split), Few16Smem::THREADS, Few16Smem::TOTAL, (unsigned)split, stream, tw, tx16,
+                      tx64, p) == cudaSuccess
+             ? SMOE_OK
+             : SMOE_ERR_LAUNCH;
 }
 
 }  // namespace smoe

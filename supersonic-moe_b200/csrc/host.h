@@ -5,6 +5,7 @@
 #include <cudaTypedefs.h>
 
 #include <mutex>
+#include <utility>
 
 namespace smoe {
 
@@ -56,6 +57,28 @@ inline bool ensure_smem_attr(Kern kern, int bytes, bool (&done)[kMaxDevices]) {
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
   done[dev] = true;
   return true;
+}
+
+// A launch that may be made ready while the kernel before it in the stream ends; the kernel waits for that one's end (and so for
+// everything before it) before it touches memory.  cluster: CTAs of a cluster, 0 where the kernel names them itself or has none.
+template <typename... P, typename... A>
+inline cudaError_t launch_early(void (*kern)(P...), unsigned blocks, unsigned threads, size_t smem, unsigned cluster, cudaStream_t stream,
+                                A&&... args) {
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster ? 2 : 1;
+  const cudaError_t rc = cudaLaunchKernelEx(&cfg, kern, std::forward<A>(args)...);
+  return rc == cudaSuccess ? cudaGetLastError() : rc;
 }
 
 }  // namespace smoe

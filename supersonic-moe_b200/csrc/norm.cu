@@ -11,6 +11,7 @@
 #include <stdint.h>
 
 #include "host.h"
+#include "ptx.cuh"
 #include "quant_groups.cuh"
 #include "smoe_b200.h"
 
@@ -382,6 +383,7 @@ constexpr int kNormRun = 256;
 template <bool XF32, bool HF32, int NC, bool WF32, bool VEC>
 __global__ void __launch_bounds__(32 * kNormMaxWarps, 1) rms_norm_bwd_kernel(const NormBwdArgs a) {
   extern __shared__ float columns[];                    // [rows, H]
+  next_kernel_may_start();                              // (the sums of the blocks' sums, which waits)
   __shared__ float sums[2][kNormMaxWarps];
   const int group = threadIdx.x / (a.warps * 32);
   const NormRow<VEC> at{(int)threadIdx.x - group * a.warps * 32, a.warps * 32, a.H, a.apart != 0};
@@ -509,6 +511,7 @@ __global__ void __launch_bounds__(32 * kNormSumWarps) rms_norm_dw_kernel(const f
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int col = blockIdx.x * 32 + lane;
   double s = 0.0;
+  wait_for_kernel_before();
   if (col < H) {
 #pragma unroll 8
     for (int64_t i = warp; i < n; i += kNormSumWarps) s += part[i * H + col];
@@ -666,9 +669,10 @@ int smoe_rms_norm_bwd(const void* dy, int x_f32, const void* h, int h_f32, int64
   if (x_f32) rc = norm_bwd_launch_any<true, true>(a, sh, blocks, st);
   else rc = h_f32 ? norm_bwd_launch_any<false, true>(a, sh, blocks, st) : norm_bwd_launch_any<false, false>(a, sh, blocks, st);
   if (rc || !dw) return rc;
-  rms_norm_dw_kernel<<<(unsigned)((H + 31) / 32), 32 * kNormSumWarps, 0, st>>>((const float*)workspace, (int64_t)blocks * a.flushes, (int)H, dw,
-                                                               dw_f32 != 0, dw_accumulate != 0);
-  return cudaGetLastError() == cudaSuccess ? SMOE_OK : SMOE_ERR_LAUNCH;
+  return launch_early(rms_norm_dw_kernel, (unsigned)((H + 31) / 32), 32 * kNormSumWarps, 0, 0, st, (const float*)workspace,
+                      (int64_t)blocks * a.flushes, (int)H, dw, (int)(dw_f32 != 0), (int)(dw_accumulate != 0)) == cudaSuccess
+             ? SMOE_OK
+             : SMOE_ERR_LAUNCH;
 }
 
 }  // extern "C"
