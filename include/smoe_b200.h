@@ -566,10 +566,12 @@ int smoe_block128_experts(const void* x_bf16, const int32_t* idx, const float* s
 int smoe_grouped_rows(const void* x_bf16, int64_t ldx, const void* w_bf16, int w_transposed, const int32_t* efo, const int32_t* counts,
                       void* y_bf16, int64_t rows, int64_t N, int64_t K, int64_t E, int32_t* status, int32_t* pinned_host_word,
                       void* stream);
-/* dw[e] (N x K) = the sum over e's live rows of dy[r,:]^T x[r,:]: f32, added to dw or stored, or rounded to bf16. */
+/* dw[e] (N x K) = the sum over e's live rows of dy[r,:]^T x[r,:]: f32, added to dw or stored, or rounded to bf16.  workspace:
+ * smoe_grouped_wgrad_workspace bytes (0: none is used; -1 for sizes that are not taken). */
+int64_t smoe_grouped_wgrad_workspace(int64_t N, int64_t K, int64_t rows, int64_t E);
 int smoe_grouped_wgrad(const void* dy_bf16, int64_t ldy, const void* x_bf16, int64_t ldx, const int32_t* efo, const int32_t* counts,
-                       void* dw, int64_t N, int64_t K, int64_t rows, int64_t E, int out_bf16, int accumulate, int32_t* status,
-                       int32_t* pinned_host_word, void* stream);
+                       void* dw, int64_t N, int64_t K, int64_t rows, int64_t E, int out_bf16, int accumulate, void* workspace,
+                       int32_t* status, int32_t* pinned_host_word, void* stream);
 
 /* ---- the norm in front of the experts -------------------------------------------
  * No counterpart in the reference, whose layer begins behind it.

@@ -27,22 +27,27 @@ struct Gemm16Params {
   int b_mn;
   void* c;                   // ROWS16: bf16 [rows, N], rows that are not live become zero; WGRAD16: [E, M, N] f32 or bf16
   int out_bf16, accumulate;  // WGRAD16
+  int split;                 // WGRAD16: stretches that a segment's rows are cut into; stretch s goes to the s-th [E, M, N] of c
   int* status;
   volatile int* host_word;
 };
 
+constexpr int kPiece16 = 64 * 128;      // bytes of 64 x 64 values
+
+// BN: columns of a tile, 256, or 128 where tiles are few or narrow
+template <int COLS>
 struct Gemm16Smem {
-  static constexpr int BN = 256;
-  static constexpr int A_BYTES = BM * 128, B_BYTES = BN / 2 * 128, PIECE = 64 * 128;      // PIECE: 64 x 64 values
-  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES, STAGES = 5;
+  static constexpr int BN = COLS;
+  static constexpr int A_BYTES = BM * 128, B_BYTES = BN / 2 * 128, B_PIECES = BN / 128;
+  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES, STAGES = BN == 256 ? 5 : 7;
   static constexpr int BUFS = 2;
   static constexpr int EPI_WARPS = 8, STG_BYTES = 4096;       // staging of a warp: 32 rows of 128 bytes
   static constexpr int BAR_BYTES = (4 * STAGES + 2 * BUFS) * 8;
-  static constexpr int AUX_BYTES = 256 + 3 * (kG128Segs + 1) * 4;
+  static constexpr int AUX_BYTES = 512 + 3 * (kG128Segs + 1) * 4;
   static constexpr int TOTAL = 1024 + STAGES * STAGE_BYTES + EPI_WARPS * STG_BYTES + AUX_BYTES;
   static constexpr int THREADS = 32 * (EPI_WARPS + 4);
   static_assert(TOTAL <= 227 * 1024, "shared memory budget");
-  static_assert(BAR_BYTES <= 240, "barrier storage");
+  static_assert(BAR_BYTES <= 496, "barrier storage");
 };
 
 // tcgen05.mma kind::f16: bf16 x bf16 -> f32
@@ -65,7 +70,7 @@ __device__ __forceinline__ void mma_bf16_pair_lo(uint32_t d_tmem, uint32_t a_lo,
 constexpr uint32_t kDescHi16 = (1024u >> 4) | (1u << 14) | (2u << 29);
 // low word: start, and for an MN-major operand the distance between its pieces of 64
 __device__ __forceinline__ uint32_t desc_lo16(uint32_t saddr, bool mn) {
-  return ((saddr & 0x3FFFF) >> 4) | (mn ? (uint32_t)(Gemm16Smem::PIECE >> 4) << 16 : 1u << 16);
+  return ((saddr & 0x3FFFF) >> 4) | (mn ? (uint32_t)(kPiece16 >> 4) << 16 : 1u << 16);
 }
 // of an MMA's 16 values of the reduction: 32 bytes, or 16 rows of 128
 __device__ __forceinline__ uint32_t desc_step16(bool mn) { return mn ? 128u : 2u; }
@@ -81,20 +86,23 @@ struct Tile16 {
   int e, m0, n0;             // m0: first row of this CTA's 128
   int t0, nkt, tail;         // WGRAD16: first row of the reduction; blocks of 64; rows of the last one if it is not full
   int live;                  // rows below it are stored
+  int out;                   // WGRAD16: which of c's [M, N]
 };
-template <int MODE>
+template <int MODE, int BN>
 __device__ __forceinline__ Tile16 tile16(int tile, int rank, const Gemm16Params& p, const Segs128& s) {
   Tile16 t;
-  constexpr int BN = Gemm16Smem::BN;
   const int nt = (p.N + BN - 1) / BN;
   if (MODE == WGRAD16) {
     const int mt = (p.M + 255) / 256, per = mt * nt;
-    t.e = tile / per;
-    const int r = tile - t.e * per;
+    t.out = tile / per;
+    const int r = tile - t.out * per, part = t.out / p.E;
+    t.e = t.out - part * p.E;
     t.m0 = (r / nt) * 256 + rank * 128;
     t.n0 = (r % nt) * BN;
-    t.t0 = s.start[t.e];
-    const int n = s.live[t.e] - t.t0;
+    const int all = s.live[t.e] - s.start[t.e];
+    const int stretch = ((all + p.split - 1) / p.split + kBK16 - 1) / kBK16 * kBK16;
+    const int n = max(min(all - part * stretch, stretch), 0);
+    t.t0 = s.start[t.e] + part * stretch;
     t.nkt = (n + kBK16 - 1) / kBK16;
     t.tail = n % kBK16;
     t.live = p.M;
@@ -103,7 +111,7 @@ __device__ __forceinline__ Tile16 tile16(int tile, int rank, const Gemm16Params&
     t.n0 = (tile - pr * nt) * BN;
     t.e = seg_of_tile_warp(s.tiles, p.E, pr);
     t.m0 = s.start[t.e] + (pr - s.tiles[t.e]) * 256 + rank * 128;
-    t.t0 = t.tail = 0;
+    t.t0 = t.tail = t.out = 0;
     t.nkt = (p.K + kBK16 - 1) / kBK16;
     t.live = s.live[t.e];
   }
@@ -126,21 +134,21 @@ __device__ __forceinline__ void zero_gaps16(const Segs128& s, int E, __nv_bfloat
   }
 }
 
-template <int MODE>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Gemm16Smem::THREADS, 1)
+template <int MODE, int COLS>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Gemm16Smem<COLS>::THREADS, 1)
 gemm16_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
               const __grid_constant__ CUtensorMap tmap_c, const Gemm16Params p) {
-  using S = Gemm16Smem;
+  using S = Gemm16Smem<COLS>;
   constexpr int BN = S::BN;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* epi = smem + S::STAGES * S::STAGE_BYTES;
   uint8_t* aux = epi + S::EPI_WARPS * S::STG_BYTES;
   uint64_t* bars = reinterpret_cast<uint64_t*>(aux);            // full[S], empty[S], tail[S], fixed[S], tfull[BUFS], tempty[BUFS]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(aux + 240);
-  volatile int* s_abort = reinterpret_cast<volatile int*>(aux + 244);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(aux + 496);
+  volatile int* s_abort = reinterpret_cast<volatile int*>(aux + 500);
   Segs128 segs;
-  segs.start = reinterpret_cast<int*>(aux + 256);
+  segs.start = reinterpret_cast<int*>(aux + 512);
   segs.live = segs.start + kG128Segs + 1;
   segs.tiles = segs.live + kG128Segs + 1;
 
@@ -168,7 +176,7 @@ gemm16_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
     fence_proxy_async_smem();
   }
   if (warp == ISSUER) {
-    tmem_alloc2(smem_u32(tmem_slot), 512);
+    tmem_alloc2(smem_u32(tmem_slot), S::BUFS * BN);
     tmem_relinquish2();
   }
   wait_for_kernel_before();                   // so far nothing in memory has been touched
@@ -181,7 +189,7 @@ gemm16_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
   const uint32_t tmem_base = *tmem_slot;
   const uint32_t smem_base = smem_u32(smem);
   const int nt = (p.N + BN - 1) / BN;
-  const int n_total = MODE == WGRAD16 ? p.E * ((p.M + 255) / 256) * nt : segs.tiles[p.E + 1] * nt;
+  const int n_total = MODE == WGRAD16 ? p.split * p.E * ((p.M + 255) / 256) * nt : segs.tiles[p.E + 1] * nt;
 
   if (warp == PRODUCER) {
     // ------------------------------------------------------------ producer (both CTAs), one elected lane issues
@@ -191,7 +199,7 @@ gemm16_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
     uint32_t phase = 0;
     bool ok = true;
     for (int tile = pair_id; tile < n_total && ok; tile += n_pairs) {
-      const Tile16 t = tile16<MODE>(tile, rank, p, segs);
+      const Tile16 t = tile16<MODE, BN>(tile, rank, p, segs);
       const int nkt = __shfl_sync(0xffffffffu, t.nkt, 0), m0 = __shfl_sync(0xffffffffu, t.m0, 0);
       const int n_row = __shfl_sync(0xffffffffu, t.n0, 0) + (int)rank * (BN / 2);
       const int e = __shfl_sync(0xffffffffu, t.e, 0), t0 = __shfl_sync(0xffffffffu, t.t0, 0);
@@ -203,25 +211,25 @@ gemm16_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
         const uint32_t a_dst = smem_base + stage * S::STAGE_BYTES, b_dst = a_dst + S::A_BYTES;
         if (elect_one()) {
           if (MODE == WGRAD16 && tail && k == nkt - 1) {      // to a barrier of this CTA, for its FIXER
-            mbar_expect_tx(bar_tail + 8 * stage, S::STAGE_BYTES);
+            const uint32_t last = bar_tail + 8 * stage;
+            mbar_expect_tx(last, S::STAGE_BYTES);
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              tma_load_2d(a_dst + c * S::PIECE, &tmap_a, bar_tail + 8 * stage, m0 + c * 64, t0 + k * kBK16);
-              tma_load_2d(b_dst + c * S::PIECE, &tmap_b, bar_tail + 8 * stage, n_row + c * 64, t0 + k * kBK16);
-            }
+            for (int c = 0; c < 2; ++c) tma_load_2d(a_dst + c * kPiece16, &tmap_a, last, m0 + c * 64, t0 + k * kBK16);
+#pragma unroll
+            for (int c = 0; c < S::B_PIECES; ++c) tma_load_2d(b_dst + c * kPiece16, &tmap_b, last, n_row + c * 64, t0 + k * kBK16);
           } else {
             if (rank == 0) mbar_expect_tx(bar_full + 8 * stage, 2 * S::STAGE_BYTES);
             if (MODE == WGRAD16) {
 #pragma unroll
-              for (int c = 0; c < 2; ++c) {
-                tma_load_2d_pair(a_dst + c * S::PIECE, &tmap_a, full, m0 + c * 64, t0 + k * kBK16);
-                tma_load_2d_pair(b_dst + c * S::PIECE, &tmap_b, full, n_row + c * 64, t0 + k * kBK16);
-              }
+              for (int c = 0; c < 2; ++c) tma_load_2d_pair(a_dst + c * kPiece16, &tmap_a, full, m0 + c * 64, t0 + k * kBK16);
+#pragma unroll
+              for (int c = 0; c < S::B_PIECES; ++c)
+                tma_load_2d_pair(b_dst + c * kPiece16, &tmap_b, full, n_row + c * 64, t0 + k * kBK16);
             } else {
               tma_load_2d_pair(a_dst, &tmap_a, full, k * kBK16, m0);
               if (p.b_mn) {
 #pragma unroll
-                for (int c = 0; c < 2; ++c) tma_load_3d_pair(b_dst + c * S::PIECE, &tmap_b, full, n_row + c * 64, k * kBK16, e);
+                for (int c = 0; c < S::B_PIECES; ++c) tma_load_3d_pair(b_dst + c * kPiece16, &tmap_b, full, n_row + c * 64, k * kBK16, e);
               } else {
                 tma_load_3d_pair(b_dst, &tmap_b, full, k * kBK16, n_row, e);
               }
@@ -243,7 +251,7 @@ gemm16_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
       uint32_t fulls = 0, fixes = 0, aphase = 0;              // a stage's phase on either barrier it may be announced by: one bit each
       bool ok = true;
       for (int tile = pair_id; tile < n_total && ok; tile += n_pairs) {
-        const Tile16 t = tile16<MODE>(tile, 0, p, segs);
+        const Tile16 t = tile16<MODE, BN>(tile, 0, p, segs);
         const int nkt = __shfl_sync(0xffffffffu, t.nkt, 0), tail = __shfl_sync(0xffffffffu, t.tail, 0);
         if (nkt == 0) continue;
         ok = __all_sync(0xffffffffu, mbar_wait(bar_tempty + 8 * as, aphase ^ 1));
@@ -280,7 +288,7 @@ gemm16_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
     uint32_t tails = 0;
     bool ok = true;
     for (int tile = pair_id; tile < n_total && ok; tile += n_pairs) {
-      const Tile16 t = tile16<MODE>(tile, rank, p, segs);
+      const Tile16 t = tile16<MODE, BN>(tile, rank, p, segs);
       stage = (stage + t.nkt) % S::STAGES;
       if (t.tail == 0) continue;
       const int st = stage == 0 ? S::STAGES - 1 : stage - 1;
@@ -289,8 +297,8 @@ gemm16_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
       if (!ok) break;
       const uint32_t at = smem_base + st * S::STAGE_BYTES;
 #pragma unroll
-      for (int c = 0; c < 4; ++c)                             // two pieces of either operand, a row 128 bytes of each
-        for (int b = t.tail * 128 + lane * 16; b < S::PIECE; b += 512) st_shared_v4(at + c * S::PIECE + b, 0u, 0u, 0u, 0u);
+      for (int c = 0; c < 2 + S::B_PIECES; ++c)               // the pieces of both operands, a row 128 bytes of each
+        for (int b = t.tail * 128 + lane * 16; b < kPiece16; b += 512) st_shared_v4(at + c * kPiece16 + b, 0u, 0u, 0u, 0u);
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(fixed0 + 8 * st);
@@ -307,7 +315,7 @@ gemm16_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
     if (MODE == ROWS16)
       zero_gaps16(segs, p.E, (__nv_bfloat16*)p.c, p.N, (int)blockIdx.x * S::EPI_WARPS + warp, (int)gridDim.x * S::EPI_WARPS, lane);
     for (int tile = pair_id; tile < n_total; tile += n_pairs) {
-      const Tile16 t = tile16<MODE>(tile, rank, p, segs);
+      const Tile16 t = tile16<MODE, BN>(tile, rank, p, segs);
       const int row0 = t.m0 + q * 32, col0 = t.n0 + half * (BN / 2);
       if (t.nkt == 0 && p.accumulate) continue;               // an empty sum
       if (t.nkt) {
@@ -318,7 +326,7 @@ gemm16_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
       const uint32_t src = tmem_base + ((uint32_t)(q * 32) << 16) + as * BN + half * (BN / 2);
       const bool stored = row0 < t.live && col0 < p.N;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {                           // 64 columns
+      for (int h = 0; h < BN / 128; ++h) {                    // 64 columns
         uint32_t r[2][32];
         if (t.nkt) {
           tmem_ld32(src + h * 64, r[0]);
@@ -326,7 +334,7 @@ gemm16_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
           tmem_ld_wait();
           tmem_values(r[0]);
           tmem_values(r[1]);
-          if (h == 1) {                                       // the buffer's values are in registers
+          if (h == BN / 128 - 1) {                            // the buffer's values are in registers
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster_relaxed(tempty0 + 8 * as);
@@ -352,7 +360,7 @@ gemm16_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
-              tma_store_3d(&tmap_c, stg, col, row0, MODE == WGRAD16 ? t.e : 0);        // (the map has three dimensions)
+              tma_store_3d(&tmap_c, stg, col, row0, MODE == WGRAD16 ? t.out : 0);      // (the map has three dimensions)
               bulk_commit_group();
             }
           } else {
@@ -370,8 +378,8 @@ gemm16_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
-              if (p.accumulate) tma_reduce_add_3d(&tmap_c, stg, col + u * 32, row0, t.e);
-              else tma_store_3d(&tmap_c, stg, col + u * 32, row0, t.e);
+              if (p.accumulate) tma_reduce_add_3d(&tmap_c, stg, col + u * 32, row0, t.out);
+              else tma_store_3d(&tmap_c, stg, col + u * 32, row0, t.out);
               bulk_commit_group();
             }
           }
@@ -392,7 +400,7 @@ gemm16_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
   tc_fence_before();
   cluster_sync_all();                         // the peer may still be signalling this CTA's barriers
   tc_fence_after();
-  if (warp == ISSUER) tmem_dealloc2(tmem_base, 512);
+  if (warp == ISSUER) tmem_dealloc2(tmem_base, S::BUFS * BN);
 }
 
 }  // namespace smoe

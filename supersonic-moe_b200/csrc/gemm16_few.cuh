@@ -139,7 +139,7 @@ gemm16_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
           mbar_expect_tx(full, S::A_BYTES + (t.live <= 16 ? 16 : NT) * 128);
           if (p.w_mn) {
             tma_load_3d(at, &tmap_w, full, t.w0, k * kBK16, t.e);
-            tma_load_3d(at + Gemm16Smem::PIECE, &tmap_w, full, t.w0 + 64, k * kBK16, t.e);
+            tma_load_3d(at + kPiece16, &tmap_w, full, t.w0 + 64, k * kBK16, t.e);
           } else {
             tma_load_3d(at, &tmap_w, full, k * kBK16, t.w0, t.e);
           }

@@ -18,7 +18,7 @@ namespace smoe {
 
 constexpr int kGradThreads = 256;
 constexpr int kGradBlocks = 4;               // a block an SM takes at a time
-constexpr int kGradStep = kGradThreads * 16; // values of a block's step: two pieces of eight a thread
+constexpr int kGradStep = kGradThreads * 8;  // values of a block's step: eight a thread
 
 // A list of tensors; `first` counts pieces of `chunk` values.  Small lists travel as small parameters.
 template <int N>
@@ -208,9 +208,9 @@ grad_scale_kernel(const __grid_constant__ GradList<N> l, const double* __restric
 constexpr int kGradSmall = 48, kGradLarge = 640;      // tensors of a launch
 
 static int64_t grad_chunk(int64_t total) {
-  // some four pieces a block, so that the blocks end together, of one step to 16
-  const int64_t want = total / ((int64_t)sm_count() * kGradBlocks * 4) / kGradStep + 1;
-  return (want < 16 ? want : 16) * kGradStep;
+  // some eight pieces a block, so that the blocks end together, of one step to 32
+  const int64_t want = total / ((int64_t)sm_count() * kGradBlocks * 8) / kGradStep + 1;
+  return (want < 32 ? want : 32) * kGradStep;
 }
 
 // blocks of a launch over the tensors [from, to): as many as there are pieces, or find room together
@@ -287,7 +287,7 @@ static int grad_check(const smoe_gradient* list, int64_t count, int64_t* total, 
     if (((uintptr_t)g.grad & (g.grad_f32 ? 3 : 1)) || (outs && ((uintptr_t)g.out & (g.out_f32 ? 3 : 1)))) return SMOE_ERR_ALIGN;
     *total += g.numel;
   }
-  return *total / kGradStep / 16 < (int64_t)1 << 30 ? SMOE_OK : SMOE_ERR_SHAPE;
+  return *total / (32 * kGradStep) < (int64_t)1 << 30 ? SMOE_OK : SMOE_ERR_SHAPE;
 }
 
 }  // namespace smoe

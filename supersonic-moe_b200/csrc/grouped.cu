@@ -48,20 +48,33 @@ static int check16(int64_t rows, int64_t N, int64_t K, int64_t E, const int* efo
   return SMOE_OK;
 }
 
-template <int MODE>
+template <int MODE, int COLS>
 static int launch16(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, const Gemm16Params& p, int64_t tiles,
                     cudaStream_t stream) {
+  using S = Gemm16Smem<COLS>;
   static bool attr_set[kMaxDevices] = {};
-  auto kern = gemm16_kernel<MODE>;
-  if (!ensure_smem_attr(kern, Gemm16Smem::TOTAL, attr_set)) return SMOE_ERR_LAUNCH;
+  auto kern = gemm16_kernel<MODE, COLS>;
+  if (!ensure_smem_attr(kern, S::TOTAL, attr_set)) return SMOE_ERR_LAUNCH;
   int64_t pairs = sm_count() / 2;
   if (tiles < pairs) pairs = tiles;
-  return launch_early(kern, (unsigned)(2 * pairs), Gemm16Smem::THREADS, Gemm16Smem::TOTAL, 0, stream, ta, tb, tc, p) == cudaSuccess
-             ? SMOE_OK
-             : SMOE_ERR_LAUNCH;
+  return launch_early(kern, (unsigned)(2 * pairs), S::THREADS, S::TOTAL, 0, stream, ta, tb, tc, p) == cudaSuccess ? SMOE_OK
+                                                                                                                 : SMOE_ERR_LAUNCH;
 }
+// Narrow tiles where the wide ones would leave half of the CTA pairs without any, or have no use for their width (us, wide / narrow: 512 x
+// 4096 x 4096 24.6 / 18.1, 256 x 8192 x 2048 15.9 / 12.4, 8192 x 128 x 2048 15.3 / 12.1; of 64 tiles, 2048 x 2048 x 2048, 16.3 / 18.4)
+static bool narrow16(int64_t tiles, int64_t cols) { return tiles <= sm_count() / 4 || cols <= 128; }
 
-static bool few_rows16(int64_t rows, int64_t E) { return rows <= Few16Smem::NT || rows <= 32 * E; }
+// Weights as the wide operand: where the rows of an expert make one tile of 64, evenly routed, or the tiles are few: one for each SM of
+// a single projection, two of experts, whose 256-row tiles are then mostly empty (us, the other kernel / few: 1 expert 4096 x 4096, 256
+// rows 17.4 / 15.8, 512 18.1 / 26.4; 1024 x 4096, 1024 rows 16.8 / 15.3, 2048 18.0 / 26.1; 1000 x 720, 2000 7.7 / 9.1; 8 of 512 x 512, 2048
+// 8.2 / 5.9, 4096 8.5 / 7.7, 8192 9.0 / 11.8; of 1024 x 1024, 1024 11.3 / 8.1, 2048 9.2 / 10.9; of 4096 x 2048, 512 31 / 26, 2048 35 /
+// 50; 128 of 1536 x 2048, 4096 177 / 128, 8192 170 / 133, 12288 168 / 170; the same unevenly routed 166 / 142, 182 / 171, 189 / 206.  The
+// gradient of the rows reads its weights across and takes up to a sixth longer with few.)
+static bool few_rows16(int64_t rows, int64_t N, int64_t E) {
+  if (rows <= Few16Smem::NT * E) return true;
+  const int64_t busy = rows < E ? rows : E;
+  return (rows + (Few16Smem::NT - 1) * busy) / Few16Smem::NT * up16(N, 128) <= (E == 1 ? 1 : 2) * sm_count();
+}
 
 static int few16(const void* x, int64_t ldx, const void* w, const int* efo, const int* counts, void* y, int64_t rows, int64_t N, int64_t K,
                  int64_t E, int w_mn, int* status, int* host_word, cudaStream_t stream) {
@@ -76,8 +89,13 @@ static int few16(const void* x, int64_t ldx, const void* w, const int* efo, cons
   const int64_t busy = rows < E ? rows : E;
   const int64_t tiles = (rows + (Few16Smem::NT - 1) * busy) / Few16Smem::NT * up16(N, 128);      // as many as there can be
   const int64_t kb = up16(K, kBK16);
+  // Few tiles are shared by clusters, where the reduction is long enough for what the sums' exchange costs, some 1.7 us (us with 1 / 2 / 4
+  // / 8 CTAs, one row: 4096 x 1024 6.4 / 7.3 / 7.3 / -, x 1792 8.4 / 8.5 / 8.1 / -, x 4096 15.6 / 13.1 / 11.0 / -; 1024 x 1280 6.6 / 6.7 /
+  // 5.9 / 6.2, x 16384 47 / 28 / 17.7 / -; 8192 x 2560 11.2 / 11.8 / 16 / -, x 4096 16.5 / 15.6 / 19 / -; 64 rows: 4096 x 1536 8.4 / 10.4 /
+  // 9.5 / -, 2048 x 2048 9.5 / 10.8 / 8.9 / -).  Eight find room together on half of the SMs only (2048 x 1536 7.0 with four, 13.2).
   int split = 1;
-  while (split < 8 && kb >= 12 && split * 6 <= kb && tiles * split * (split == 4 ? 4 : 2) <= sms) split *= 2;
+  if (tiles * 4 <= sms && kb >= (rows > 16 ? 32 : 20)) split = tiles * 16 <= sms && kb >= 64 ? 8 : 4;
+  else if (tiles * 2 <= sms && kb >= 64) split = 2;
   Few16Params p{(int)rows, (int)N, (int)K, (int)E, efo, counts, w_mn, (__nv_bfloat16*)y, split, status, host_word};
   int64_t groups = sms / split;
   if (tiles < groups) groups = tiles;
@@ -85,6 +103,40 @@ static int few16(const void* x, int64_t ldx, const void* w, const int* efo, cons
                       tx64, p) == cudaSuccess
              ? SMOE_OK
              : SMOE_ERR_LAUNCH;
+}
+
+// Weight gradients of few tiles: a segment's rows are cut into stretches, so that every CTA pair has a tile; a stretch's sums pass through
+// memory once, and a launch adds them up in their order.  Where that pays: it costs some 5 us, a block of 64 rows some 0.2 of a narrow
+// tile and 0.3 of a wide one (us, 1 stretch with narrow tiles / 2 / 4 / 8 / 16, one expert: 512 x 512, 16384 rows 55 / 33 / 21 / 16 /
+// 17; 64 x 512 54 / 31 / 19 / 14 / 12; 1024 x 1024 56 / 36 / 33 / 36 / 49, 2048 rows 11.4 / 11.5 / 12.5 / 16 / 25; 8 of 512 x 256, 16384
+// rows 12.0 / 13.0 / 14.4 / 18 / 27).
+static int wgrad_split16(int64_t N, int64_t K, int64_t rows, int64_t E) {
+  const int64_t tiles = E * up16(N, 256) * up16(K, K <= 128 ? 128 : 256), pairs = sm_count() / 2, blocks = rows / E / kBK16;
+  int64_t split = pairs / tiles;
+  if (split > blocks / 8) split = blocks / 8;
+  if (split > 16) split = 16;
+  return split >= 2 && blocks * (2 * split - 3) > 50 * split ? (int)split : 1;
+}
+
+// out = (out +) the sum of `split` partial sums, each `fours` of four values
+__global__ void __launch_bounds__(256) wgrad_sum_kernel(const float4* __restrict__ part, int split, int64_t fours, void* out, int bf16,
+                                                        int accumulate) {
+  wait_for_kernel_before();
+  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < fours; i += (int64_t)gridDim.x * blockDim.x) {
+    float4 v = part[i];
+#pragma unroll 4
+    for (int s = 1; s < split; ++s) {
+      const float4 u = part[s * fours + i];
+      v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
+    }
+    if (bf16) {
+      ((uint2*)out)[i] = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
+    } else {
+      float4* o = (float4*)out + i;
+      if (accumulate) atomicAdd(o, v);                    // (once for each value: another stream's sums into it are not lost)
+      else *o = v;
+    }
+  }
 }
 
 }  // namespace smoe
@@ -102,25 +154,34 @@ int smoe_grouped_rows(const void* x_bf16, int64_t ldx, const void* w_bf16, int w
   if (rows == 0) return SMOE_OK;
   if (!x_bf16 || !w_bf16 || !y_bf16) return SMOE_ERR_ARG;
   if (!on16(x_bf16) || !on16(w_bf16) || !on16(y_bf16)) return SMOE_ERR_ALIGN;
-  if (few_rows16(rows, E))
+  if (few_rows16(rows, N, E))
     return few16(x_bf16, ldx, w_bf16, efo, counts, y_bf16, rows, N, K, E, w_transposed != 0, status, pinned_host_word,
                  (cudaStream_t)stream);
+  // every segment may end in a tile that is not full
+  const int64_t row_tiles = efo ? (rows + 255 * (rows < E ? rows : E)) / 256 : up16(rows, 256);
+  const bool narrow = narrow16(row_tiles * up16(N, 256), N);
   CUtensorMap ta, tb, tc;
   rc = make_tmap16(&ta, x_bf16, 1, rows, K, ldx, 128, 2);
-  if (!rc) rc = w_transposed ? make_tmap16(&tb, w_bf16, E, K, N, N, 64, 3) : make_tmap16(&tb, w_bf16, E, N, K, K, 128, 3);
+  if (!rc) rc = w_transposed ? make_tmap16(&tb, w_bf16, E, K, N, N, 64, 3) : make_tmap16(&tb, w_bf16, E, N, K, K, narrow ? 64 : 128, 3);
   if (!rc) rc = make_tmap16_out(&tc, y_bf16, true, 1, rows, N);
   if (rc) return rc;
   Gemm16Params p{};
-  p.rows = (int)rows; p.N = (int)N; p.K = (int)K; p.E = (int)E;
+  p.rows = (int)rows; p.N = (int)N; p.K = (int)K; p.E = (int)E; p.split = 1;
   p.efo = efo; p.counts = counts; p.b_mn = w_transposed != 0; p.c = y_bf16;
   p.status = status; p.host_word = pinned_host_word;
-  // every segment may end in a tile that is not full
-  return launch16<ROWS16>(ta, tb, tc, p, (rows / 256 + E) * up16(N, 256), (cudaStream_t)stream);
+  return narrow ? launch16<ROWS16, 128>(ta, tb, tc, p, row_tiles * up16(N, 128), (cudaStream_t)stream)
+                : launch16<ROWS16, 256>(ta, tb, tc, p, row_tiles * up16(N, 256), (cudaStream_t)stream);
+}
+
+int64_t smoe_grouped_wgrad_workspace(int64_t N, int64_t K, int64_t rows, int64_t E) {
+  if (!size16(N) || !size16(K) || rows < 0 || rows >= (int64_t)1 << 30 || E <= 0 || E > kMaxExperts2) return -1;
+  const int split = wgrad_split16(N, K, rows, E);
+  return split > 1 ? split * E * N * K * 4 : 0;
 }
 
 int smoe_grouped_wgrad(const void* dy_bf16, int64_t ldy, const void* x_bf16, int64_t ldx, const int32_t* efo, const int32_t* counts,
-                       void* dw, int64_t N, int64_t K, int64_t rows, int64_t E, int out_bf16, int accumulate, int32_t* status,
-                       int32_t* pinned_host_word, void* stream) {
+                       void* dw, int64_t N, int64_t K, int64_t rows, int64_t E, int out_bf16, int accumulate, void* workspace,
+                       int32_t* status, int32_t* pinned_host_word, void* stream) {
   int rc = check16(rows, N, K, E, efo, counts, status);
   if (rc) return rc;
   if (!rows16(rows, N, ldy) || !rows16(rows, K, ldx)) return SMOE_ERR_SHAPE;
@@ -133,16 +194,29 @@ int smoe_grouped_wgrad(const void* dy_bf16, int64_t ldy, const void* x_bf16, int
   }
   if (!dy_bf16 || !x_bf16) return SMOE_ERR_ARG;
   if (!on16(dy_bf16) || !on16(x_bf16)) return SMOE_ERR_ALIGN;
+  const int split = wgrad_split16(N, K, rows, E);
+  if (split > 1 && !workspace) return SMOE_ERR_ARG;
+  if (split > 1 && !on16(workspace)) return SMOE_ERR_ALIGN;
   CUtensorMap ta, tb, tc;
   rc = make_tmap16(&ta, dy_bf16, 1, rows, N, ldy, 64, 2);
   if (!rc) rc = make_tmap16(&tb, x_bf16, 1, rows, K, ldx, 64, 2);
-  if (!rc) rc = make_tmap16_out(&tc, dw, out_bf16 != 0, E, N, K);
+  if (!rc) rc = make_tmap16_out(&tc, split > 1 ? workspace : dw, split == 1 && out_bf16, split * E, N, K);
   if (rc) return rc;
   Gemm16Params p{};
-  p.rows = (int)rows; p.M = (int)N; p.N = (int)K; p.E = (int)E;
-  p.efo = efo; p.counts = counts; p.c = dw; p.out_bf16 = out_bf16 != 0; p.accumulate = accumulate != 0;
+  p.rows = (int)rows; p.M = (int)N; p.N = (int)K; p.E = (int)E; p.split = split;
+  p.efo = efo; p.counts = counts; p.c = split > 1 ? workspace : dw; p.out_bf16 = split == 1 && out_bf16;
+  p.accumulate = split == 1 && accumulate;
   p.status = status; p.host_word = pinned_host_word;
-  return launch16<WGRAD16>(ta, tb, tc, p, E * up16(N, 256) * up16(K, 256), (cudaStream_t)stream);
+  const cudaStream_t st = (cudaStream_t)stream;
+  const int64_t row_tiles = split * E * up16(N, 256);
+  rc = narrow16(row_tiles * up16(K, 256), K) ? launch16<WGRAD16, 128>(ta, tb, tc, p, row_tiles * up16(K, 128), st)
+                                             : launch16<WGRAD16, 256>(ta, tb, tc, p, row_tiles * up16(K, 256), st);
+  if (rc || split == 1) return rc;
+  const int64_t fours = E * N * K / 4, blocks = up16(fours, 256), most = (int64_t)sm_count() * 8;
+  return launch_early(wgrad_sum_kernel, (unsigned)(blocks < most ? blocks : most), 256, 0, 0, st, (const float4*)workspace, split, fours, dw,
+                      (int)(out_bf16 != 0), (int)(accumulate != 0)) == cudaSuccess
+             ? SMOE_OK
+             : SMOE_ERR_LAUNCH;
 }
 
 }  // extern "C"

@@ -187,8 +187,10 @@ Tensor grouped_wgrad(const Tensor& dy, const Tensor& x, const Tensor& efo, const
   // (what is added leaves in pieces that start on 16 bytes)
   const bool direct = add && (uintptr_t)main_grad.data_ptr() % 16 == 0;
   Tensor dw = direct ? main_grad : add ? at::zeros({E, N, K}, o.dtype(at::kFloat)) : at::empty({E, N, K}, o);
+  const int64_t bytes = smoe_grouped_wgrad_workspace(N, K, rows, E);
+  const Tensor ws = bytes > 0 ? at::empty({bytes}, o.dtype(at::kByte)) : Tensor();
   check(smoe_grouped_wgrad(dy.data_ptr(), distance(dy), x.data_ptr(), distance(x), (const int32_t*)ptr(efo), (const int32_t*)ptr(counts),
-                           dw.data_ptr(), N, K, rows, E, !add, add, (int32_t*)at.status, (int32_t*)at.host, stream()),
+                           dw.data_ptr(), N, K, rows, E, !add, add, ptr(ws), (int32_t*)at.status, (int32_t*)at.host, stream()),
         "grouped_wgrad");
   if (!add) return dw;
   if (!direct) Tensor(main_grad).add_(dw.view(main_grad.sizes()));

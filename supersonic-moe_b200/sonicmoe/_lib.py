@@ -103,7 +103,8 @@ SIGNATURES = {
     "smoe_block128_experts_bytes": (_L, [_L] * 5),
     "smoe_block128_experts": (_I, [_P] * 9 + [_L] * 5 + [_P, _P, _P]),
     "smoe_grouped_rows": (_I, [_P, _L, _P, _I, _P, _P, _P] + [_L] * 4 + [_P, _P, _P]),
-    "smoe_grouped_wgrad": (_I, [_P, _L, _P, _L, _P, _P, _P] + [_L] * 4 + [_I, _I, _P, _P, _P]),
+    "smoe_grouped_wgrad_workspace": (_L, [_L] * 4),
+    "smoe_grouped_wgrad": (_I, [_P, _L, _P, _L, _P, _P, _P] + [_L] * 4 + [_I, _I, _P, _P, _P, _P]),
     "smoe_rms_norm": (_I, [_P, _I, _L, _P, _I, _L, _P, _I, _L, _L, _D, _P, _P, _P, _I, _P, _P, _P]),
     "smoe_rms_norm_bwd_workspace": (_L, [_L, _L]),
     "smoe_rms_norm_bwd": (_I, [_P, _I, _P, _I, _L, _P, _I, _P, _P, _L, _L, _P, _P, _P, _I, _I, _P, _P]),

@@ -123,6 +123,23 @@ def test_large(sonicmoe):
     check(sonicmoe, [3000, 0, 1, 5011, 777, 64, 2500, 129], 2048, 1536, main_grad=True)
 
 
+@pytest.mark.parametrize("counts,N,K", [([5000], 136, 72), ([5000], 64, 512), ([13001, 0, 4999], 264, 136), ([19000, 1, 700], 128, 256),
+                                        ([20000], 1000, 520), ([40000], 8, 8)])
+def test_weight_gradients_of_few_tiles_are_summed_in_stretches(sonicmoe, counts, N, K):
+    from sonicmoe._lib import lib
+    for kw in (dict(), dict(padded=True, tail=100)):
+        rows = segments(counts, **kw)[3]
+        assert lib.smoe_grouped_wgrad_workspace(N, K, rows, len(counts)) > 0
+        check(sonicmoe, counts, N, K, **kw)
+        check(sonicmoe, counts, N, K, main_grad=True, **kw)
+
+
+@pytest.mark.parametrize("rows,N,K", [(600, 1024, 200), (3000, 512, 136), (5000, 128, 64), (5000, 72, 264), (300, 4096, 520)])
+def test_narrow_tiles(sonicmoe, rows, N, K):
+    check(sonicmoe, [rows], N, K)
+    check(sonicmoe, [rows // 2, 3, 0, rows - rows // 2 - 3], N, K, main_grad=True)
+
+
 def test_few_rows_of_a_wide_weight_are_shared_by_clusters(sonicmoe):
     for rows in (1, 15, 16, 17, 33, 64):
         for N, K in ((4096, 4096), (1024, 2048), (136, 8192), (4096, 760)):

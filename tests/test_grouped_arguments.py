@@ -55,9 +55,10 @@ def test_c_entry_points_check_their_arguments():
     assert rows(E=1, efo=None, counts=16) == ARG
     assert rows(x=8) == rows(w=24) == rows(y=2) == ALIGN
     assert rows(rows=0, x=None, y=None) == 0
-    wg = lambda **k: lib.smoe_grouped_wgrad(*({**dict(dy=16, ldy=8, x=16, ldx=64, efo=16, counts=None, dw=16, N=8, K=64, rows=4, E=2, bf16=1, acc=0,
+    wg = lambda **k: lib.smoe_grouped_wgrad(*({**dict(dy=16, ldy=8, x=16, ldx=64, efo=16, counts=None, dw=16, N=8, K=64, rows=4, E=2, bf16=1, acc=0, ws=None,
                                                       status=16, host=None, stream=None), **k}.values()))
     assert wg(N=4) == wg(ldy=0) == wg(ldx=65) == SHAPE
     assert wg(acc=1) == wg(dw=None) == wg(dy=None) == wg(efo=None) == ARG
     assert wg(dw=8) == wg(dy=2) == wg(x=8) == ALIGN
     assert wg(rows=0, bf16=0, acc=1) == 0
+    assert lib.smoe_grouped_wgrad_workspace(8, 64, 4, 2) == 0 and lib.smoe_grouped_wgrad_workspace(8, 60, 4, 2) == -1
