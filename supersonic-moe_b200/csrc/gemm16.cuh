@@ -82,6 +82,14 @@ __device__ __forceinline__ void tmem_values(uint32_t (&r)[N]) {
   for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
 }
 
+// The L2 fetches what a sum is added to when the sum arrives, and the sums wait for that: the old values of a warp's next pieces are
+// asked for kReduceAhead ahead, in tiles of few blocks, which this traffic bounds (us with / without, by rows an expert: 32 of 1536 x
+// 2048, 128 rows 149 / 168; 8 of 2048 x 2048, 512 54 / 66; 128 of 1536 x 2048, 256 631 / 648, 1024 846 / 827).
+constexpr int kAheadBlocks16 = 10;
+__device__ __forceinline__ void tma_prefetch_l2_3d(const void* tmap, int c0, int c1, int c2) {
+  asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];" ::"l"(tmap), "r"(c0), "r"(c1), "r"(c2) : "memory");
+}
+
 struct Tile16 {
   int e, m0, n0;             // m0: first row of this CTA's 128
   int t0, nkt, tail;         // WGRAD16: first row of the reduction; blocks of 64; rows of the last one if it is not full
@@ -318,13 +326,19 @@ gemm16_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
       const Tile16 t = tile16<MODE, BN>(tile, rank, p, segs);
       const int row0 = t.m0 + q * 32, col0 = t.n0 + half * (BN / 2);
       if (t.nkt == 0 && p.accumulate) continue;               // an empty sum
+      const bool stored = row0 < t.live && col0 < p.N;
+      const bool ahead = MODE == WGRAD16 && p.accumulate && stored && t.nkt <= kAheadBlocks16 && lane == 0;
+      auto prefetch_piece = [&](int i) {
+        if (ahead && i < BN / 64 && col0 + i * 32 < p.N) tma_prefetch_l2_3d(&tmap_c, col0 + i * 32, row0, t.out);
+      };
+#pragma unroll
+      for (int i = 0; i < kReduceAhead; ++i) prefetch_piece(i);
       if (t.nkt) {
         ok = __all_sync(0xffffffffu, mbar_wait(bar_tfull + 8 * as, aphase));
         if (!ok) break;
         tc_fence_after();
       }
       const uint32_t src = tmem_base + ((uint32_t)(q * 32) << 16) + as * BN + half * (BN / 2);
-      const bool stored = row0 < t.live && col0 < p.N;
 #pragma unroll
       for (int h = 0; h < BN / 128; ++h) {                    // 64 columns
         uint32_t r[2][32];
@@ -372,6 +386,7 @@ gemm16_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
 #pragma unroll
           for (int u = 0; u < 2; ++u) {                       // 32 columns
             if (col + u * 32 >= p.N) break;
+            prefetch_piece(2 * h + u + kReduceAhead);
             if (lane == 0) bulk_wait_group_read<0>();
             __syncwarp();
             stage_f32_32(stg, lane, r[u]);
