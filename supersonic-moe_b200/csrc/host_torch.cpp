@@ -1,7 +1,7 @@
 // The host side of the operators around the experts, on torch tensors: outputs from the caching allocator, the current stream, autograd
 // nodes.  What Python and ctypes take for it is longer than the kernels of a small batch, or than the look at a list of a few hundred
-// gradients (us a call through Python / here: one decoded token's norm 21 / 13, norm with its backward pass 114 / 70, the norm of 300
-// gradients 205 / 29).  The kernels are those of the C ABI; nothing here computes.
+// gradients (us a call through Python / here: one decoded token's norm 21 / 11, norm with its backward pass 114 / 68, the norm of 300
+// gradients 205 / 28).  The kernels are those of the C ABI; nothing here computes.
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
@@ -15,6 +15,7 @@
 #include <torch/csrc/utils/pybind.h>
 
 #include <algorithm>
+#include <cmath>
 #include <optional>
 #include <string>
 #include <tuple>
@@ -160,6 +161,64 @@ struct NormNode : torch::autograd::Function<NormNode> {
   }
 };
 
+const char* type_name(at::ScalarType t) { return at::toString(t); }
+bool needs_grad(std::initializer_list<const Tensor*> ts) {
+  return at::GradMode::is_enabled() && std::any_of(ts.begin(), ts.end(), [](const Tensor* t) { return t->defined() && t->requires_grad(); });
+}
+// [..., H] as [rows, H] whose values lie side by side; the rows may be any distance apart
+Tensor as_rows(const Tensor& t) {
+  const Tensor r = t.dim() == 2 ? t : t.reshape({-1, t.size(-1)});
+  return (r.stride(1) == 1 || r.size(1) == 1) && (r.stride(0) >= r.size(1) || r.size(0) <= 1) ? r : r.contiguous();
+}
+
+constexpr int64_t kNormMaxH = 16384;
+// x and residual as rows, and the weight, of a call that is allowed; kind: see smoe_rms_norm
+std::tuple<Tensor, Tensor, Tensor> norm_checked(const Tensor& x, const Tensor& w, const Tensor& residual, double eps, int kind) {
+  const char* const what = kind ? "rms_norm_quantized" : "rms_norm";
+  const auto tx = x.scalar_type();
+  TORCH_CHECK_VALUE(tx == at::kBFloat16 || (tx == at::kFloat && !kind), what, ": x is bf16", kind ? "" : " or f32", ", got ", type_name(tx));
+  const int64_t H = x.dim() ? x.size(-1) : 0;
+  TORCH_CHECK_VALUE(H >= 1 && H <= kNormMaxH, what, ": rows have 1 to ", std::to_string(kNormMaxH), " values, got ", text(x.sizes()));
+  TORCH_CHECK_VALUE((w.scalar_type() == at::kBFloat16 || f32(w)) && w.dim() == 1 && w.size(0) == H, what, ": the weight is bf16 or f32 [",
+                    std::to_string(H), "], got ", type_name(w.scalar_type()), " ", text(w.sizes()));
+  TORCH_CHECK_VALUE(!residual.defined() || (residual.sizes() == x.sizes() && (residual.scalar_type() == tx || f32(residual))), what,
+                    ": the residual is of x's type or f32, of its shape ", text(x.sizes()), ", got ",
+                    type_name(residual.defined() ? residual.scalar_type() : tx), " ", residual.defined() ? text(residual.sizes()) : "");
+  TORCH_CHECK_VALUE(eps >= 0 && eps < INFINITY, what, ": eps=", std::to_string(eps));
+  const int64_t unit = kind == 1 ? kMxGroup : kind == 2 ? 8 : 1;
+  TORCH_CHECK_VALUE(H % unit == 0, what, ": ", std::to_string(H), " columns are no multiple of ", std::to_string(unit));
+  return {as_rows(x), w.is_contiguous() ? w : w.contiguous(), residual.defined() ? as_rows(residual) : residual};
+}
+
+using Four = std::tuple<Maybe, Maybe, Maybe, Maybe>;
+Maybe some(const Tensor& t) { return t.defined() ? Maybe(t) : Maybe(); }
+// results of rows in x's leading dimensions
+Four in_shape(const Tensor& x, Tensor q, Tensor s, Tensor y, Tensor h) {
+  if (x.dim() != 2) {
+    const auto lead = x.sizes().slice(0, x.dim() - 1);
+    auto apart = [&](const Tensor& t) { return !t.defined() ? t : lead.empty() ? t.select(0, 0) : t.unflatten(0, lead); };
+    q = apart(q);
+    s = apart(s);
+    y = apart(y);
+    h = apart(h);
+  }
+  return {some(q), some(s), some(y), some(h)};
+}
+
+// -> payload, scales, y, h
+Four norm_call(const Tensor& x, const Tensor& weight, const Maybe& residual, double eps, int kind, bool with_output) {
+  const auto [rows, w, res] = norm_checked(x, weight, of(residual), eps, kind);
+  if (needs_grad({&rows, &w, &res})) {
+    TORCH_CHECK_VALUE(!kind || with_output,
+                      "rms_norm_quantized: no gradient flows through the payload; with_output=True gives the rows it flows through");
+    const variable_list out = NormNode::apply(rows, w, some(res), eps, (int64_t)kind);
+    const size_t n = out.size();
+    return in_shape(x, kind ? out[n - 2] : Tensor(), kind ? out[n - 1] : Tensor(), out[0], res.defined() ? out[1] : Tensor());
+  }
+  const Norm n = norm(rows, w, res, eps, kind, !kind || with_output, false);
+  return in_shape(x, n.q, n.s, n.y, n.h);
+}
+
 // ---------------------------------------------------------------- products of bf16 rows grouped by expert
 struct Words {                                           // see failure_words in ops.py
   int64_t status, host;
@@ -238,6 +297,44 @@ struct GroupedNode : torch::autograd::Function<GroupedNode> {
     return once_only(grads, {dx, dw, Tensor(), Tensor(), Tensor(), Tensor()});
   }
 };
+
+// x, weight as the kernels read them, of a call that is allowed
+std::tuple<Tensor, Tensor> grouped_checked(const Tensor& x, const Tensor& w, const Tensor& efo, const Tensor& counts) {
+  const char* const what = "grouped_linear";
+  TORCH_CHECK_VALUE(x.scalar_type() == at::kBFloat16 && x.dim() > 0, what, ": x is bf16 [rows,K], got ", type_name(x.scalar_type()), " ",
+                    text(x.sizes()));
+  TORCH_CHECK_VALUE(w.scalar_type() == at::kBFloat16 && (w.dim() == 2 || w.dim() == 3), what, ": the weight is bf16 [E,N,K], got ",
+                    type_name(w.scalar_type()), " ", text(w.sizes()));
+  const int64_t E = w.dim() == 3 ? w.size(0) : 1, N = w.size(-2), K = w.size(-1);
+  TORCH_CHECK_VALUE(x.size(-1) == K, what, ": x has ", std::to_string(x.size(-1)), " columns, the weight ", std::to_string(K));
+  TORCH_CHECK_VALUE(N > 0 && K > 0 && N % 8 == 0 && K % 8 == 0 && E >= 1 && E <= 256, what, ": ", std::to_string(E), " experts of ",
+                    std::to_string(N), " x ", std::to_string(K), ": sizes are multiples of 8, 1 to 256 experts");
+  TORCH_CHECK_VALUE(efo.defined() || (E == 1 && !counts.defined()), what, ": several experts, or counts, need efo");
+  TORCH_CHECK_VALUE(!efo.defined() || x.dim() == 2, what, ": x is [rows,K] where efo is given");
+  TORCH_CHECK_VALUE(!efo.defined() || (efo.scalar_type() == at::kInt && efo.dim() == 1 && efo.size(0) == E + 1 && efo.is_contiguous()), what,
+                    ": efo is i32 [", std::to_string(E + 1), "], got ", efo.defined() ? text(efo.sizes()) : "");
+  TORCH_CHECK_VALUE(!counts.defined() || (counts.scalar_type() == at::kInt && counts.dim() == 1 && counts.size(0) == E &&
+                                          counts.is_contiguous()),
+                    what, ": counts is i32 [", std::to_string(E), "], got ", counts.defined() ? text(counts.sizes()) : "");
+  same_gpu(what, x, {&w, &efo, &counts});
+  const Tensor rows = x.dim() == 2 ? x : x.reshape({-1, K});
+  return {rows_lie(rows) ? rows : dense(rows), w};
+}
+
+Tensor grouped_call(const Tensor& x, const Tensor& weight, const Maybe& efo, const Maybe& counts, int64_t status, int64_t host) {
+  const auto [rows, w] = grouped_checked(x, weight, of(efo), of(counts));
+  Tensor y;
+  if (needs_grad({&rows, &w})) {
+    y = GroupedNode::apply(rows, w, efo, counts, status, host)[0];
+  } else {
+    const Tensor d = dense(w.detach());
+    y = grouped_rows(rows, d.dim() == 3 ? d : d.unsqueeze(0), of(efo), of(counts), false, {status, host});
+  }
+  if (x.dim() == 2) return y;
+  auto shape = x.sizes().vec();
+  shape.back() = y.size(1);
+  return y.view(shape);
+}
 
 // ---------------------------------------------------------------- the norm of the gradients
 // Gradient tensors of parameters (main_grad before grad; those with neither left out), tensors as they are
@@ -376,28 +473,31 @@ Tensor clip_gradients(const py::object& items, double max_norm, const Maybe& giv
 PYBIND11_MODULE(_host, m) {
   m.def("rms_norm", [](const Tensor& x, const Tensor& w, const Maybe& residual, double eps, int kind, bool with_y, bool keep) {
     const Norm n = norm(x, w, of(residual), eps, kind, with_y, keep);
-    auto some = [](const Tensor& t) { return t.defined() ? Maybe(t) : Maybe(); };
     return std::make_tuple(some(n.y), some(n.h), some(n.q), some(n.s), some(n.r));
   });
   m.def("rms_norm_bwd", [](const Tensor& dy, const Tensor& h, const Tensor& w, const Tensor& r, const Maybe& dh, bool want_x, bool want_res,
                            bool want_w, const Maybe& main_grad) {
     const auto [gx, gr, gw] = norm_backward(dy, h, w, r, of(dh), want_x, want_res, want_w, of(main_grad));
-    auto some = [](const Tensor& t) { return t.defined() ? Maybe(t) : Maybe(); };
     return std::make_tuple(some(gx), some(gr), some(gw));
   });
-  m.def("rms_norm_grad", [](const Tensor& x, const Tensor& w, const Maybe& residual, double eps, int64_t kind) {
-    return NormNode::apply(x, w, residual, eps, kind);
+  m.def("norm_checked", [](const Tensor& x, const Tensor& w, const Maybe& residual, double eps, int kind) {
+    const auto [rows, weight, res] = norm_checked(x, w, of(residual), eps, kind);
+    return std::make_tuple(rows, weight, some(res));
+  });
+  m.def("norm_call", &norm_call);
+  m.def("norm_in_shape", [](const Tensor& x, const Maybe& q, const Maybe& s, const Maybe& y, const Maybe& h) {
+    return in_shape(x, of(q), of(s), of(y), of(h));
   });
   m.def("grouped_rows", [](const Tensor& x, const Tensor& w, const Maybe& efo, const Maybe& counts, bool transposed, int64_t status,
                            int64_t host) { return grouped_rows(x, w, of(efo), of(counts), transposed, {status, host}); });
   m.def("grouped_wgrad", [](const Tensor& dy, const Tensor& x, const Maybe& efo, const Maybe& counts, int64_t E, const Maybe& main_grad,
                             int64_t status, int64_t host) {
-    const Tensor dw = grouped_wgrad(dy, x, of(efo), of(counts), E, of(main_grad), {status, host});
-    return dw.defined() ? Maybe(dw) : Maybe();
+    return some(grouped_wgrad(dy, x, of(efo), of(counts), E, of(main_grad), {status, host}));
   });
-  m.def("grouped_linear_grad", [](const Tensor& x, const Tensor& w, const Maybe& efo, const Maybe& counts, int64_t status, int64_t host) {
-    return GroupedNode::apply(x, w, efo, counts, status, host)[0];
+  m.def("grouped_checked", [](const Tensor& x, const Tensor& w, const Maybe& efo, const Maybe& counts) {
+    return grouped_checked(x, w, of(efo), of(counts));
   });
+  m.def("grouped_call", &grouped_call);
   m.def("gradient_norm", &gradient_norm);
   m.def("clip_gradients", &clip_gradients);
 }

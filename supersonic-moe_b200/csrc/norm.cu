@@ -525,7 +525,8 @@ __global__ void __launch_bounds__(32 * kNormSumWarps) rms_norm_dw_kernel(const f
   if (lane || col >= H) return;
   if (f32) {
     float* p = (float*)dw + col;
-    *p = accumulate ? (float)(*p + s) : (float)s;
+    if (accumulate) atomicAdd(p, (float)s);             // (once for each value: another stream's sums into it are not lost)
+    else *p = (float)s;
   } else {
     ((__nv_bfloat16*)dw)[col] = __float2bfloat16_rn(norm_for_bf16(s));
   }

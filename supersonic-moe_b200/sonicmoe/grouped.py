@@ -68,25 +68,16 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, efo: torch.Tensor | No
 
     Sums are f32, results bf16.  Differentiable in x and weight; a weight's gradient is added to the parameter's f32 `main_grad` where it
     has one, else returned in bf16.  Gradients cannot be differentiated again."""
-    what = "grouped_linear"
-    if x.dtype != torch.bfloat16 or x.ndim == 0:
-        raise ValueError(f"{what}: x is bf16 [rows,K], got {x.dtype} {tuple(x.shape)}")
-    if weight.dtype != torch.bfloat16 or weight.ndim not in (2, 3):
-        raise ValueError(f"{what}: the weight is bf16 [E,N,K], got {weight.dtype} {tuple(weight.shape)}")
-    E, N, K = weight.shape if weight.ndim == 3 else (1, *weight.shape)
-    if x.shape[-1] != K:
-        raise ValueError(f"{what}: x has {x.shape[-1]} columns, the weight {K}")
-    if efo is not None and x.ndim != 2:
-        raise ValueError(f"{what}: x is [rows,K] where efo is given")
-    ops.check_grouped(efo, counts, E, N, K, what)
     ops.poll_status(x.device)                 # a device-side failure of an earlier call surfaces here, without a sync
-    rows = _rows16(x if x.ndim == 2 else x.reshape(-1, K))
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
-        if ops._recorder is not None or (weight.requires_grad and getattr(_base_of(weight), "main_grad", None) is not None):
-            y = _GroupedLinear.apply(rows, weight, efo, counts)
-        else:
-            y = _host.grouped_linear_grad(rows, weight, efo, counts, *ops.failure_words(rows.device))
+    grad = torch.is_grad_enabled()
+    if not x.is_cuda:
+        _host.grouped_checked(x, weight, efo, counts)      # (which refuses it, by the arguments or for want of a GPU)
+    if ops._recorder is None and not (grad and weight.requires_grad and getattr(_base_of(weight), "main_grad", None) is not None):
+        return _host.grouped_call(x, weight, efo, counts, *ops.failure_words(x.device))
+    rows, _ = _host.grouped_checked(x, weight, efo, counts)
+    if grad and (x.requires_grad or weight.requires_grad):
+        y = _GroupedLinear.apply(rows, weight, efo, counts)
     else:
         w = _weight16(weight)
         y = ops.grouped_rows(rows, w if w.ndim == 3 else w[None], efo, counts)
-    return y if x.ndim == 2 else y.view(*x.shape[:-1], N)
+    return y if x.ndim == 2 else y.view(*x.shape[:-1], weight.shape[-2])

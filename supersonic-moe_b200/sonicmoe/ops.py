@@ -1145,12 +1145,6 @@ def block128_experts(x, idx, scores, w1, w1_s, w2, w2_s, E, I):
 
 
 # ---------------------------------------------------------------- products of bf16 rows grouped by expert
-def check_grouped(efo, counts, E, N, K, what):
-    check_segments(efo, counts, E, what)
-    if N <= 0 or K <= 0 or N % 8 or K % 8 or not 1 <= E <= 256:
-        raise ValueError(f"{what}: {E} experts of {N} x {K}: sizes are multiples of 8, 1 to 256 experts")
-
-
 @_timed
 def grouped_rows(x, w, efo=None, counts=None, transposed=False):
     """x bf16 [rows,K] (rows any multiple of 8 values apart, from a 16-byte boundary on), w bf16 [E,N,K], or `transposed` [E,K,N] -> bf16
@@ -1166,7 +1160,6 @@ def grouped_wgrad(dy, x, efo, counts, E, main_grad=None):
 
 # ---------------------------------------------------------------- the norm in front of the experts
 NORM_SCALES = {None: 0, "mx": 1, "block128": 2}
-NORM_MAX_H = 16384
 
 
 @_timed

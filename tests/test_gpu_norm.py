@@ -162,6 +162,21 @@ def test_weight_gradient_goes_to_main_grad(sonicmoe):
         check_backward(sonicmoe, x, w, res, dy, dh, 1e-6, main_grad=True)
 
 
+def test_main_grad_where_the_sum_alone_is_used(sonicmoe):
+    x, w, res, dy, dh = make(5, 136, BF, BF, F32, seed=4)
+    p = torch.nn.Parameter(w.to(DEV))
+    p.main_grad = torch.full((136,), 3.0, device=DEV)
+    calls = []
+    p._apply_backward_hook = lambda: calls.append(1)
+    gx = x.to(DEV).requires_grad_(True)
+    y, h = sonicmoe.rms_norm(gx, p, res.to(DEV))
+    h.backward(dh.to(DEV))
+    assert p.grad is None and (p.main_grad == 3).all() and calls == [1] and torch.equal(gx.grad.cpu(), dh)
+    y, h = sonicmoe.rms_norm(gx, p, res.to(DEV))
+    y.backward(dy.to(DEV))
+    assert p.grad is None and calls == [1, 1] and (p.main_grad != 3).any()
+
+
 def test_long_column_sums(sonicmoe):
     """More rows than a block adds up in one f32 sum."""
     T = 300_000
