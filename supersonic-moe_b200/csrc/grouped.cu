@@ -1,6 +1,7 @@
 // Host side of the products of bf16 rows grouped by expert.
 #include "gemm16.cuh"
 #include "gemm16_few.cuh"
+#include "gemv16.cuh"
 #include "host.h"
 #include "smoe_b200.h"
 
@@ -139,6 +140,23 @@ __global__ void __launch_bounds__(256) wgrad_sum_kernel(const float4* __restrict
   }
 }
 
+// A handful of rows without tensor cores: one an expert, or so few products that a warp's reading of x again for every two weight rows does
+// not matter (us, tensor cores / without: one row of 4096 x 4096 10.9 / 9.0, of 1024 x 1024 5.8 / 2.5, of 1000 x 720 5.2 / 2.6; 2 of 4096 x
+// 4096 11.0 / 10.6, 4 11.0 / 12.6, 8 11.1 / 21; 8 of 1024 x 1024 5.8 / 4.3; one for each of 8 experts of 1536 x 2048 11.5 / 10.1, of 4096
+// x 2048 23.2 / 23.7, two each 23.4 / 31; 8 and 16 of 128 of 1536 x 2048 11.6 / 10.2 and 23.3 / 18.3).
+static bool gemv_rows16(int64_t rows, int64_t N, int64_t K, int64_t E) {
+  return rows <= kGemvMost && (rows <= E || rows * N * K <= (int64_t)12 << 20);
+}
+
+static int gemv16(const void* x, int64_t ldx, const void* w, const int* efo, const int* counts, void* y, int64_t rows, int64_t N, int64_t K,
+                  int64_t E, cudaStream_t stream) {
+  const Gemv16Params p{(int)rows, (int)N, (int)K, (int)E, ldx, efo, counts, (const __nv_bfloat16*)x, (const __nv_bfloat16*)w, (__nv_bfloat16*)y};
+  const int64_t blocks = up16(rows * N, kGemvCols * kGemvWarps), most = (int64_t)sm_count() * 4;
+  return launch_early(gemv16_kernel, (unsigned)(blocks < most ? blocks : most), 32 * kGemvWarps, 0, 0, stream, p) == cudaSuccess
+             ? SMOE_OK
+             : SMOE_ERR_LAUNCH;
+}
+
 }  // namespace smoe
 
 using namespace smoe;
@@ -154,6 +172,8 @@ int smoe_grouped_rows(const void* x_bf16, int64_t ldx, const void* w_bf16, int w
   if (rows == 0) return SMOE_OK;
   if (!x_bf16 || !w_bf16 || !y_bf16) return SMOE_ERR_ARG;
   if (!on16(x_bf16) || !on16(w_bf16) || !on16(y_bf16)) return SMOE_ERR_ALIGN;
+  if (!w_transposed && gemv_rows16(rows, N, K, E))
+    return gemv16(x_bf16, ldx, w_bf16, efo, counts, y_bf16, rows, N, K, E, (cudaStream_t)stream);
   if (few_rows16(rows, N, E))
     return few16(x_bf16, ldx, w_bf16, efo, counts, y_bf16, rows, N, K, E, w_transposed != 0, status, pinned_host_word,
                  (cudaStream_t)stream);

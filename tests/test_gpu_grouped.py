@@ -140,6 +140,17 @@ def test_narrow_tiles(sonicmoe, rows, N, K):
     check(sonicmoe, [rows // 2, 3, 0, rows - rows // 2 - 3], N, K, main_grad=True)
 
 
+@pytest.mark.parametrize("counts", [[1], [7], [16], [0, 0, 1, 0], [1] * 16, [2, 0, 5, 0, 9], [0] * 200 + [8] + [0] * 55, [0] * 100 + [3, 0, 1] + [0] * 100 + [4]])
+@pytest.mark.parametrize("N,K", [(8, 8), (136, 72), (264, 1032), (1000, 720)])
+def test_a_handful_of_rows(sonicmoe, counts, N, K):
+    check(sonicmoe, counts, N, K)
+    if sum(counts) < 12:
+        check(sonicmoe, counts, N, K, first=1, tail=2)
+        gaps = [0] * len(counts)
+        gaps[0], gaps[-1] = 1, 1
+        check(sonicmoe, counts, N, K, gaps=gaps)
+
+
 def test_few_rows_of_a_wide_weight_are_shared_by_clusters(sonicmoe):
     for rows in (1, 15, 16, 17, 33, 64):
         for N, K in ((4096, 4096), (1024, 2048), (136, 8192), (4096, 760)):
