@@ -3,9 +3,12 @@
 //   h = x + residual (held in the residual's type)      r = 1 / sqrt(mean(h^2) + eps)      y = h r w
 //   backward, g = dy w:  dh = r (g - h r^2 mean(g h)) + the gradient that comes in for h;   dw = sum over rows of dy h r
 //
-// A row is held in registers between its one read and its one write.  bf16 results and what is quantised from them are those of 64
-// bits: the mean and r are f64 (8 conversions and 8 f64 additions a thread's 16 bytes, in the shadow of HBM), y is made in f32 and
-// looked at: where it lies within kNormNear of the border between two bf16 values it is made again in f64 (one in 7000).
+// A row is held in registers between its one read and its one write; a block stays and asks for its next row before it adds this one up.
+// bf16 results and what is quantised from them are those of 64 bits: the mean and r are f64, y is made in f32 and looked at: where it
+// lies within kNormNear of the border between two bf16 values it is made again in f64 (one in 7000).
+//   What bounds it: HBM.  8192 x 4096 bf16 with residual, rows 43 us (6.2 TB/s), rows and payload 50 (6.1 TB/s); residual in f32 64 (6.2
+//   TB/s).  Backward, 16384 x 2048 bf16 49 us (5.5 TB/s), 8192 x 4096 with h in f32 94 (5.7): the column sums of dw take the registers that
+//   would keep more rows on their way.  A single row takes 2.4 to 2.9 us.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -398,9 +401,9 @@ __global__ void __launch_bounds__(32 * kNormMaxWarps, 1) rms_norm_bwd_kernel(con
   const float inv_H = 1.f / a.H;
   int turn = 0;
   int64_t row = (int64_t)blockIdx.x * a.rows + group;
-  // A row's loads leave before the one ahead of it is added up, which by then is held as h r and g.  (Four pieces a thread: neither, for
-  // want of registers.)
-  constexpr bool AHEAD = NC == 2;
+  // A row's loads leave before the one ahead of it is added up, which by then is held as h r and g.  (Rows in f32, or four pieces a thread:
+  // neither, for want of registers; 8192 x 4096 with h in f32 109 us ahead and 94 so.)
+  constexpr bool AHEAD = NC == 2 && !HF32;
   NormVec<XF32> dy[NC];
   NormVec<HF32> h[NC], dh[NC], next_dh[AHEAD ? NC : 1];
   double next_r = 1.0;
@@ -419,10 +422,14 @@ __global__ void __launch_bounds__(32 * kNormMaxWarps, 1) rms_norm_bwd_kernel(con
   for (int flush = 0; flush < a.flushes; ++flush) {
     for (int n = 0; n < kNormRun && row < a.T; ++n, row += stride) {
       if (!AHEAD) ask(row);
+      if (AHEAD) {                                      // (the weights unpacked anew: 16 registers less)
+#pragma unroll
+        for (int c = 0; c < NC; ++c) w[c].anew();
+      }
       // r as a product of two f32, the first a power of two, so that rows of very large or very small values keep their precision
       const double r64 = next_r;
       const float pre = r64 < 1e-30 ? 0x1p-64f : r64 > 1e30 ? 0x1p64f : 1.f;
-      const float r = (float)(r64 / pre);
+      const float r = (float)(r64 * (r64 < 1e-30 ? 0x1p64 : r64 > 1e30 ? 0x1p-64 : 1.0));
       const P2 pre2 = p2(pre, pre), r2 = p2(r, r);
       P2 s2 = p2(0.f, 0.f), hr[AHEAD ? NC : 1][4], g[AHEAD ? NC : 1][4];
 #pragma unroll
