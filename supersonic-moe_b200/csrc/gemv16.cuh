@@ -11,10 +11,11 @@
 namespace smoe {
 
 constexpr int kGemvRows = 4;               // routed rows of a warp
-// weight rows of a warp (with four: one row of 4096 x 4096 9.0 -> 9.1 us, of 1024 x 1024 2.5 -> 2.8, 8 of 128 experts of 1536 x 2048 10.2 -> 10.8)
+// weight rows of a warp (with four: one row of 1024 x 1024 2.5 -> 2.8 us, 8 of 128 experts of 1536 x 2048 10.2 -> 10.8)
 constexpr int kGemvCols = 2;
 constexpr int kGemvMost = 16;              // rows of a call
 constexpr int kGemvWarps = 8;
+constexpr int kGemvBlocks = 4;             // of an SM at a time (three: one row of 4096 x 4096 8.2 -> 9.1 us, of 8192 x 8192 23.7 -> 26.1)
 constexpr int kGemvAhead = 4;              // 16-byte pieces of a weight row on their way
 
 struct Gemv16Params {
@@ -81,7 +82,7 @@ __device__ __forceinline__ void gemv_task(const Gemv16Params& p, const uint4* w,
   }
 }
 
-__global__ void __launch_bounds__(32 * kGemvWarps) gemv16_kernel(const Gemv16Params p) {
+__global__ void __launch_bounds__(32 * kGemvWarps, kGemvBlocks) gemv16_kernel(const Gemv16Params p) {
   // Up to four rows of an expert each, and runs of rows that are nobody's, found by a thread an expert.  The units are put in one order,
   // since blocks divide them by their places; that of the runs says nothing.
   __shared__ int n_units, n_gaps, found_e[kGemvMost], found_row[kGemvMost], found_live[kGemvMost];

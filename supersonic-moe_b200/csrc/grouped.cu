@@ -141,9 +141,10 @@ __global__ void __launch_bounds__(256) wgrad_sum_kernel(const float4* __restrict
 }
 
 // A handful of rows without tensor cores: one an expert, or so few products that a warp's reading of x again for every two weight rows does
-// not matter (us, tensor cores / without: one row of 4096 x 4096 10.9 / 9.0, of 1024 x 1024 5.8 / 2.5, of 1000 x 720 5.2 / 2.6; 2 of 4096 x
-// 4096 11.0 / 10.6, 4 11.0 / 12.6, 8 11.1 / 21; 8 of 1024 x 1024 5.8 / 4.3; one for each of 8 experts of 1536 x 2048 11.5 / 10.1, of 4096
-// x 2048 23.2 / 23.7, two each 23.4 / 31; 8 and 16 of 128 of 1536 x 2048 11.6 / 10.2 and 23.3 / 18.3).
+// not matter (us, tensor cores / without: one row of 4096 x 4096 10.9 / 8.2, of 8192 x 8192 26.0 / 23.7, of 1024 x 1024 5.8 / 2.7, of 1000 x
+// 720 5.2 / 2.6; of 4096 x 4096 2 rows 11.0 / 10.6, 4 11.0 / 12.6, 8 11.1 / 21; 8 of 1024 x 1024 5.8 / 4.3; one for each of 8 experts of 4096
+// x 2048 23.2 / 23.6, two each 23.4 / 31; of 128 experts of 1536 x 2048 8 rows 11.7 / 11.8, all of one expert 10.2 / 6.9, 16 23.3 / 18.9, of
+// 2048 x 768 7.2 / 7.3 and 11.2 / 11.9).
 static bool gemv_rows16(int64_t rows, int64_t N, int64_t K, int64_t E) {
   return rows <= kGemvMost && (rows <= E || rows * N * K <= (int64_t)12 << 20);
 }
@@ -151,7 +152,7 @@ static bool gemv_rows16(int64_t rows, int64_t N, int64_t K, int64_t E) {
 static int gemv16(const void* x, int64_t ldx, const void* w, const int* efo, const int* counts, void* y, int64_t rows, int64_t N, int64_t K,
                   int64_t E, cudaStream_t stream) {
   const Gemv16Params p{(int)rows, (int)N, (int)K, (int)E, ldx, efo, counts, (const __nv_bfloat16*)x, (const __nv_bfloat16*)w, (__nv_bfloat16*)y};
-  const int64_t blocks = up16(rows * N, kGemvCols * kGemvWarps), most = (int64_t)sm_count() * 4;
+  const int64_t blocks = up16(rows * N, kGemvCols * kGemvWarps), most = (int64_t)sm_count() * kGemvBlocks;
   return launch_early(gemv16_kernel, (unsigned)(blocks < most ? blocks : most), 32 * kGemvWarps, 0, 0, stream, p) == cudaSuccess
              ? SMOE_OK
              : SMOE_ERR_LAUNCH;
