@@ -37,10 +37,10 @@ __device__ __forceinline__ void gemv_dot8(float& s, const uint4& a, const uint4&
         : "+f"(s)
         : "r"(u[i]), "r"(v[i]));
 }
-// weights pass once: not kept in L1
+// Weights pass once: not kept in L1.  (No read-only load: the kernel begins while the one before it, which may write them, ends.)
 __device__ __forceinline__ uint4 gemv_load(const uint4* p) {
   uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
   return v;
 }
 

@@ -106,7 +106,7 @@ __device__ __forceinline__ double grad_block_sum(double s, double* shared) {
 // partial[block]: sum of the squares of the pieces block, block + blocks, ...
 template <int N>
 __global__ void __launch_bounds__(kGradThreads, kGradBlocks)
-grad_squares_kernel(const __grid_constant__ GradList<N> l, double* __restrict__ partial) {
+grad_squares_kernel(const __grid_constant__ GradList<N> l, double* partial) {
   __shared__ double sums[kGradThreads / 32];
   next_kernel_may_start();                   // (which waits for this one's end)
   double s = 0.0;
@@ -145,13 +145,14 @@ grad_squares_kernel(const __grid_constant__ GradList<N> l, double* __restrict__ 
   if (threadIdx.x == 0) partial[blockIdx.x] = s;
 }
 
-__device__ __forceinline__ double grad_total(const double* __restrict__ partial, int n, double* shared) {
+// (a kernel that begins while the one before ends: no pointer here promises memory that nobody writes meanwhile)
+__device__ __forceinline__ double grad_total(const double* partial, int n, double* shared) {
   double s = 0.0;
   for (int i = threadIdx.x; i < n; i += kGradThreads) s += partial[i];
   return grad_block_sum(s, shared);
 }
 
-__global__ void __launch_bounds__(kGradThreads) grad_norm_kernel(const double* __restrict__ partial, int n, float* norm) {
+__global__ void __launch_bounds__(kGradThreads) grad_norm_kernel(const double* partial, int n, float* norm) {
   __shared__ double sums[kGradThreads / 32];
   wait_for_kernel_before();
   const double s = grad_total(partial, n, sums);
@@ -161,8 +162,8 @@ __global__ void __launch_bounds__(kGradThreads) grad_norm_kernel(const double* _
 // Pieces from the last one on: what the first launch read last is what L2 still holds.
 template <int N>
 __global__ void __launch_bounds__(kGradThreads, kGradBlocks)
-grad_scale_kernel(const __grid_constant__ GradList<N> l, const double* __restrict__ partial, int n_partial,
-                  const float* __restrict__ given, double max_norm, float* norm) {
+grad_scale_kernel(const __grid_constant__ GradList<N> l, const double* partial, int n_partial,
+                  const float* given, double max_norm, float* norm) {
   __shared__ double sums[kGradThreads / 32];
   wait_for_kernel_before();
   const double total = given ? (double)*given : sqrt(grad_total(partial, n_partial, sums));

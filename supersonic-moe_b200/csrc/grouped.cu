@@ -120,7 +120,7 @@ static int wgrad_split16(int64_t N, int64_t K, int64_t rows, int64_t E) {
 }
 
 // out = (out +) the sum of `split` partial sums, each `fours` of four values
-__global__ void __launch_bounds__(256) wgrad_sum_kernel(const float4* __restrict__ part, int split, int64_t fours, void* out, int bf16,
+__global__ void __launch_bounds__(256) wgrad_sum_kernel(const float4* part, int split, int64_t fours, void* out, int bf16,
                                                         int accumulate) {
   wait_for_kernel_before();
   for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < fours; i += (int64_t)gridDim.x * blockDim.x) {

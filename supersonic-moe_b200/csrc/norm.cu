@@ -512,7 +512,7 @@ __global__ void __launch_bounds__(32 * kNormMaxWarps, 1) rms_norm_bwd_kernel(con
 
 // dw[col] (+)= the sum of its column, 32 columns a block
 constexpr int kNormSumWarps = 32;
-__global__ void __launch_bounds__(32 * kNormSumWarps) rms_norm_dw_kernel(const float* __restrict__ part, int64_t n, int H, void* dw,
+__global__ void __launch_bounds__(32 * kNormSumWarps) rms_norm_dw_kernel(const float* part, int64_t n, int H, void* dw,
                                                                          int f32, int accumulate) {
   __shared__ double sums[kNormSumWarps][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;

@@ -192,3 +192,105 @@ def test_a_captured_step(sonicmoe):
             assert torch.equal(a, b)
         # (the weighted sum is torch's, whose order varies)
         assert relative(outs[0], want[0]) < 2.0 ** -7
+
+
+def calls(m, rows):
+    """The calls whose kernels are made ready while what is ahead of them ends, each as the first of its kind behind it."""
+    x, w, dy = randn(rows, 136, seed=1), randn(3, 264, 136, seed=2), randn(rows, 264, seed=3)
+    efo = torch.tensor([0, rows // 2, rows // 2, rows], dtype=torch.int32, device=DEV)
+    grads, outs, norm = [randn(500, 33, seed=4), randn(7, seed=5)], [torch.empty(500, 33, device=DEV), torch.empty(7, device=DEV)], torch.full(
+        (), 40.0, device=DEV)
+    return [(x, lambda: [m.grouped_linear(x, w, efo)]), (dy, lambda: [m.ops.grouped_rows(dy, w, efo, None, True)]),
+            (dy, lambda: [m.ops.grouped_wgrad(dy, x, efo, None, 3)]),
+            (grads[0], lambda: [m.clip_gradients(grads, 10.0, norm=norm, out=outs), *outs]), (grads[0], lambda: [m.gradient_norm(grads)])]
+
+
+@pytest.mark.parametrize("rows", [3, 60, 3000])
+@pytest.mark.parametrize("ahead", ["copy", "join", "copy of another stream", "fill"])
+def test_calls_right_behind_what_makes_their_input(sonicmoe, rows, ahead):
+    """A copy, a kernel of another stream, a fill: eager and captured, the call sees what they leave."""
+    m = sonicmoe
+    for value, call in calls(m, rows):
+        fresh = [torch.randn(value.shape, generator=torch.Generator(device=DEV).manual_seed(i), device=DEV).to(BF) for i in range(3)]
+        source, scratch = fresh[0].clone(), torch.empty(1 << 24, device=DEV)
+        other = torch.cuda.Stream()
+
+        def run():
+            here = torch.cuda.current_stream()
+            if ahead == "copy":
+                value.copy_(source)
+            elif ahead == "fill":
+                value.zero_()
+                value.add_(source)
+            else:
+                other.wait_stream(here)
+                with torch.cuda.stream(other):
+                    scratch.fill_(1.0)                        # takes a while
+                    if ahead == "join":
+                        torch.mul(source, 1, out=value)
+                    else:
+                        value.copy_(source)
+                here.wait_stream(other)
+            return call()
+
+        wants = []
+        for f in fresh[:2]:
+            value.copy_(f)
+            torch.cuda.synchronize()
+            wants.append([v.clone() for v in call()])
+        for f, want in zip(fresh[:2], wants):
+            source.copy_(f)
+            value.fill_(float("nan"))
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(run(), want))
+        value.copy_(fresh[2])
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = run()
+        for f, want in zip(fresh[:2], wants):
+            source.copy_(f)
+            value.fill_(float("nan"))
+            torch.cuda.synchronize()
+            graph.replay()
+            assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+def test_two_streams_at_once(sonicmoe):
+    """Calls of two streams overlap: each has outputs and workspaces of its own."""
+    m = sonicmoe
+    sets = [calls(m, rows) for rows in (2500, 40)]
+    wants = [[[v.clone() for v in call()] for _, call in s] for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [[] for _ in sets]
+    for turn in range(20):
+        for i, (stream, s) in enumerate(zip(streams, sets)):
+            with torch.cuda.stream(stream):
+                got[i].append([[v.clone() for v in call()] for _, call in s])
+    torch.cuda.synchronize()
+    for want, runs in zip(wants, got):
+        for run in runs:
+            assert all(torch.equal(a, b) for x, y in zip(run, want) for a, b in zip(x, y))
+
+
+def test_the_graph_kept_for_a_second_backward_pass(sonicmoe):
+    m = sonicmoe
+    x, w, g = (t.requires_grad_(True) for t in (randn(50, 136, seed=1), randn(264, 136, seed=2), randn(136, seed=3)))
+    y = m.grouped_linear(m.rms_norm(x, g), w)
+    dy = randn(50, 264, seed=4)
+    first = torch.autograd.grad(y, (x, w, g), dy, retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(first, torch.autograd.grad(y, (x, w, g), dy)))
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(y, (x, w, g), dy)
+
+
+def test_one_weight_for_all_experts(sonicmoe):
+    """A weight that is expanded over the experts gets the sum of their gradients."""
+    m = sonicmoe
+    x, w, dy = randn(90, 72, seed=1), randn(1, 80, 72, seed=2).requires_grad_(True), randn(90, 80, seed=3)
+    efo = torch.tensor([0, 40, 47, 90], dtype=torch.int32, device=DEV)
+    y = m.grouped_linear(x, w.expand(3, 80, 72), efo)
+    dw, = torch.autograd.grad(y, w, dy)
+    parts = sum((dy[a:b].double().T @ x[a:b].double() for a, b in ((0, 40), (40, 47), (47, 90))))
+    assert torch.equal(y, m.grouped_linear(x, w.detach()[0].expand(3, 80, 72), efo)) and relative(dw[0], parts) < 2.0 ** -7
