@@ -4,7 +4,7 @@
 //
 // One launch adds up squares, one more scales: the list travels in the launch's parameters, so that a captured graph keeps it and
 // nothing is uploaded, and every block of the second launch adds the first one's partial sums up again instead of waiting for a
-// kernel between the two.  Bound by HBM: f32 sums of 32 values, f64 beyond, cost less than their loads.
+// kernel between the two.  Bound by HBM: f32 sums of eight values, f64 beyond, cost less than their loads.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>

@@ -398,14 +398,32 @@ Tensor gradient_norm(const py::object& items) {
   return n;
 }
 
-// starts of what holds values, each once
-void once(const std::vector<smoe_gradient>& t, const char* which) {
-  std::vector<const void*> at;
-  at.reserve(t.size());
-  for (const auto& g : t)
-    if (g.numel) at.push_back(g.out);
-  std::sort(at.begin(), at.end());
-  TORCH_CHECK_VALUE(std::adjacent_find(at.begin(), at.end()) == at.end(), "clip_gradients: one of the ", which, " is given twice");
+// Memory of one tensor, of a strided one its first value
+struct Span {
+  uintptr_t from, to;
+  size_t i;
+};
+Span span(const Tensor& t, size_t i) {
+  const uintptr_t at = (uintptr_t)t.data_ptr();
+  return {at, at + (t.is_contiguous() ? (size_t)t.numel() : 1) * t.element_size(), i};
+}
+// of what is written, in its order in memory, each once
+std::vector<Span> written_spans(const std::vector<Tensor>& ts, const char* which) {
+  std::vector<Span> at;
+  at.reserve(ts.size());
+  for (size_t i = 0; i < ts.size(); ++i)
+    if (ts[i].numel()) at.push_back(span(ts[i], i));
+  std::sort(at.begin(), at.end(), [](const Span& a, const Span& b) { return a.from < b.from; });
+  for (size_t i = 1; i < at.size(); ++i)
+    TORCH_CHECK_VALUE(at[i - 1].to <= at[i].from, "clip_gradients: one of the ", which, " is given twice, or overlaps another");
+  return at;
+}
+// what is read, and written by one at most: the tensor itself
+bool read_apart(const Span& in, const std::vector<Span>& written, bool itself) {
+  auto w = std::upper_bound(written.begin(), written.end(), in.from, [](uintptr_t at, const Span& s) { return at < s.to; });
+  for (; w != written.end() && w->from < in.to; ++w)
+    if (!itself || w->i != in.i || w->from != in.from || w->to != in.to) return false;
+  return true;
 }
 
 void written(const std::vector<Tensor>& ts) {            // autograd sees that they are others now
@@ -434,20 +452,12 @@ Tensor clip_gradients(const py::object& items, double max_norm, const Maybe& giv
                         text(grads[i].sizes()));
   }
   const auto t = table(grads, out.is_none() ? nullptr : &outs, "clip_gradients");
-  once(t, out.is_none() ? "gradients" : "outputs");
-  if (!out.is_none()) {
-    std::vector<std::pair<const void*, size_t>> at;
-    at.reserve(t.size());
-    for (size_t i = 0; i < t.size(); ++i)
-      if (t[i].numel) at.emplace_back(t[i].grad, i);
-    std::sort(at.begin(), at.end());
-    for (size_t i = 0; i < t.size(); ++i) {
-      if (!t[i].numel) continue;
-      for (auto g = std::lower_bound(at.begin(), at.end(), std::make_pair((const void*)t[i].out, (size_t)0));
-           g != at.end() && g->first == t[i].out; ++g)
-        TORCH_CHECK_VALUE(g->second == i && t[i].grad_f32 == t[i].out_f32, "clip_gradients: an output lies where another gradient does");
-    }
-  }
+  const auto spans = written_spans(out.is_none() ? before : outs, out.is_none() ? "gradients" : "outputs");
+  if (!out.is_none())
+    for (size_t i = 0; i < grads.size(); ++i)
+      TORCH_CHECK_VALUE(!grads[i].numel() || read_apart(span(grads[i], i), spans, f32(grads[i]) == f32(outs[i])),
+                        "clip_gradients: an output lies where another gradient does");
+  TORCH_CHECK_VALUE(!norm.defined() || read_apart(span(norm, 0), spans, false), "clip_gradients: the norm lies in what is written");
   on_gpu(grads[0]);
   const c10::cuda::CUDAGuard guard(grads[0].device());
   Tensor n = norm, ws;

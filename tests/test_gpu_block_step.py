@@ -294,3 +294,30 @@ def test_one_weight_for_all_experts(sonicmoe):
     dw, = torch.autograd.grad(y, w, dy)
     parts = sum((dy[a:b].double().T @ x[a:b].double() for a, b in ((0, 40), (40, 47), (47, 90))))
     assert torch.equal(y, m.grouped_linear(x, w.detach()[0].expand(3, 80, 72), efo)) and relative(dw[0], parts) < 2.0 ** -7
+
+
+def test_recorded_calls_are_the_same_calls(sonicmoe):
+    """With a recorder the calls go kernel by kernel: the same results and gradients, each launch named."""
+    m = sonicmoe
+    rows, efo = 77, torch.tensor([0, 30, 30, 61, 77], dtype=torch.int32, device=DEV)
+
+    def step():
+        x, g, w = randn(rows, 96, seed=1).requires_grad_(True), randn(96, seed=2).requires_grad_(True), randn(4, 40, 96, seed=3).requires_grad_(True)
+        res = randn(rows, 96, seed=4).float().requires_grad_(True)
+        n = m.rms_norm_quantized(x, g, res, scales="block128", with_output=True)
+        y = m.grouped_linear(n.y, w, efo)
+        grads = torch.autograd.grad([y, n.h], [x, g, res, w], [randn(rows, 40, seed=5), randn(rows, 96, seed=6).float()])
+        total = m.clip_gradients(grads, 1.0)
+        with torch.no_grad():
+            alone = m.grouped_linear(m.rms_norm(x, g), w, efo)
+        return [n.payload.view(torch.uint8), n.scales, n.y, n.h, y, *grads, total, m.gradient_norm(grads), alone]
+
+    want, record = step(), []
+    m.ops.set_recorder(record)
+    try:
+        got = step()
+    finally:
+        m.ops.set_recorder(None)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert [n for n, _, _ in record] == ["rms_norm", "grouped_rows", "grouped_rows", "grouped_wgrad", "rms_norm_bwd", "clip_gradients",
+                                         "rms_norm", "grouped_rows", "gradient_norm"]

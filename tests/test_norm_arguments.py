@@ -69,6 +69,29 @@ def test_clipping_refusals():
         sonicmoe.clip_gradients([g, torch.zeros(8)], 1.0, out=[o, o])
 
 
+def test_clipping_refuses_memory_that_it_writes_twice():
+    """Also where the tensors only overlap: the order of reads and writes would make the result."""
+    g, other = torch.zeros(64), torch.zeros(64)
+    bf = g.view(torch.bfloat16)
+    for grads, kw in (([g, g[8:16]], {}), ([g[:40], other, g[32:]], {}), ([g[:8], bf[15:]], {}), ([g.view(8, 8).T, g.view(8, 8).T], {}),
+                      ([g.view(8, 8)[:, :4], g], {}),
+                      ([other, other.clone()], dict(out=[g, g])),
+                      ([other[:8], other[8:16]], dict(out=[g[:8], g[4:12]])),
+                      ([g[:8], other[:8]], dict(out=[other[8:16], g[7:15]])),          # another gradient's end
+                      ([g[:8]], dict(out=[g[4:12]])), ([g[4:12]], dict(out=[g[:8]])),       # its own, shifted
+                      ([g[:8]], dict(out=[bf[:8]])), ([bf[:8]], dict(out=[g[:8]])), ([g[:8]], dict(out=[bf[8:16]])),
+                      ([g], dict(norm=g[3])), ([g[:8]], dict(out=[other[:8]], norm=other[7:8]))):
+        with pytest.raises(ValueError, match="twice|lies"):
+            sonicmoe.clip_gradients(grads, 1.0, **kw)
+    # beside one another, within one another's gaps, over themselves, empty ones anywhere: these pass the checks and want a GPU
+    for grads, kw in (([g[:8], g[8:]], {}), ([g.view(8, 8)[:, :4], g.view(8, 8)[:, 4:]], {}), ([g, g[8:8], g[8:8]], {}),
+                      ([g[:8], g[8:16]], dict(out=[g[:8], g[8:16]])), ([g[:8], g[8:16]], dict(out=[g[16:24], g[8:16]])),
+                      ([g[:8]], dict(norm=g[8])), ([g[:8]], dict(out=[other[:8]], norm=g[0])),
+                      ([g.view(8, 8).T], dict(out=[g.view(8, 8)]))):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            sonicmoe.clip_gradients(grads, 1.0, **kw)
+
+
 def test_c_entry_points_check_their_arguments():
     from sonicmoe._lib import lib
     SHAPE, ALIGN, ARG = 1, 2, 6
