@@ -112,6 +112,35 @@ def test_parameters_stand_for_their_gradients(sonicmoe):
     assert torch.equal(p[0].grad, kept) and p[1].grad._version > version
 
 
+class OwnAccumulator(torch.nn.Parameter):
+    """A parameter that keeps its accumulator elsewhere."""
+    @property
+    def main_grad(self):
+        return self.kept[0]
+
+
+def test_wherever_an_accumulator_is_kept(sonicmoe):
+    def parameter(cls=torch.nn.Parameter):
+        p = cls(torch.zeros(40, device=DEV))
+        p.grad = torch.full_like(p, 100.0)
+        return p
+
+    plain, none, attribute, own, frozen = parameter(), parameter(), parameter(), parameter(OwnAccumulator), parameter()
+    none.main_grad = None
+    attribute.main_grad = torch.full((40,), 2.0, device=DEV)
+    own.kept = [torch.full((40,), 3.0, device=DEV)]
+    frozen.grad = None
+    buffer = torch.full((40,), 4.0, device=DEV).requires_grad_(False)
+    items = [plain, none, attribute, own, frozen, buffer]
+    total = (40 * (2 * 100.0 ** 2 + 4 + 9 + 16)) ** 0.5
+    assert abs(float(sonicmoe.gradient_norm(items)) / total - 1) <= NORM
+    versions = [t._version for t in (plain.grad, attribute.main_grad, own.kept[0], buffer)]
+    assert abs(float(sonicmoe.clip_gradients(iter(items), total / 2)) / total - 1) <= NORM
+    for t, v, was in zip((plain.grad, attribute.main_grad, own.kept[0], buffer), (100.0, 2.0, 3.0, 4.0), versions):
+        assert torch.allclose(t, torch.full_like(t, v / 2), rtol=8 * U) and t._version == was + 1
+    assert abs(float(sonicmoe.gradient_norm(attribute)) / (160 ** 0.5 / 2) - 1) <= NORM + 8 * U      # alone, without a list
+
+
 def test_a_given_norm(sonicmoe):
     g = make([(1000,), (7, 9)], (F32, BF))
     dev = on(g)
