@@ -39,7 +39,7 @@ def _host_command():
             + [a for i in (INCLUDE, os.path.join(at, "include"), os.path.join(at, "include", "torch", "csrc", "api", "include"),
                            sysconfig.get_paths()["include"], "/usr/local/cuda/include") for a in ("-I", i)]
             + [HOST_SOURCE, "-o", HOST_OUT, "-L", os.path.dirname(OUT), "-lsmoe_b200", "-L", os.path.join(at, "lib"), "-ltorch_python",
-               "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"])
+               "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"])
 
 
 def build(force=False, verbose=False):

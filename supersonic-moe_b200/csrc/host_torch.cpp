@@ -1,10 +1,9 @@
 // The host side of the operators around the experts, on torch tensors: outputs from the caching allocator, the current stream, autograd
 // nodes.  What Python and ctypes take for it is longer than the kernels of a small batch, or than the look at a list of a few hundred
-// gradients (us a call through Python / here: one decoded token's norm 21 / 11, norm with its backward pass 114 / 68, the norm of 300
-// gradients 205 / 28).  The kernels are those of the C ABI; nothing here computes.
+// gradients (us a call through Python / here: one decoded token's norm 21 / 10, norm with its backward pass 114 / 63, the norm of 300
+// gradients 205 / 22).  The kernels are those of the C ABI; nothing here computes.
 #include <ATen/core/Tensor.h>
-#include <ATen/ops/empty.h>
-#include <ATen/ops/empty_like.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <ATen/ops/zeros.h>
 #include <ATen/ops/zeros_like.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -50,6 +49,11 @@ void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 Tensor of(const Maybe& t) { return t ? *t : Tensor(); }
 int64_t distance(const Tensor& rows) { return rows.size(0) > 1 ? rows.stride(0) : rows.size(1); }
 
+// (not through the dispatcher, which takes 0.3 us: a token's norm with payload 8.4 us of the host, 7.4 so)
+Tensor fresh(at::IntArrayRef size, at::ScalarType type, const Tensor& like) {
+  return Tensor(at::detail::empty_cuda(size, type, like.device(), std::nullopt));
+}
+
 void* stream() { return c10::cuda::getCurrentCUDAStream().stream(); }
 
 void same_gpu(const char* what, const Tensor& first, std::initializer_list<const Tensor*> others) {
@@ -81,18 +85,17 @@ Norm norm(const Tensor& x, const Tensor& w, const Tensor& residual, double eps, 
   same_gpu("rms_norm", x, {&w, &residual});
   const c10::cuda::CUDAGuard guard(x.device());
   const int64_t T = x.size(0), H = x.size(1);
-  const auto o = x.options().requires_grad(false);
   Norm n;
-  if (with_y || !kind) n.y = at::empty({T, H}, o);
-  if (residual.defined()) n.h = at::empty({T, H}, residual.options().requires_grad(false));
-  if (keep) n.r = at::empty({T}, o.dtype(at::kDouble));
+  if (with_y || !kind) n.y = fresh({T, H}, x.scalar_type(), x);
+  if (residual.defined()) n.h = fresh({T, H}, residual.scalar_type(), x);
+  if (keep) n.r = fresh({T}, at::kDouble, x);
   if (kind == 1) {
-    n.q = at::empty({T, H}, o.dtype(at::kFloat8_e4m3fn));
-    n.s = at::empty({T, H / kMxGroup}, o.dtype(at::kByte));
+    n.q = fresh({T, H}, at::kFloat8_e4m3fn, x);
+    n.s = fresh({T, H / kMxGroup}, at::kByte, x);
   } else if (kind == 2) {
-    n.q = at::empty({T, (H + 15) / 16 * 16}, o.dtype(at::kFloat8_e4m3fn));
+    n.q = fresh({T, (H + 15) / 16 * 16}, at::kFloat8_e4m3fn, x);
     if (H % 16) n.q = n.q.narrow(1, 0, H);
-    n.s = at::empty({T, (H + kBlock - 1) / kBlock}, o.dtype(at::kFloat));
+    n.s = fresh({T, (H + kBlock - 1) / kBlock}, at::kFloat, x);
   }
   check(smoe_rms_norm(x.data_ptr(), f32(x), distance(x), ptr(residual), residual.defined() && f32(residual),
                       residual.defined() ? distance(residual) : H, w.data_ptr(), f32(w), T, H, eps, ptr(n.y), ptr(n.h),
@@ -107,13 +110,12 @@ std::tuple<Tensor, Tensor, Tensor> norm_backward(const Tensor& dy, const Tensor&
   same_gpu("rms_norm_bwd", dy, {&h, &w, &r, &dh, &main_grad});
   const c10::cuda::CUDAGuard guard(dy.device());
   const int64_t T = dy.size(0), H = dy.size(1);
-  const auto o = dy.options().requires_grad(false);
   Tensor gx, gr, gw, ws;
-  if (want_x) gx = at::empty({T, H}, o);
-  if (want_res) gr = at::empty({T, H}, o.dtype(h.scalar_type()));
+  if (want_x) gx = fresh({T, H}, dy.scalar_type(), dy);
+  if (want_res) gr = fresh({T, H}, h.scalar_type(), dy);
   if (want_w) {
-    gw = main_grad.defined() ? main_grad : at::empty({H}, o.dtype(w.scalar_type()));
-    ws = at::empty({smoe_rms_norm_bwd_workspace(T, H)}, o.dtype(at::kByte));
+    gw = main_grad.defined() ? main_grad : fresh({H}, w.scalar_type(), dy);
+    ws = fresh({smoe_rms_norm_bwd_workspace(T, H)}, at::kByte, dy);
   }
   check(smoe_rms_norm_bwd(dy.data_ptr(), f32(dy), h.data_ptr(), f32(h), distance(h), w.data_ptr(), f32(w), (const double*)r.data_ptr(),
                           ptr(dh), T, H, ptr(gx), ptr(gr), ptr(gw), want_w && f32(gw), main_grad.defined(), ptr(ws), stream()),
@@ -229,7 +231,7 @@ Tensor grouped_rows(const Tensor& x, const Tensor& w, const Tensor& efo, const T
   same_gpu("grouped_rows", x, {&w, &efo, &counts});
   const c10::cuda::CUDAGuard guard(x.device());
   const int64_t rows = x.size(0), K = x.size(1), E = w.size(0), N = w.size(transposed ? 2 : 1);
-  Tensor y = at::empty({rows, N}, x.options().requires_grad(false));
+  Tensor y = fresh({rows, N}, at::kBFloat16, x);
   check(smoe_grouped_rows(x.data_ptr(), distance(x), w.data_ptr(), transposed, (const int32_t*)ptr(efo), (const int32_t*)ptr(counts),
                           y.data_ptr(), rows, N, K, E, (int32_t*)at.status, (int32_t*)at.host, stream()),
         "grouped_rows");
@@ -242,13 +244,12 @@ Tensor grouped_wgrad(const Tensor& dy, const Tensor& x, const Tensor& efo, const
   same_gpu("grouped_wgrad", dy, {&x, &efo, &counts, &main_grad});
   const c10::cuda::CUDAGuard guard(dy.device());
   const int64_t rows = dy.size(0), N = dy.size(1), K = x.size(1);
-  const auto o = dy.options().requires_grad(false);
   const bool add = main_grad.defined();
   // (what is added leaves in pieces that start on 16 bytes)
   const bool direct = add && (uintptr_t)main_grad.data_ptr() % 16 == 0;
-  Tensor dw = direct ? main_grad : add ? at::zeros({E, N, K}, o.dtype(at::kFloat)) : at::empty({E, N, K}, o);
+  Tensor dw = direct ? main_grad : add ? at::zeros({E, N, K}, dy.options().dtype(at::kFloat).requires_grad(false)) : fresh({E, N, K}, at::kBFloat16, dy);
   const int64_t bytes = smoe_grouped_wgrad_workspace(N, K, rows, E);
-  const Tensor ws = bytes > 0 ? at::empty({bytes}, o.dtype(at::kByte)) : Tensor();
+  const Tensor ws = bytes > 0 ? fresh({bytes}, at::kByte, dy) : Tensor();
   check(smoe_grouped_wgrad(dy.data_ptr(), distance(dy), x.data_ptr(), distance(x), (const int32_t*)ptr(efo), (const int32_t*)ptr(counts),
                            dw.data_ptr(), N, K, rows, E, !add, add, ptr(ws), (int32_t*)at.status, (int32_t*)at.host, stream()),
         "grouped_wgrad");
@@ -361,7 +362,7 @@ struct Tensors {
 Tensors gradients(const py::handle items, const char* what) {
   static PyTypeObject* const parameter = (PyTypeObject*)py::object(py::module_::import("torch.nn").attr("Parameter")).release().ptr();
   static PyObject* const name = PyUnicode_InternFromString("main_grad");
-  // (an attribute that is missing is dear to ask for: 300 parameters with .grad only 150 us, with a look into their dictionaries 30)
+  // (an attribute that is missing is dear to ask for: 300 parameters with .grad only 150 us, with a look into their dictionaries 26)
   const bool in_dict = !PyObject_HasAttr((PyObject*)parameter, name);
   auto main_grad = [&](PyObject* o) -> py::object {
     if (!in_dict || Py_TYPE(o) != parameter) return py::getattr(o, name, py::none());
@@ -415,9 +416,9 @@ std::vector<smoe_gradient> table(Tensors& grads, const Tensors* outs, const char
 
 void on_gpu(const Tensor& t) { TORCH_CHECK(t.is_cuda(), "sonicmoe kernels need CUDA tensors (no CPU fallback)"); }
 Tensor gradient_workspace(const Tensor& like, size_t n) {
-  return at::empty({smoe_gradient_workspace((int64_t)n)}, at::TensorOptions().device(like.device()).dtype(at::kByte));
+  return fresh({smoe_gradient_workspace((int64_t)n)}, at::kByte, like);
 }
-Tensor gradient_scalar(const Tensor& like) { return at::empty({}, at::TensorOptions().device(like.device()).dtype(at::kFloat)); }
+Tensor gradient_scalar(const Tensor& like) { return fresh({}, at::kFloat, like); }
 
 Tensor gradient_norm(const py::object& items) {
   auto grads = gradients(items, "gradient_norm");
