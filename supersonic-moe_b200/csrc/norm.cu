@@ -167,12 +167,14 @@ struct NormRow {
   }
 };
 
-// over the warps of a row, in one order; `group` of the block's rows it is, each with sums and a barrier of its own
-template <typename T>
-__device__ __forceinline__ T norm_sum(T s, int warps, int group, T* shared) {
+// over the threads of a row, in one order; `group` of the block's rows it is, each of several warps with sums and a barrier of its own
+template <bool NARROW, typename T>
+__device__ __forceinline__ T norm_sum(T s, int threads, int group, T* shared) {
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-  if (warps == 1) return s;
+  for (int d = 16; d > 0; d >>= 1)
+    if (!NARROW || d < threads) s += __shfl_xor_sync(0xffffffffu, s, d);
+  if (NARROW || threads == 32) return s;
+  const int warps = threads >> 5;
   if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = s;
   asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(warps * 32) : "memory");
   shared += group * warps;
@@ -211,7 +213,7 @@ __device__ __forceinline__ float norm_for_bf16(double d) {
 struct NormArgs {
   const void *x, *res, *w;
   int64_t ldx, ldr, T;
-  int H, warps, rows;                    // warps of a row, rows of a block
+  int H, lanes, rows;                    // threads of a row, rows of a block
   int w_f32, vec, apart;                 // vec: see NormRow
   double eps, inv_H;
   void *y, *h;                           // null: not written
@@ -223,32 +225,43 @@ struct NormArgs {
 
 enum NormQuant : int { NORM_PLAIN = 0, NORM_MX = 1, NORM_BLOCK128 = 2 };
 
+// Blocks an SM has at a time: two where h is f32, for the registers of the next row (us, two / three without it: 8192 x 4096 with residual
+// in f32, rows and payload 69 / 71, 131072 x 128 39 / 45, 3001 x 1000 7.4 / 6.7, for which two take three turns instead of two).
+constexpr int norm_blocks(bool h_f32, int pieces) { return pieces > 2 ? 1 : h_f32 ? 2 : 3; }
+
 // RES: 0 none, 1 of x's type, 2 f32 (beside bf16).  A block stays and takes rows in turn, several at a time, each by threads of its own;
-// a row's loads leave before the one ahead of it is added up.
-template <bool XF32, int RES, int QUANT, int NC, bool WF32, bool VEC>
-__global__ void __launch_bounds__(NC == 2 ? 256 : 512, NC == 2 ? 3 : 1) rms_norm_kernel(const NormArgs a) {
+// a row's loads leave before the one ahead of it is added up.  NARROW: several rows a warp, of which those behind the last one have no
+// columns.
+template <bool XF32, int RES, int QUANT, int NC, bool WF32, bool VEC, bool NARROW>
+__global__ void __launch_bounds__(NC == 2 ? 256 : 512, norm_blocks(XF32 || RES == 2, NC)) rms_norm_kernel(const NormArgs a) {
   constexpr bool HF32 = XF32 || RES == 2;
-  constexpr bool AHEAD = VEC && !HF32;                  // (rows in f32 would need more registers)
+  // (x and residual both in f32 would need more registers: 8192 x 2048 53 us ahead and 44 so)
+  constexpr bool AHEAD = VEC && (NC == 2 ? !(XF32 && RES) : !HF32);
   __shared__ double sums[2][kNormMaxWarps];
   const int lane = threadIdx.x & 31;
-  const int group = threadIdx.x / (a.warps * 32);
-  const NormRow<VEC> at{(int)threadIdx.x - group * a.warps * 32, a.warps * 32, a.H, QUANT == NORM_PLAIN && a.apart};
+  const int group = threadIdx.x / a.lanes, in_warp = NARROW ? lane / a.lanes : 0;
+  NormRow<VEC> at{(int)threadIdx.x - group * a.lanes, a.lanes, a.H, QUANT == NORM_PLAIN && a.apart};
   const int64_t stride = (int64_t)gridDim.x * a.rows;
-  int64_t row = (int64_t)blockIdx.x * a.rows + group;
-  if (row >= a.T) return;                               // all threads of the row
+  int64_t first = (int64_t)blockIdx.x * a.rows + group - in_warp;   // of the rows of this warp
+  if (first >= a.T) return;
   NormVec<XF32> x[NC];
   NormVec<HF32> res[RES ? NC : 1];
-  auto ask = [&](int64_t of) {
-    if (of >= a.T) return;
-    at.load(x, a.x, of * a.ldx);
-    if constexpr (RES != 0) at.load(res, a.res, of * a.ldr);
+  auto ask = [&](int64_t first) {
+    if (first >= a.T) return;
+    const int64_t of = first + in_warp;
+    NormRow<VEC> in = at;
+    in.H = !NARROW || of < a.T ? a.H : 0;
+    in.load(x, a.x, of * a.ldx);
+    if constexpr (RES != 0) in.load(res, a.res, of * a.ldr);
   };
-  if (AHEAD) ask(row);
+  if (AHEAD) ask(first);
   NormVec<WF32> w[NC];
   at.load(w, a.w, 0);
   int turn = 0;
-  for (; row < a.T; row += stride) {
-  if (!AHEAD) ask(row);
+  for (; first < a.T; first += stride) {
+  if (!AHEAD) ask(first);
+  const int64_t row = first + in_warp;
+  if (NARROW) at.H = row < a.T ? a.H : 0;
   NormVec<HF32> h[NC];
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
@@ -262,7 +275,7 @@ __global__ void __launch_bounds__(NC == 2 ? 256 : 512, NC == 2 ? 3 : 1) rms_norm
       }
     }
   }
-  if (AHEAD) ask(row + stride);
+  if (AHEAD) ask(first + stride);
   if constexpr (RES != 0) {
 #pragma unroll
     for (int c = 0; c < NC; ++c) at.store(h[c], a.h, row * a.H, c);
@@ -278,12 +291,32 @@ __global__ void __launch_bounds__(NC == 2 ? 256 : 512, NC == 2 ? 3 : 1) rms_norm
       s1 = fma(q, q, s1);
     }
   }
-  const double r64 = norm_rsqrt(norm_sum<double>(s0 + s1, a.warps, group, sums[turn]) * a.inv_H + a.eps);
+  const double r64 = norm_rsqrt(norm_sum<NARROW>(s0 + s1, a.lanes, group, sums[turn]) * a.inv_H + a.eps);
   turn ^= 1;                                            // the next row's sums do not wait for this one's readers
   const float r = (float)r64;
-  if (a.rstd && at.t == 0) a.rstd[row] = r64;
+  if (a.rstd && at.t == 0 && (!NARROW || at.H)) a.rstd[row] = r64;
   const bool far = !(r64 > 1e-30 && r64 < 1e30);        // r in f32 would not have its full precision
   const P2 r2 = p2(r, r);
+  NormVec<false> kept[NARROW && QUANT == NORM_BLOCK128 ? NC : 1];
+  // y of columns from col on, whose group's largest magnitude is m
+  auto quantise128 = [&](const NormVec<false>& y, uint32_t m, int col, bool first_of_group) {
+    m &= 0x7FFF7FFFu;
+    const float amax = fmaxf(fmaxf(__uint_as_float(m << 16), __uint_as_float(m & 0xFFFF0000u)), kAmaxFloor);
+    // one division a lane, of either kind
+    const float quotient = ((lane & 1) ? kE4m3Max : amax) / ((lane & 1) ? amax : kE4m3Max);
+    const float qs = __shfl_sync(0xffffffffu, quotient, lane | 1);
+    float2 b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) b[i] = p2_get(y.pair(i) * p2(qs, qs));
+    if (col < at.H) {
+      *reinterpret_cast<uint2*>(a.q + row * a.pitch + col) =
+          make_uint2(q_pack4(b[0].x, b[0].y, b[1].x, b[1].y), q_pack4(b[2].x, b[2].y, b[3].x, b[3].y));
+      if (first_of_group) ((float*)a.s)[row * ((a.H + 127) >> 7) + (col >> 7)] = quotient;
+    }
+  };
+  auto largest = [](const NormVec<false>& y) {
+    return q_max_abs_bf16x2(q_max_abs_bf16x2(y.w[0], y.w[1]), q_max_abs_bf16x2(y.w[2], y.w[3]));
+  };
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
     const int col = at.col(c);
@@ -331,36 +364,38 @@ __global__ void __launch_bounds__(NC == 2 ? 256 : 512, NC == 2 ? 3 : 1) rms_norm
       for (int i = 0; i < 4; ++i) y.set(i, v[i]);
       if (QUANT == NORM_PLAIN || a.y) at.store(y, a.y, row * a.H, c);
       if constexpr (QUANT == NORM_MX) {                 // four lanes a group
-        uint32_t m = q_max_abs_bf16x2(q_max_abs_bf16x2(y.w[0], y.w[1]), q_max_abs_bf16x2(y.w[2], y.w[3]));
+        uint32_t m = largest(y);
         m = q_max_abs_bf16x2(m, __shfl_xor_sync(0xffffffffu, m, 1));
         m = q_max_abs_bf16x2(m, __shfl_xor_sync(0xffffffffu, m, 2));
         m &= 0x7FFF7FFFu;
         const int e = q_e8m0_of(fmaxf(fmaxf(0.f, __uint_as_float(m << 16)), __uint_as_float(m & 0xFFFF0000u)));
         const uint32_t qs = (__float_as_uint(q_scale_of(e)) >> 16) * 0x10001u;      // a power of two is a bf16
-        if (col < a.H) {
+        if (col < at.H) {
           *reinterpret_cast<uint2*>(a.q + row * a.pitch + col) =
               make_uint2(q_pack4_scaled(y.w[0], y.w[1], qs, qs), q_pack4_scaled(y.w[2], y.w[3], qs, qs));
           if ((lane & 3) == 0) ((uint8_t*)a.s)[row * (a.H >> 5) + (col >> 5)] = (uint8_t)e;
         }
       }
-      if constexpr (QUANT == NORM_BLOCK128) {           // sixteen
-        uint32_t m = q_max_abs_bf16x2(q_max_abs_bf16x2(y.w[0], y.w[1]), q_max_abs_bf16x2(y.w[2], y.w[3]));
+      if constexpr (QUANT == NORM_BLOCK128 && NARROW) kept[c] = y;
+      if constexpr (QUANT == NORM_BLOCK128 && !NARROW) {      // sixteen
+        uint32_t m = largest(y);
 #pragma unroll
         for (int d = 1; d < 16; d <<= 1) m = q_max_abs_bf16x2(m, __shfl_xor_sync(0xffffffffu, m, d));
-        m &= 0x7FFF7FFFu;
-        const float amax = fmaxf(fmaxf(__uint_as_float(m << 16), __uint_as_float(m & 0xFFFF0000u)), kAmaxFloor);
-        // one division a lane, of either kind
-        const float quotient = ((lane & 1) ? kE4m3Max : amax) / ((lane & 1) ? amax : kE4m3Max);
-        const float qs = __shfl_sync(0xffffffffu, quotient, lane | 1);
-        float2 b[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) b[i] = p2_get(y.pair(i) * p2(qs, qs));
-        if (col < a.H) {
-          *reinterpret_cast<uint2*>(a.q + row * a.pitch + col) =
-              make_uint2(q_pack4(b[0].x, b[0].y, b[1].x, b[1].y), q_pack4(b[2].x, b[2].y, b[3].x, b[3].y));
-          if ((lane & 15) == 0) ((float*)a.s)[row * ((a.H + 127) >> 7) + (col >> 7)] = quotient;
-        }
+        quantise128(y, m, col, (lane & 15) == 0);
       }
+    }
+  }
+  if constexpr (QUANT == NORM_BLOCK128 && NARROW) {     // sixteen lanes, or all of a row's two pieces
+    const bool one = a.lanes < 16;
+    uint32_t both = largest(kept[0]);
+    if (one) both = q_max_abs_bf16x2(both, largest(kept[NC - 1]));
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      uint32_t m = c == 0 || one ? both : largest(kept[c]);
+#pragma unroll
+      for (int d = 1; d < 16; d <<= 1)
+        if (d < a.lanes) m = q_max_abs_bf16x2(m, __shfl_xor_sync(0xffffffffu, m, d));
+      quantise128(kept[c], m, at.col(c), at.t == 0 && (c == 0 || !one));
     }
   }
   }
@@ -371,7 +406,7 @@ struct NormBwdArgs {
   const void *dy, *h, *w, *dh;           // dh: null if none comes in
   const double* rstd;
   int64_t ldh, T;
-  int H, warps, rows;
+  int H, lanes, rows;
   int w_f32, vec, apart;
   void *dx, *dres;                       // null: not wanted
   float* part;                           // [blocks * flushes, H], null: no gradient of the weight
@@ -383,13 +418,13 @@ constexpr int kNormRun = 256;
 
 // dx of x's type, dres of h's (where the two types differ; else dx serves both).  A block stays and takes rows in turn, several at a
 // time, each by threads of its own, which keep their columns' part of dw in registers.
-template <bool XF32, bool HF32, int NC, bool WF32, bool VEC>
+template <bool XF32, bool HF32, int NC, bool WF32, bool VEC, bool NARROW>
 __global__ void __launch_bounds__(32 * kNormMaxWarps, 1) rms_norm_bwd_kernel(const NormBwdArgs a) {
-  extern __shared__ float columns[];                    // [rows, H]
+  extern __shared__ float columns[];                    // [rows, or warps if they are fewer, H]
   next_kernel_may_start();                              // (the sums of the blocks' sums, which waits)
   __shared__ float sums[2][kNormMaxWarps];
-  const int group = threadIdx.x / (a.warps * 32);
-  const NormRow<VEC> at{(int)threadIdx.x - group * a.warps * 32, a.warps * 32, a.H, a.apart != 0};
+  const int group = threadIdx.x / a.lanes, in_warp = NARROW ? (threadIdx.x & 31) / a.lanes : 0;
+  const NormRow<VEC> at{(int)threadIdx.x - group * a.lanes, a.lanes, a.H, a.apart != 0};
   const int64_t stride = (int64_t)gridDim.x * a.rows;
   NormVec<WF32> w[NC];
   at.load(w, a.w, 0);
@@ -400,28 +435,34 @@ __global__ void __launch_bounds__(32 * kNormMaxWarps, 1) rms_norm_bwd_kernel(con
     for (int i = 0; i < 4; ++i) dw[c][i] = p2(0.f, 0.f);
   const float inv_H = 1.f / a.H;
   int turn = 0;
-  int64_t row = (int64_t)blockIdx.x * a.rows + group;
+  int64_t first = (int64_t)blockIdx.x * a.rows + group - in_warp;   // of the rows of this warp
   // A row's loads leave before the one ahead of it is added up, which by then is held as h r and g.  (Rows in f32, or four pieces a thread:
   // neither, for want of registers; 8192 x 4096 with h in f32 109 us ahead and 94 so.)
   constexpr bool AHEAD = NC == 2 && !HF32;
   NormVec<XF32> dy[NC];
   NormVec<HF32> h[NC], dh[NC], next_dh[AHEAD ? NC : 1];
   double next_r = 1.0;
-  auto ask = [&](int64_t of) {
-    if (of >= a.T) return;
-    at.load(dy, a.dy, of * a.H);
-    at.load(h, a.h, of * a.ldh);
+  auto ask = [&](int64_t first) {                       // (a row behind the last one adds zeros)
+    if (first >= a.T) return;
+    const int64_t of = first + in_warp;
+    NormRow<VEC> in = at;
+    in.H = !NARROW || of < a.T ? a.H : 0;
+    in.load(dy, a.dy, of * a.H);
+    in.load(h, a.h, of * a.ldh);
     if constexpr (AHEAD) {
-      if (a.dh) at.load(next_dh, a.dh, of * a.H);
+      if (a.dh) in.load(next_dh, a.dh, of * a.H);
     } else {
-      if (a.dh) at.load(dh, a.dh, of * a.H);
+      if (a.dh) in.load(dh, a.dh, of * a.H);
     }
-    next_r = a.rstd[of];
+    next_r = !NARROW || in.H ? a.rstd[of] : 0.0;
   };
-  if (AHEAD) ask(row);
+  if (AHEAD) ask(first);
   for (int flush = 0; flush < a.flushes; ++flush) {
-    for (int n = 0; n < kNormRun && row < a.T; ++n, row += stride) {
-      if (!AHEAD) ask(row);
+    for (int n = 0; n < kNormRun && first < a.T; ++n, first += stride) {
+      if (!AHEAD) ask(first);
+      const int64_t row = first + in_warp;
+      NormRow<VEC> to = at;
+      to.H = !NARROW || row < a.T ? a.H : 0;
       if (AHEAD) {                                      // (the weights unpacked anew: 16 registers less)
 #pragma unroll
         for (int c = 0; c < NC; ++c) w[c].anew();
@@ -447,10 +488,10 @@ __global__ void __launch_bounds__(32 * kNormMaxWarps, 1) rms_norm_bwd_kernel(con
       if constexpr (AHEAD) {
 #pragma unroll
         for (int c = 0; c < NC; ++c) dh[c] = next_dh[c];
-        ask(row + stride);
+        ask(first + stride);
       }
       const float2 both = p2_get(s2);
-      const float s = norm_sum<float>(both.x + both.y, a.warps, group, sums[turn]) * -inv_H;
+      const float s = norm_sum<NARROW>(both.x + both.y, a.lanes, group, sums[turn]) * -inv_H;
       turn ^= 1;                                        // the next row's sums do not wait for this one's readers
       const P2 minus = p2(s, s);
 #pragma unroll
@@ -471,35 +512,46 @@ __global__ void __launch_bounds__(32 * kNormMaxWarps, 1) rms_norm_bwd_kernel(con
           NormVec<XF32> o;
 #pragma unroll
           for (int i = 0; i < 4; ++i) o.set(i, d[i]);
-          at.store(o, a.dx, row * a.H, c);
+          to.store(o, a.dx, row * a.H, c);
         }
         if constexpr (XF32 != HF32) {
           if (a.dres) {
             NormVec<HF32> o;
 #pragma unroll
             for (int i = 0; i < 4; ++i) o.set(i, d[i]);
-            at.store(o, a.dres, row * a.H, c);
+            to.store(o, a.dres, row * a.H, c);
           }
         }
       }
     }
     if (!a.part) continue;
     float* part = a.part + ((int64_t)blockIdx.x * a.flushes + flush) * a.H;
-    float* mine = a.rows > 1 ? columns + group * a.H : part;
-    if (a.rows > 1) __syncthreads();                    // the flush before has been read
+    const int sums_of = NARROW ? kNormMaxWarps : a.rows;
+    float* mine = sums_of > 1 ? columns + (NARROW ? threadIdx.x >> 5 : group) * a.H : part;
+    if (NARROW) {                                       // the warp's rows first
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1)
+        if (d >= a.lanes) {
+#pragma unroll
+          for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) dw[c][i] = dw[c][i] + P2{__shfl_xor_sync(0xffffffffu, dw[c][i].v, d)};
+        }
+    }
+    if (sums_of > 1) __syncthreads();                   // the flush before has been read
 #pragma unroll
     for (int c = 0; c < NC; ++c)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int col = at.col(c) + i * at.step();
         const float2 v = p2_get(dw[c][i >> 1]);
-        if (col < a.H) mine[col] = i & 1 ? v.y : v.x;
+        if (col < a.H && in_warp == 0) mine[col] = i & 1 ? v.y : v.x;
       }
-    if (a.rows > 1) {                                   // the block's rows first
+    if (sums_of > 1) {                                  // the block's rows first
       __syncthreads();
       for (int col = threadIdx.x; col < a.H; col += blockDim.x) {
         float v = columns[col];
-        for (int k = 1; k < a.rows; ++k) v += columns[k * a.H + col];
+        for (int k = 1; k < sums_of; ++k) v += columns[k * a.H + col];
         part[col] = v;
       }
     }
@@ -540,20 +592,25 @@ __global__ void __launch_bounds__(32 * kNormSumWarps) rms_norm_dw_kernel(const f
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------
-// Warps of a row of `nc` pieces a thread, and rows a block has at a time
+// Threads of a row of `nc` pieces a thread, at least `least`, and rows a block has at a time.  Narrow rows share a warp (us, one / several a
+// warp, bf16: 262144 x 128 85 / 26, with mx payload too 113 / 36, with 128-blocks alone 128 / 38, backward 100 / 39; x 64 85 / 14, backward
+// 96 / 22; 131072 x 256 45 / 27).
 struct NormShape {
-  int warps, rows;
-  NormShape(int H, int nc, int block_warps) {
-    warps = 1;
-    while (warps * 32 * 8 * nc < H) warps *= 2;
-    rows = warps < block_warps ? block_warps / warps : 1;
+  int lanes, rows;
+  NormShape(int H, int nc, int block_warps, int least) {
+    lanes = least;
+    while (lanes * 8 * nc < H) lanes *= 2;
+    rows = lanes < block_warps * 32 ? block_warps * 32 / lanes : 1;
   }
-  int threads() const { return 32 * warps * rows; }
+  int threads() const { return lanes * rows; }
 };
 static int norm_pieces(int H) { return H > 4096 ? 4 : 2; }
-static NormShape norm_forward_shape(int H) { return NormShape(H, norm_pieces(H), 8); }
+// (a group that is quantised together lies side by side in a warp)
+static NormShape norm_forward_shape(int H, int quant) {
+  return NormShape(H, norm_pieces(H), 8, quant == NORM_MX ? 4 : quant == NORM_BLOCK128 ? 2 : 1);
+}
 static int norm_bwd_pieces(int H) { return H > kNormMaxWarps * 512 ? 4 : 2; }
-static NormShape norm_bwd_shape(int H) { return NormShape(H, norm_bwd_pieces(H), kNormMaxWarps); }
+static NormShape norm_bwd_shape(int H) { return NormShape(H, norm_bwd_pieces(H), kNormMaxWarps, 1); }
 
 // rows of it can be read by 16 bytes (null: there are none)
 static bool norm_vec(const void* p, bool f32, int64_t ld, int64_t H) {
@@ -561,22 +618,24 @@ static bool norm_vec(const void* p, bool f32, int64_t ld, int64_t H) {
   return ((uintptr_t)p & 15) == 0 && H % 8 == 0 && ld % (f32 ? 4 : 8) == 0;
 }
 
-template <bool XF32, int RES, int QUANT, int NC>
+template <bool XF32, int RES, int QUANT, int NC, bool NARROW>
 static cudaError_t norm_launch_pieces(const NormArgs& a, const NormShape& sh, cudaStream_t stream) {
-  const int64_t all = (a.T + sh.rows - 1) / sh.rows, most = (int64_t)sm_count() * (NC == 2 ? 3 : 512 / sh.threads());
+  const int64_t all = (a.T + sh.rows - 1) / sh.rows, most = (int64_t)sm_count() * (NC == 2 ? norm_blocks(XF32 || RES == 2, NC) : 512 / sh.threads());
   const unsigned blocks = (unsigned)(all < most ? all : most);
   if (a.vec) {
-    if (a.w_f32) rms_norm_kernel<XF32, RES, QUANT, NC, true, true><<<blocks, sh.threads(), 0, stream>>>(a);
-    else rms_norm_kernel<XF32, RES, QUANT, NC, false, true><<<blocks, sh.threads(), 0, stream>>>(a);
+    if (a.w_f32) rms_norm_kernel<XF32, RES, QUANT, NC, true, true, NARROW><<<blocks, sh.threads(), 0, stream>>>(a);
+    else rms_norm_kernel<XF32, RES, QUANT, NC, false, true, NARROW><<<blocks, sh.threads(), 0, stream>>>(a);
   } else {
-    if (a.w_f32) rms_norm_kernel<XF32, RES, QUANT, NC, true, false><<<blocks, sh.threads(), 0, stream>>>(a);
-    else rms_norm_kernel<XF32, RES, QUANT, NC, false, false><<<blocks, sh.threads(), 0, stream>>>(a);
+    if (a.w_f32) rms_norm_kernel<XF32, RES, QUANT, NC, true, false, NARROW><<<blocks, sh.threads(), 0, stream>>>(a);
+    else rms_norm_kernel<XF32, RES, QUANT, NC, false, false, NARROW><<<blocks, sh.threads(), 0, stream>>>(a);
   }
   return cudaGetLastError();
 }
 template <bool XF32, int RES, int QUANT>
 static cudaError_t norm_launch(const NormArgs& a, const NormShape& sh, cudaStream_t stream) {
-  return norm_pieces(a.H) == 2 ? norm_launch_pieces<XF32, RES, QUANT, 2>(a, sh, stream) : norm_launch_pieces<XF32, RES, QUANT, 4>(a, sh, stream);
+  if (sh.lanes < 32) return norm_launch_pieces<XF32, RES, QUANT, 2, true>(a, sh, stream);
+  return norm_pieces(a.H) == 2 ? norm_launch_pieces<XF32, RES, QUANT, 2, false>(a, sh, stream)
+                               : norm_launch_pieces<XF32, RES, QUANT, 4, false>(a, sh, stream);
 }
 template <int RES>
 static cudaError_t norm_launch_bf16(const NormArgs& a, const NormShape& sh, int quant, cudaStream_t stream) {
@@ -585,22 +644,24 @@ static cudaError_t norm_launch_bf16(const NormArgs& a, const NormShape& sh, int 
                                   : norm_launch<false, RES, NORM_PLAIN>(a, sh, stream);
 }
 
-template <bool XF32, bool HF32, int NC>
+template <bool XF32, bool HF32, int NC, bool NARROW>
 static int norm_bwd_launch(const NormBwdArgs& a, const NormShape& sh, int blocks, cudaStream_t stream) {
-  const size_t smem = sh.rows > 1 && a.part ? (size_t)sh.rows * a.H * 4 : 0;       // at most 16 x 512 x 4 bytes
+  const int sums = sh.rows < kNormMaxWarps ? sh.rows : kNormMaxWarps;
+  const size_t smem = sums > 1 && a.part ? (size_t)sums * a.H * 4 : 0;              // at most 16 x 512 x 4 bytes
   if (a.vec) {
-    if (a.w_f32) rms_norm_bwd_kernel<XF32, HF32, NC, true, true><<<blocks, sh.threads(), smem, stream>>>(a);
-    else rms_norm_bwd_kernel<XF32, HF32, NC, false, true><<<blocks, sh.threads(), smem, stream>>>(a);
+    if (a.w_f32) rms_norm_bwd_kernel<XF32, HF32, NC, true, true, NARROW><<<blocks, sh.threads(), smem, stream>>>(a);
+    else rms_norm_bwd_kernel<XF32, HF32, NC, false, true, NARROW><<<blocks, sh.threads(), smem, stream>>>(a);
   } else {
-    if (a.w_f32) rms_norm_bwd_kernel<XF32, HF32, NC, true, false><<<blocks, sh.threads(), smem, stream>>>(a);
-    else rms_norm_bwd_kernel<XF32, HF32, NC, false, false><<<blocks, sh.threads(), smem, stream>>>(a);
+    if (a.w_f32) rms_norm_bwd_kernel<XF32, HF32, NC, true, false, NARROW><<<blocks, sh.threads(), smem, stream>>>(a);
+    else rms_norm_bwd_kernel<XF32, HF32, NC, false, false, NARROW><<<blocks, sh.threads(), smem, stream>>>(a);
   }
   return cudaGetLastError() == cudaSuccess ? SMOE_OK : SMOE_ERR_LAUNCH;
 }
 template <bool XF32, bool HF32>
 static int norm_bwd_launch_any(const NormBwdArgs& a, const NormShape& sh, int blocks, cudaStream_t stream) {
-  return norm_bwd_pieces(a.H) == 2 ? norm_bwd_launch<XF32, HF32, 2>(a, sh, blocks, stream)
-                                   : norm_bwd_launch<XF32, HF32, 4>(a, sh, blocks, stream);
+  if (sh.lanes < 32) return norm_bwd_launch<XF32, HF32, 2, true>(a, sh, blocks, stream);
+  return norm_bwd_pieces(a.H) == 2 ? norm_bwd_launch<XF32, HF32, 2, false>(a, sh, blocks, stream)
+                                   : norm_bwd_launch<XF32, HF32, 4, false>(a, sh, blocks, stream);
 }
 
 static int norm_bwd_blocks(int64_t T, const NormShape& sh) {
@@ -628,10 +689,10 @@ int smoe_rms_norm(const void* x, int x_f32, int64_t ldx, const void* residual, i
   if (T == 0) return SMOE_OK;
   if (!x || !w || (residual && !h) || (scale_kind ? !q || !scales : !y)) return SMOE_ERR_ARG;
   if (scale_kind && (uintptr_t)q & 15) return SMOE_ERR_ALIGN;
-  const NormShape sh = norm_forward_shape((int)H);
+  const NormShape sh = norm_forward_shape((int)H, scale_kind);
   NormArgs a{};
   a.x = x; a.res = residual; a.w = w; a.ldx = ldx; a.ldr = ldr; a.T = T; a.H = (int)H;
-  a.warps = sh.warps; a.rows = sh.rows; a.w_f32 = w_f32 != 0; a.apart = H % 8 != 0; a.eps = eps; a.inv_H = 1.0 / (double)H;
+  a.lanes = sh.lanes; a.rows = sh.rows; a.w_f32 = w_f32 != 0; a.apart = H % 8 != 0; a.eps = eps; a.inv_H = 1.0 / (double)H;
   const bool h_f32 = x_f32 || (residual && residual_f32);
   a.vec = norm_vec(x, x_f32, ldx, H) && norm_vec(residual, h_f32, ldr, H) && norm_vec(w, w_f32, H, H) && norm_vec(y, x_f32, H, H) &&
           norm_vec(h, h_f32, H, H);
@@ -667,7 +728,7 @@ int smoe_rms_norm_bwd(const void* dy, int x_f32, const void* h, int h_f32, int64
   const int blocks = norm_bwd_blocks(T, sh);
   NormBwdArgs a{};
   a.dy = dy; a.h = h; a.w = w; a.dh = dh; a.rstd = rstd; a.ldh = ldh; a.T = T; a.H = (int)H;
-  a.warps = sh.warps; a.rows = sh.rows; a.w_f32 = w_f32 != 0; a.apart = H % 8 != 0;
+  a.lanes = sh.lanes; a.rows = sh.rows; a.w_f32 = w_f32 != 0; a.apart = H % 8 != 0;
   a.vec = norm_vec(dy, x_f32, H, H) && norm_vec(h, h_f32, ldh, H) && norm_vec(w, w_f32, H, H) && norm_vec(dh, h_f32, H, H) &&
           norm_vec(dx, x_f32, H, H) && norm_vec(dres, h_f32, H, H);
   a.dx = dx; a.dres = dres;

@@ -156,6 +156,63 @@ def test_gradients(sonicmoe, T, H, tx, tr, tw):
     check_backward(sonicmoe, x, w, res, dy, dh, 1e-5)
 
 
+# rows that share a warp: from one value on, the last warp and the last block not full, more rows than one turn of all blocks
+NARROW = [(1, 2), (33, 1), (7, 16), (333, 24), (50, 64), (1001, 72), (77, 95), (300, 128), (131, 136), (64, 255), (3001, 256), (90001, 8),
+          (20011, 100), (13000, 256)]
+
+
+@pytest.mark.parametrize("T,H", NARROW)
+@pytest.mark.parametrize("tx,tr,tw", TYPES)
+def test_narrow_rows(sonicmoe, T, H, tx, tr, tw):
+    x, w, res, dy, dh = make(T, H, tx, tr, tw, seed=3)
+    out = sonicmoe.rms_norm(*on(x, w, res), eps=1e-5)
+    y, h = (out, None) if res is None else out
+    check_forward(y, h, x, w, res, 1e-5)
+    check_backward(sonicmoe, x, w, res, dy, dh, 1e-5)
+
+
+@pytest.mark.parametrize("H", [24, 64, 100, 256])
+def test_a_narrow_row_of_nan_is_alone(sonicmoe, H):
+    """Rows of one warp share nothing, forward and backward; only the weight's gradient takes all of them in."""
+    x, w, res, dy, dh = on(*make(70, H, BF, F32, F32, seed=4))
+    bad = [0, 13, 38, 69]
+    px = x.clone()
+    px[bad] = torch.tensor([float("nan"), float("inf"), 0.0, float("nan")], device=DEV, dtype=BF)[:, None]
+    keep = [i for i in range(70) if i not in bad]
+
+    def grads(x):
+        x, r = x.clone().requires_grad_(True), res.clone().requires_grad_(True)
+        y, h = sonicmoe.rms_norm(x, w, r)
+        return y.detach(), h.detach(), *torch.autograd.grad((y, h), (x, r), (dy, dh))
+
+    for a, b in zip(grads(x), grads(px)):
+        assert torch.equal(a[keep], b[keep])
+    if H % 8 == 0:
+        for scales in ("mx", "block128")[H % 32 != 0:]:
+            a, b = (sonicmoe.rms_norm_quantized(v, w, res, scales=scales) for v in (x, px))
+            assert torch.equal(a.payload.view(torch.uint8)[keep], b.payload.view(torch.uint8)[keep]) and torch.equal(a.scales[keep], b.scales[keep])
+
+
+def test_heads_norm_in_place_of_a_view(sonicmoe):
+    """Queries and keys as they lie in one projection: [tokens, heads, 128] with a stride, forward and backward."""
+    T, heads, D = 45, 6, 128
+    g = torch.Generator().manual_seed(8)
+    qkv = torch.randn(T, 3 * heads * D, generator=g).to(BF)
+    w, dy = (1 + torch.randn(D, generator=g) * 0.1).to(BF), torch.randn(T, heads, D, generator=g).to(BF)
+    dq, dw = qkv.to(DEV).requires_grad_(True), w.to(DEV).requires_grad_(True)
+    y = sonicmoe.rms_norm(dq[:, heads * D:2 * heads * D].view(T, heads, D), dw)
+    gq, gw = torch.autograd.grad(y, (dq, dw), dy.to(DEV))
+    k = qkv[:, heads * D:2 * heads * D].reshape(-1, D)
+    assert torch.equal(y.cpu().view(-1, D), O.bf16(O.rms_norm(k, w, 1e-6)[0]))
+    want, _ = O.rms_norm_backward(k, w, 1e-6, dy.view(-1, D), None)
+    assert (gq[:, :heads * D] == 0).all() and (gq[:, 2 * heads * D:] == 0).all()
+    got = gq[:, heads * D:2 * heads * D].cpu().double().reshape(-1, D)
+    r = O.rms_norm(k, w, 1e-6)[1]
+    gr, hr = (dy.view(-1, D).double() * w.double()).abs(), (k.double() * r).abs()
+    err = U * (r * (6 * gr + hr * (gr * hr).mean(1, keepdim=True) * (32 + 21 + 12)) + 2 * want.abs())      # as in check_backward
+    within(got, want, rounded(want, BF, err))
+
+
 def test_weight_gradient_goes_to_main_grad(sonicmoe):
     for tw in (BF, F32):
         x, w, res, dy, dh = make(33, 520, BF, F32, tw, seed=2)
@@ -238,7 +295,7 @@ def test_gradients_against_differences(sonicmoe):
 
 
 # ------------------------------------------------------------------------------------------------ payloads
-@pytest.mark.parametrize("T,H", [(1, 32), (3, 96), (40, 512), (7, 1056), (64, 4096), (2, 8224), (1, 16384)])
+@pytest.mark.parametrize("T,H", [(1, 32), (3, 96), (135, 64), (77, 128), (2001, 256), (9, 288), (40, 512), (7, 1056), (64, 4096), (2, 8224), (1, 16384)])
 @pytest.mark.parametrize("tr", [None, BF, F32])
 def test_mx_payload_is_the_row_quantisers(sonicmoe, T, H, tr):
     x, w, res, _, _ = make(T, H, BF, tr, BF, seed=7)
@@ -251,7 +308,7 @@ def test_mx_payload_is_the_row_quantisers(sonicmoe, T, H, tr):
     assert alone.y is None and torch.equal(alone.payload.view(torch.uint8), q) and torch.equal(alone.scales, s)
 
 
-@pytest.mark.parametrize("T,H", [(1, 8), (3, 136), (40, 512), (7, 1000), (64, 4096), (2, 8208), (1, 16384)])
+@pytest.mark.parametrize("T,H", [(1, 8), (131, 16), (135, 64), (77, 128), (3, 136), (2001, 256), (9, 264), (40, 512), (7, 1000), (64, 4096), (2, 8208), (1, 16384)])
 @pytest.mark.parametrize("tr", [None, BF, F32])
 def test_block128_payload_is_that_of_64_bits(sonicmoe, T, H, tr):
     x, w, res, _, _ = make(T, H, BF, tr, F32, seed=8)
