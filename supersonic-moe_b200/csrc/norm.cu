@@ -6,8 +6,8 @@
 // A row is held in registers between its one read and its one write; a block stays and asks for its next row before it adds this one up.
 // bf16 results and what is quantised from them are those of 64 bits: the mean and r are f64, y is made in f32 and looked at: where it
 // lies within kNormNear of the border between two bf16 values it is made again in f64 (one in 7000).
-//   What bounds it: HBM.  8192 x 4096 bf16 with residual, rows 43 us (6.2 TB/s), rows and payload 50 (6.1 TB/s); residual in f32 64 (6.2
-//   TB/s).  Backward, 16384 x 2048 bf16 49 us (5.5 TB/s), 8192 x 4096 with h in f32 94 (5.7): the column sums of dw take the registers that
+//   What bounds it: HBM.  8192 x 4096 bf16 with residual, rows 43 us (6.2 TB/s), rows and payload 50 (6.1 TB/s); residual in f32 65 (6.2
+//   TB/s); 262144 x 128 47 (5.7 TB/s).  Backward, 16384 x 2048 bf16 49 us (5.5 TB/s), 8192 x 4096 with h in f32 94 (5.7): the column sums of dw take the registers that
 //   would keep more rows on their way.  A single row takes 2.4 to 2.9 us.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -417,7 +417,8 @@ struct NormBwdArgs {
 constexpr int kNormRun = 256;
 
 // dx of x's type, dres of h's (where the two types differ; else dx serves both).  A block stays and takes rows in turn, several at a
-// time, each by threads of its own, which keep their columns' part of dw in registers.
+// time, each by threads of its own, which keep their columns' part of dw in registers.  NARROW: as in
+// the forward pass.
 template <bool XF32, bool HF32, int NC, bool WF32, bool VEC, bool NARROW>
 __global__ void __launch_bounds__(32 * kNormMaxWarps, 1) rms_norm_bwd_kernel(const NormBwdArgs a) {
   extern __shared__ float columns[];                    // [rows, or warps if they are fewer, H]
@@ -620,7 +621,8 @@ static bool norm_vec(const void* p, bool f32, int64_t ld, int64_t H) {
 
 template <bool XF32, int RES, int QUANT, int NC, bool NARROW>
 static cudaError_t norm_launch_pieces(const NormArgs& a, const NormShape& sh, cudaStream_t stream) {
-  const int64_t all = (a.T + sh.rows - 1) / sh.rows, most = (int64_t)sm_count() * (NC == 2 ? norm_blocks(XF32 || RES == 2, NC) : 512 / sh.threads());
+  const int64_t all = (a.T + sh.rows - 1) / sh.rows;
+  const int64_t most = (int64_t)sm_count() * (NC == 2 ? norm_blocks(XF32 || RES == 2, NC) : 512 / sh.threads());
   const unsigned blocks = (unsigned)(all < most ? all : most);
   if (a.vec) {
     if (a.w_f32) rms_norm_kernel<XF32, RES, QUANT, NC, true, true, NARROW><<<blocks, sh.threads(), 0, stream>>>(a);
