@@ -178,8 +178,8 @@ __device__ __forceinline__ T norm_sum(T s, int threads, int group, T* shared) {
   if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = s;
   asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(warps * 32) : "memory");
   shared += group * warps;
-  s = shared[0] + shared[1];                            // (a power of two)
-  for (int i = 2; i < warps; i += 2) s += shared[i] + shared[i + 1];
+  s = shared[0] + shared[1];
+  for (int i = 2; i < warps; i += 2) s += shared[i] + (i + 1 < warps ? shared[i + 1] : T(0));
   return s;
 }
 
@@ -593,7 +593,9 @@ __global__ void __launch_bounds__(32 * kNormSumWarps) rms_norm_dw_kernel(const f
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------
-// Threads of a row of `nc` pieces a thread, at least `least`, and rows a block has at a time.  Narrow rows share a warp (us, one / several a
+// Threads of a row of `nc` pieces a thread, at least `least`, and rows a block has at a time: as many warps as it fills, not a power of two
+// (us, a power / so, bf16 with residual, rows and payload: 8192 x 2560 42.4 / 33.4, x 5120 74 / 66; backward 41 / 35, 80 / 73; 3968 x 5088
+// without residual 34 / 28.6).  Narrow rows share a warp (us, one / several a
 // warp, bf16: 262144 x 128 85 / 26, with mx payload too 113 / 36, with 128-blocks alone 128 / 38, backward 100 / 39; x 64 85 / 14, backward
 // 96 / 22; 131072 x 256 45 / 27).
 struct NormShape {
@@ -601,6 +603,10 @@ struct NormShape {
   NormShape(int H, int nc, int block_warps, int least) {
     lanes = least;
     while (lanes * 8 * nc < H) lanes *= 2;
+    if (lanes > 32) {                                    // (seven warps of a row burden an SM's quarters unevenly: 4096 x 7168 42 us, eight 39)
+      const int warps = (H + 256 * nc - 1) / (256 * nc);
+      lanes = (warps == 7 ? 8 : warps) * 32;
+    }
     rows = lanes < block_warps * 32 ? block_warps * 32 / lanes : 1;
   }
   int threads() const { return lanes * rows; }
@@ -622,7 +628,7 @@ static bool norm_vec(const void* p, bool f32, int64_t ld, int64_t H) {
 template <bool XF32, int RES, int QUANT, int NC, bool NARROW>
 static cudaError_t norm_launch_pieces(const NormArgs& a, const NormShape& sh, cudaStream_t stream) {
   const int64_t all = (a.T + sh.rows - 1) / sh.rows;
-  const int64_t most = (int64_t)sm_count() * (NC == 2 ? norm_blocks(XF32 || RES == 2, NC) : 512 / sh.threads());
+  const int64_t most = (int64_t)sm_count() * ((NC == 2 ? 256 * norm_blocks(XF32 || RES == 2, NC) : 512) / sh.threads());
   const unsigned blocks = (unsigned)(all < most ? all : most);
   if (a.vec) {
     if (a.w_f32) rms_norm_kernel<XF32, RES, QUANT, NC, true, true, NARROW><<<blocks, sh.threads(), 0, stream>>>(a);
