@@ -126,8 +126,10 @@ __device__ __forceinline__ Tile16 tile16(int tile, int rank, const Gemm16Params&
   return t;
 }
 
-// Rows that belong to no segment, or lie behind a segment's live ones, become zero: warp w of n, N a multiple of 8
+// Rows that belong to no segment, or lie behind a segment's live ones, become zero: warp w of n, N a multiple of 8.  The warps take the rows
+// in turn over all gaps (each gap from warp 0 on: 128 experts of 1472 x 288, 10101 rows in 26496, 85 us instead of 49).
 __device__ __forceinline__ void zero_gaps16(const Segs128& s, int E, __nv_bfloat16* c, int N, int w, int n, int lane) {
+  int mine = w;                                         // rows of gaps until this warp's next one
   for (int e0 = -1; e0 <= E; e0 += 32) {
     const int e = e0 + lane;
     const int a = e < 0 ? 0 : e <= E ? s.live[e] : 0, end = e < 0 ? s.start[0] : e <= E ? s.start[e + 1] : 0;
@@ -136,8 +138,10 @@ __device__ __forceinline__ void zero_gaps16(const Segs128& s, int E, __nv_bfloat
       const int l = __ffs((int)some) - 1;
       some &= some - 1;
       const int from = __shfl_sync(0xffffffffu, a, l), to = __shfl_sync(0xffffffffu, end, l);
-      for (int r = from + w; r < to; r += n)
+      int r = from + mine;
+      for (; r < to; r += n)
         for (int col = lane * 8; col < N; col += 256) *reinterpret_cast<uint4*>(c + (int64_t)r * N + col) = make_uint4(0, 0, 0, 0);
+      mine = r - to;
     }
   }
 }
