@@ -4,8 +4,9 @@
 //   WGRAD16   c[e][m, n] (+)= sum over the rows r of e's segment of a[r, m] b[r, n]
 //
 // Segments begin and end at any row.  A tile of rows that reaches into the next segment computes rows that it does not store; a
-// reduction over rows must not take any in, so that the operands' rows behind a segment's last one are overwritten with zeros in
-// shared memory (by a warp of its own, one block of 64 rows a tile) before the MMAs read them.
+// reduction over rows must not take any in: the last block of 64 gets as many MMAs of 16 rows as it needs, and the operands' rows behind
+// the segment's last one, at most 15, are overwritten with zeros in shared memory by a warp of its own before they are read (us, all of
+// the block / so, weight gradients of 128 experts of 1536 x 2048: 4 rows each 191 / 143, 65 244 / 192, 96 217 / 177; zeros alone 139).
 //
 // Operands by TMA in the 128-byte swizzle, 64 values of the reduction a stage: [128 rows][64] where the reduction lies along memory
 // (K-major), two pieces of [64 of the reduction][64] where it lies across (MN-major), as weights do for the gradient of the rows and
@@ -222,7 +223,7 @@ gemm16_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
         const uint32_t full = full0 + 8 * stage;
         const uint32_t a_dst = smem_base + stage * S::STAGE_BYTES, b_dst = a_dst + S::A_BYTES;
         if (elect_one()) {
-          if (MODE == WGRAD16 && tail && k == nkt - 1) {      // to a barrier of this CTA, for its FIXER
+          if (MODE == WGRAD16 && (tail & 15) && k == nkt - 1) {      // to a barrier of this CTA, for its FIXER
             const uint32_t last = bar_tail + 8 * stage;
             mbar_expect_tx(last, S::STAGE_BYTES);
 #pragma unroll
@@ -269,7 +270,7 @@ gemm16_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
         ok = __all_sync(0xffffffffu, mbar_wait(bar_tempty + 8 * as, aphase ^ 1));
         if (!ok) break;
         for (int k = 0; k < nkt; ++k) {
-          if (MODE == WGRAD16 && tail && k == nkt - 1) {
+          if (MODE == WGRAD16 && (tail & 15) && k == nkt - 1) {
             ok = __all_sync(0xffffffffu, mbar_wait_cluster(bar_fixed + 8 * stage, fixes >> stage & 1));
             fixes ^= 1u << stage;
           } else {
@@ -279,10 +280,12 @@ gemm16_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
           if (!ok) break;
           tc_fence_after();
           const uint32_t a_lo = a_lo0 + stage * (S::STAGE_BYTES >> 4), b_lo = b_lo0 + stage * (S::STAGE_BYTES >> 4);
+          const int steps = MODE == WGRAD16 && tail && k == nkt - 1 ? (tail + 15) / 16 : kBK16 / 16;
           if (elect_one()) {
 #pragma unroll
             for (int kb = 0; kb < kBK16 / 16; ++kb)
-              mma_bf16_pair_lo(tmem_base + as * BN, a_lo + a_step * kb, b_lo + b_step * kb, kDescHi16, idesc, (k | kb) != 0);
+              if (kb < steps)
+                mma_bf16_pair_lo(tmem_base + as * BN, a_lo + a_step * kb, b_lo + b_step * kb, kDescHi16, idesc, (k | kb) != 0);
             tc_commit_pair(bar_empty + 8 * stage, 3);
             if (k == nkt - 1) tc_commit_pair(bar_tfull + 8 * as, 3);
           }
@@ -302,7 +305,8 @@ gemm16_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
     for (int tile = pair_id; tile < n_total && ok; tile += n_pairs) {
       const Tile16 t = tile16<MODE, BN>(tile, rank, p, segs);
       stage = (stage + t.nkt) % S::STAGES;
-      if (t.tail == 0) continue;
+      const int end = (t.tail + 15) & ~15;
+      if (t.tail == end) continue;
       const int st = stage == 0 ? S::STAGES - 1 : stage - 1;
       ok = __all_sync(0xffffffffu, mbar_wait(bar_tail + 8 * st, tails >> st & 1));
       tails ^= 1u << st;
@@ -310,7 +314,7 @@ gemm16_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
       const uint32_t at = smem_base + st * S::STAGE_BYTES;
 #pragma unroll
       for (int c = 0; c < 2 + S::B_PIECES; ++c)               // the pieces of both operands, a row 128 bytes of each
-        for (int b = t.tail * 128 + lane * 16; b < kPiece16; b += 512) st_shared_v4(at + c * kPiece16 + b, 0u, 0u, 0u, 0u);
+        for (int b = t.tail * 128 + lane * 16; b < end * 128; b += 512) st_shared_v4(at + c * kPiece16 + b, 0u, 0u, 0u, 0u);
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(fixed0 + 8 * st);

@@ -118,6 +118,15 @@ def test_sizes_and_main_grad(sonicmoe, N, K, counts):
     check(sonicmoe, counts, N, K, seed=5, padded=True)
 
 
+@pytest.mark.parametrize("N,K", [(136, 72), (264, 520)])
+@pytest.mark.parametrize("gaps", [False, True])
+def test_every_length_of_a_segment(sonicmoe, gaps, N, K):
+    """A block of the reduction ends anywhere; what lies behind it belongs to the next expert, or to nobody."""
+    counts = list(range(131))
+    check(sonicmoe, counts, N, K, **(dict(gaps=[(5 * i) % 37 for i in counts]) if gaps else {}))
+    check(sonicmoe, counts[::-1], N, K, seed=5, main_grad=True, **(dict(gaps=[300] + [0] * 128 + [700, 1], first=40) if gaps else {}))
+
+
 def test_large(sonicmoe):
     check(sonicmoe, [3000, 0, 1, 5011, 777, 64, 2500, 129], 4096, 2048)
     check(sonicmoe, [3000, 0, 1, 5011, 777, 64, 2500, 129], 2048, 1536, main_grad=True)
