@@ -171,6 +171,22 @@ def test_narrow_rows(sonicmoe, T, H, tx, tr, tw):
     check_backward(sonicmoe, x, w, res, dy, dh, 1e-5)
 
 
+# rows of three, five, six, seven (of eight), nine and thirteen warps, several of them a block and several turns of all blocks
+@pytest.mark.parametrize("T,H", [(37, 1536), (1901, 2560), (11, 2880), (1000, 2817), (950, 3584), (601, 5120), (5, 6656), (160, 9216), (3, 13000)])
+@pytest.mark.parametrize("tx,tr,tw", [(BF, BF, BF), (BF, F32, F32), (F32, None, BF), (F32, F32, F32)])
+def test_rows_of_any_number_of_warps(sonicmoe, T, H, tx, tr, tw):
+    x, w, res, dy, dh = make(T, H, tx, tr, tw, seed=5)
+    out = sonicmoe.rms_norm(*on(x, w, res), eps=1e-5)
+    check_forward(*((out, None) if res is None else out), x, w, res, 1e-5)
+    check_backward(sonicmoe, x, w, res, dy, dh, 1e-5)
+    if tx == BF and H % 32 == 0:
+        for scales, quantise in (("mx", lambda y: sonicmoe.ops.quant_rows(y)[:2]), ("block128", sonicmoe.ops.quant128_rows)):
+            got = sonicmoe.rms_norm_quantized(*on(x, w, res), eps=1e-5, scales=scales, with_output=True)
+            q, s = quantise(got.y)
+            assert torch.equal(got.y.cpu(), (out if res is None else out[0]).cpu())
+            assert torch.equal(got.payload.view(torch.uint8), q.view(torch.uint8)) and torch.equal(got.scales, s)
+
+
 @pytest.mark.parametrize("H", [24, 64, 100, 256])
 def test_a_narrow_row_of_nan_is_alone(sonicmoe, H):
     """Rows of one warp share nothing, forward and backward; only the weight's gradient takes all of them in."""
