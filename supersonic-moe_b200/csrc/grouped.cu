@@ -70,9 +70,13 @@ static bool narrow16(int64_t tiles, int64_t cols) { return tiles <= sm_count() /
 // rows 17.4 / 15.8, 512 18.1 / 26.4; 1024 x 4096, 1024 rows 16.8 / 15.3, 2048 18.0 / 26.1; 1000 x 720, 2000 7.7 / 9.1; 8 of 512 x 512, 2048
 // 8.2 / 5.9, 4096 8.5 / 7.7, 8192 9.0 / 11.8; of 1024 x 1024, 1024 11.3 / 8.1, 2048 9.2 / 10.9; of 4096 x 2048, 512 31 / 26, 2048 35 /
 // 50; 128 of 1536 x 2048, 4096 177 / 128, 8192 170 / 133, 12288 168 / 170; the same unevenly routed 166 / 142, 182 / 171, 189 / 206.  The
-// gradient of the rows reads its weights across and takes up to a sixth longer with few.)
-static bool few_rows16(int64_t rows, int64_t N, int64_t E) {
-  if (rows <= Few16Smem::NT * E) return true;
+// gradient of the rows reads its weights across and takes up to a sixth longer with few.)  Segments with counts are padded, as a rule to
+// multiples of 128, and their live rows are not known here: as many rows as one such block an expert and an eighth more (us, the other / few
+// by live rows an expert of 128: 128 experts of 1536 x 2048, 8 179 / 136, 64 176 / 149, 100 of 149 180 / 173, 128 187 / 176, 140 of 202
+// 194 / 227; of 264 x 808, 8 37 / 20, 128 37 / 30; 37 of 1024 x 1024, 9 20.5 / 13.3, 128 20.4 / 22.9; 8 of 4096 x 2048, 8 33 / 27, 128 33.4 /
+// 34.2).
+static bool few_rows16(int64_t rows, int64_t N, int64_t E, bool padded) {
+  if (rows <= (padded ? 9 * 128 * E / 8 : Few16Smem::NT * E)) return true;
   const int64_t busy = rows < E ? rows : E;
   return (rows + (Few16Smem::NT - 1) * busy) / Few16Smem::NT * up16(N, 128) <= (E == 1 ? 1 : 2) * sm_count();
 }
@@ -175,7 +179,7 @@ int smoe_grouped_rows(const void* x_bf16, int64_t ldx, const void* w_bf16, int w
   if (!on16(x_bf16) || !on16(w_bf16) || !on16(y_bf16)) return SMOE_ERR_ALIGN;
   if (!w_transposed && gemv_rows16(rows, N, K, E))
     return gemv16(x_bf16, ldx, w_bf16, efo, counts, y_bf16, rows, N, K, E, (cudaStream_t)stream);
-  if (few_rows16(rows, N, E))
+  if (few_rows16(rows, N, E, counts != nullptr))
     return few16(x_bf16, ldx, w_bf16, efo, counts, y_bf16, rows, N, K, E, w_transposed != 0, status, pinned_host_word,
                  (cudaStream_t)stream);
   // every segment may end in a tile that is not full

@@ -247,7 +247,9 @@ Tensor grouped_wgrad(const Tensor& dy, const Tensor& x, const Tensor& efo, const
   const bool add = main_grad.defined();
   // (what is added leaves in pieces that start on 16 bytes)
   const bool direct = add && (uintptr_t)main_grad.data_ptr() % 16 == 0;
-  Tensor dw = direct ? main_grad : add ? at::zeros({E, N, K}, dy.options().dtype(at::kFloat).requires_grad(false)) : fresh({E, N, K}, at::kBFloat16, dy);
+  Tensor dw = direct ? main_grad
+              : add  ? at::zeros({E, N, K}, dy.options().dtype(at::kFloat).requires_grad(false))
+                     : fresh({E, N, K}, at::kBFloat16, dy);
   const int64_t bytes = smoe_grouped_wgrad_workspace(N, K, rows, E);
   const Tensor ws = bytes > 0 ? fresh({bytes}, at::kByte, dy) : Tensor();
   check(smoe_grouped_wgrad(dy.data_ptr(), distance(dy), x.data_ptr(), distance(x), (const int32_t*)ptr(efo), (const int32_t*)ptr(counts),

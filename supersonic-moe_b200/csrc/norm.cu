@@ -6,9 +6,10 @@
 // A row is held in registers between its one read and its one write; a block stays and asks for its next row before it adds this one up.
 // bf16 results and what is quantised from them are those of 64 bits: the mean and r are f64, y is made in f32 and looked at: where it
 // lies within kNormNear of the border between two bf16 values it is made again in f64 (one in 7000).
-//   What bounds it: HBM.  8192 x 4096 bf16 with residual, rows 43 us (6.2 TB/s), rows and payload 50 (6.1 TB/s); residual in f32 65 (6.2
-//   TB/s); 262144 x 128 47 (5.7 TB/s).  Backward, 16384 x 2048 bf16 49 us (5.5 TB/s), 8192 x 4096 with h in f32 94 (5.7): the column sums of dw take the registers that
-//   would keep more rows on their way.  A single row takes 2.4 to 2.9 us.
+//   What bounds it: HBM.  8192 x 4096 bf16 with residual, rows 43 us (6.2 TB/s), rows and payload 50 (6.1 TB/s); residual in f32 67 (6.0
+//   TB/s), with payload 70 (6.2); 262144 x 128 47 (5.7 TB/s).  Without residual issue: 8192 x 4096 31 us (4.4 TB/s).  Backward, 16384 x 2048
+//   bf16 49 us (5.5 TB/s), 8192 x 4096 with h in f32 94 (5.7): the column sums of dw take the registers that would keep more rows on their
+//   way.  A single row takes 2.4 to 2.9 us.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
