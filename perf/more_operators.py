@@ -84,8 +84,7 @@ def draw(rng):
     if rng.random() < 0.3:
         case.update(shapes="experts", tensors=8, E=rng.choice((8, 32, 64)), H=64 * rng.randint(4, 32), I=64 * rng.randint(2, 12))
     if kind == "clip":
-        case.update(out=rng.choice(("f32", "bf16")), max_norm=rng.choice((0.1, 1.0, 1e6)),
-                    tensors=min(case["tensors"], 60))          # each is an output of the call, of which 64 can be compared
+        case.update(out=rng.choice(("f32", "bf16")), max_norm=rng.choice((0.1, 1.0, 1e6)))
     return case
 
 
