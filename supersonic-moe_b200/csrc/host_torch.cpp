@@ -278,9 +278,9 @@ struct GroupedNode : torch::autograd::Function<GroupedNode> {
     const Tensor w3 = wd.dim() == 3 ? wd : wd.unsqueeze(0);
     const Tensor e = of(efo), c = of(counts);
     Tensor y = grouped_rows(x, w3, e, c, false, {status, host});
-    // (the weight itself where it is read as it lies: autograd then sees a change in place between the passes)
-    ctx->save_for_backward({ctx->needs_input_grad(1) ? x : Tensor(), ctx->needs_input_grad(0) ? (wd.data_ptr() == w.data_ptr() ? w : wd) : Tensor(),
-                            e, c});
+    // (the weight itself where it is read as it lies: autograd then sees a change in place between the passes; what is saved goes by the
+    // inputs, since needs_input_grad speaks of the backward pass that is running, which one that makes this pass again is not)
+    ctx->save_for_backward({w.requires_grad() ? x : Tensor(), x.requires_grad() ? (wd.data_ptr() == w.data_ptr() ? w : wd) : Tensor(), e, c});
     ctx->saved_data["shape"] = w3.sizes().vec();
     ctx->saved_data["dims"] = w.dim();
     ctx->saved_data["status"] = status;
@@ -293,8 +293,10 @@ struct GroupedNode : torch::autograd::Function<GroupedNode> {
     const Words at{ctx->saved_data["status"].toInt(), ctx->saved_data["host"].toInt()};
     const Tensor dy = rows_lie(grads[0]) ? grads[0] : dense(grads[0]);
     Tensor dx, dw;
-    if (ctx->needs_input_grad(0) && saved[1].defined()) dx = grouped_rows(dy, saved[1].view(shape), saved[2], saved[3], true, at);
-    if (ctx->needs_input_grad(1) && saved[0].defined()) {
+    const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
+    TORCH_CHECK((saved[1].defined() || !need_x) && (saved[0].defined() || !need_w), "grouped_linear: a gradient is asked for whose operand was not kept");
+    if (need_x) dx = grouped_rows(dy, saved[1].view(shape), saved[2], saved[3], true, at);
+    if (need_w) {
       dw = grouped_wgrad(dy, saved[0], saved[2], saved[3], shape[0], Tensor(), at);
       if (ctx->saved_data["dims"].toInt() == 2) dw = dw.squeeze(0);
     }
