@@ -5,7 +5,8 @@
 //
 // A row is held in registers between its one read and its one write; a block stays and asks for its next row before it adds this one up.
 // bf16 results and what is quantised from them are those of 64 bits: the mean and r are f64, y is made in f32 and looked at: where it
-// lies within kNormNear of the border between two bf16 values it is made again in f64 (one in 7000).
+// lies within kNormNear of the border between two bf16 values it is made again in f64 (one in 7000), where one that is a tie but for the
+// roundings of f64 counts as a tie.
 //   What bounds it: HBM.  8192 x 4096 bf16 with residual, rows 43 us (6.2 TB/s), rows and payload 50 (6.1 TB/s); residual in f32 67 (6.0
 //   TB/s), with payload 70 (6.2); 262144 x 128 47 (5.7 TB/s).  Without residual issue: 8192 x 4096 31 us (4.4 TB/s).  Backward, 16384 x 2048
 //   bf16 49 us (5.5 TB/s), 8192 x 4096 with h in f32 94 (5.7): the column sums of dw take the registers that would keep more rows on their
@@ -184,13 +185,15 @@ __device__ __forceinline__ T norm_sum(T s, int threads, int group, T* shared) {
   return s;
 }
 
-// 1 / sqrt(v): the f32 approximation and one step of Newton's method, which leaves some 2^-43; v is brought into the range of f32
+// 1 / sqrt(v) to the last place: with y the f32 approximation and e = 1 - v y^2, y (1 - e)^(-1/2) = y (1 + e / 2 + 3 e^2 / 8 + 5 e^3 / 16 ...), of
+// which the third power, 2^-66, is left out; v is brought into the range of f32
 __device__ __forceinline__ double norm_rsqrt(double v) {
   const double scale = v < 1e-30 ? 0x1p200 : v > 1e30 ? 0x1p-200 : 1.0, back = v < 1e-30 ? 0x1p100 : v > 1e30 ? 0x1p-100 : 1.0;
   v *= scale;
   const float r = rsqrtf((float)v);
   if (!(r > 0.f && r < __int_as_float(0x7f800000))) return r;      // of 0, infinity, NaN
-  return (double)r * (1.5 - 0.5 * v * r * r) * back;
+  const double y = r, e = fma(-v * y, y, 1.0);
+  return fma(y, e * fma(0.375, e, 0.5), y) * back;
 }
 
 // h r w in f32 is off by three roundings (r, two products), each up to one unit of the last place
@@ -200,16 +203,19 @@ __device__ __forceinline__ uint32_t norm_min_u16x2(uint32_t a, uint32_t b) {
   asm("min.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
-// f32 that rounds to the bf16 nearest to d: a tie of f32 that is none of f64 is moved off
-__device__ __forceinline__ float norm_for_bf16(double d) {
+// f32 that rounds to the bf16 nearest to d: a tie of f32 that is none of f64 is moved off.  What is a tie but for `slack` of its size is one.
+__device__ __forceinline__ float norm_for_bf16(double d, double slack) {
   float f = (float)d;
   if ((__float_as_uint(f) & 0xFFFFu) == 0x8000u) {
-    const double away = fabs(d) - fabs((double)f);
-    if (away > 0) f = __uint_as_float(__float_as_uint(f) + 1);
-    if (away < 0) f = __uint_as_float(__float_as_uint(f) - 1);
+    const double away = fabs(d) - fabs((double)f), least = fabs(d) * slack;
+    if (away > least) f = __uint_as_float(__float_as_uint(f) + 1);
+    if (away < -least) f = __uint_as_float(__float_as_uint(f) - 1);
   }
   return f;
 }
+// Rounding of the mean (of its quotient, which is a product, and of eps's addition), r and h w r in f64: 2^-51 of a value that is a tie, as
+// those of equal magnitudes whose weight lies between two bf16 are
+constexpr double kNormTie = 0x1p-50;
 
 struct NormArgs {
   const void *x, *res, *w;
@@ -357,7 +363,7 @@ __global__ void __launch_bounds__(NC == 2 ? 256 : 512, norm_blocks(XF32 || RES =
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float2 f = p2_get(hc.pair(i)), g = p2_get(wc.pair(i));
-          v[i] = p2(norm_for_bf16((double)f.x * r64 * (double)g.x), norm_for_bf16((double)f.y * r64 * (double)g.y));
+          v[i] = p2(norm_for_bf16((double)f.x * (double)g.x * r64, kNormTie), norm_for_bf16((double)f.y * (double)g.y * r64, kNormTie));
         }
       }
       NormVec<false> y;
@@ -589,7 +595,7 @@ __global__ void __launch_bounds__(32 * kNormSumWarps) rms_norm_dw_kernel(const f
     if (accumulate) atomicAdd(p, (float)s);             // (once for each value: another stream's sums into it are not lost)
     else *p = (float)s;
   } else {
-    ((__nv_bfloat16*)dw)[col] = __float2bfloat16_rn(norm_for_bf16(s));
+    ((__nv_bfloat16*)dw)[col] = __float2bfloat16_rn(norm_for_bf16(s, 0.0));
   }
 }
 
