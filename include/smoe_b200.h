@@ -578,7 +578,7 @@ int smoe_grouped_wgrad(const void* dy_bf16, int64_t ldy, const void* x_bf16, int
  * h = x + residual, held in the residual's type (without one h = x and nothing is written); r = 1 / sqrt(mean(h^2) + eps), one a
  * row; y = h r w.  x, y bf16 or f32 [T,H], rows of x ldx values apart; residual, h of x's type or f32, rows of the residual ldr
  * apart; w bf16 or f32 [H]; rstd f64 [T] or null.  H <= 16384.  The mean and r are f64, and bf16 results those of 64 bits (what lies within
- * 2^-50 of the middle between two bf16 goes to the even one).
+ * 2^-50 of the middle between two bf16 goes to the even one).  eps is 0 or at least 1e-90.
  * scale_kind 1 (x bf16, H % 32 == 0): of y, q e4m3 [T,H] and scales u8 [T,H/32] as smoe_quant_rows makes them; 2 (x bf16, H % 8 == 0): q, rows
  * ceil(H/16)*16 bytes apart, and scales f32 [T,ceil(H/128)] as smoe_quant128_rows does; y may then be null. */
 int smoe_rms_norm(const void* x, int x_f32, int64_t ldx, const void* residual, int residual_f32, int64_t ldr, const void* w, int w_f32,

@@ -175,6 +175,7 @@ Tensor as_rows(const Tensor& t) {
 }
 
 constexpr int64_t kNormMaxH = 16384;
+constexpr double kNormLeastEps = 1e-90;                  // (what a root brought into the range of f32 can be taken of)
 // x and residual as rows, and the weight, of a call that is allowed; kind: see smoe_rms_norm
 std::tuple<Tensor, Tensor, Tensor> norm_checked(const Tensor& x, const Tensor& w, const Tensor& residual, double eps, int kind) {
   const char* const what = kind ? "rms_norm_quantized" : "rms_norm";
@@ -187,7 +188,8 @@ std::tuple<Tensor, Tensor, Tensor> norm_checked(const Tensor& x, const Tensor& w
   TORCH_CHECK_VALUE(!residual.defined() || (residual.sizes() == x.sizes() && (residual.scalar_type() == tx || f32(residual))), what,
                     ": the residual is of x's type or f32, of its shape ", text(x.sizes()), ", got ",
                     type_name(residual.defined() ? residual.scalar_type() : tx), " ", residual.defined() ? text(residual.sizes()) : "");
-  TORCH_CHECK_VALUE(eps >= 0 && eps < INFINITY, what, ": eps=", std::to_string(eps));
+  TORCH_CHECK_VALUE((eps == 0 || eps >= kNormLeastEps) && eps < INFINITY, what, ": eps=", py::str(py::float_(eps)).cast<std::string>(),
+                    ": 0 or at least 1e-90, finite");
   const int64_t unit = kind == 1 ? kMxGroup : kind == 2 ? 8 : 1;
   TORCH_CHECK_VALUE(H % unit == 0, what, ": ", std::to_string(H), " columns are no multiple of ", std::to_string(unit));
   return {as_rows(x), w.is_contiguous() ? w : w.contiguous(), residual.defined() ? as_rows(residual) : residual};

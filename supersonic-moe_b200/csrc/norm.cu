@@ -24,6 +24,7 @@ namespace smoe {
 
 constexpr int kNormMaxH = 16384;
 constexpr int kNormMaxWarps = 16;
+constexpr double kNormLeastEps = 1e-90;    // the root's argument is brought into the range of f32: so far (a row that is not zero has 1e-94)
 
 // ---- pairs of f32 in one instruction (round to nearest, as the scalar forms)
 struct P2 {
@@ -699,7 +700,7 @@ int smoe_rms_norm(const void* x, int x_f32, int64_t ldx, const void* residual, i
                   int64_t T, int64_t H, double eps, void* y, void* h, double* rstd, int scale_kind, void* q, void* scales,
                   void* stream) {
   if (!norm_sizes(T, H) || ldx < H || (residual && ldr < H)) return SMOE_ERR_SHAPE;
-  if (scale_kind < 0 || scale_kind > 2 || !(eps >= 0) || (x_f32 && (scale_kind || (residual && !residual_f32)))) return SMOE_ERR_ARG;
+  if (scale_kind < 0 || scale_kind > 2 || !(eps == 0 || eps >= kNormLeastEps) || (x_f32 && (scale_kind || (residual && !residual_f32)))) return SMOE_ERR_ARG;
   if ((scale_kind == NORM_MX && H % 32) || (scale_kind == NORM_BLOCK128 && H % 8)) return SMOE_ERR_SHAPE;
   if (T == 0) return SMOE_OK;
   if (!x || !w || (residual && !h) || (scale_kind ? !q || !scales : !y)) return SMOE_ERR_ARG;

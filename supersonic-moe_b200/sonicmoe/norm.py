@@ -80,6 +80,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | Non
     f32.  y is of x's type, h of the residual's: it is rounded to that type, and the norm is that of the rounded sum, so that the next
     layer and the backward pass see the same rows.  Mean and root are f64; bf16 results are those of 64 bits (but where h / sqrt(...) lies
     below f32's normal range, 2^-126), and what lies within 2^-50 of the middle between two bf16 goes to the even one.
+    eps is 0 or at least 1e-90.
 
     Differentiable in x, weight and residual (the gradient of h included); a weight's gradient goes to the parameter's f32 `main_grad`
     where it has one.  Gradients cannot be differentiated again."""
