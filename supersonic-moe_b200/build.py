@@ -35,7 +35,7 @@ def _host_command():
     import torch
     at = os.path.dirname(torch.__file__)
     return ([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f'-DSMOE_TORCH_VERSION="{torch.__version__}"']
             + [a for i in (INCLUDE, os.path.join(at, "include"), os.path.join(at, "include", "torch", "csrc", "api", "include"),
                            sysconfig.get_paths()["include"], "/usr/local/cuda/include") for a in ("-I", i)]
             + [HOST_SOURCE, "-o", HOST_OUT, "-L", os.path.dirname(OUT), "-lsmoe_b200", "-L", os.path.join(at, "lib"), "-ltorch_python",

@@ -521,6 +521,7 @@ Tensor clip_gradients(const py::object& items, double max_norm, const Maybe& giv
 }  // namespace
 
 PYBIND11_MODULE(_host, m) {
+  m.attr("torch_version") = SMOE_TORCH_VERSION;
   m.def("rms_norm", [](const Tensor& x, const Tensor& w, const Maybe& residual, double eps, int kind, bool with_y, bool keep) {
     const Norm n = norm(x, w, of(residual), eps, kind, with_y, keep);
     return std::make_tuple(some(n.y), some(n.h), some(n.q), some(n.s), some(n.r));

@@ -6,11 +6,15 @@ the import of this module raises.
 from __future__ import annotations
 
 import ctypes
+import importlib
 import os
 from ctypes import c_double, c_float, c_int, c_int64, c_void_p
 
+import torch
+
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libsmoe_b200.so")
+HOST_PATH = os.path.join(_HERE, "_host.so")
 
 _P, _I, _L, _F, _D = c_void_p, c_int, c_int64, c_float, c_double
 
@@ -142,6 +146,27 @@ def _load():
 
 
 lib = _load()
+
+
+class _Host:
+    """The functions of csrc/host_torch.cpp, loaded with the first call that goes through them: the rest of the package needs the C ABI
+    alone, whatever PyTorch it runs under."""
+
+    def __getattr__(self, name):
+        if name.startswith("__"):
+            raise AttributeError(name)
+        advice = "build it with `python supersonic-moe_b200/build.py` under the installed PyTorch (there is no fallback for the calls that need it)"
+        try:
+            native = importlib.import_module("._host", __package__)
+        except ImportError as e:
+            raise ImportError(f"{HOST_PATH} is missing or cannot be loaded ({e}): {advice}") from e
+        if native.torch_version != str(torch.__version__):
+            raise ImportError(f"{HOST_PATH} was built with PyTorch {native.torch_version}, this is {torch.__version__}: {advice}")
+        self.__dict__.update((k, v) for k, v in vars(native).items() if not k.startswith("__"))
+        return getattr(native, name)
+
+
+host = _Host()
 
 
 def check(rc: int, what: str):

@@ -24,4 +24,4 @@ def clip_gradients(gradients, max_norm: float, *, norm: torch.Tensor | None = No
     contiguous f32 or bf16 tensors of the gradients' shapes, one for each, which receive the results (accumulators in f32, gradients
     for the optimizer in bf16, from one pass); the gradients stay as they are then.  An output may be its own gradient and lies apart
     from every other one.  Without `out` they change in place, and where nothing is to be clipped nothing is written.  A norm of NaN makes every result NaN, an infinite one 0 (NaN where the gradient is infinite)."""
-    return ops.gradient_clip(gradients, float(max_norm), norm, out)
+    return ops.clip_gradients(gradients, float(max_norm), norm, out)

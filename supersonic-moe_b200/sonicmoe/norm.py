@@ -8,7 +8,8 @@ from typing import NamedTuple
 import torch
 from torch.autograd.function import once_differentiable
 
-from . import _host, ops
+from . import ops
+from ._lib import host as _host
 from .functional import _after_accumulate, _base_of, _grad_target
 
 

@@ -9,8 +9,7 @@ import ctypes
 
 import torch
 
-from ._lib import check, lib  # (loads the library that _host calls)
-from . import _host
+from ._lib import check, host as _host, lib
 
 _U8 = torch.uint8
 _I32 = torch.int32
@@ -1177,5 +1176,13 @@ def rms_norm_bwd(dy, h, w, rstd, dh=None, dx=True, dres=False, dw=True, main_gra
 
 
 # ---------------------------------------------------------------- the norm of the gradients
-gradient_norm = _timed(_host.gradient_norm)
-gradient_clip = _timed(_host.clip_gradients)
+@_timed
+def gradient_norm(gradients):
+    """Tensors or parameters -> f32 []; see `sonicmoe.gradient_norm`."""
+    return _host.gradient_norm(gradients)
+
+
+@_timed
+def clip_gradients(gradients, max_norm, norm=None, out=None):
+    """-> the norm f32 []; see `sonicmoe.clip_gradients`."""
+    return _host.clip_gradients(gradients, max_norm, norm, out)
