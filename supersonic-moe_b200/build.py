@@ -4,7 +4,9 @@
 
 The library lands next to the Python package (sonicmoe/libsmoe_b200.so) and is
 loaded with ctypes; it links nothing but the CUDA runtime.  Beside it lies
-sonicmoe/_host.so, which calls it on torch tensors (csrc/host_torch.cpp).
+sonicmoe/_host.so, which calls it on torch tensors (csrc/host_torch.cpp): made
+with the installed PyTorch, and again when that is another; without one it is
+left out.
 """
 import os
 import subprocess
@@ -20,6 +22,7 @@ SOURCES = ["routing.cu", "quant.cu", "combine.cu", "glu.cu", "ep_plan.cu", "ep_p
            "norm.cu", "grad_norm.cu", "grouped.cu"]
 HOST_SOURCE = os.path.join(CSRC, "host_torch.cpp")
 HOST_OUT = os.path.join(HERE, "sonicmoe", "_host.so")
+HOST_MADE = os.path.join(HERE, "build", "_host.command")      # what it was made by
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", "-I", INCLUDE, "-I", CSRC]
 
@@ -31,8 +34,12 @@ def _stale(target, deps):
     return any(os.path.getmtime(d) > t for d in deps)
 
 
-def _host_command():
-    import torch
+def host_command():
+    """What compiles _host.so with the PyTorch and the Python that run this; None without a PyTorch."""
+    try:
+        import torch
+    except ImportError:
+        return None
     at = os.path.dirname(torch.__file__)
     return ([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
              f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f'-DSMOE_TORCH_VERSION="{torch.__version__}"']
@@ -40,6 +47,18 @@ def _host_command():
                            sysconfig.get_paths()["include"], "/usr/local/cuda/include") for a in ("-I", i)]
             + [HOST_SOURCE, "-o", HOST_OUT, "-L", os.path.dirname(OUT), "-lsmoe_b200", "-L", os.path.join(at, "lib"), "-ltorch_python",
                "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"])
+
+
+def _made_by(command):
+    return "\n".join([sys.version, *command]) + "\n"
+
+
+def host_stale(command):
+    """Older than what it is made of, or made by another command, PyTorch or Python."""
+    if not os.path.exists(HOST_MADE) or _stale(HOST_OUT, [HOST_SOURCE, os.path.join(INCLUDE, "smoe_b200.h")]):
+        return True
+    with open(HOST_MADE) as f:
+        return f.read() != _made_by(command)
 
 
 def build(force=False, verbose=False):
@@ -65,8 +84,15 @@ def build(force=False, verbose=False):
     if force or procs or _stale(OUT, objs):
         cmd = [nvcc, "-shared", "-o", OUT] + objs + ["-lcudart"]
         subprocess.check_call(cmd)
-    if force or _stale(HOST_OUT, [HOST_SOURCE, headers[-1]]):
-        subprocess.check_call(_host_command())
+    command = host_command()
+    if command is None:
+        print("no PyTorch: _host.so, which the operators around the experts are called through, is not built")
+    elif force or host_stale(command):
+        if os.path.exists(HOST_MADE):
+            os.remove(HOST_MADE)
+        subprocess.check_call(command)
+        with open(HOST_MADE, "w") as f:
+            f.write(_made_by(command))
     return OUT
 
 
