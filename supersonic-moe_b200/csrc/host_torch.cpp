@@ -63,6 +63,12 @@ void same_gpu(const char* what, const Tensor& first, std::initializer_list<const
                 t->device().str(), ")");
 }
 
+// A tangent would be lost without a word where no node stands for the call, which refuses it by itself
+void no_tangent(const char* what, std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), what, ": no forward-mode derivatives");
+}
+
 // Gradients of gradients that could be differentiated again are not: their use raises
 variable_list once_only(const variable_list& in, variable_list out) {
   if (!at::GradMode::is_enabled() ||
@@ -179,6 +185,7 @@ constexpr double kNormLeastEps = 1e-90;                  // (what a root brought
 // x and residual as rows, and the weight, of a call that is allowed; kind: see smoe_rms_norm
 std::tuple<Tensor, Tensor, Tensor> norm_checked(const Tensor& x, const Tensor& w, const Tensor& residual, double eps, int kind) {
   const char* const what = kind ? "rms_norm_quantized" : "rms_norm";
+  no_tangent(what, {&x, &w, &residual});
   const auto tx = x.scalar_type();
   TORCH_CHECK_VALUE(tx == at::kBFloat16 || (tx == at::kFloat && !kind), what, ": x is bf16", kind ? "" : " or f32", ", got ", type_name(tx));
   const int64_t H = x.dim() ? x.size(-1) : 0;
@@ -309,6 +316,7 @@ struct GroupedNode : torch::autograd::Function<GroupedNode> {
 // x, weight as the kernels read them, of a call that is allowed
 std::tuple<Tensor, Tensor> grouped_checked(const Tensor& x, const Tensor& w, const Tensor& efo, const Tensor& counts) {
   const char* const what = "grouped_linear";
+  no_tangent(what, {&x, &w});
   TORCH_CHECK_VALUE(x.scalar_type() == at::kBFloat16 && x.dim() > 0, what, ": x is bf16 [rows,K], got ", type_name(x.scalar_type()), " ",
                     text(x.sizes()));
   TORCH_CHECK_VALUE(w.scalar_type() == at::kBFloat16 && (w.dim() == 2 || w.dim() == 3), what, ": the weight is bf16 [E,N,K], got ",
@@ -409,6 +417,7 @@ std::vector<smoe_gradient> table(Tensors& grads, const Tensors* outs, const char
   std::vector<smoe_gradient> t(grads.size());
   for (size_t i = 0; i < grads.size(); ++i) {
     const Tensor& o = outs ? (*outs)[i] : grads[i];
+    no_tangent(what, {&grads[i], &o});
     TORCH_CHECK_VALUE(taken(grads[i].scalar_type()) && taken(o.scalar_type()), what, ": gradients are f32 or bf16, got ",
                       at::toString(grads[i].scalar_type()), outs ? " into another type or that" : "");
     TORCH_CHECK(grads[i].device() == device && o.device() == device, what, ": tensors on different devices (", device.str(), ", ",
@@ -473,6 +482,7 @@ Tensor clip_gradients(const py::object& items, double max_norm, const Maybe& giv
   TORCH_CHECK_VALUE(max_norm >= 0, "clip_gradients: max_norm=", std::to_string(max_norm));
   auto grads = gradients(items, "clip_gradients");
   const Tensor norm = of(given);
+  no_tangent("clip_gradients", {&norm});
   TORCH_CHECK_VALUE(!norm.defined() || (norm.numel() == 1 && f32(norm) && norm.device() == grads[0].device()),
                     "clip_gradients: the norm is one f32 on ", grads[0].device().str());
   const auto before = grads.at;

@@ -12,7 +12,7 @@ def gradient_norm(gradients) -> torch.Tensor:
     """sqrt(sum of the squares of all values of all gradients) -> f32 [] on their GPU.
 
     gradients: tensors, f32 or bf16, of any shapes, or parameters, which stand for their `main_grad`, else their `.grad` (those with
-    neither are left out).  f32 sums of a few values, f64 beyond, in one order.  Nothing is copied to the host.  Across ranks that hold
+    neither are left out).  f32 sums of a few values, f64 beyond, in one order.  Nothing is copied to the host, and no gradient flows through it.  Across ranks that hold
     different parameters the squares of their norms add up: all-reduce those and hand the root to `clip_gradients(norm=...)`."""
     return ops.gradient_norm(gradients)
 

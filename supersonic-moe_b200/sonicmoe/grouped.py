@@ -68,7 +68,8 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, efo: torch.Tensor | No
     weight's.  Without efo there is one weight ([1,N,K] or [N,K]), every row is live, and x may have leading dimensions.
 
     Sums are f32, results bf16.  Differentiable in x and weight; a weight's gradient is added to the parameter's f32 `main_grad` where it
-    has one, else returned in bf16.  Gradients cannot be differentiated again."""
+    has one, else returned in bf16.  Gradients cannot be differentiated again, and there are no forward-mode
+    derivatives."""
     ops.poll_status(x.device)                 # a device-side failure of an earlier call surfaces here, without a sync
     grad = torch.is_grad_enabled()
     if not x.is_cuda:

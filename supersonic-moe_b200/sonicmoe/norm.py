@@ -84,7 +84,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | Non
     eps is 0 or at least 1e-90.
 
     Differentiable in x, weight and residual (the gradient of h included); a weight's gradient goes to the parameter's f32 `main_grad`
-    where it has one.  Gradients cannot be differentiated again."""
+    where it has one.  Gradients cannot be differentiated again, and there are no forward-mode derivatives."""
     _, _, y, h = _call(x, weight, residual, eps, None, True)
     return y if residual is None else (y, h)
 
