@@ -104,6 +104,7 @@ def block128_linear(x: torch.Tensor, weight, efo: torch.Tensor | None = None, co
         if weight.ndim not in (2, 3) or weight.dtype != torch.bfloat16:
             raise ValueError(f"block128_linear: the weight is bf16 [E,N,K], got {weight.dtype} {tuple(weight.shape)}")
         E, N, K = weight.shape if weight.ndim == 3 else (1, *weight.shape)
+    ops.no_tangent("block128_linear", x, weight)
     if x.shape[-1] != K:
         raise ValueError(f"block128_linear: x has {x.shape[-1]} columns, the weight {K}")
     if efo is not None and x.ndim != 2:

@@ -40,6 +40,13 @@ def isa_bytes(rows: int, cols: int) -> int:
     return -(-rows // 128) * -(-cols // 128) * 512
 
 
+def no_tangent(what, *tensors):
+    """Forward-mode derivatives are refused where no autograd node stands for a call, which would refuse them by itself."""
+    for t in tensors:
+        if t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{what}: no forward-mode derivatives")
+
+
 _status = {}
 
 # Optional per-op CUDA-event recorder (bench / profiling): a list that receives

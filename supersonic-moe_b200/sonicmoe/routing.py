@@ -69,6 +69,7 @@ def group_limited_routing(router_logits: torch.Tensor, K: int, *, score: str = "
             raise ValueError(f"bias {tuple(bias.shape)}: one value for each of {E} experts")
         if bias.dtype != torch.float32 or not bias.is_contiguous():
             bias = bias.detach().float().contiguous()
+    ops.no_tangent("group_limited_routing", router_logits)
     rule = (bias, groups, top_groups, group_score, score == "softmax", bool(normalize), float(scale))
     logits = router_logits if router_logits.is_contiguous() else router_logits.contiguous()
     if logits.requires_grad and torch.is_grad_enabled():
