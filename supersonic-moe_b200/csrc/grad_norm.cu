@@ -27,7 +27,7 @@ struct GradList {
   void* out[N];
   int64_t n[N];
   int first[N + 1];
-  uint8_t in_f32[N], out_f32[N], vec[N];     // vec: both start on 16 bytes
+  uint8_t in_f32[N], out_f32[N], vec[N];     // vec: they start on 16 bytes (the output where there is one)
   int count, chunk;
 };
 
@@ -223,7 +223,7 @@ static int grad_blocks(const smoe_gradient* list, int64_t from, int64_t to, int6
 }
 
 template <int N>
-static void grad_fill(GradList<N>& l, const smoe_gradient* list, int64_t from, int64_t to, int64_t chunk) {
+static void grad_fill(GradList<N>& l, const smoe_gradient* list, int64_t from, int64_t to, int64_t chunk, bool outs) {
   l.count = (int)(to - from);
   l.chunk = (int)chunk;
   int64_t pieces = 0;
@@ -236,7 +236,7 @@ static void grad_fill(GradList<N>& l, const smoe_gradient* list, int64_t from, i
     l.first[j] = (int)pieces;
     l.in_f32[j] = g.grad_f32 != 0;
     l.out_f32[j] = g.out_f32 != 0;
-    l.vec[j] = (((uintptr_t)g.grad | (uintptr_t)g.out) & 15) == 0;
+    l.vec[j] = (((uintptr_t)g.grad | (outs ? (uintptr_t)g.out : 0)) & 15) == 0;
     pieces += (g.numel + chunk - 1) / chunk;
   }
   l.first[l.count] = (int)pieces;
@@ -255,7 +255,7 @@ struct GradCall {
 template <int N>
 static cudaError_t grad_launch(const GradCall& c, int64_t from, int64_t to, int blocks, bool scale, int at) {
   GradList<N> l;
-  grad_fill(l, c.list, from, to, c.chunk);
+  grad_fill(l, c.list, from, to, c.chunk, scale);
   if (scale)
     return launch_early(grad_scale_kernel<N>, blocks, kGradThreads, 0, 0, c.stream, l, (const double*)c.partial, at, c.given, c.max_norm,
                         from == 0 ? c.norm : nullptr);
