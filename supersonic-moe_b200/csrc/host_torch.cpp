@@ -488,7 +488,7 @@ Tensor clip_gradients(const py::object& items, double max_norm, const Maybe& giv
   const auto before = grads.at;
   Tensors outs;
   if (!out.is_none()) {
-    outs = Tensors(out);
+    outs = Tensors(THPVariable_Check(out.ptr()) ? py::object(py::make_tuple(out)) : out);      // (one tensor, as of the gradients)
     for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(outs.items.ptr()); ++i) {
       PyObject* const o = PyTuple_GET_ITEM(outs.items.ptr(), i);
       TORCH_CHECK_TYPE(THPVariable_Check(o), "clip_gradients: outputs are tensors");

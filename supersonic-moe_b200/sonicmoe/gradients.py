@@ -21,7 +21,7 @@ def clip_gradients(gradients, max_norm: float, *, norm: torch.Tensor | None = No
     """gradients *= min(1, max_norm / (n + 1e-6)), n their norm, which is returned (f32 [], before clipping, on their GPU).
 
     gradients: as `gradient_norm` takes them, none overlapping another.  `norm`: f32 [], instead of theirs (that of all ranks).  `out`:
-    contiguous f32 or bf16 tensors of the gradients' shapes, one for each, which receive the results (accumulators in f32, gradients
+    contiguous f32 or bf16 tensors of the gradients' shapes, one for each (a single one as the gradients), which receive the results (accumulators in f32, gradients
     for the optimizer in bf16, from one pass); the gradients stay as they are then.  An output may be its own gradient and lies apart
     from every other one.  Without `out` they change in place, and where nothing is to be clipped nothing is written.  A norm of NaN makes every result NaN, an infinite one 0 (NaN where the gradient is infinite)."""
     return ops.clip_gradients(gradients, float(max_norm), norm, out)
