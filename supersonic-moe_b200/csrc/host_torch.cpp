@@ -2,6 +2,7 @@
 // nodes.  What Python and ctypes take for it is longer than the kernels of a small batch, or than the look at a list of a few hundred
 // gradients (us a call through Python / here: one decoded token's norm 21 / 10, norm with its backward pass 114 / 63, the norm of 300
 // gradients 205 / 22).  The kernels are those of the C ABI; nothing here computes.
+#include <ATen/MemoryOverlap.h>
 #include <ATen/core/Tensor.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <ATen/ops/zeros.h>
@@ -486,6 +487,10 @@ Tensor clip_gradients(const py::object& items, double max_norm, const Maybe& giv
   TORCH_CHECK_VALUE(!norm.defined() || (norm.numel() == 1 && f32(norm) && norm.device() == grads[0].device()),
                     "clip_gradients: the norm is one f32 on ", grads[0].device().str());
   const auto before = grads.at;
+  if (out.is_none())                                     // (before anything is launched)
+    for (const Tensor* t : before)
+      TORCH_CHECK_VALUE(at::has_internal_overlap(*t) != at::MemOverlap::Yes, "clip_gradients: a gradient ", text(t->sizes()),
+                        " holds one value in several places (an expanded tensor) and cannot be changed in place");
   Tensors outs;
   if (!out.is_none()) {
     outs = Tensors(THPVariable_Check(out.ptr()) ? py::object(py::make_tuple(out)) : out);      // (one tensor, as of the gradients)

@@ -23,5 +23,7 @@ def clip_gradients(gradients, max_norm: float, *, norm: torch.Tensor | None = No
     gradients: as `gradient_norm` takes them, none overlapping another.  `norm`: f32 [], instead of theirs (that of all ranks).  `out`:
     contiguous f32 or bf16 tensors of the gradients' shapes, one for each (a single one as the gradients), which receive the results (accumulators in f32, gradients
     for the optimizer in bf16, from one pass); the gradients stay as they are then.  An output may be its own gradient and lies apart
-    from every other one.  Without `out` they change in place, and where nothing is to be clipped nothing is written.  A norm of NaN makes every result NaN, an infinite one 0 (NaN where the gradient is infinite)."""
+    from every other one.  Without `out` they change in place (an expanded gradient is refused, a strided one goes through a copy and is
+    written always), and where nothing is to be clipped nothing else is written.  A norm of NaN makes every result NaN, an infinite one 0
+    (NaN where the gradient is infinite)."""
     return ops.clip_gradients(gradients, float(max_norm), norm, out)

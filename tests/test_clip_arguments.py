@@ -19,6 +19,19 @@ def test_a_single_output_for_a_single_gradient():
         sonicmoe.clip_gradients(torch.zeros(2), 1.0, out=torch.zeros(3))
 
 
+def test_expanded_gradients_are_not_changed_in_place():
+    """What torch.autograd.grad returns for a sum: one value in every place.  Refused before the others are touched."""
+    wide = torch.ones(1).expand(6)
+    for bad in (wide, torch.ones(3, 1).expand(3, 4), torch.ones(4).expand(2, 4)):
+        with pytest.raises(ValueError, match="several places"):
+            sonicmoe.clip_gradients([torch.zeros(8), bad], 1.0)
+    # into other tensors, and one that only looks expanded
+    for grads, kw in (([wide], dict(out=[torch.zeros(6)])), ([torch.zeros(1).expand(1)], {}), ([torch.zeros(0, 1).expand(0, 5)], {}),
+                      ([torch.zeros(4, 4).T], {}), ([torch.zeros(8)[::2]], {})):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            sonicmoe.clip_gradients(grads, 1.0, **kw)
+
+
 @pytest.mark.gpu
 def test_a_single_output_receives_the_result():
     g = torch.randn(5, 7, device="cuda")
@@ -26,3 +39,16 @@ def test_a_single_output_receives_the_result():
     n = sonicmoe.clip_gradients(g, 0.5, out=o)
     want = g.double() * (0.5 / (float(n) + 1e-6))
     assert ((o.double() - want).abs() <= want.abs() * (2.0 ** -8 + 2.0 ** -20)).all()
+
+
+@pytest.mark.gpu
+def test_nothing_is_changed_by_a_call_that_is_refused():
+    g, wide = torch.randn(64, device="cuda"), torch.ones(1, device="cuda").expand(6)
+    kept = g.clone()
+    with pytest.raises(ValueError, match="several places"):
+        sonicmoe.clip_gradients([g, wide], 1e-3)
+    assert torch.equal(g, kept)
+    o = [torch.empty(64, device="cuda"), torch.empty(6, device="cuda")]
+    n = float(sonicmoe.clip_gradients([g, wide], 1e-3, out=o))
+    assert abs(n - float(torch.cat([g, wide]).double().norm())) <= n * 2.0 ** -21
+    assert (o[1] == o[1][0]).all() and abs(float(o[1][0]) * n / 1e-3 - 1) <= 2.0 ** -20 + 1e-6 / n
