@@ -65,16 +65,23 @@ static int launch16(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensor
 // 4096 x 4096 24.6 / 18.1, 256 x 8192 x 2048 15.9 / 12.4, 8192 x 128 x 2048 15.3 / 12.1; of 64 tiles, 2048 x 2048 x 2048, 16.3 / 18.4)
 static bool narrow16(int64_t tiles, int64_t cols) { return tiles <= sm_count() / 4 || cols <= 128; }
 
-// Weights as the wide operand: where the rows of an expert make one tile of 64, evenly routed, or the tiles are few: one for each SM of
-// a single projection, two of experts, whose 256-row tiles are then mostly empty (us, the other kernel / few: 1 expert 4096 x 4096, 256
-// rows 17.4 / 15.8, 512 18.1 / 26.4; 1024 x 4096, 1024 rows 16.8 / 15.3, 2048 18.0 / 26.1; 1000 x 720, 2000 7.7 / 9.1; 8 of 512 x 512, 2048
-// 8.2 / 5.9, 4096 8.5 / 7.7, 8192 9.0 / 11.8; of 1024 x 1024, 1024 11.3 / 8.1, 2048 9.2 / 10.9; of 4096 x 2048, 512 31 / 26, 2048 35 /
-// 50; 128 of 1536 x 2048, 4096 177 / 128, 8192 170 / 133, 12288 168 / 170; the same unevenly routed 166 / 142, 182 / 171, 189 / 206.  The
-// gradient of the rows reads its weights across and takes up to a sixth longer with few.)  Segments with counts are padded, as a rule to
-// multiples of 128, and their live rows are not known here: as many rows as one such block an expert and an eighth more (us, the other / few
-// by live rows an expert of 128: 128 experts of 1536 x 2048, 8 179 / 136, 64 176 / 149, 100 of 149 180 / 173, 128 187 / 176, 140 of 202
-// 194 / 227; of 264 x 808, 8 37 / 20, 128 37 / 30; 37 of 1024 x 1024, 9 20.5 / 13.3, 128 20.4 / 22.9; 8 of 4096 x 2048, 8 33 / 27, 128 33.4 /
-// 34.2).
+// Weights as the wide operand: where the rows of an expert make one tile of 64, or the tiles are few: one for each SM of a single
+// projection, two of experts, whose 256-row tiles are then mostly empty (us, the other kernel / few):
+//   1 expert    4096 x 4096  256 rows 17.4 / 15.8, 512 18.1 / 26.4;  1024 x 4096  1024 rows 16.8 / 15.3, 2048 18.0 / 26.1;
+//               1000 x 720  2000 rows 7.7 / 9.1
+//   8 experts   512 x 512  2048 rows 8.2 / 5.9, 4096 8.5 / 7.7, 8192 9.0 / 11.8;  1024 x 1024  1024 rows 11.3 / 8.1, 2048 9.2 / 10.9;
+//               4096 x 2048  512 rows 31 / 26, 2048 35 / 50
+//   128         1536 x 2048  4096 rows 177 / 128, 8192 170 / 133, 12288 168 / 170;  unevenly routed 166 / 142, 182 / 171, 189 / 206
+// The gradient of the rows reads its weights across and takes up to a sixth longer with few.
+//   Segments that are padded to multiples of 128, which counts and a table of a multiple of 128 rows stand for, have live rows that are not
+// known here, and two tiles an expert at most: one such block an expert and an eighth more, as the metadata allocates for up to 16 rows an
+// expert (us, the other kernel / few, y; gradient of the rows, by live rows an expert of allocated ones):
+//   128 of 1536 x 2048  16 of 144 177 / 139; 173 / 141   1 to 128 of 128 178 / 148; 174 / 150   90 on average 181 / 173; 175 / 181
+//   128 of 2048 x 768   16 of 144 126 / 85; 117 / 81     1 to 128 of 128 124 / 95; 118 / 89     90 on average 104 / 103; 103 / 100
+//   37 of 1024 x 1024    4 of 135 21.1 / 12.9; 19.3 / 12.4   1 to 128 of 128 21.5 / 21.8; 20.4 / 22.2   90 21.1 / 22.9; 19.6 / 23.1
+//   8 of 4096 x 2048    16 of 144 32.8 / 26.7; 31.0 / 24.9   1 to 128 of 128 33.0 / 29.5; 31.0 / 34.9   90 32.6 / 34.2; 30.7 / 33.1
+// Blocks that are all full pay: 0 to 20 %, 128 of 2048 x 768 a third on a GPU at lower clocks (115 / 150; at full clocks 89 / 98).
+//   Of segments with gaps all rows may live, and those above 128 take a third tile (129 of 136 rows, 128 of 1536 x 2048: 170 / 219; 164 / 255).
 static bool few_rows16(int64_t rows, int64_t N, int64_t E, bool padded) {
   if (rows <= (padded ? 9 * 128 * E / 8 : Few16Smem::NT * E)) return true;
   const int64_t busy = rows < E ? rows : E;
@@ -179,7 +186,7 @@ int smoe_grouped_rows(const void* x_bf16, int64_t ldx, const void* w_bf16, int w
   if (!on16(x_bf16) || !on16(w_bf16) || !on16(y_bf16)) return SMOE_ERR_ALIGN;
   if (!w_transposed && gemv_rows16(rows, N, K, E))
     return gemv16(x_bf16, ldx, w_bf16, efo, counts, y_bf16, rows, N, K, E, (cudaStream_t)stream);
-  if (few_rows16(rows, N, E, counts != nullptr))
+  if (few_rows16(rows, N, E, counts && rows % 128 == 0))
     return few16(x_bf16, ldx, w_bf16, efo, counts, y_bf16, rows, N, K, E, w_transposed != 0, status, pinned_host_word,
                  (cudaStream_t)stream);
   // every segment may end in a tile that is not full
