@@ -473,6 +473,14 @@ bool read_apart(const Span& in, const std::vector<Span>& written, bool itself) {
     if (!itself || w->i != in.i || w->from != in.from || w->to != in.to) return false;
   return true;
 }
+// a value, of the memory between a strided tensor's first value and its last one
+bool outside(const Tensor& value, const Tensor& t) {
+  if (!t.numel()) return true;
+  int64_t last = 0;
+  for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+  const uintptr_t at = (uintptr_t)value.data_ptr(), from = (uintptr_t)t.data_ptr();
+  return at + value.element_size() <= from || at >= from + (last + 1) * t.element_size();
+}
 
 void written(const std::vector<const Tensor*>& ts) {     // autograd sees that they are others now
   for (const Tensor* t : ts)
@@ -513,6 +521,9 @@ Tensor clip_gradients(const py::object& items, double max_norm, const Maybe& giv
       TORCH_CHECK_VALUE(!grads[i].numel() || read_apart(span(grads[i], i), spans, f32(grads[i]) == f32(outs[i])),
                         "clip_gradients: an output lies where another gradient does");
   TORCH_CHECK_VALUE(!norm.defined() || read_apart(span(norm, 0), spans, false), "clip_gradients: the norm lies in what is written");
+  if (norm.defined() && out.is_none())                   // (a strided gradient is written last, from its first value to its last one)
+    for (const Tensor* t : before)
+      TORCH_CHECK_VALUE(t->is_contiguous() || outside(norm, *t), "clip_gradients: the norm lies in what is written");
   on_gpu(grads[0]);
   const c10::cuda::CUDAGuard guard(grads[0].device());
   Tensor n = norm, ws;

@@ -32,6 +32,17 @@ def test_expanded_gradients_are_not_changed_in_place():
             sonicmoe.clip_gradients(grads, 1.0, **kw)
 
 
+def test_the_norm_does_not_lie_in_a_strided_gradient():
+    """Which is written from a copy at the end: the norm that is returned would be a clipped value."""
+    base = torch.zeros(100)
+    for grads, at in (([base[:64].view(8, 8).T], 13), ([base[10:50].view(5, 8)[:, :4]], 45), ([base[60:90:3]], 87), ([base[60:90:3]], 60)):
+        with pytest.raises(ValueError, match="norm lies"):
+            sonicmoe.clip_gradients(grads, 1.0, norm=base[at])
+    for grads, at in (([base[:64].view(8, 8).T], 64), ([base[10:50].view(5, 8)[:, :4]], 46), ([base[60:90:3]], 88), ([base[60:90:3]], 59)):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            sonicmoe.clip_gradients(grads, 1.0, norm=base[at])
+
+
 @pytest.mark.gpu
 def test_a_single_output_receives_the_result():
     g = torch.randn(5, 7, device="cuda")
