@@ -234,7 +234,7 @@ struct NormArgs {
 enum NormQuant : int { NORM_PLAIN = 0, NORM_MX = 1, NORM_BLOCK128 = 2 };
 
 // Blocks an SM has at a time: two where h is f32, for the registers of the next row (us, two / three without it: 8192 x 4096 with residual
-// in f32, rows and payload 69 / 71, 131072 x 128 39 / 45, 3001 x 1000 7.4 / 6.7, for which two take three turns instead of two).
+// in f32, rows and payload 69 / 71, 131072 x 128 39 / 45, 3001 x 1000, rows alone, 7.4 / 6.7, for which two take three turns instead of two).
 constexpr int norm_blocks(bool h_f32, int pieces) { return pieces > 2 ? 1 : h_f32 ? 2 : 3; }
 
 // RES: 0 none, 1 of x's type, 2 f32 (beside bf16).  A block stays and takes rows in turn, several at a time, each by threads of its own;
@@ -267,145 +267,145 @@ __global__ void __launch_bounds__(NC == 2 ? 256 : 512, norm_blocks(XF32 || RES =
   at.load(w, a.w, 0);
   int turn = 0;
   for (; first < a.T; first += stride) {
-  if (!AHEAD) ask(first);
-  const int64_t row = first + in_warp;
-  if (NARROW) at.H = row < a.T ? a.H : 0;
-  NormVec<HF32> h[NC];
-#pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    if constexpr (RES == 0) {
-      h[c] = x[c];
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (!HF32) asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(h[c].w[i]) : "r"(x[c].w[i]), "r"(res[c].w[i]));
-        else h[c].set(i, x[c].pair(i) + res[c].pair(i));
-      }
-    }
-  }
-  if (AHEAD) ask(first + stride);
-  if constexpr (RES != 0) {
-#pragma unroll
-    for (int c = 0; c < NC; ++c) at.store(h[c], a.h, row * a.H, c);
-  }
-  double s0 = 0.0, s1 = 0.0;
-#pragma unroll
-  for (int c = 0; c < NC; ++c) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = p2_get(h[c].pair(i));
-      const double p = f.x, q = f.y;
-      s0 = fma(p, p, s0);
-      s1 = fma(q, q, s1);
-    }
-  }
-  const double r64 = norm_rsqrt(norm_sum<NARROW>(s0 + s1, a.lanes, group, sums[turn]) * a.inv_H + a.eps);
-  turn ^= 1;                                            // the next row's sums do not wait for this one's readers
-  const float r = (float)r64;
-  if (a.rstd && at.t == 0 && (!NARROW || at.H)) a.rstd[row] = r64;
-  const bool far = !(r64 > 1e-30 && r64 < 1e30);        // r in f32 would not have its full precision
-  const P2 r2 = p2(r, r);
-  NormVec<false> kept[NARROW && QUANT == NORM_BLOCK128 ? NC : 1];
-  // y of columns from col on, whose group's largest magnitude is m
-  auto quantise128 = [&](const NormVec<false>& y, uint32_t m, int col, bool first_of_group) {
-    m &= 0x7FFF7FFFu;
-    const float amax = fmaxf(fmaxf(__uint_as_float(m << 16), __uint_as_float(m & 0xFFFF0000u)), kAmaxFloor);
-    // one division a lane, of either kind
-    const float quotient = ((lane & 1) ? kE4m3Max : amax) / ((lane & 1) ? amax : kE4m3Max);
-    const float qs = __shfl_sync(0xffffffffu, quotient, lane | 1);
-    float2 b[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) b[i] = p2_get(y.pair(i) * p2(qs, qs));
-    if (col < at.H) {
-      *reinterpret_cast<uint2*>(a.q + row * a.pitch + col) =
-          make_uint2(q_pack4(b[0].x, b[0].y, b[1].x, b[1].y), q_pack4(b[2].x, b[2].y, b[3].x, b[3].y));
-      if (first_of_group) ((float*)a.s)[row * ((a.H + 127) >> 7) + (col >> 7)] = quotient;
-    }
-  };
-  auto largest = [](const NormVec<false>& y) {
-    return q_max_abs_bf16x2(q_max_abs_bf16x2(y.w[0], y.w[1]), q_max_abs_bf16x2(y.w[2], y.w[3]));
-  };
-#pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    const int col = at.col(c);
-    P2 v[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = h[c].pair(i) * r2 * w[c].pair(i);
-    if constexpr (XF32) {
-      NormVec<true> y;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) y.set(i, v[i]);
-      if (far) {
-        NormVec<HF32> hc = h[c];
-        NormVec<WF32> wc = w[c];
-        hc.anew();
-        wc.anew();
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float2 f = p2_get(hc.pair(i >> 1)), g = p2_get(wc.pair(i >> 1));
-          y.f[i] = (float)((double)(i & 1 ? f.y : f.x) * r64 * (double)(i & 1 ? g.y : g.x));
-        }
-      }
-      at.store(y, a.y, row * a.H, c);
-    } else {
-      // least distances above a border less kNormNear, of the even and the odd values (a carry makes an odd one's one more)
-      uint32_t near = 0xFFFFFFFFu;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 f = p2_get(v[i]);
-        near = norm_min_u16x2(near, __byte_perm(__float_as_uint(f.x), __float_as_uint(f.y), 0x5410) + (0x8000u + kNormNear) * 0x10001u);
-      }
-      if ((near & 0xFFFFu) <= 2 * kNormNear || near < (2 * kNormNear + 2) << 16 || far) {
-        // (anew: what is f64 of these values here would otherwise be kept from the sum of squares, and the weights' over all rows)
-        NormVec<HF32> hc = h[c];
-        NormVec<WF32> wc = w[c];
-        hc.anew();
-        wc.anew();
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 f = p2_get(hc.pair(i)), g = p2_get(wc.pair(i));
-          v[i] = p2(norm_for_bf16((double)f.x * (double)g.x * r64, kNormTie), norm_for_bf16((double)f.y * (double)g.y * r64, kNormTie));
-        }
-      }
-      NormVec<false> y;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) y.set(i, v[i]);
-      if (QUANT == NORM_PLAIN || a.y) at.store(y, a.y, row * a.H, c);
-      if constexpr (QUANT == NORM_MX) {                 // four lanes a group
-        uint32_t m = largest(y);
-        m = q_max_abs_bf16x2(m, __shfl_xor_sync(0xffffffffu, m, 1));
-        m = q_max_abs_bf16x2(m, __shfl_xor_sync(0xffffffffu, m, 2));
-        m &= 0x7FFF7FFFu;
-        const int e = q_e8m0_of(fmaxf(fmaxf(0.f, __uint_as_float(m << 16)), __uint_as_float(m & 0xFFFF0000u)));
-        const uint32_t qs = (__float_as_uint(q_scale_of(e)) >> 16) * 0x10001u;      // a power of two is a bf16
-        if (col < at.H) {
-          *reinterpret_cast<uint2*>(a.q + row * a.pitch + col) =
-              make_uint2(q_pack4_scaled(y.w[0], y.w[1], qs, qs), q_pack4_scaled(y.w[2], y.w[3], qs, qs));
-          if ((lane & 3) == 0) ((uint8_t*)a.s)[row * (a.H >> 5) + (col >> 5)] = (uint8_t)e;
-        }
-      }
-      if constexpr (QUANT == NORM_BLOCK128 && NARROW) kept[c] = y;
-      if constexpr (QUANT == NORM_BLOCK128 && !NARROW) {      // sixteen
-        uint32_t m = largest(y);
-#pragma unroll
-        for (int d = 1; d < 16; d <<= 1) m = q_max_abs_bf16x2(m, __shfl_xor_sync(0xffffffffu, m, d));
-        quantise128(y, m, col, (lane & 15) == 0);
-      }
-    }
-  }
-  if constexpr (QUANT == NORM_BLOCK128 && NARROW) {     // sixteen lanes, or all of a row's two pieces
-    const bool one = a.lanes < 16;
-    uint32_t both = largest(kept[0]);
-    if (one) both = q_max_abs_bf16x2(both, largest(kept[NC - 1]));
+    if (!AHEAD) ask(first);
+    const int64_t row = first + in_warp;
+    if (NARROW) at.H = row < a.T ? a.H : 0;
+    NormVec<HF32> h[NC];
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      uint32_t m = c == 0 || one ? both : largest(kept[c]);
+      if constexpr (RES == 0) {
+        h[c] = x[c];
+      } else {
 #pragma unroll
-      for (int d = 1; d < 16; d <<= 1)
-        if (d < a.lanes) m = q_max_abs_bf16x2(m, __shfl_xor_sync(0xffffffffu, m, d));
-      quantise128(kept[c], m, at.col(c), at.t == 0 && (c == 0 || !one));
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (!HF32) asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(h[c].w[i]) : "r"(x[c].w[i]), "r"(res[c].w[i]));
+          else h[c].set(i, x[c].pair(i) + res[c].pair(i));
+        }
+      }
     }
-  }
+    if (AHEAD) ask(first + stride);
+    if constexpr (RES != 0) {
+#pragma unroll
+      for (int c = 0; c < NC; ++c) at.store(h[c], a.h, row * a.H, c);
+    }
+    double s0 = 0.0, s1 = 0.0;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = p2_get(h[c].pair(i));
+        const double p = f.x, q = f.y;
+        s0 = fma(p, p, s0);
+        s1 = fma(q, q, s1);
+      }
+    }
+    const double r64 = norm_rsqrt(norm_sum<NARROW>(s0 + s1, a.lanes, group, sums[turn]) * a.inv_H + a.eps);
+    turn ^= 1;                                            // the next row's sums do not wait for this one's readers
+    const float r = (float)r64;
+    if (a.rstd && at.t == 0 && (!NARROW || at.H)) a.rstd[row] = r64;
+    const bool far = !(r64 > 1e-30 && r64 < 1e30);        // r in f32 would not have its full precision
+    const P2 r2 = p2(r, r);
+    NormVec<false> kept[NARROW && QUANT == NORM_BLOCK128 ? NC : 1];
+    // y of columns from col on, whose group's largest magnitude is m
+    auto quantise128 = [&](const NormVec<false>& y, uint32_t m, int col, bool first_of_group) {
+      m &= 0x7FFF7FFFu;
+      const float amax = fmaxf(fmaxf(__uint_as_float(m << 16), __uint_as_float(m & 0xFFFF0000u)), kAmaxFloor);
+      // one division a lane, of either kind
+      const float quotient = ((lane & 1) ? kE4m3Max : amax) / ((lane & 1) ? amax : kE4m3Max);
+      const float qs = __shfl_sync(0xffffffffu, quotient, lane | 1);
+      float2 b[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) b[i] = p2_get(y.pair(i) * p2(qs, qs));
+      if (col < at.H) {
+        *reinterpret_cast<uint2*>(a.q + row * a.pitch + col) =
+            make_uint2(q_pack4(b[0].x, b[0].y, b[1].x, b[1].y), q_pack4(b[2].x, b[2].y, b[3].x, b[3].y));
+        if (first_of_group) ((float*)a.s)[row * ((a.H + 127) >> 7) + (col >> 7)] = quotient;
+      }
+    };
+    auto largest = [](const NormVec<false>& y) {
+      return q_max_abs_bf16x2(q_max_abs_bf16x2(y.w[0], y.w[1]), q_max_abs_bf16x2(y.w[2], y.w[3]));
+    };
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int col = at.col(c);
+      P2 v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = h[c].pair(i) * r2 * w[c].pair(i);
+      if constexpr (XF32) {
+        NormVec<true> y;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y.set(i, v[i]);
+        if (far) {
+          NormVec<HF32> hc = h[c];
+          NormVec<WF32> wc = w[c];
+          hc.anew();
+          wc.anew();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float2 f = p2_get(hc.pair(i >> 1)), g = p2_get(wc.pair(i >> 1));
+            y.f[i] = (float)((double)(i & 1 ? f.y : f.x) * r64 * (double)(i & 1 ? g.y : g.x));
+          }
+        }
+        at.store(y, a.y, row * a.H, c);
+      } else {
+        // least distances above a border less kNormNear, of the even and the odd values (a carry makes an odd one's one more)
+        uint32_t near = 0xFFFFFFFFu;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 f = p2_get(v[i]);
+          near = norm_min_u16x2(near, __byte_perm(__float_as_uint(f.x), __float_as_uint(f.y), 0x5410) + (0x8000u + kNormNear) * 0x10001u);
+        }
+        if ((near & 0xFFFFu) <= 2 * kNormNear || near < (2 * kNormNear + 2) << 16 || far) {
+          // (anew: what is f64 of these values here would otherwise be kept from the sum of squares, and the weights' over all rows)
+          NormVec<HF32> hc = h[c];
+          NormVec<WF32> wc = w[c];
+          hc.anew();
+          wc.anew();
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 f = p2_get(hc.pair(i)), g = p2_get(wc.pair(i));
+            v[i] = p2(norm_for_bf16((double)f.x * (double)g.x * r64, kNormTie), norm_for_bf16((double)f.y * (double)g.y * r64, kNormTie));
+          }
+        }
+        NormVec<false> y;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y.set(i, v[i]);
+        if (QUANT == NORM_PLAIN || a.y) at.store(y, a.y, row * a.H, c);
+        if constexpr (QUANT == NORM_MX) {                 // four lanes a group
+          uint32_t m = largest(y);
+          m = q_max_abs_bf16x2(m, __shfl_xor_sync(0xffffffffu, m, 1));
+          m = q_max_abs_bf16x2(m, __shfl_xor_sync(0xffffffffu, m, 2));
+          m &= 0x7FFF7FFFu;
+          const int e = q_e8m0_of(fmaxf(fmaxf(0.f, __uint_as_float(m << 16)), __uint_as_float(m & 0xFFFF0000u)));
+          const uint32_t qs = (__float_as_uint(q_scale_of(e)) >> 16) * 0x10001u;      // a power of two is a bf16
+          if (col < at.H) {
+            *reinterpret_cast<uint2*>(a.q + row * a.pitch + col) =
+                make_uint2(q_pack4_scaled(y.w[0], y.w[1], qs, qs), q_pack4_scaled(y.w[2], y.w[3], qs, qs));
+            if ((lane & 3) == 0) ((uint8_t*)a.s)[row * (a.H >> 5) + (col >> 5)] = (uint8_t)e;
+          }
+        }
+        if constexpr (QUANT == NORM_BLOCK128 && NARROW) kept[c] = y;
+        if constexpr (QUANT == NORM_BLOCK128 && !NARROW) {      // sixteen
+          uint32_t m = largest(y);
+#pragma unroll
+          for (int d = 1; d < 16; d <<= 1) m = q_max_abs_bf16x2(m, __shfl_xor_sync(0xffffffffu, m, d));
+          quantise128(y, m, col, (lane & 15) == 0);
+        }
+      }
+    }
+    if constexpr (QUANT == NORM_BLOCK128 && NARROW) {     // sixteen lanes, or all of a row's two pieces
+      const bool one = a.lanes < 16;
+      uint32_t both = largest(kept[0]);
+      if (one) both = q_max_abs_bf16x2(both, largest(kept[NC - 1]));
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        uint32_t m = c == 0 || one ? both : largest(kept[c]);
+#pragma unroll
+        for (int d = 1; d < 16; d <<= 1)
+          if (d < a.lanes) m = q_max_abs_bf16x2(m, __shfl_xor_sync(0xffffffffu, m, d));
+        quantise128(kept[c], m, at.col(c), at.t == 0 && (c == 0 || !one));
+      }
+    }
   }
 }
 
