@@ -74,7 +74,7 @@ static bool narrow16(int64_t tiles, int64_t cols) { return tiles <= sm_count() /
 //   128         1536 x 2048  4096 rows 177 / 128, 8192 170 / 133, 12288 168 / 170;  unevenly routed 166 / 142, 182 / 171, 189 / 206
 // The gradient of the rows reads its weights across and takes up to a sixth longer with few.
 //   Segments that are padded to multiples of 128, which counts and a table of a multiple of 128 rows stand for, have live rows that are not
-// known here, and two tiles an expert at most: one such block an expert and an eighth more, as the metadata allocates for up to 16 rows an
+// known here, and two tiles a block at most: one such block an expert and an eighth more, as the metadata allocates for up to 16 rows an
 // expert (us, the other kernel / few, y; gradient of the rows, by live rows an expert of allocated ones):
 //   128 of 1536 x 2048  16 of 144 177 / 139; 173 / 141   1 to 128 of 128 178 / 148; 174 / 150   90 on average 181 / 173; 175 / 181
 //   128 of 2048 x 768   16 of 144 126 / 85; 117 / 81     1 to 128 of 128 124 / 95; 118 / 89     90 on average 104 / 103; 103 / 100
